@@ -352,6 +352,91 @@ int rmi_gqa_flash_decode_noalloc(const float* q, const uint16_t* kcache, const u
                                  float scale, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------------
+ * K/V caches in 16, 8 or 4 bits, attention for trees of drafted tokens over them, and the logits of a tree's nodes
+ * (no counterpart in the reference, whose cache is fp16, whose draft is one token and whose logits go out as they are)
+ * ------------------------------------------------------------------------------------------------------------- */
+
+/* Cache types.  One cache holds the K or the V rows of one layer, [max_ctx] positions x n_kv heads x head_dim (128 or
+ * 256) dims, 16-byte aligned:
+ *   F16  the layout of the fp16 caches above, [position][kv head][dim];
+ *   I8   codes [kv head][position][dim], one byte code + 128, then scales [kv head][position][dim / 32], one byte each;
+ *   I4   codes [kv head][position][dim / 8], a little-endian 32-bit word per 8 dims with code + 8 of dim 2 k at bits
+ *        4 k and of dim 2 k + 1 at bits 16 + 4 k, then scales as I8.
+ * A block of 32 dims shares the scale s: a scale byte b is the fp16 number with the bits b << 7 (five exponent and three
+ * mantissa bits).  s is the smallest such number with Q s >= max|x| (Q = 127 / 7, at most 512 / 8192: larger values
+ * saturate), code = x / s rounded to the nearest integer (half to even), |code| <= Q, and the cache holds code * s, which
+ * is an fp16 number exactly.  A block with an infinity or a NaN gets s = NaN and reads back as NaN. */
+enum { RMI_KV_F16 = 0, RMI_KV_I8 = 1, RMI_KV_I4 = 2 };
+
+/* bytes of one cache; 0 on a bad type or shape */
+size_t rmi_kv_cache_bytes(int type, int max_ctx, int n_kv, int head_dim);
+/* n rows [n_kv x head_dim] of fp32 (src_f16 = 0) or fp16 (1), src_stride elements apart, to positions [first, first + n)
+ * of the cache; n = 0 does nothing.  The source may not overlap the cache. */
+int rmi_kv_write(int type, const void* src, int src_f16, int src_stride, void* cache, int first, int n, int n_kv,
+                 int head_dim, int max_ctx, void* stream);
+/* positions [first, first + n) back to rows of fp32 or fp16 (both exact for I8 and I4), out_stride elements apart */
+int rmi_kv_read(int type, const void* cache, void* out, int out_f16, int out_stride, int first, int n, int n_kv,
+                int head_dim, int max_ctx, void* stream);
+/* Moves rows pos[0] + path[i] to pos[0] + i for i < min(count[0], max_path) in each of n_caches (1..64) caches of one
+ * type: the accepted path of a drafted tree becomes the context's next rows.  `caches` is a host array of device
+ * pointers, read during the call; pos, path and count are device words.  All rows are read before any is written.  A
+ * move from or to a position outside [0, max_ctx) is left out.  max_path <= 64. */
+int rmi_kv_compact(int type, void* const* caches, int n_caches, const int* pos, const int* path, const int* count,
+                   int max_path, int n_kv, int head_dim, int max_ctx, void* stream);
+
+/* Which position turns pair i of n_rot / 2: `section` pairs of each of three axes (time, height, width), which add up to
+ * n_rot / 2; in runs (interleaved = 0), or dealt out in turn (1): axis 1 at i % 3 == 1 and axis 2 at i % 3 == 2 while
+ * i < 3 * section of that axis, axis 0 elsewhere. */
+typedef struct rmi_rope_axes {
+    int section[3];
+    int interleaved;
+} rmi_rope_axes;
+/* rmi_attn_prep_rope for caches of any type and positions that are not slots: token t's K and V rows go to slot
+ * pos[0] + t (nothing is written for a slot outside [0, max_ctx)) and its rotation is at axis_pos[a * ntok + t] of axis a
+ * (null: the slot, on every axis).  For F16 with a null axis_pos the results are bitwise rmi_attn_prep_rope's.  K rows
+ * that are quantised are normed and rotated in fp64 and rounded to fp32 once, so their codes do not hang on the order of
+ * a sum.  ntok >= 1. */
+int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* qn, const float* kn, int ktype, void* kcache,
+                       int vtype, void* vcache, const int* pos, const int* axis_pos, float* qout, int n_head, int n_kv,
+                       int head_dim, int n_rot, const rmi_rope_params* rope, const rmi_rope_axes* axes, float eps,
+                       int ntok, int max_ctx, void* stream);
+
+/* Attention of ntok drafted tokens, whose K and V rows are at slots pos[0] + 0 .. ntok - 1, over the context before them
+ * and each other: token t sees every position below pos[0] and slot pos[0] + j where bit j of masks[t] is set (ntok <=
+ * 64; a token that sees nothing gives zeros), or with null masks the chain j <= t (ntok <= 1024: decode, verify and
+ * prompt chunks).  q is [ntok][n_head][head_dim]; kcache / vcache types: both F16, both I8, both I4, or I8 and I4;
+ * sigmoid gate as rmi_gqa_flash_decode's (gate of head h at + h * 2 * head_dim + head_dim; null: no gate); fp32 y
+ * (nullable) and Q8_1 (nullable).  Rows a token does not see have no part in its result, whatever they hold.  If a slot
+ * lies outside [0, max_ctx) nothing is written.
+ * The context is split into chunks of 128 * nsub positions; rmi_gqa_tree_nsub gives the split for a context of `ctx`
+ * positions, to be settled once (results differ in the last bits between splits).  workspace holds
+ * rmi_gqa_tree_workspace_bytes(...) bytes, 16-byte aligned, and needs no initial state; calls that may overlap need one
+ * each.  Same inputs, same bits; I8 and I4 caches give the bits of an F16 cache that holds their values. */
+int rmi_gqa_tree_nsub(int ctx, int n_head, int n_kv, int head_dim, int ntok);
+size_t rmi_gqa_tree_workspace_bytes(int max_ctx, int n_head, int n_kv, int head_dim, int ntok, int nsub);
+int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache, int vtype, const void* vcache, const int* pos,
+                        const uint64_t* masks, const float* gate_src, int gate_stride, float* y, int y_stride,
+                        uint8_t* q8, int q8_stride, void* workspace, int n_head, int n_kv, int head_dim, int ntok,
+                        int max_ctx, int nsub, float scale, void* stream);
+
+/* What a sampler wants done to ncols (1..64) columns of n logits before rmi_argmax / rmi_topk.  Column c's text is
+ * history[0 .. min(history_len[0], max_history)) (device words; null: empty) and then, with a draft of ndraft <= 64
+ * tokens, those draft[j] whose bit j of masks[c] is set, in ascending order (the path to a tree's node); ids outside
+ * [0, n) count for nothing.  m = how often v stands in the text's last `window` tokens (window <= 0: in all of it).
+ *   x = logits[v] + bias of v (bias_ids / bias_vals, n_bias entries; of entries with one id the last counts)
+ *   m > 0:  x = x > 0 ? x / repetition : x * repetition;   x -= m * frequency + presence
+ *   bit v % 32 of allow[c * allow_stride + v / 32] clear:  x = -infinity     (null allow: every token)
+ * out may be logits (with the same stride).  repetition > 0. */
+typedef struct rmi_penalties {
+    float repetition, presence, frequency;
+    int window;
+} rmi_penalties;
+int rmi_logits_process(const float* logits, int n, int ncols, int col_stride, float* out, int out_stride,
+                       const int* history, const int* history_len, int max_history, const int* draft,
+                       const uint64_t* masks, int ndraft, const rmi_penalties* penalties, const int* bias_ids,
+                       const float* bias_vals, int n_bias, const uint32_t* allow, int allow_stride, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
  * Seeded synthetic tensors in HBM (stand-in for a GGUF file: random-init weights; no reference counterpart)
  * ------------------------------------------------------------------------------------------------------------- */
 int rmi_gen_q6_k(void* w, size_t nblocks, uint64_t seed, float d_std, void* stream);

@@ -18,6 +18,7 @@ CSRC = os.path.join(_HERE, "csrc")
 
 RMI_OK, RMI_ERR_SHAPE, RMI_ERR_POINTER, RMI_ERR_STREAM, RMI_ERR_LAUNCH, RMI_ERR_UNSUPPORTED, RMI_ERR_STATE = range(7)
 GGML_Q8_0, GGML_Q6_K = 8, 14
+KV_F16, KV_I8, KV_I4 = range(3)   # K/V cache types
 Q6K_BYTES, Q8_0_BYTES, Q8_1_BYTES = 210, 34, 36
 
 _lib = None
@@ -104,6 +105,18 @@ SIGNATURES = {
                                           _vp]),
     "rmi_gqa_flash_decode": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f,
                                   _vp]),
+    "rmi_kv_cache_bytes": (_sz, [_i, _i, _i, _i]),
+    "rmi_kv_write": (_i, [_i, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _vp]),
+    "rmi_kv_read": (_i, [_i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "rmi_kv_compact": (_i, [_i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "rmi_attn_prep_axes": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _f, _i,
+                                _i, _vp]),
+    "rmi_gqa_tree_nsub": (_i, [_i, _i, _i, _i, _i]),
+    "rmi_gqa_tree_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "rmi_gqa_tree_decode": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i,
+                                 _i, _f, _vp]),
+    "rmi_logits_process": (_i, [_vp, _i, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i,
+                                _vp]),
 }
 
 
@@ -528,3 +541,92 @@ def gqa_flash_decode_noalloc(q, kcache, vcache, pos, gate_src, gate_stride, y, y
     scratch array (rmi_gqa_noalloc_scratch_max() bytes); no allocation.  Calls that overlap on one GPU race."""
     _call("rmi_gqa_flash_decode_noalloc", _p(q), _p(kcache), _p(vcache), _p(pos), _p(gate_src), gate_stride, _p(y),
           y_stride, _p(q8), q8_stride, n_head, n_kv, head_dim, ntok, max_ctx, nsub, scale, _stream(stream))
+
+
+# ---- K/V caches in 16, 8 or 4 bits, attention for drafted trees over them, logits of a tree's nodes ---------------------
+
+def kv_cache_bytes(type_, max_ctx, n_kv, head_dim) -> int:
+    n = lib().rmi_kv_cache_bytes(type_, max_ctx, n_kv, head_dim)
+    if n == 0:
+        raise ValueError(last_error())
+    return n
+
+
+def _is_f16(t):
+    """1 for 16-bit rows (float16, or int16 / uint16 that hold its bits), 0 for float32"""
+    return 1 if t.element_size() == 2 else 0
+
+
+def kv_write(type_, src, src_stride, cache, first, n, n_kv, head_dim, max_ctx, stream=None):
+    """n rows [n_kv x head_dim] of float32 or float16, src_stride elements apart, to positions [first, first + n)"""
+    _call("rmi_kv_write", type_, _p(src), _is_f16(src), src_stride, _p(cache), first, n, n_kv, head_dim, max_ctx,
+          _stream(stream))
+
+
+def kv_read(type_, cache, out, out_stride, first, n, n_kv, head_dim, max_ctx, stream=None):
+    """positions [first, first + n) of a cache back to float32 or float16 rows"""
+    _call("rmi_kv_read", type_, _p(cache), _p(out), _is_f16(out), out_stride, first, n, n_kv, head_dim, max_ctx,
+          _stream(stream))
+
+
+def kv_compact(type_, caches, pos, path, count, max_path, n_kv, head_dim, max_ctx, stream=None):
+    """rows pos[0] + path[i] -> pos[0] + i, i < min(count[0], max_path), in each of the caches (a list of tensors)"""
+    ptrs = (ctypes.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches])
+    _call("rmi_kv_compact", type_, ptrs, len(caches), _p(pos), _p(path), _p(count), max_path, n_kv, head_dim, max_ctx,
+          _stream(stream))
+
+
+class RopeAxes(ctypes.Structure):
+    """rmi_rope_axes: the pairs of each axis and how they are dealt out"""
+    _fields_ = [("section", ctypes.c_int * 3), ("interleaved", ctypes.c_int)]
+
+
+def attn_prep_axes(q3, q3_stride, qn, kn, ktype, kcache, vtype, vcache, pos, axis_pos, qout, n_head, n_kv, head_dim,
+                   n_rot, freq_base, factor, orig_ctx, sections, interleaved, eps, ntok, max_ctx, ext_factor=1.0,
+                   attn_factor=1.0, beta_fast=32.0, beta_slow=1.0, stream=None):
+    """per-head norm, rotation at axis_pos ([3][ntok]; None: the slots) and the cache write at slots pos[0] + t"""
+    rope = RopeParams(freq_base, factor, orig_ctx, ext_factor, attn_factor, beta_fast, beta_slow)
+    axes = RopeAxes((ctypes.c_int * 3)(*sections), int(interleaved))
+    _call("rmi_attn_prep_axes", _p(q3), q3_stride, _p(qn), _p(kn), ktype, _p(kcache), vtype, _p(vcache), _p(pos),
+          _p(axis_pos), _p(qout), n_head, n_kv, head_dim, n_rot, ctypes.byref(rope), ctypes.byref(axes), eps, ntok,
+          max_ctx, _stream(stream))
+
+
+def gqa_tree_nsub(ctx, n_head, n_kv, head_dim, ntok) -> int:
+    """the split of a context of ctx positions (chunks of 128 * nsub)"""
+    n = lib().rmi_gqa_tree_nsub(ctx, n_head, n_kv, head_dim, ntok)
+    if n == 0:
+        raise ValueError(last_error())
+    return n
+
+
+def gqa_tree_workspace_bytes(max_ctx, n_head, n_kv, head_dim, ntok, nsub) -> int:
+    n = lib().rmi_gqa_tree_workspace_bytes(max_ctx, n_head, n_kv, head_dim, ntok, nsub)
+    if n == 0:
+        raise ValueError(last_error())
+    return n
+
+
+def gqa_tree_decode(q, ktype, kcache, vtype, vcache, pos, masks, gate_src, gate_stride, y, y_stride, q8, q8_stride,
+                    workspace, n_head, n_kv, head_dim, ntok, max_ctx, nsub, scale, stream=None):
+    """attention of ntok drafted tokens at slots pos[0] + t: all of the context before them, and of each other what
+    masks[t] (int64 bit patterns) says; masks None: the chain j <= t"""
+    _call("rmi_gqa_tree_decode", _p(q), ktype, _p(kcache), vtype, _p(vcache), _p(pos), _p(masks), _p(gate_src),
+          gate_stride, _p(y), y_stride, _p(q8), q8_stride, _p(workspace), n_head, n_kv, head_dim, ntok, max_ctx, nsub,
+          scale, _stream(stream))
+
+
+class Penalties(ctypes.Structure):
+    """rmi_penalties"""
+    _fields_ = [("repetition", ctypes.c_float), ("presence", ctypes.c_float), ("frequency", ctypes.c_float),
+                ("window", ctypes.c_int)]
+
+
+def logits_process(logits, n, ncols, col_stride, out, out_stride, history, history_len, max_history, window=0,
+                   draft=None, masks=None, ndraft=0, repetition=1.0, presence=0.0, frequency=0.0, bias_ids=None,
+                   bias_vals=None, n_bias=0, allow=None, allow_stride=0, stream=None):
+    """biases, penalties over history (+ the draft path of each column's mask) and grammar masks, before argmax / topk"""
+    pen = Penalties(repetition, presence, frequency, window)
+    _call("rmi_logits_process", _p(logits), n, ncols, col_stride, _p(out), out_stride, _p(history), _p(history_len),
+          max_history, _p(draft), _p(masks), ndraft, ctypes.byref(pen), _p(bias_ids), _p(bias_vals), n_bias, _p(allow),
+          allow_stride, _stream(stream))

@@ -1,0 +1,514 @@
+// kv_cache.hip - K/V caches in 16, 8 or 4 bits (types and quantiser: kv_cache.h) for gfx950:
+//   kv_write     fp32 / fp16 rows -> cache rows; a lane owns eight dims, four lanes a scale block
+//   kv_read      cache rows -> fp32 / fp16 rows
+//   kv_compact   the accepted path's rows of a drafted tree to the front of the draft, for all caches of a model at once
+//   prep_axes    per-head RMSNorm, rotary embedding with three position axes, and the K / V write of new tokens
+// No counterpart in the reference, whose cache is fp16 (store_kv2_kernel, qw:340-345) and whose draft is one token.
+#include "kv_cache.h"
+#include "rope.h"
+
+#include <cmath>
+
+namespace rmi {
+namespace {
+
+// ---- rows in and out ---------------------------------------------------------------------------------------------------
+// Both are copies with a little arithmetic, bound by the memory they touch.  The unit is eight dims: 16 bytes of fp16,
+// 8 bytes of I8 codes, one word of I4 codes.
+
+struct F8 {
+    float v[8];
+};
+
+template <bool SRC16, bool VEC>
+__device__ __forceinline__ F8 load8(const void* src, size_t e) {
+    F8 x;
+    if constexpr (SRC16) {
+        const auto* p = static_cast<const uint16_t*>(src) + e;
+        if constexpr (VEC) {
+            const uint4 w = *reinterpret_cast<const uint4*>(p);
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x.v[2 * i] = half_bits_to_float(ws[i]);
+                x.v[2 * i + 1] = half_bits_to_float(ws[i] >> 16);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x.v[i] = half_bits_to_float(p[i]);
+        }
+    } else {
+        const auto* p = static_cast<const float*>(src) + e;
+        if constexpr (VEC) {
+            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+            x = {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x.v[i] = p[i];
+        }
+    }
+    return x;
+}
+
+__device__ __forceinline__ uint32_t half_bits(float v) {
+    return static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(v)));
+}
+
+template <bool OUT16, bool VEC>
+__device__ __forceinline__ void store8(void* out, size_t e, const F8& x) {
+    if constexpr (OUT16) {
+        auto* p = static_cast<uint16_t*>(out) + e;
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = half_bits(x.v[2 * i]) | (half_bits(x.v[2 * i + 1]) << 16);
+        if constexpr (VEC) {
+            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+        }
+    } else {
+        auto* p = static_cast<float*>(out) + e;
+        if constexpr (VEC) {
+            reinterpret_cast<float4*>(p)[0] = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
+            reinterpret_cast<float4*>(p)[1] = make_float4(x.v[4], x.v[5], x.v[6], x.v[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = x.v[i];
+        }
+    }
+}
+
+constexpr int kRowThreads = 256;
+
+template <int T, bool SRC16, bool VEC>
+__global__ __launch_bounds__(kRowThreads) void kv_write_kernel(const void* __restrict__ src, int src_stride,
+                                                               uint8_t* __restrict__ cache, int first, size_t units,
+                                                               int n_kv, int head_dim, int max_ctx) {
+    const size_t u = static_cast<size_t>(blockIdx.x) * kRowThreads + threadIdx.x;
+    if (u >= units) return;   // units is a multiple of 16 (a row): the lanes of a block stay or go together
+    const int per = head_dim >> 3;                       // units per (position, head) row
+    const size_t hr = u / per;
+    const int g = static_cast<int>(u - hr * per);        // eight dims 8 g ..
+    const int row = static_cast<int>(hr / n_kv), kv = static_cast<int>(hr - static_cast<size_t>(row) * n_kv);
+    const F8 x = load8<SRC16, VEC>(src, static_cast<size_t>(row) * src_stride + kv * head_dim + 8 * g);
+    const KvRow<T> at = kv_row<T>(first + row, kv, n_kv, max_ctx, head_dim);
+    if constexpr (T == kKvF16) {
+        store8<true, true>(cache + at.code, 8 * g, x);
+        return;
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x.v[i]) & 0x7fffffffu);
+    m = max(m, xor_lane<1>(m));
+    m = max(m, xor_lane<2>(m));
+    const uint32_t sb = kv_scale_byte<T>(m);
+    const float s = kv_scale_value(sb), inv = 1.0f / s;
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = static_cast<uint32_t>(kv_code<T>(x.v[i], s, inv) + kv_bias(T));
+    if constexpr (T == kKvI8) {
+        *reinterpret_cast<uint2*>(cache + at.code + 8 * g) =
+            make_uint2(c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24), c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24));
+    } else {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w |= c[i] << kv_i4_shift(i);
+        *reinterpret_cast<uint32_t*>(cache + at.code + 4 * g) = w;
+    }
+    uint32_t w = sb | (xor_lane<4>(sb) << 8);   // in the lanes of block 0 of four
+    w |= xor_lane<8>(w) << 16;
+    if ((g & 15) == 0) *reinterpret_cast<uint32_t*>(cache + at.scale + (g >> 2)) = w;
+}
+
+template <int T, bool OUT16, bool VEC>
+__global__ __launch_bounds__(kRowThreads) void kv_read_kernel(const uint8_t* __restrict__ cache, void* __restrict__ out,
+                                                              int out_stride, int first, size_t units, int n_kv,
+                                                              int head_dim, int max_ctx) {
+    const size_t u = static_cast<size_t>(blockIdx.x) * kRowThreads + threadIdx.x;
+    if (u >= units) return;
+    const int per = head_dim >> 3;
+    const size_t hr = u / per;
+    const int g = static_cast<int>(u - hr * per);
+    const int row = static_cast<int>(hr / n_kv), kv = static_cast<int>(hr - static_cast<size_t>(row) * n_kv);
+    const KvRow<T> at = kv_row<T>(first + row, kv, n_kv, max_ctx, head_dim);
+    F8 x;
+    if constexpr (T == kKvF16) {
+        x = load8<true, true>(cache + at.code, 8 * g);
+    } else {
+        const float s = kv_scale_value(cache[at.scale + (g >> 2)]);
+        if constexpr (T == kKvI8) {
+            const uint2 w = *reinterpret_cast<const uint2*>(cache + at.code + 8 * g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t b = ((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xffu;
+                x.v[i] = static_cast<float>(static_cast<int>(b) - kv_bias(T)) * s;
+            }
+        } else {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(cache + at.code + 4 * g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x.v[i] = static_cast<float>(static_cast<int>((w >> kv_i4_shift(i)) & 15u) - kv_bias(T)) * s;
+        }
+    }
+    store8<OUT16, VEC>(out, static_cast<size_t>(row) * out_stride + kv * head_dim + 8 * g, x);
+}
+
+// ---- the accepted path's rows --------------------------------------------------------------------------------------------
+// Workgroup (cache, head): up to 64 rows of up to 512 bytes are read into registers, a barrier, then written, so a source
+// row that is another's destination is read before it goes.  Latency-bound (one read, one write).
+constexpr int kMaxPath = 64;
+constexpr int kMaxCaches = 64;
+constexpr int kMoves = kMaxPath * 32 / 256;   // 16-byte pieces per lane
+
+struct CachePtrs {
+    uint8_t* p[kMaxCaches];
+};
+
+template <int T>
+__global__ __launch_bounds__(256) void kv_compact_kernel(CachePtrs caches, const int* __restrict__ pos,
+                                                         const int* __restrict__ path, const int* __restrict__ count,
+                                                         int max_path, int n_kv, int head_dim, int max_ctx) {
+    __shared__ int from[kMaxPath];
+    uint8_t* cache = caches.p[blockIdx.x];
+    const int kv = blockIdx.y, tid = threadIdx.x;
+    const int base = pos[0], n = min(max(count[0], 0), max_path);
+    if (tid < n) {
+        const long long s = static_cast<long long>(base) + path[tid], d = static_cast<long long>(base) + tid;
+        from[tid] = s >= 0 && s < max_ctx && d >= 0 && d < max_ctx ? static_cast<int>(s) : -1;
+    }
+    __syncthreads();
+    const int per = kv_row_bytes(T, head_dim) / 16, sper = T == kKvF16 ? 0 : head_dim / 128;   // pieces, scale words
+    uint4 x[kMoves];
+    uint32_t sc = 0;
+#pragma unroll
+    for (int k = 0; k < kMoves; ++k) {
+        const int i = tid + 256 * k, r = i / per;
+        x[k] = make_uint4(0, 0, 0, 0);
+        if (r < n && from[r] >= 0)
+            x[k] = *reinterpret_cast<const uint4*>(cache + kv_row<T>(from[r], kv, n_kv, max_ctx, head_dim).code + 16 * (i - r * per));
+    }
+    const int sr = T == kKvF16 ? n : tid / sper;
+    if (sr < n && from[sr] >= 0)
+        sc = *reinterpret_cast<const uint32_t*>(cache + kv_row<T>(from[sr], kv, n_kv, max_ctx, head_dim).scale + 4 * (tid - sr * sper));
+    // every load has returned before any lane passes the barrier
+#pragma unroll
+    for (int k = 0; k < kMoves; ++k) asm volatile("" : "+v"(x[k].x), "+v"(x[k].y), "+v"(x[k].z), "+v"(x[k].w));
+    asm volatile("" : "+v"(sc));
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kMoves; ++k) {
+        const int i = tid + 256 * k, r = i / per;
+        if (r < n && from[r] >= 0)
+            *reinterpret_cast<uint4*>(cache + kv_row<T>(base + r, kv, n_kv, max_ctx, head_dim).code + 16 * (i - r * per)) = x[k];
+    }
+    if (sr < n && from[sr] >= 0)
+        *reinterpret_cast<uint32_t*>(cache + kv_row<T>(base + sr, kv, n_kv, max_ctx, head_dim).scale + 4 * (tid - sr * sper)) = sc;
+}
+
+// ---- norm, rotation, cache write ------------------------------------------------------------------------------------------
+// Workgroup (token, part): the token's (cos, sin) per pair once into LDS, then a wave per head row, lane l holding dims
+// l + 64 k: the norm is attn_prep's tree (a 64-lane butterfly per 64 dims, summed in order), the rotation's partner comes
+// through the wave's LDS row.  K rows that are quantised go through the same steps in fp64.  A scale block is 32 lanes at
+// one k.  `per_wave` rows a wave: one for few tokens (latency), all of the token's rows on four waves for many, where the
+// fp64 angles of a workgroup are then shared by all heads.
+constexpr int kPrepWaves = 4;
+
+struct PrepArgs {
+    const float* q3;
+    int q3_stride;
+    const float *qn, *kn;
+    uint8_t *kc, *vc;
+    const int *pos, *axis_pos;
+    float* qout;
+    int n_head, n_kv, n_rot, max_ctx, ntok, per_wave;
+    float theta, eps;
+    Yarn yarn;
+    rmi_rope_axes axes;
+};
+
+__device__ __forceinline__ int rope_axis(const rmi_rope_axes& a, int i) {
+    if (a.interleaved) {
+        const int m = i % 3;
+        return m == 1 && i < 3 * a.section[1] ? 1 : m == 2 && i < 3 * a.section[2] ? 2 : 0;
+    }
+    return i < a.section[0] ? 0 : i < a.section[0] + a.section[1] ? 1 : 2;
+}
+
+// orders a wave's own LDS accesses
+__device__ __forceinline__ void wave_lds_sync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ double group_sum64(double v) {
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) v += __shfl_xor(v, k, 64);
+    return v;
+}
+
+// the wave's row (lane: dims lane + 64 k) into position p of a cache
+template <int T, int HD>
+__device__ __forceinline__ void store_row(const float (&x)[HD / 64], uint8_t* cache, int p, int kv, int n_kv, int max_ctx,
+                                          int lane) {
+    const KvRow<T> at = kv_row<T>(p, kv, n_kv, max_ctx, HD);
+#pragma unroll
+    for (int k = 0; k < HD / 64; ++k) {
+        const int d = lane + 64 * k;
+        if constexpr (T == kKvF16) {
+            reinterpret_cast<uint16_t*>(cache + at.code)[d] = static_cast<uint16_t>(half_bits(x[k]));
+        } else {
+            uint32_t m = __float_as_uint(x[k]) & 0x7fffffffu;
+            m = max(m, xor_lane<16>(m));
+            m = max(m, xor_lane<8>(m));
+            m = max(m, xor_lane<4>(m));
+            m = max(m, xor_lane<2>(m));
+            m = max(m, xor_lane<1>(m));
+            const uint32_t sb = kv_scale_byte<T>(m);
+            const float s = kv_scale_value(sb);
+            const uint32_t c = static_cast<uint32_t>(kv_code<T>(x[k], s, 1.0f / s) + kv_bias(T));
+            if constexpr (T == kKvI8) {
+                cache[at.code + d] = static_cast<uint8_t>(c);
+            } else {
+                uint32_t w = c << kv_i4_shift(d);
+                w |= xor_lane<1>(w);
+                w |= xor_lane<2>(w);
+                w |= xor_lane<4>(w);
+                if ((d & 7) == 0) *reinterpret_cast<uint32_t*>(cache + at.code + d / 2) = w;
+            }
+            if ((d & 31) == 0) cache[at.scale + d / 32] = static_cast<uint8_t>(sb);
+        }
+    }
+}
+
+template <int KT, int VT, int HD>
+__global__ __launch_bounds__(64 * kPrepWaves) void prep_axes_kernel(PrepArgs a) {
+    constexpr int N = HD / 64;
+    __shared__ double cs[HD / 2][2];
+    __shared__ double rows[kPrepWaves][HD];
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int base = a.pos[0], half = a.n_rot / 2;
+    if (base < -t || base >= a.max_ctx - t) return;   // uniform: a slot outside the cache stores nothing
+    const int p = base + t;
+    if (tid < half) {
+        const int ap = a.axis_pos ? a.axis_pos[static_cast<size_t>(rope_axis(a.axes, tid)) * a.ntok + t] : p;
+        rope_cos_sin_d(ap, rope_freq(tid, a.n_rot, a.theta), tid, a.yarn, &cs[tid][0], &cs[tid][1]);
+    }
+    __syncthreads();
+    const float* src = a.q3 + static_cast<size_t>(t) * a.q3_stride;
+    const int items = a.n_head + 2 * a.n_kv, first = (blockIdx.y * kPrepWaves + wv) * a.per_wave;
+    for (int it = first; it < min(first + a.per_wave, items); ++it) {
+        const bool is_q = it < a.n_head, is_v = it >= a.n_head + a.n_kv;
+        const int kv = is_v ? it - a.n_head - a.n_kv : it - a.n_head;
+        const float* row = is_q ? src + it * 2 * HD : src + 2 * a.n_head * HD + ((is_v ? a.n_kv : 0) + kv) * HD;
+        float x[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] = row[lane + 64 * k];
+        if (is_v) {
+            store_row<VT, HD>(x, a.vc, p, kv, a.n_kv, a.max_ctx, lane);
+            continue;
+        }
+        const float* w = is_q ? a.qn : a.kn;
+        if (is_q || KT == kKvF16) {
+            float* xs = reinterpret_cast<float*>(rows[wv]);
+            float ss = 0.0f;
+#pragma unroll
+            for (int k = 0; k < N; ++k)   // lane 0's sum, as attn_prep takes it
+                ss += __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(group_sum<64>(x[k] * x[k]))));
+            const float inv = rsqrtf(ss / static_cast<float>(HD) + a.eps);
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                x[k] = x[k] * inv * w[lane + 64 * k];
+                xs[lane + 64 * k] = x[k];
+            }
+            wave_lds_sync();
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int d = lane + 64 * k;
+                if (d < a.n_rot) {
+                    const int i = d < half ? d : d - half;
+                    const float c = static_cast<float>(cs[i][0]), s = static_cast<float>(cs[i][1]);
+                    x[k] = d < half ? rope_lo(x[k], xs[d + half], c, s) : rope_hi(xs[d - half], x[k], c, s);
+                }
+            }
+            wave_lds_sync();   // the next row overwrites the exchange
+            if (is_q) {
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                    a.qout[(static_cast<size_t>(t) * a.n_head + it) * HD + lane + 64 * k] = x[k];
+            } else {
+                store_row<KT, HD>(x, a.kc, p, kv, a.n_kv, a.max_ctx, lane);
+            }
+        } else {
+            double* xs = rows[wv];
+            double y[N], ss = 0.0;
+#pragma unroll
+            for (int k = 0; k < N; ++k) ss += static_cast<double>(x[k]) * static_cast<double>(x[k]);
+            const double inv = 1.0 / sqrt(group_sum64(ss) / HD + static_cast<double>(a.eps));
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                y[k] = static_cast<double>(x[k]) * inv * static_cast<double>(w[lane + 64 * k]);
+                xs[lane + 64 * k] = y[k];
+            }
+            wave_lds_sync();
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int d = lane + 64 * k;
+                if (d < a.n_rot) {
+                    const int i = d < half ? d : d - half;
+                    y[k] = d < half ? y[k] * cs[i][0] - xs[d + half] * cs[i][1] : xs[d - half] * cs[i][1] + y[k] * cs[i][0];
+                }
+                x[k] = static_cast<float>(y[k]);
+            }
+            wave_lds_sync();
+            store_row<KT, HD>(x, a.kc, p, kv, a.n_kv, a.max_ctx, lane);
+        }
+    }
+}
+
+bool aligned_to(const void* p, size_t n) { return p && (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// calls f with the type as a constant
+template <typename F>
+int with_type(int type, F&& f) {
+    if (type == kKvI8) return f(std::integral_constant<int, kKvI8>{});
+    if (type == kKvI4) return f(std::integral_constant<int, kKvI4>{});
+    return f(std::integral_constant<int, kKvF16>{});
+}
+
+int row_args(const char* what, int type, const void* cache, const void* rows, int rows16, int stride, int first, int n,
+             int n_kv, int head_dim, int max_ctx) {
+    if (!kv_type_ok(type)) return fail(RMI_ERR_UNSUPPORTED, what);
+    if (!kv_shape_ok(max_ctx, n_kv, head_dim) || first < 0 || n < 0 || n > max_ctx || first > max_ctx - n ||
+        static_cast<long long>(n_kv) * head_dim > stride)
+        return fail(RMI_ERR_SHAPE, what);
+    if (!aligned16(cache) || !aligned_to(rows, rows16 ? 2 : 4)) return fail(RMI_ERR_POINTER, what);
+    return RMI_OK;
+}
+
+}  // namespace
+}  // namespace rmi
+
+using namespace rmi;
+
+extern "C" size_t rmi_kv_cache_bytes(int type, int max_ctx, int n_kv, int head_dim) {
+    if (!kv_type_ok(type) || !kv_shape_ok(max_ctx, n_kv, head_dim)) {
+        set_error("kv_cache_bytes: type F16, I8 or I4, positive max_ctx and n_kv, head_dim 128 or 256");
+        return 0;
+    }
+    const size_t rows = static_cast<size_t>(max_ctx) * n_kv;
+    return rows * kv_row_bytes(type, head_dim) + (type == kKvF16 ? 0 : rows * (head_dim / kKvBlock));
+}
+
+extern "C" int rmi_kv_write(int type, const void* src, int src_f16, int src_stride, void* cache, int first, int n,
+                            int n_kv, int head_dim, int max_ctx, void* stream) {
+    RMI_TRY(row_args("kv_write: invalid arguments", type, cache, src, src_f16, src_stride, first, n, n_kv, head_dim, max_ctx));
+    if (n == 0) return RMI_OK;
+    const size_t units = static_cast<size_t>(n) * n_kv * (head_dim / 8);
+    const size_t blocks = (units + kRowThreads - 1) / kRowThreads;
+    if (blocks > 0x7fffffffu) return fail(RMI_ERR_SHAPE, "kv_write: too many rows for one call");
+    const bool vec = aligned16(src) && src_stride % (src_f16 ? 8 : 4) == 0;   // 16-byte loads, else one by one
+    auto* out = static_cast<uint8_t*>(cache);
+    return with_type(type, [&](auto t) {
+        auto go = [&](auto* kernel) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRowThreads), 0, static_cast<hipStream_t>(stream),
+                               src, src_stride, out, first, units, n_kv, head_dim, max_ctx);
+            return launch_status("kv_write");
+        };
+        constexpr int T = decltype(t)::value;
+        if (src_f16) return vec ? go(&kv_write_kernel<T, true, true>) : go(&kv_write_kernel<T, true, false>);
+        return vec ? go(&kv_write_kernel<T, false, true>) : go(&kv_write_kernel<T, false, false>);
+    });
+}
+
+extern "C" int rmi_kv_read(int type, const void* cache, void* out, int out_f16, int out_stride, int first, int n,
+                           int n_kv, int head_dim, int max_ctx, void* stream) {
+    RMI_TRY(row_args("kv_read: invalid arguments", type, cache, out, out_f16, out_stride, first, n, n_kv, head_dim, max_ctx));
+    if (n == 0) return RMI_OK;
+    const size_t units = static_cast<size_t>(n) * n_kv * (head_dim / 8);
+    const size_t blocks = (units + kRowThreads - 1) / kRowThreads;
+    if (blocks > 0x7fffffffu) return fail(RMI_ERR_SHAPE, "kv_read: too many rows for one call");
+    const bool vec = aligned16(out) && out_stride % (out_f16 ? 8 : 4) == 0;
+    const auto* in = static_cast<const uint8_t*>(cache);
+    return with_type(type, [&](auto t) {
+        auto go = [&](auto* kernel) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRowThreads), 0, static_cast<hipStream_t>(stream),
+                               in, out, out_stride, first, units, n_kv, head_dim, max_ctx);
+            return launch_status("kv_read");
+        };
+        constexpr int T = decltype(t)::value;
+        if (out_f16) return vec ? go(&kv_read_kernel<T, true, true>) : go(&kv_read_kernel<T, true, false>);
+        return vec ? go(&kv_read_kernel<T, false, true>) : go(&kv_read_kernel<T, false, false>);
+    });
+}
+
+extern "C" int rmi_kv_compact(int type, void* const* caches, int n_caches, const int* pos, const int* path,
+                              const int* count, int max_path, int n_kv, int head_dim, int max_ctx, void* stream) {
+    if (!kv_type_ok(type)) return fail(RMI_ERR_UNSUPPORTED, "kv_compact: unknown cache type");
+    if (!kv_shape_ok(max_ctx, n_kv, head_dim) || n_caches < 1 || n_caches > kMaxCaches || max_path < 1 || max_path > kMaxPath)
+        return fail(RMI_ERR_SHAPE, "kv_compact: invalid arguments");
+    if (!caches || !aligned4(pos) || !aligned4(path) || !aligned4(count))
+        return fail(RMI_ERR_POINTER, "kv_compact: invalid arguments");
+    CachePtrs ptrs{};
+    for (int i = 0; i < n_caches; ++i) {
+        if (!aligned16(caches[i])) return fail(RMI_ERR_POINTER, "kv_compact: null or misaligned cache");
+        ptrs.p[i] = static_cast<uint8_t*>(caches[i]);
+    }
+    return with_type(type, [&](auto t) {
+        hipLaunchKernelGGL((kv_compact_kernel<decltype(t)::value>), dim3(n_caches, n_kv), dim3(256), 0,
+                           static_cast<hipStream_t>(stream), ptrs, pos, path, count, max_path, n_kv, head_dim, max_ctx);
+        return launch_status("kv_compact");
+    });
+}
+
+extern "C" int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* qn, const float* kn, int ktype,
+                                  void* kcache, int vtype, void* vcache, const int* pos, const int* axis_pos, float* qout,
+                                  int n_head, int n_kv, int head_dim, int n_rot, const rmi_rope_params* rope,
+                                  const rmi_rope_axes* axes, float eps, int ntok, int max_ctx, void* stream) {
+    const char* what = "attn_prep_axes: invalid arguments";
+    if (!kv_type_ok(ktype) || !kv_type_ok(vtype)) return fail(RMI_ERR_UNSUPPORTED, "attn_prep_axes: unknown cache type");
+    if (!kv_shape_ok(max_ctx, n_kv, head_dim) || n_head <= 0 || n_head > 65535 || n_head % n_kv || n_rot < 0 || n_rot > head_dim || n_rot % 2 ||
+        ntok < 1 || ntok > max_ctx || !rope || !(rope->freq_base > 1.0f) || !axes ||
+        2LL * n_head * head_dim + 2LL * n_kv * head_dim > 0x7fffffffLL)
+        return fail(RMI_ERR_SHAPE, what);
+    const int* s = axes->section;
+    const int half = n_rot / 2;
+    if (s[0] < 0 || s[1] < 0 || s[2] < 0 || s[0] > half || s[1] > half || s[2] > half || s[0] + s[1] + s[2] != half)
+        return fail(RMI_ERR_SHAPE, "attn_prep_axes: the axes' sections must add up to n_rot / 2");
+    // dealt out in turn, the last pairs of axes 1 and 2 are 3 s - 2 and 3 s - 1
+    if (axes->interleaved && ((s[1] > 0 && 3 * s[1] - 2 >= half) || (s[2] > 0 && 3 * s[2] - 1 >= half)))
+        return fail(RMI_ERR_SHAPE, "attn_prep_axes: an interleaved axis has more pairs than its turns");
+    if (!aligned4(q3) || !aligned4(qn) || !aligned4(kn) || !aligned16(kcache) || !aligned16(vcache) || !aligned4(pos) ||
+        (axis_pos && !aligned4(axis_pos)) || !aligned4(qout))
+        return fail(RMI_ERR_POINTER, what);
+    PrepArgs a{};
+    if (!yarn_setup(*rope, n_rot, &a.yarn)) return fail(RMI_ERR_SHAPE, "attn_prep_axes: invalid YaRN parameters");
+    a.q3 = q3;
+    a.q3_stride = q3_stride;
+    a.qn = qn;
+    a.kn = kn;
+    a.kc = static_cast<uint8_t*>(kcache);
+    a.vc = static_cast<uint8_t*>(vcache);
+    a.pos = pos;
+    a.axis_pos = axis_pos;
+    a.qout = qout;
+    a.n_head = n_head;
+    a.n_kv = n_kv;
+    a.n_rot = n_rot;
+    a.max_ctx = max_ctx;
+    a.ntok = ntok;
+    a.theta = rope->freq_base;
+    a.eps = eps;
+    a.axes = *axes;
+    const int items = n_head + 2 * n_kv;
+    // a row per wave up to 64 tokens, then a token per workgroup
+    a.per_wave = ntok <= 64 ? 1 : (items + kPrepWaves - 1) / kPrepWaves;
+    const int parts = (items + kPrepWaves * a.per_wave - 1) / (kPrepWaves * a.per_wave);
+    return with_type(ktype, [&](auto k) {
+        return with_type(vtype, [&](auto v) {
+            auto go = [&](auto* kernel) {
+                hipLaunchKernelGGL(kernel, dim3(ntok, parts), dim3(64 * kPrepWaves), 0, static_cast<hipStream_t>(stream), a);
+                return launch_status("attn_prep_axes");
+            };
+            constexpr int KT = decltype(k)::value, VT = decltype(v)::value;
+            return head_dim == 256 ? go(&prep_axes_kernel<KT, VT, 256>) : go(&prep_axes_kernel<KT, VT, 128>);
+        });
+    });
+}

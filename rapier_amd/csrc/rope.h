@@ -44,8 +44,8 @@ __device__ __forceinline__ double rope_freq(int i, int n_rot, float theta) {
     return pow(static_cast<double>(theta), -2.0 * i / static_cast<double>(n_rot));
 }
 
-// cos and sin of pair i at position p from its frequency (angle in fp64, rounded to fp32 once)
-__device__ __forceinline__ void rope_cos_sin_f(int p, double freq, int i, const Yarn& yarn, float* c, float* s) {
+// cos and sin of pair i at position p from its frequency, in fp64
+__device__ __forceinline__ void rope_cos_sin_d(int p, double freq, int i, const Yarn& yarn, double* c, double* s) {
     double ang = static_cast<double>(p) * freq;
     double sn, cs;
     if (yarn.on) {
@@ -58,6 +58,14 @@ __device__ __forceinline__ void rope_cos_sin_f(int p, double freq, int i, const 
     } else {
         sincos(ang, &sn, &cs);
     }
+    *c = cs;
+    *s = sn;
+}
+
+// the same rounded to fp32 once
+__device__ __forceinline__ void rope_cos_sin_f(int p, double freq, int i, const Yarn& yarn, float* c, float* s) {
+    double cs, sn;
+    rope_cos_sin_d(p, freq, i, yarn, &cs, &sn);
     *c = static_cast<float>(cs);
     *s = static_cast<float>(sn);
 }
