@@ -177,6 +177,8 @@ def _p(t):
 def _stream(stream):
     if stream is None:
         import torch
+        if torch.cuda.is_initialized():   # the raw handle: current_stream() builds a Stream object for it, 3 us
+            return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
         return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
     if isinstance(stream, int):
         return ctypes.c_void_p(stream)

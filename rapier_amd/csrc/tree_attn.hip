@@ -2,20 +2,15 @@
 // (rmi_gqa_tree_decode; caches: kv_cache.h).  No counterpart in the reference, whose draft is one token (gqa_head_kernel,
 // qw:384-442, per column).
 //
-//   partial   workgroup (chunk of 128 nsub positions, KV head, group of 16 query rows); row r = token r / G, head r % G of
-//             the KV head's G.  Each of the four waves streams a quarter of the chunk in steps of 32 positions with a
-//             running maximum, sum and output per row, and the four are joined at the end: one record (m, l, o) a row.
-//   merge     workgroup (token, head): joins the chunks' records, gates, writes fp32 and Q8_1.
+//   partial   workgroup (chunk of 128 nsub positions, KV head, group of query rows); row r = token r / G, head r % G of the
+//             KV head's G.  Each wave streams its part of the chunk in steps of 32 positions with a running maximum, sum and
+//             output per row; the waves' parts are joined at the end, one record (m, l, o) a row.
+//   merge     workgroup (token, head, 64 dims): joins the chunks' records, gates, writes fp32 and Q8_1.  A call of one chunk
+//             needs none: the partial launch writes the result.
 //
-// Both products run on v_mfma_f32_16x16x32_f16 (lane: l16 = l % 16, g4 = l / 16; A rows, B and D columns are l16; A and B
-// hold k = 8 g4 + 0..7; D rows are 4 g4 + 0..3).  The cache's values are fp16 numbers in every type; the fp32 operand
-// (q, p) goes as fp16 high + low part, 22 bits, in two products, so the result keeps fp32's accuracy.
-//   scores    D[position][row] += K[position][dims] . q[row][dims]: lane (l16, g4) takes 16 neighbouring dims of position
-//             l16 at a time, 64 i + 16 g4 + [0, 16), as two operands of eight, straight from the cache.
-//   P V       D[row][dim] += P[row][positions] V[positions][dim]: the score lane (row l16, positions 4 g4 + r of two tiles)
-//             holds P in the A layout already, k slot j being position 4 g4 + j or 16 + 4 g4 + j - 4.  V comes by lane
-//             (l16, g4) as HD / 16 neighbouring dims of those eight positions; operand e gathers dim e of the eight.
-// The scores' exponent is base 2 (q is scaled by log2 e once).
+// Both products run on fp16 MFMAs.  The cache's values are fp16 numbers in every type; the fp32 operand (q, p) goes as fp16
+// high + low part, 22 bits, so the result keeps fp32's accuracy.  fp16's subnormals would cut the low parts short: a row's q
+// is scaled by a power of two to [2^13, 2^14) and p by 2^8.  The scores' exponent is base 2.
 //
 // What a token does not see has no part in it: scores are masked before the maximum, and in the steps that reach into the
 // draft a V that is not finite is taken out of the product and added to the rows that see it alone (an infinity times a
@@ -31,14 +26,20 @@ namespace {
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kRows = 16;          // query rows of a group
 constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
 constexpr int kStep = 32;          // positions of a step
 constexpr int kUnit = kWaves * kStep;
 constexpr int kMaxChunks = 2048;
 constexpr int kMaxTree = 64, kMaxChain = 1024;
+constexpr int kOct = 8;            // rows joined at a time
+constexpr int kFewRows = 8;        // query rows per KV head of the 16 x 16 form
+constexpr int kBlockRows = 32;     // rows of a wave in the 32 x 32 form
+constexpr float kPScale = 8.0f;    // p goes as 2^8 p
+constexpr float kLazy = 7.0f;      // a maximum moves once a score passes it by more than 2^7 (2^15 p is an fp16 number)
 
 struct TreeArgs {
     const float* q;
@@ -46,7 +47,10 @@ struct TreeArgs {
     const int* pos;
     const uint64_t* masks;
     float *wo, *wml;   // records: o [chunk][kv][row][HD], (m, l) [chunk][kv][row][2]
-    int n_head, n_kv, ntok, rows, rows_pad, groups, npairs, nsub, max_ctx;
+    const float* gate;
+    float* y;
+    uint8_t* q8;
+    int n_head, n_kv, ntok, rows, rows_pad, groups, npairs, nsub, max_ctx, gate_stride, y_stride, q8_stride, direct;
     float scale;
 };
 
@@ -109,14 +113,20 @@ __device__ __forceinline__ half8 k_operand(const Dims16<T>& x, int hf, half2v s)
     }
 }
 
-// VD neighbouring dims of one position's V
+// VD neighbouring dims of one position's V (I4 at VD = 4: half the dims of a word, brought down to the bits of the first)
 template <int T, int VD>
 struct DimsV {
     static constexpr int kBytes = T == kKvF16 ? 2 * VD : T == kKvI8 ? VD : VD / 2;
-    uint32_t w[kBytes / 4];
+    uint32_t w[kBytes <= 4 ? 1 : kBytes / 4];
 };
+// the lane's first byte in a row (lane index n)
 template <int T, int VD>
-__device__ __forceinline__ DimsV<T, VD> load_v(const uint8_t* p) {
+__device__ __forceinline__ int v_offset(int n) {
+    constexpr int kB = DimsV<T, VD>::kBytes;
+    return kB == 2 ? 4 * (n >> 1) : kB * n;
+}
+template <int T, int VD>
+__device__ __forceinline__ DimsV<T, VD> load_v(const uint8_t* p, int n) {
     DimsV<T, VD> x;
     constexpr int kB = DimsV<T, VD>::kBytes;
     if constexpr (kB >= 16) {
@@ -130,6 +140,7 @@ __device__ __forceinline__ DimsV<T, VD> load_v(const uint8_t* p) {
         x.w[0] = v.x, x.w[1] = v.y;
     } else {
         x.w[0] = *reinterpret_cast<const uint32_t*>(p);
+        if constexpr (kB == 2) x.w[0] >>= 8 * (n & 1);
     }
     return x;
 }
@@ -153,8 +164,9 @@ __device__ __forceinline__ void v_pair(const DimsV<T, VD>& a, const DimsV<T, VD>
 }
 
 __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ floatx16 mfma(half8 a, half8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-// fp16 high and low parts of eight fp32 values
+// fp16 high part of eight fp32 values, and what is left of them
 __device__ __forceinline__ void split8(const float (&x)[8], half8& hi, half8& lo) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -167,56 +179,143 @@ __device__ __forceinline__ void split8(const float (&x)[8], half8& hi, half8& lo
 __device__ __forceinline__ bool finite16(uint32_t w) {   // both halves
     return (w & 0x7c00u) != 0x7c00u && (w & 0x7c000000u) != 0x7c000000u;
 }
+// a word of fp16 V without its infinities and NaN
+__device__ __forceinline__ uint32_t zero_odd(uint32_t w) {
+    if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
+    if ((w & 0x7c000000u) == 0x7c000000u) w &= 0xffffu;
+    return w;
+}
 
+// the power of two that brings a row's largest |q| to [2^13, 2^14), as its exponent
+__device__ __forceinline__ int q_shift(float amax) {
+    if (!(amax > 0.0f && amax <= FLT_MAX)) return 0;
+    return min(14 - __builtin_amdgcn_frexp_expf(amax), 126);
+}
+
+// what a workgroup works on; false where it has nothing to do (uniform)
+struct Work {
+    int chunk, kv, row0, base, last;   // row0: its first row, last: the last position any of its rows sees
+};
+template <int ROWS>
+__device__ __forceinline__ bool tree_work(const TreeArgs& a, Work& w) {
+    // the groups of a (chunk, head) pair are consecutive workgroups of one XCD (workgroups go to the XCDs round robin),
+    // so the pair's rows come from HBM once
+    const int k8 = static_cast<int>(blockIdx.x >> 3), q8 = k8 / a.groups;
+    const int pair = 8 * q8 + static_cast<int>(blockIdx.x & 7);
+    if (pair >= a.npairs) return false;
+    w.chunk = pair / a.n_kv;
+    w.kv = pair - w.chunk * a.n_kv;
+    w.row0 = ROWS * (k8 - q8 * a.groups);
+    w.base = a.pos[0];
+    if (w.base < 0 || w.base > a.max_ctx - a.ntok) return false;   // a slot outside the cache
+    const int G = a.n_head / a.n_kv;
+    w.last = w.base + (a.masks ? a.ntok - 1 : min(w.row0 + ROWS - 1, a.rows - 1) / G);
+    return w.chunk * kUnit * a.nsub <= w.last;   // else the merge does not read this record
+}
+
+// which of a step's positions (first + 0..31, bit by bit) row `row` of token tok sees: lim is the last of its unbroken run
+__device__ __forceinline__ bool sees(int p, int lim, uint64_t mask, int base, int ntok) {
+    return p <= lim || (mask && p >= base && p - base < ntok && ((mask >> (p - base)) & 1));
+}
+
+// Joins the waves' parts of 8 * RB rows (rows 8 oct .. of each of RB row blocks) from their LDS slabs [wave][8][HD] and
+// either writes records or, for a call of one chunk, the result: fac[wave][row of the block] is a part's weight, sum[row]
+// the joined l.  Wave w holds part w / RB of row block w % RB.
+template <int HD, int RB, int BLOCK>
+__device__ __forceinline__ void join_rows(const TreeArgs& a, const Work& w, const float (&slab)[kWaves][kOct][HD],
+                                          const float (&fac)[kWaves][BLOCK], const float (&top)[RB][BLOCK],
+                                          const float (&sum)[RB][BLOCK], int oct) {
+    constexpr int PB = kWaves / RB;
+    const int G = a.n_head / a.n_kv;
+#pragma unroll
+    for (int i = 0; i < RB * kOct * HD / kThreads; ++i) {
+        const int e = static_cast<int>(threadIdx.x) + kThreads * i, d = e % HD, r8 = e / HD;   // r8: uniform in a wave
+        const int rb = r8 / kOct, rr = r8 % kOct, rk = kOct * oct + rr, row = w.row0 + BLOCK * rb + rk;
+        float v = slab[rb][rr][d] * fac[rb][rk];
+#pragma unroll
+        for (int p = 1; p < PB; ++p) v = __builtin_fmaf(slab[rb + RB * p][rr][d], fac[rb + RB * p][rk], v);
+        if (row < a.rows && !a.direct) {
+            const size_t rec = (static_cast<size_t>(w.chunk) * a.n_kv + w.kv) * a.rows_pad + row;
+            a.wo[rec * HD + d] = v;
+            if (d == 0) *reinterpret_cast<float2*>(a.wml + 2 * rec) = make_float2(top[rb][rk], sum[rb][rk]);
+        } else if (row < a.rows) {
+            const int t = row / G, h = w.kv * G + row - t * G;
+            v = top[rb][rk] == -INFINITY ? 0.0f : v / sum[rb][rk];
+            if (a.gate) v *= 1.0f / (1.0f + expf(-a.gate[static_cast<size_t>(t) * a.gate_stride + h * 2 * HD + HD + d]));
+            if (a.y) a.y[static_cast<size_t>(t) * a.y_stride + h * HD + d] = v;
+            if (a.q8) q8_1_store_lane(v, a.q8 + static_cast<size_t>(t) * a.q8_stride + (h * (HD / 32) + d / 32) * kQ8_1Bytes);
+        }
+    }
+}
+
+// the parts' weights and the joined sum of every row, from stat[wave][m, l][row of the block]
+template <int RB, int BLOCK>
+__device__ __forceinline__ void join_stats(const float (&stat)[kWaves][2][BLOCK], float (&fac)[kWaves][BLOCK], float (&top)[RB][BLOCK],
+                                           float (&sum)[RB][BLOCK]) {
+    constexpr int PB = kWaves / RB;
+    const int i = threadIdx.x;
+    if (i >= RB * BLOCK) return;
+    const int rb = i / BLOCK, r = i % BLOCK;
+    float m = stat[rb][0][r];
+#pragma unroll
+    for (int p = 1; p < PB; ++p) m = fmaxf(m, stat[rb + RB * p][0][r]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+#pragma unroll
+    for (int p = 0; p < PB; ++p) {
+        const float f = __builtin_amdgcn_exp2f(stat[rb + RB * p][0][r] - ref);
+        fac[rb + RB * p][r] = f;
+        l = __builtin_fmaf(stat[rb + RB * p][1][r], f, l);
+    }
+    top[rb][r] = m;
+    sum[rb][r] = l;
+}
+
+// ---- up to 8 query rows: v_mfma_f32_16x16x32_f16 -------------------------------------------------------------------------
+// Lane: l16 = l % 16, g4 = l / 16; A rows, B and D columns are l16; A and B hold k = 8 g4 + 0..7; D rows are 4 g4 + 0..3.
+//   scores    D[position][n] += K[position][dims] . q_n[dims]: column n < 8 is the high part of row n, column n >= 8 the low
+//             part of row n - 8, so one chain gives both.  Lane (l16, g4) takes 16 neighbouring dims of position l16 at a
+//             time, 64 i + 16 g4 + [0, 16), as two operands of eight, straight from the cache.
+//   P V       D[m][dim] += P_m[positions] V[positions][dim], rows m split the same way.  The score lane (row, positions
+//             4 g4 + r of two tiles) holds P in the A layout already, k slot j being position 4 g4 + j or 16 + 4 g4 + j - 4.
+//             V comes by lane (l16, g4) as HD / 16 neighbouring dims of those eight positions; operand e gathers dim e.
+// The waves take quarters of the chunk.  K of the next step is loaded when this step's scores are done, V when its product is:
+// each has half a step to arrive.
 template <int KT, int VT, int HD>
-__global__ __launch_bounds__(64 * kWaves, 1) void tree_partial_kernel(TreeArgs a) {
+__global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kernel(TreeArgs a) {
     constexpr int NI = HD / 64;        // K: 16-dim pieces a lane takes of a position
     constexpr int VD = HD / 16;        // V: dims a lane takes of a position
     constexpr int NB = HD / kKvBlock;  // scale bytes of a row
     constexpr int kKB = kv_row_bytes(KT, HD), kVB = kv_row_bytes(VT, HD);
-    __shared__ __attribute__((aligned(16))) float ob[kWaves / 2][kRows][HD];   // joins; V of a step that is not finite
-    __shared__ float pb[kWaves][kRows][kStep];
-    __shared__ float stat[kWaves][2][kRows];
+    __shared__ __attribute__((aligned(16))) float slab[kWaves][kOct][HD];
+    __shared__ float stat[kWaves][2][kFewRows], fac[kWaves][kFewRows], top[1][kFewRows], sum[1][kFewRows];
 
-    // the groups of a (chunk, head) pair are consecutive workgroups of one XCD (workgroups go to the XCDs round robin),
-    // so the pair's rows come from HBM once
-    const int k8 = static_cast<int>(blockIdx.x >> 3), q8 = k8 / a.groups;
-    const int group = k8 - q8 * a.groups, pair = 8 * q8 + static_cast<int>(blockIdx.x & 7);
-    if (pair >= a.npairs) return;
-    const int chunk = pair / a.n_kv, kv = pair - chunk * a.n_kv;
+    Work w;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l16 = lane & 15, g4 = lane >> 4;
-    const int G = a.n_head / a.n_kv;
-    const int base = a.pos[0];
-    if (base < 0 || base > a.max_ctx - a.ntok) return;   // uniform: a slot outside the cache
-    const int row = kRows * group + l16, rowc = min(row, a.rows - 1), tok = rowc / G;
-    // the last position any row of the group sees
-    const int last = a.masks ? base + a.ntok - 1 : base + min(kRows * group + kRows - 1, a.rows - 1) / G;
-    const int wlen = kStep * a.nsub, cbase = chunk * kWaves * wlen;
-    if (cbase > last) return;   // uniform; the merge does not read this record
+    if (!tree_work<kFewRows>(a, w)) return;
+    const int G = a.n_head / a.n_kv, base = w.base, last = w.last, kv = w.kv;
+    const int row = l16 & 7, rowc = min(row, a.rows - 1), tok = rowc / G;
+    const bool low = l16 >= 8;
+    const float* qr = a.q + (static_cast<size_t>(tok) * a.n_head + kv * G + (rowc - tok * G)) * HD + 16 * g4;
+    float qx[NI][16];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+            const float4 u = reinterpret_cast<const float4*>(qr + 64 * i)[f];
+            qx[i][4 * f] = u.x, qx[i][4 * f + 1] = u.y, qx[i][4 * f + 2] = u.z, qx[i][4 * f + 3] = u.w;
+        }
+    const int wlen = kStep * a.nsub, wbase = (w.chunk * kWaves + wv) * wlen;
+    const int nsteps = wbase > last ? 0 : min(a.nsub, (last - wbase) / kStep + 1);
     uint64_t mask = 0;   // of the row's token: bit j = draft slot base + j
     if (a.masks && row < a.rows) mask = a.masks[tok];
     const int lim = row >= a.rows ? -1 : a.masks ? base - 1 : base + tok;   // the row sees every position up to here
-
-    half8 qh[NI][2], ql[NI][2];
-    {
-        const float* qr = a.q + (static_cast<size_t>(tok) * a.n_head + kv * G + (rowc - tok * G)) * HD + 16 * g4;
-        const float c = a.scale * 1.44269504088896340736f;
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const float4 u = reinterpret_cast<const float4*>(qr + 64 * i + 8 * hf)[0];
-                const float4 v = reinterpret_cast<const float4*>(qr + 64 * i + 8 * hf)[1];
-                const float x[8] = {u.x * c, u.y * c, u.z * c, u.w * c, v.x * c, v.y * c, v.z * c, v.w * c};
-                split8(x, qh[i][hf], ql[i][hf]);
-            }
-    }
 
     // the head's rows: position p at kp + p * kstride
     const size_t kstride = KT == kKvF16 ? static_cast<size_t>(a.n_kv) * kKB : kKB;
     const size_t vstride = VT == kKvF16 ? static_cast<size_t>(a.n_kv) * kVB : kVB;
     const uint8_t* kp = a.kc + kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD).code + g4 * (kKB / (HD / 16));
-    const uint8_t* vp = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).code + l16 * DimsV<VT, VD>::kBytes;
+    const uint8_t* vp = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).code + v_offset<VT, VD>(l16);
     const uint8_t* ks = a.kc + kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD).scale;
     const uint8_t* vs = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).scale + VD * l16 / kKvBlock;
 
@@ -224,8 +323,6 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_partial_kernel(TreeArgs a
     uint32_t ksc[2][2];
     DimsV<VT, VD> vx[8];
     uint32_t vsc[8];
-    const int wbase = cbase + wv * wlen;
-    const int nsteps = wbase > last ? 0 : min(a.nsub, (last - wbase) / kStep + 1);
     auto load_k = [&](int sb) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -246,26 +343,51 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_partial_kernel(TreeArgs a
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const size_t p = min(sb + 4 * g4 + (j < 4 ? j : 12 + j), last);
-            vx[j] = load_v<VT, VD>(vp + p * vstride);
+            vx[j] = load_v<VT, VD>(vp + p * vstride, l16);
             if constexpr (VT != kKvF16) vsc[j] = vs[p * NB];
         }
     };
+    if (nsteps > 0) {
+        load_k(wbase);
+        load_vs(wbase);
+    }
+
+    half8 qb[NI][2];
+    float post;   // score = product * post, in base 2
+    {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(qx[i][e]));
+        m = fmaxf(m, xor_lane<16>(m));
+        m = fmaxf(m, xor_lane<32>(m));
+        const int sh = q_shift(m);
+        const float f = ldexpf(1.0f, sh);
+        post = a.scale * 1.44269504088896340736f * ldexpf(1.0f, -sh);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = qx[i][8 * hf + e] * f;
+                    const _Float16 h = static_cast<_Float16>(x);
+                    qb[i][hf][e] = low ? static_cast<_Float16>(x - static_cast<float>(h)) : h;
+                }
+    }
 
     floatx4 o[VD];
 #pragma unroll
     for (int e = 0; e < VD; ++e) o[e] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = -INFINITY, l_run = 0.0f;   // l_run: this lane's positions only
 
-    if (nsteps > 0) {
-        load_k(wbase);
-        load_vs(wbase);
-    }
     for (int st = 0; st < nsteps; ++st) {
         const int sb = wbase + st * kStep;
-        float sc[8];   // j: position sb + 4 g4 + j, or 16 further from j = 4 on
+        float sc[8];   // j: position sb + 4 g4 + j, or 16 + 4 g4 + j - 4 further
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            floatx4 dh = {0.0f, 0.0f, 0.0f, 0.0f}, dl = dh;
+            floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 half2v s = {};
@@ -274,14 +396,10 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_partial_kernel(TreeArgs a
                     s = scale2(b, b);
                 }
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const half8 kk = k_operand<KT>(kx[t][i], hf, s);
-                    dh = mfma(kk, qh[i][hf], dh);
-                    dl = mfma(kk, ql[i][hf], dl);
-                }
+                for (int hf = 0; hf < 2; ++hf) acc = mfma(k_operand<KT>(kx[t][i], hf, s), qb[i][hf], acc);
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sc[4 * t + r] = dh[r] + dl[r];
+            for (int r = 0; r < 4; ++r) sc[4 * t + r] = (acc[r] + xor_lane<8>(acc[r])) * post;
         }
         const bool more = st + 1 < nsteps;
         if (more) load_k(sb + kStep);
@@ -291,26 +409,22 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_partial_kernel(TreeArgs a
             seen = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int p = sb + 4 * g4 + (j < 4 ? j : 12 + j);
-                bool ok = p <= lim;
-                if (mask && p >= base && p - base < a.ntok) ok = ok || ((mask >> (p - base)) & 1);
-                if (ok) seen |= 1u << j;
+                if (sees(sb + 4 * g4 + (j < 4 ? j : 12 + j), lim, mask, base, a.ntok)) seen |= 1u << j;
+                else sc[j] = -INFINITY;
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sc[j] = seen >> j & 1 ? sc[j] : -INFINITY;
         }
         float mloc = sc[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) mloc = fmaxf(mloc, sc[j]);
         mloc = fmaxf(mloc, xor_lane<16>(mloc));
         mloc = fmaxf(mloc, xor_lane<32>(mloc));
-        const float m_new = fmaxf(m_run, mloc);
+        const float m_new = mloc > m_run + kLazy ? mloc : m_run;
         const float m_ref = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: exp2(-inf) = 0, no NaN
         const float alpha = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_ref);
         float p[8], lsum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(sc[j] - m_ref);
+            p[j] = __builtin_amdgcn_exp2f(sc[j] - m_ref + kPScale);
             lsum += p[j];
         }
         l_run = l_run * alpha + lsum;
@@ -318,25 +432,25 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_partial_kernel(TreeArgs a
         if (__ballot(alpha != 1.0f)) {   // uniform: some row's maximum moved
             float al[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) al[r] = __shfl(alpha, 4 * g4 + r, 64);
+            for (int r = 0; r < 4; ++r) al[r] = __shfl(alpha, 4 * (g4 & 1) + r, 64);
 #pragma unroll
             for (int e = 0; e < VD; ++e)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[e][r] *= al[r];
         }
-        half8 ph, pl;
-        split8(p, ph, pl);
+        half8 pa;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const _Float16 h = static_cast<_Float16>(p[j]);
+            pa[j] = low ? static_cast<_Float16>(p[j] - static_cast<float>(h)) : h;
+        }
         half2v vsp[4];
-        if constexpr (VT != kKvF16) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) vsp[j] = scale2(vsc[2 * j], vsc[2 * j + 1]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) vsp[j] = half2v{};
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (VT != kKvF16) vsp[j] = scale2(vsc[2 * j], vsc[2 * j + 1]);
+            else vsp[j] = half2v{};
         }
         if (tail) {
-            // V rows that are not finite (of tokens that others do not see, or never written): zeroed in the product and
-            // added by hand to the rows that see them
             bool odd = false;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -348,28 +462,23 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_partial_kernel(TreeArgs a
                 }
             }
             if (__ballot(odd)) {
-                float* pw = &pb[wv][0][0];   // [row][position in the step], -1 where not seen
+                float(*pw)[kStep] = reinterpret_cast<float(*)[kStep]>(&slab[wv][0][0]);   // [row][position], -1: not seen
+                if (!low)
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    pw[l16 * kStep + 4 * g4 + (j < 4 ? j : 12 + j)] = seen >> j & 1 ? p[j] : -1.0f;
+                    for (int j = 0; j < 8; ++j) pw[row][4 * g4 + (j < 4 ? j : 12 + j)] = seen >> j & 1 ? p[j] : -1.0f;
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                for (int pp = 0; pp < kStep; ++pp) {
+                    const size_t p1 = min(sb + pp, last);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    // this lane's dims of its position j, one lane group after another
-                    for (int g = 0; g < 4; ++g) {
+                    for (int e = 0; e < VD; ++e) {
+                        float v;
+                        if constexpr (VT == kKvF16) v = half_bits_to_float(reinterpret_cast<const uint16_t*>(vp + p1 * vstride)[e]);
+                        else v = kv_scale_value(vs[p1 * NB]);   // NaN: every value of the block
+                        if (fabsf(v) <= FLT_MAX) continue;
 #pragma unroll
-                        for (int e = 0; e < VD; ++e) {
-                            float v;
-                            if constexpr (VT == kKvF16) v = half_bits_to_float(vx[j].w[e >> 1] >> (16 * (e & 1)));
-                            else v = static_cast<float>(vsp[j >> 1][j & 1]);   // a NaN scale: every value of the block
-                            v = __shfl(v, 16 * g + l16, 64);
-                            if (!(fabsf(v) <= FLT_MAX)) {
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    const float w = pw[(4 * g4 + r) * kStep + 4 * g + (j < 4 ? j : 12 + j)];
-                                    if (w >= 0.0f || w != w) o[e][r] = __builtin_fmaf(w, v, o[e][r]);
-                                }
-                            }
+                        for (int r = 0; r < 4; ++r) {
+                            const float x = g4 < 2 ? pw[4 * (g4 & 1) + r][pp] : -1.0f;
+                            if (!(x < 0.0f)) o[e][r] = __builtin_fmaf(x, v, o[e][r]);
                         }
                     }
                 }
@@ -377,16 +486,11 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_partial_kernel(TreeArgs a
                 for (int j = 0; j < 8; ++j) {
                     if constexpr (VT == kKvF16) {
 #pragma unroll
-                        for (int e = 0; e < VD / 2; ++e) {
-                            uint32_t& w = vx[j].w[e];
-                            if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
-                            if ((w & 0x7c000000u) == 0x7c000000u) w &= 0xffffu;
-                        }
-                    } else if (!finite16(u2(vsp[j >> 1]) >> (16 * (j & 1)) & 0xffffu)) {
-                        vsp[j >> 1][j & 1] = static_cast<_Float16>(0.0f);
+                        for (int e = 0; e < VD / 2; ++e) vx[j].w[e] = zero_odd(vx[j].w[e]);
+                    } else if ((j & 1) == 0) {
+                        vsp[j >> 1] = h2(zero_odd(u2(vsp[j >> 1])));
                     }
                 }
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
         }
 #pragma unroll
@@ -394,140 +498,397 @@ __global__ __launch_bounds__(64 * kWaves, 1) void tree_partial_kernel(TreeArgs a
             uint32_t ev[4], od[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) v_pair<VT, VD>(vx[2 * j], vx[2 * j + 1], e, vsp[j], ev[j], od[j]);
-            const half8 b0 = h8(ev[0], ev[1], ev[2], ev[3]), b1 = h8(od[0], od[1], od[2], od[3]);
-            o[2 * e] = mfma(ph, b0, o[2 * e]);
-            o[2 * e] = mfma(pl, b0, o[2 * e]);
-            o[2 * e + 1] = mfma(ph, b1, o[2 * e + 1]);
-            o[2 * e + 1] = mfma(pl, b1, o[2 * e + 1]);
+            o[2 * e] = mfma(pa, h8(ev[0], ev[1], ev[2], ev[3]), o[2 * e]);
+            o[2 * e + 1] = mfma(pa, h8(od[0], od[1], od[2], od[3]), o[2 * e + 1]);
         }
         if (more) load_vs(sb + kStep);
     }
 
-    // join the waves: (0 + 1) + (2 + 3), scaled to the common maximum
     l_run += xor_lane<16>(l_run);
     l_run += xor_lane<32>(l_run);
-    if (g4 == 0) {
-        stat[wv][0][l16] = m_run;
-        stat[wv][1][l16] = l_run;
+    if (g4 == 0 && !low) {
+        stat[wv][0][row] = m_run;
+        stat[wv][1][row] = l_run;
     }
-    __syncthreads();
-    float f[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int rr = 4 * g4 + r;
-        const float mm = fmaxf(fmaxf(stat[0][0][rr], stat[1][0][rr]), fmaxf(stat[2][0][rr], stat[3][0][rr]));
-        f[r] = __builtin_amdgcn_exp2f(stat[wv][0][rr] - (mm == -INFINITY ? 0.0f : mm));
-    }
+    // high rows + low rows: lanes g4 < 2 end with o[row 4 g4 + r]
 #pragma unroll
     for (int e = 0; e < VD; ++e)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[e][r] *= f[r];
-    if (wv & 1) {
+        for (int r = 0; r < 4; ++r) o[e][r] += xor_lane<32>(o[e][r]);
+    if (g4 < 2) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int e = 0; e < VD; ++e) ob[wv >> 1][4 * g4 + r][VD * l16 + e] = o[e][r];
+            for (int e = 0; e < VD; e += 4)
+                *reinterpret_cast<float4*>(&slab[wv][4 * g4 + r][VD * l16 + e]) = make_float4(o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]);
     }
     __syncthreads();
-    if (!(wv & 1)) {
+    join_stats<1, kFewRows>(stat, fac, top, sum);
+    __syncthreads();
+    join_rows<HD, 1, kFewRows>(a, w, slab, fac, top, sum, 0);
+}
+
+// ---- more rows: v_mfma_f32_32x32x16_f16 -----------------------------------------------------------------------------------
+// Lane: l32 = l % 32, h = l / 32; A rows, B and D columns are l32; A and B hold k = 8 h + 0..7; D row of register r is
+// 8 (r / 4) + 4 h + r % 4.  A wave holds 32 query rows (q in high and low parts, o) in registers and walks its positions as
+// above, 32 at a time: scores D[position][row], P in the A layout of two products of 16 positions each (k slot j of product
+// m is position 16 m + 4 h + j, or + 4 more from j = 4 on, which are registers 8 m + j of the scores).
+// Of the four waves, RB hold different rows and 4 / RB different parts of the chunk.
+template <int KT, int VT, int HD, int RB>
+__global__ __launch_bounds__(kThreads, 1) void tree_rows_kernel(TreeArgs a) {
+    constexpr int NI = HD / 32;        // K: 16-dim pieces a lane takes of a position
+    constexpr int VD = HD / 32;        // V: dims a lane takes of a position
+    constexpr int NB = HD / kKvBlock;
+    constexpr int kKB = kv_row_bytes(KT, HD), kVB = kv_row_bytes(VT, HD);
+    __shared__ __attribute__((aligned(16))) float slab[kWaves][kOct][HD];
+    __shared__ float stat[kWaves][2][kBlockRows], fac[kWaves][kBlockRows], top[RB][kBlockRows], sum[RB][kBlockRows];
+
+    Work w;
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l32 = lane & 31, h = lane >> 5;
+    if (!tree_work<kBlockRows * RB>(a, w)) return;
+    const int G = a.n_head / a.n_kv, base = w.base, kv = w.kv;
+    const int rb = wv % RB, part = wv / RB;
+    const int row0 = w.row0 + kBlockRows * rb, row = row0 + l32, rowc = min(row, a.rows - 1), tok = rowc / G;
+    // the last position the wave's rows see
+    const int last = a.masks ? w.last : base + min(row0 + kBlockRows - 1, a.rows - 1) / G;
+    const int wsteps = RB * a.nsub, wbase = w.chunk * kUnit * a.nsub + part * wsteps * kStep;
+    const int nsteps = wbase > last || row0 >= a.rows ? 0 : min(wsteps, (last - wbase) / kStep + 1);
+    uint64_t mask = 0;
+    if (a.masks && row < a.rows) mask = a.masks[tok];
+    const int lim = row >= a.rows ? -1 : a.masks ? base - 1 : base + tok;
+
+    half8 qh[NI][2], ql[NI][2];
+    float post;
+    {
+        const float* qr = a.q + (static_cast<size_t>(tok) * a.n_head + kv * G + (rowc - tok * G)) * HD + 16 * h;
+        float4 u[NI][4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int e = 0; e < VD; ++e) {
-                float& w = ob[wv >> 1][4 * g4 + r][VD * l16 + e];
-                w = o[e][r] + w;
+            for (int f = 0; f < 4; ++f) u[i][f] = reinterpret_cast<const float4*>(qr + 32 * i)[f];
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+                m = fmaxf(m, fmaxf(fmaxf(fabsf(u[i][f].x), fabsf(u[i][f].y)), fmaxf(fabsf(u[i][f].z), fabsf(u[i][f].w))));
+        m = fmaxf(m, xor_lane<32>(m));
+        const int sh = q_shift(m);
+        const float f = ldexpf(1.0f, sh);
+        post = a.scale * 1.44269504088896340736f * ldexpf(1.0f, -sh);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const float4 b = u[i][2 * hf], c = u[i][2 * hf + 1];
+                const float x[8] = {b.x * f, b.y * f, b.z * f, b.w * f, c.x * f, c.y * f, c.z * f, c.w * f};
+                split8(x, qh[i][hf], ql[i][hf]);
             }
     }
-    __syncthreads();
-    const size_t rec = (static_cast<size_t>(chunk) * a.n_kv + kv) * a.rows_pad + kRows * group;
-    for (int i = threadIdx.x; i < kRows * HD / 4; i += 64 * kWaves) {
-        const float4 x = reinterpret_cast<const float4*>(&ob[0][0][0])[i], y = reinterpret_cast<const float4*>(&ob[1][0][0])[i];
-        reinterpret_cast<float4*>(a.wo + rec * HD)[i] = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
-    }
-    if (threadIdx.x < kRows) {
-        const int r = threadIdx.x;
-        const float mm = fmaxf(fmaxf(stat[0][0][r], stat[1][0][r]), fmaxf(stat[2][0][r], stat[3][0][r]));
-        const float ref = mm == -INFINITY ? 0.0f : mm;
-        float l = 0.0f;
+
+    const size_t kstride = KT == kKvF16 ? static_cast<size_t>(a.n_kv) * kKB : kKB;
+    const size_t vstride = VT == kKvF16 ? static_cast<size_t>(a.n_kv) * kVB : kVB;
+    const uint8_t* kp = a.kc + kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD).code + h * (kKB / (HD / 16));
+    const uint8_t* vp = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).code + v_offset<VT, VD>(l32);
+    const uint8_t* ks = a.kc + kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD).scale;
+    const uint8_t* vs = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).scale + VD * l32 / kKvBlock;
+
+    Dims16<KT> kx[NI];
+    uint32_t ksc[2];
+    DimsV<VT, VD> vx[16];
+    uint32_t vsc[16];
+    auto load_k = [&](int sb) {
+        const size_t p = min(sb + l32, last);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) l = __builtin_fmaf(stat[w][1][r], __builtin_amdgcn_exp2f(stat[w][0][r] - ref), l);
-        a.wml[2 * (rec + r)] = mm;
-        a.wml[2 * (rec + r) + 1] = l;
+        for (int i = 0; i < NI; ++i) kx[i] = load_k16<KT>(kp + p * kstride + i * (kKB / NI));
+        if constexpr (KT != kKvF16) {
+            if constexpr (NB == 8) {
+                const uint2 s = *reinterpret_cast<const uint2*>(ks + p * NB);
+                ksc[0] = s.x, ksc[1] = s.y;
+            } else {
+                ksc[0] = *reinterpret_cast<const uint32_t*>(ks + p * NB);
+            }
+        }
+    };
+    auto slot = [&](int j) { return 8 * (j >> 2) + 4 * h + (j & 3); };   // the position of score register j in its step
+    auto load_vs = [&](int sb) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const size_t p = min(sb + slot(j), last);
+            vx[j] = load_v<VT, VD>(vp + p * vstride, l32);
+            if constexpr (VT != kKvF16) vsc[j] = vs[p * NB];
+        }
+    };
+    floatx16 o[VD];
+#pragma unroll
+    for (int e = 0; e < VD; ++e)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[e][r] = 0.0f;
+    float m_run = -INFINITY, l_run = 0.0f;
+
+    if (nsteps > 0) {
+        load_k(wbase);
+        load_vs(wbase);
+    }
+    for (int st = 0; st < nsteps; ++st) {
+        const int sb = wbase + st * kStep;
+        floatx16 sc;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            half2v s = {};
+            if constexpr (KT != kKvF16) {   // block i
+                const uint32_t b = (ksc[i >> 2] >> (8 * (i & 3))) & 0xffu;
+                s = scale2(b, b);
+            }
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const half8 kk = k_operand<KT>(kx[i], hf, s);
+                sc = mfma(kk, qh[i][hf], sc);
+                sc = mfma(kk, ql[i][hf], sc);
+            }
+        }
+        const bool more = st + 1 < nsteps;
+        if (more) load_k(sb + kStep);
+        const bool tail = sb + kStep > base;   // uniform
+        uint32_t seen = 0xffffu;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sc[j] *= post;
+        if (tail || row >= a.rows) {
+            seen = 0;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                if (sees(sb + slot(j), lim, mask, base, a.ntok)) seen |= 1u << j;
+                else sc[j] = -INFINITY;
+            }
+        }
+        float mloc = sc[0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) mloc = fmaxf(mloc, sc[j]);
+        mloc = fmaxf(mloc, xor_lane<32>(mloc));
+        const float m_new = mloc > m_run + kLazy ? mloc : m_run;
+        const float m_ref = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_ref);
+        float p[16], lsum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            p[j] = __builtin_amdgcn_exp2f(sc[j] - m_ref + kPScale);
+            lsum += p[j];
+        }
+        l_run = l_run * alpha + lsum;
+        m_run = m_new;
+        if (__ballot(alpha != 1.0f)) {
+            float al[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) al[r] = __shfl(alpha, slot(r), 64);
+#pragma unroll
+            for (int e = 0; e < VD; ++e)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[e][r] *= al[r];
+        }
+        half8 ph[2], pl[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const float x[8] = {p[8 * m], p[8 * m + 1], p[8 * m + 2], p[8 * m + 3], p[8 * m + 4], p[8 * m + 5], p[8 * m + 6], p[8 * m + 7]};
+            split8(x, ph[m], pl[m]);
+        }
+        half2v vsp[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (VT != kKvF16) vsp[j] = scale2(vsc[2 * j], vsc[2 * j + 1]);
+            else vsp[j] = half2v{};
+        }
+        if (tail) {
+            bool odd = false;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (VT != kKvF16) {
+                    odd = odd || !finite16(u2(vsp[j]));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VD / 2; ++e) odd = odd || !finite16(vx[2 * j].w[e]) || !finite16(vx[2 * j + 1].w[e]);
+                }
+            }
+            if (__ballot(odd)) {
+                float(*pw)[kStep] = reinterpret_cast<float(*)[kStep]>(&slab[wv][0][0]);   // [row][position], -1: not seen
+#pragma unroll
+                for (int j = 0; j < 16; ++j) pw[l32][slot(j)] = seen >> j & 1 ? p[j] : -1.0f;
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                for (int pp = 0; pp < kStep; ++pp) {
+                    const size_t p1 = min(sb + pp, last);
+#pragma unroll
+                    for (int e = 0; e < VD; ++e) {
+                        float v;
+                        if constexpr (VT == kKvF16) v = half_bits_to_float(reinterpret_cast<const uint16_t*>(vp + p1 * vstride)[e]);
+                        else v = kv_scale_value(vs[p1 * NB]);
+                        if (fabsf(v) <= FLT_MAX) continue;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const float x = pw[slot(r)][pp];
+                            if (!(x < 0.0f)) o[e][r] = __builtin_fmaf(x, v, o[e][r]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    if constexpr (VT == kKvF16) {
+#pragma unroll
+                        for (int e = 0; e < VD / 2; ++e) vx[j].w[e] = zero_odd(vx[j].w[e]);
+                    } else if ((j & 1) == 0) {
+                        vsp[j >> 1] = h2(zero_odd(u2(vsp[j >> 1])));
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < VD / 2; ++e)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                uint32_t ev[4], od[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v_pair<VT, VD>(vx[8 * m + 2 * j], vx[8 * m + 2 * j + 1], e, vsp[4 * m + j], ev[j], od[j]);
+                const half8 b0 = h8(ev[0], ev[1], ev[2], ev[3]), b1 = h8(od[0], od[1], od[2], od[3]);
+                o[2 * e] = mfma(ph[m], b0, o[2 * e]);
+                o[2 * e + 1] = mfma(ph[m], b1, o[2 * e + 1]);
+                o[2 * e] = mfma(pl[m], b0, o[2 * e]);
+                o[2 * e + 1] = mfma(pl[m], b1, o[2 * e + 1]);
+            }
+        if (more) load_vs(sb + kStep);
+    }
+
+    l_run += xor_lane<32>(l_run);
+    if (h == 0) {
+        stat[wv][0][l32] = m_run;
+        stat[wv][1][l32] = l_run;
+    }
+    __syncthreads();
+    join_stats<RB, kBlockRows>(stat, fac, top, sum);
+#pragma unroll
+    for (int oct = 0; oct < kBlockRows / kOct; ++oct) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < VD; e += 4)
+                *reinterpret_cast<float4*>(&slab[wv][4 * h + r][VD * l32 + e]) =
+                    make_float4(o[e][4 * oct + r], o[e + 1][4 * oct + r], o[e + 2][4 * oct + r], o[e + 3][4 * oct + r]);
+        __syncthreads();
+        join_rows<HD, RB, kBlockRows>(a, w, slab, fac, top, sum, oct);
+        __syncthreads();
     }
 }
 
 // ---- merge -------------------------------------------------------------------------------------------------------------
-// Workgroup (token, head): the chunks' (m, l) give weights 2^(m - M) and L; lane groups of HD / 4 lanes sum every n-th
-// chunk's o (four dims a lane), the groups are added in order; gate, fp32, Q8_1.  A row that sees nothing has M = -inf.
-constexpr int kMergeThreads = 256;
+// Workgroup (token, head, 64 dims): every lane has the (m, l) of a chunk and its group's first o in flight together; weights
+// 2^(m - M) to LDS, wave g sums chunks g, g + 4, ... in order, then the four waves in order; gate, fp32, Q8_1.  A row that
+// sees nothing has M = -inf.
+constexpr int kMergeDims = 64, kMergeBatch = 16;
 
 template <int HD>
-__global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(TreeArgs a, const float* __restrict__ gsrc, int gstride,
-                                                                   float* __restrict__ y, int y_stride,
-                                                                   uint8_t* __restrict__ q8, int q8_stride) {
-    constexpr int L4 = HD / 4, NG = kMergeThreads / L4;
+__global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeArgs a) {
     __shared__ float wts[kMaxChunks];
-    __shared__ float red[2][kMergeThreads / 64];
-    __shared__ __attribute__((aligned(16))) float part[NG][HD];
-    const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+    __shared__ float red[2][kWaves];
+    __shared__ float part[kWaves][kMergeDims];
+    const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, g = tid >> 6;
+    const int d = kMergeDims * blockIdx.z + lane;
     const int G = a.n_head / a.n_kv, kv = h / G, row = t * G + (h - kv * G);
+    float gate = 0.0f;
+    if (a.gate) gate = a.gate[static_cast<size_t>(t) * a.gate_stride + h * 2 * HD + HD + d];
     const int base = a.pos[0];
     if (base < 0 || base > a.max_ctx - a.ntok) return;   // uniform: a slot outside the cache
-    const int last = base + (a.masks ? a.ntok - 1 : t);
-    const int nchunk = last / (kUnit * a.nsub) + 1;
+    const int nchunk = (base + (a.masks ? a.ntok - 1 : t)) / (kUnit * a.nsub) + 1;
     const size_t cstride = static_cast<size_t>(a.n_kv) * a.rows_pad, r0 = static_cast<size_t>(kv) * a.rows_pad + row;
-    float m = -INFINITY;
-    for (int c = tid; c < nchunk; c += kMergeThreads) m = fmaxf(m, a.wml[2 * (r0 + c * cstride)]);
+    const float2* ml = reinterpret_cast<const float2*>(a.wml) + r0;
+    const float* ro = a.wo + r0 * HD + d;
+    const float2 first = ml[min(tid, nchunk - 1) * cstride];
+    float oa[kMergeBatch];   // chunks g + 4 k, clamped (a load under a branch gets a wait of its own)
+#pragma unroll
+    for (int k = 0; k < kMergeBatch; ++k) oa[k] = ro[min(g + 4 * k, nchunk - 1) * cstride * HD];
+    float m = first.x;
+    for (int c = tid + kThreads; c < nchunk; c += kThreads) m = fmaxf(m, ml[c * cstride].x);
     m = group_max<64>(m);
-    if ((tid & 63) == 0) red[0][tid >> 6] = m;
+    if (lane == 0) red[0][g] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
     const float ref = m == -INFINITY ? 0.0f : m;
     float l = 0.0f;
-    for (int c = tid; c < nchunk; c += kMergeThreads) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.wml + 2 * (r0 + c * cstride));
-        const float w = __builtin_amdgcn_exp2f(ml.x - ref);
-        wts[c] = w;
-        l = __builtin_fmaf(ml.y, w, l);
+    for (int c = tid; c < nchunk; c += kThreads) {
+        const float2 x = c == tid ? first : ml[c * cstride];
+        const float wt = __builtin_amdgcn_exp2f(x.x - ref);
+        wts[c] = wt;
+        l = __builtin_fmaf(x.y, wt, l);
     }
     l = group_sum<64>(l);
-    if ((tid & 63) == 0) red[1][tid >> 6] = l;
+    if (lane == 0) red[1][g] = l;
     __syncthreads();
     l = ((red[1][0] + red[1][1]) + red[1][2]) + red[1][3];
-    const int g = tid / L4, d = 4 * (tid % L4);
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int c = g; c < nchunk; c += NG) {
-        const float4 x = *reinterpret_cast<const float4*>(a.wo + (r0 + c * cstride) * HD + d);
-        const float w = wts[c];
-        o.x = __builtin_fmaf(w, x.x, o.x);
-        o.y = __builtin_fmaf(w, x.y, o.y);
-        o.z = __builtin_fmaf(w, x.z, o.z);
-        o.w = __builtin_fmaf(w, x.w, o.w);
-    }
-    *reinterpret_cast<float4*>(&part[g][d]) = o;
-    __syncthreads();
-    if (tid >= HD) return;
-    float v = 0.0f;
+    float o = 0.0f;
+    for (int c0 = 0; 4 * c0 < nchunk; c0 += kMergeBatch) {
+        const bool more = 4 * (c0 + kMergeBatch) < nchunk;
+        float nx[kMergeBatch];
+        if (more) {
 #pragma unroll
-    for (int i = 0; i < NG; ++i) v += part[i][tid];
-    v = m == -INFINITY ? 0.0f : v / l;
-    if (gsrc) {
-        const float x = gsrc[static_cast<size_t>(t) * gstride + h * 2 * HD + HD + tid];
-        v *= 1.0f / (1.0f + expf(-x));
+            for (int k = 0; k < kMergeBatch; ++k) nx[k] = ro[min(g + 4 * (c0 + kMergeBatch + k), nchunk - 1) * cstride * HD];
+        }
+#pragma unroll
+        for (int k = 0; k < kMergeBatch; ++k) {
+            const int c = g + 4 * (c0 + k);
+            if (c < nchunk) o = __builtin_fmaf(wts[c], oa[k], o);
+        }
+        if (more) {
+#pragma unroll
+            for (int k = 0; k < kMergeBatch; ++k) oa[k] = nx[k];
+        }
     }
-    if (y) y[static_cast<size_t>(t) * y_stride + h * HD + tid] = v;
-    if (q8) q8_1_store_lane(v, q8 + static_cast<size_t>(t) * q8_stride + (h * (HD / 32) + tid / 32) * kQ8_1Bytes);
+    part[g][lane] = o;
+    __syncthreads();
+    if (g != 0) return;
+    float v = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
+    v = m == -INFINITY ? 0.0f : v / l;
+    if (a.gate) v *= 1.0f / (1.0f + expf(-gate));
+    if (a.y) a.y[static_cast<size_t>(t) * a.y_stride + h * HD + d] = v;
+    if (a.q8) q8_1_store_lane(v, a.q8 + static_cast<size_t>(t) * a.q8_stride + (h * (HD / 32) + d / 32) * kQ8_1Bytes);
 }
 
 bool tree_shape_ok(int max_ctx, int n_head, int n_kv, int head_dim, int ntok) {
     return kv_shape_ok(max_ctx, n_kv, head_dim) && n_head > 0 && n_head <= 65535 && n_head % n_kv == 0 && n_head / n_kv <= 64 &&
            ntok >= 1 && ntok <= kMaxChain;
 }
-int tree_rows(int n_head, int n_kv, int ntok) { return ntok * (n_head / n_kv); }
-int tree_groups(int rows) { return (rows + kRows - 1) / kRows; }
+
+// the form of a call: query rows per KV head, row blocks side by side in a workgroup (0: the 16 x 16 form), rows a
+// workgroup holds, workgroups per (chunk, KV head)
+struct Form {
+    int rows, rb, held, groups;
+};
+Form tree_form(int n_head, int n_kv, int ntok) {
+    Form f;
+    f.rows = ntok * (n_head / n_kv);
+    f.rb = f.rows <= kFewRows ? 0 : f.rows <= kBlockRows ? 1 : f.rows <= 2 * kBlockRows ? 2 : 4;
+    f.held = f.rb ? kBlockRows * f.rb : kFewRows;
+    f.groups = (f.rows + f.held - 1) / f.held;
+    return f;
+}
 long long tree_chunks(int max_ctx, int nsub) {
     const long long len = static_cast<long long>(kUnit) * nsub;
     return (max_ctx + len - 1) / len;
+}
+
+template <int KT, int VT, int HD>
+void launch_partial(const TreeArgs& a, int rb, unsigned blocks, hipStream_t s) {
+    auto go = [&](auto* kernel) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, s, a); };
+    if (rb == 0) go(&tree_few_kernel<KT, VT, HD>);
+    else if (rb == 1) go(&tree_rows_kernel<KT, VT, HD, 1>);
+    else if (rb == 2) go(&tree_rows_kernel<KT, VT, HD, 2>);
+    else go(&tree_rows_kernel<KT, VT, HD, 4>);
+}
+
+template <int HD>
+void launch_tree(const TreeArgs& a, int ktype, int vtype, int rb, unsigned blocks, hipStream_t s) {
+    if (ktype == kKvF16) launch_partial<kKvF16, kKvF16, HD>(a, rb, blocks, s);
+    else if (ktype == kKvI4) launch_partial<kKvI4, kKvI4, HD>(a, rb, blocks, s);
+    else if (vtype == kKvI8) launch_partial<kKvI8, kKvI8, HD>(a, rb, blocks, s);
+    else launch_partial<kKvI8, kKvI4, HD>(a, rb, blocks, s);
+    if (!a.direct) hipLaunchKernelGGL((tree_merge_kernel<HD>), dim3(a.ntok, a.n_head, HD / kMergeDims), dim3(kThreads), 0, s, a);
 }
 
 }  // namespace
@@ -540,9 +901,9 @@ extern "C" int rmi_gqa_tree_nsub(int ctx, int n_head, int n_kv, int head_dim, in
         set_error("gqa_tree_nsub: invalid shape");
         return 0;
     }
-    // two workgroups a compute unit
-    const long long groups = tree_groups(tree_rows(n_head, n_kv, ntok)), units = (ctx + kUnit - 1) / kUnit;
-    const long long want = (units * n_kv * groups + 511) / 512;
+    // a workgroup a compute unit
+    const long long groups = tree_form(n_head, n_kv, ntok).groups, units = (ctx + kUnit - 1) / kUnit;
+    const long long want = (units * n_kv * groups + 255) / 256;
     return static_cast<int>(std::max(std::max(1LL, (units + kMaxChunks - 1) / kMaxChunks), std::min(units, want)));
 }
 
@@ -551,8 +912,8 @@ extern "C" size_t rmi_gqa_tree_workspace_bytes(int max_ctx, int n_head, int n_kv
         set_error("gqa_tree_workspace_bytes: invalid shape");
         return 0;
     }
-    const size_t rows = static_cast<size_t>(tree_groups(tree_rows(n_head, n_kv, ntok))) * kRows;
-    return static_cast<size_t>(tree_chunks(max_ctx, nsub)) * n_kv * rows * (head_dim + 2) * sizeof(float);
+    const Form f = tree_form(n_head, n_kv, ntok);
+    return static_cast<size_t>(tree_chunks(max_ctx, nsub)) * n_kv * (static_cast<size_t>(f.groups) * f.held) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache, int vtype, const void* vcache,
@@ -568,42 +929,36 @@ extern "C" int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache
         (masks && (reinterpret_cast<uintptr_t>(masks) & 7u)) || (gate_src && !aligned4(gate_src)) || (!y && !q8) ||
         (y && !aligned4(y)) || (q8 && (!aligned4(q8) || q8_stride % 4)))
         return fail(RMI_ERR_POINTER, "gqa_tree_decode: null or misaligned pointer");
+    const Form f = tree_form(n_head, n_kv, ntok);
     TreeArgs a{};
     a.q = q;
     a.kc = static_cast<const uint8_t*>(kcache);
     a.vc = static_cast<const uint8_t*>(vcache);
     a.pos = pos;
     a.masks = masks;
+    a.gate = gate_src;
+    a.y = y;
+    a.q8 = q8;
     a.n_head = n_head;
     a.n_kv = n_kv;
     a.ntok = ntok;
-    a.rows = tree_rows(n_head, n_kv, ntok);
-    a.groups = tree_groups(a.rows);
-    a.rows_pad = a.groups * kRows;
+    a.rows = f.rows;
+    a.groups = f.groups;
+    a.rows_pad = f.groups * f.held;
     a.nsub = static_cast<int>(std::min<long long>(nsub, (static_cast<long long>(max_ctx) + kUnit - 1) / kUnit));
     a.max_ctx = max_ctx;
+    a.gate_stride = gate_stride;
+    a.y_stride = y_stride;
+    a.q8_stride = q8_stride;
     a.scale = scale;
-    const long long pairs = tree_chunks(max_ctx, nsub) * n_kv, blocks = (pairs + 7) / 8 * 8 * a.groups;
+    const long long chunks = tree_chunks(max_ctx, nsub), pairs = chunks * n_kv, blocks = (pairs + 7) / 8 * 8 * f.groups;
     if (blocks > 0x7fffffffLL) return fail(RMI_ERR_SHAPE, "gqa_tree_decode: too many workgroups");
     a.npairs = static_cast<int>(pairs);
+    a.direct = chunks == 1;
     a.wo = static_cast<float*>(workspace);
     a.wml = a.wo + static_cast<size_t>(pairs) * a.rows_pad * head_dim;
     auto* s = static_cast<hipStream_t>(stream);
-    auto go = [&](auto* kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), 0, s, a); };
-    if (head_dim == 256) {
-        if (ktype == kKvF16) go(&tree_partial_kernel<kKvF16, kKvF16, 256>);
-        else if (ktype == kKvI4) go(&tree_partial_kernel<kKvI4, kKvI4, 256>);
-        else if (vtype == kKvI8) go(&tree_partial_kernel<kKvI8, kKvI8, 256>);
-        else go(&tree_partial_kernel<kKvI8, kKvI4, 256>);
-        hipLaunchKernelGGL((tree_merge_kernel<256>), dim3(ntok, n_head), dim3(kMergeThreads), 0, s, a, gate_src, gate_stride, y,
-                           y_stride, q8, q8_stride);
-    } else {
-        if (ktype == kKvF16) go(&tree_partial_kernel<kKvF16, kKvF16, 128>);
-        else if (ktype == kKvI4) go(&tree_partial_kernel<kKvI4, kKvI4, 128>);
-        else if (vtype == kKvI8) go(&tree_partial_kernel<kKvI8, kKvI8, 128>);
-        else go(&tree_partial_kernel<kKvI8, kKvI4, 128>);
-        hipLaunchKernelGGL((tree_merge_kernel<128>), dim3(ntok, n_head), dim3(kMergeThreads), 0, s, a, gate_src, gate_stride, y,
-                           y_stride, q8, q8_stride);
-    }
+    if (head_dim == 256) launch_tree<256>(a, ktype, vtype, f.rb, static_cast<unsigned>(blocks), s);
+    else launch_tree<128>(a, ktype, vtype, f.rb, static_cast<unsigned>(blocks), s);
     return launch_status("gqa_tree_decode");
 }

@@ -159,10 +159,10 @@ def test_a_chain_by_masks_is_a_chain(rmi, types):
 
 
 @pytest.mark.parametrize("types", PAIRS, ids=IDS)
-@pytest.mark.parametrize("ntok", [2, 4])
-def test_a_short_chains_tokens_are_the_single_tokens(rmi, types, ntok):
-    """up to 16 query rows per KV head: every token of a chain has the bits of a decode step at its slot"""
-    c = Call(rmi, types, 16, 4, 256, ntok, 381, None, nsub=2)
+@pytest.mark.parametrize("nh,ntok", [(16, 2), (8, 4), (4, 8), (4, 3)])
+def test_a_short_chains_tokens_are_the_single_tokens(rmi, types, nh, ntok):
+    """up to 8 query rows per KV head: every token of a chain has the bits of a decode step at its slot"""
+    c = Call(rmi, types, nh, 4, 256, ntok, 381, None, nsub=2)
     y = c.run()
     for t in range(ntok):
         one = c.run(tokens=slice(t, t + 1), base=c.base + t)
