@@ -26,7 +26,6 @@ namespace {
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
@@ -36,8 +35,7 @@ constexpr int kUnit = kWaves * kStep;
 constexpr int kMaxChunks = 2048;
 constexpr int kMaxTree = 64, kMaxChain = 1024;
 constexpr int kOct = 8;            // rows joined at a time
-constexpr int kFewRows = 8;        // query rows per KV head of the 16 x 16 form
-constexpr int kBlockRows = 32;     // rows of a wave in the 32 x 32 form
+constexpr int kFewRows = 8;        // query rows per KV head of the form without a tile
 constexpr float kPScale = 8.0f;    // p goes as 2^8 p
 constexpr float kLazy = 7.0f;      // a maximum moves once a score passes it by more than 2^7 (2^15 p is an fp16 number)
 
@@ -164,7 +162,6 @@ __device__ __forceinline__ void v_pair(const DimsV<T, VD>& a, const DimsV<T, VD>
 }
 
 __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ floatx16 mfma(half8 a, half8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
 // fp16 high part of eight fp32 values, and what is left of them
 __device__ __forceinline__ void split8(const float (&x)[8], half8& hi, half8& lo) {
@@ -221,15 +218,15 @@ __device__ __forceinline__ bool sees(int p, int lim, uint64_t mask, int base, in
 // Joins the waves' parts of 8 * RB rows (rows 8 oct .. of each of RB row blocks) from their LDS slabs [wave][8][HD] and
 // either writes records or, for a call of one chunk, the result: fac[wave][row of the block] is a part's weight, sum[row]
 // the joined l.  Wave w holds part w / RB of row block w % RB.
-template <int HD, int RB, int BLOCK>
-__device__ __forceinline__ void join_rows(const TreeArgs& a, const Work& w, const float (&slab)[kWaves][kOct][HD],
-                                          const float (&fac)[kWaves][BLOCK], const float (&top)[RB][BLOCK],
+template <int HD, int WAVES, int RB, int BLOCK>
+__device__ __forceinline__ void join_rows(const TreeArgs& a, const Work& w, const float (&slab)[WAVES][kOct][HD],
+                                          const float (&fac)[WAVES][BLOCK], const float (&top)[RB][BLOCK],
                                           const float (&sum)[RB][BLOCK], int oct) {
-    constexpr int PB = kWaves / RB;
+    constexpr int PB = WAVES / RB;
     const int G = a.n_head / a.n_kv;
 #pragma unroll
-    for (int i = 0; i < RB * kOct * HD / kThreads; ++i) {
-        const int e = static_cast<int>(threadIdx.x) + kThreads * i, d = e % HD, r8 = e / HD;   // r8: uniform in a wave
+    for (int i = 0; i < RB * kOct * HD / (64 * WAVES); ++i) {
+        const int e = static_cast<int>(threadIdx.x) + 64 * WAVES * i, d = e % HD, r8 = e / HD;   // r8: uniform in a wave
         const int rb = r8 / kOct, rr = r8 % kOct, rk = kOct * oct + rr, row = w.row0 + BLOCK * rb + rk;
         float v = slab[rb][rr][d] * fac[rb][rk];
 #pragma unroll
@@ -249,10 +246,10 @@ __device__ __forceinline__ void join_rows(const TreeArgs& a, const Work& w, cons
 }
 
 // the parts' weights and the joined sum of every row, from stat[wave][m, l][row of the block]
-template <int RB, int BLOCK>
-__device__ __forceinline__ void join_stats(const float (&stat)[kWaves][2][BLOCK], float (&fac)[kWaves][BLOCK], float (&top)[RB][BLOCK],
+template <int WAVES, int RB, int BLOCK>
+__device__ __forceinline__ void join_stats(const float (&stat)[WAVES][2][BLOCK], float (&fac)[WAVES][BLOCK], float (&top)[RB][BLOCK],
                                            float (&sum)[RB][BLOCK]) {
-    constexpr int PB = kWaves / RB;
+    constexpr int PB = WAVES / RB;
     const int i = threadIdx.x;
     if (i >= RB * BLOCK) return;
     const int rb = i / BLOCK, r = i % BLOCK;
@@ -523,257 +520,288 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
                 *reinterpret_cast<float4*>(&slab[wv][4 * g4 + r][VD * l16 + e]) = make_float4(o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]);
     }
     __syncthreads();
-    join_stats<1, kFewRows>(stat, fac, top, sum);
+    join_stats<kWaves, 1, kFewRows>(stat, fac, top, sum);
     __syncthreads();
-    join_rows<HD, 1, kFewRows>(a, w, slab, fac, top, sum, 0);
+    join_rows<HD, kWaves, 1, kFewRows>(a, w, slab, fac, top, sum, 0);
 }
 
-// ---- more rows: v_mfma_f32_32x32x16_f16 -----------------------------------------------------------------------------------
-// Lane: l32 = l % 32, h = l / 32; A rows, B and D columns are l32; A and B hold k = 8 h + 0..7; D row of register r is
-// 8 (r / 4) + 4 h + r % 4.  A wave holds 32 query rows (q in high and low parts, o) in registers and walks its positions as
-// above, 32 at a time: scores D[position][row], P in the A layout of two products of 16 positions each (k slot j of product
-// m is position 16 m + 4 h + j, or + 4 more from j = 4 on, which are registers 8 m + j of the scores).
-// Of the four waves, RB hold different rows and 4 / RB different parts of the chunk.
+// ---- more rows: the tile in LDS ---------------------------------------------------------------------------------------------
+// Eight waves, two to a SIMD: RB hold different 16 rows (q in high and low parts and o in registers), 8 / RB different parts
+// of the chunk.  The RB waves of a part share its tile of 32 positions in LDS as fp16, [position][dim] for K and V alike, so
+// each cache value is turned into fp16 once for 16 RB rows: a thread takes 16 dims of a position per unit, the next tile's
+// loads in flight over this tile's products.
+//   scores    A = K tile rows (16-byte reads), B = q rows: D[position][row], as above with one register set per part.
+//   P V       A = P, B = V columns by transposed reads (ds_read_b64_tr_b16: the 16 lanes of a g4 give the addresses of four
+//             positions x 16 dims and get a dim's four positions each), k slots as above.
+// Row strides of 16 and 32 bytes past a power of two spread a read's rows over the banks.
+constexpr int kTileWaves = 8;
+constexpr int kTileThreads = 64 * kTileWaves;
+constexpr int kRowBlock = 16;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+template <int HD, int RB>
+struct TilePool {
+    static constexpr int kParts = kTileWaves / RB;
+    static constexpr int kKRow = 2 * HD + 16, kVRow = 2 * HD + 32;     // bytes
+    static constexpr int kBytes = kStep * (kKRow + kVRow);             // one tile
+    static constexpr int kBufs = kParts == 4 ? 1 : 2;                  // two tiles a part where they fit
+    static constexpr int kSlab = kTileWaves * kOct * HD * 4;           // the rows that are joined, after the last step
+    static constexpr int kPool = kParts * kBufs * kBytes > kSlab ? kParts * kBufs * kBytes : kSlab;
+};
+
+// The order of N groups of R LDS reads and M products in a block: AHEAD groups' reads, then a group's reads for a group's
+// products.  Left alone the compiler reads two operands ahead and waits out the latency at each.
+template <int N, int R, int M, int AHEAD>
+__device__ __forceinline__ void interleave() {
+    constexpr int kAhead = N < AHEAD ? N : AHEAD;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead * R, 0);   // LDS reads
+#pragma unroll
+    for (int i = 0; i < N - kAhead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, M, 0);        // MFMAs
+        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, M * kAhead, 0);
+}
+
 template <int KT, int VT, int HD, int RB>
-__global__ __launch_bounds__(kThreads, 1) void tree_rows_kernel(TreeArgs a) {
-    constexpr int NI = HD / 32;        // K: 16-dim pieces a lane takes of a position
-    constexpr int VD = HD / 32;        // V: dims a lane takes of a position
+__global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) {
+    using Pool = TilePool<HD, RB>;
+    constexpr int PB = Pool::kParts, BUFS = Pool::kBufs;
+    constexpr int NC = HD / 32;                                  // 32-dim pieces of a row
+    constexpr int NE = HD / 16;                                  // 16-dim columns of o
     constexpr int NB = HD / kKvBlock;
+    constexpr int kUnits = kStep * NE;                           // 16-dim units of a tile
+    constexpr int U = kUnits > 64 * RB ? kUnits / (64 * RB) : 1;   // of them a thread's, of K and of V
     constexpr int kKB = kv_row_bytes(KT, HD), kVB = kv_row_bytes(VT, HD);
-    __shared__ __attribute__((aligned(16))) float slab[kWaves][kOct][HD];
-    __shared__ float stat[kWaves][2][kBlockRows], fac[kWaves][kBlockRows], top[RB][kBlockRows], sum[RB][kBlockRows];
+    __shared__ __attribute__((aligned(16))) uint8_t pool[Pool::kPool];
+    __shared__ float pb[kTileWaves][kRowBlock][kStep];           // a step's p where a V is not finite
+    __shared__ int odd_step[PB][BUFS];                           // the last step whose V had one
+    __shared__ float stat[kTileWaves][2][kRowBlock], fac[kTileWaves][kRowBlock], top[RB][kRowBlock], sum[RB][kRowBlock];
 
     Work w;
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l32 = lane & 31, h = lane >> 5;
-    if (!tree_work<kBlockRows * RB>(a, w)) return;
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l16 = lane & 15, g4 = lane >> 4;
+    if (!tree_work<kRowBlock * RB>(a, w)) return;
+    if (threadIdx.x < PB * BUFS) odd_step[threadIdx.x / BUFS][threadIdx.x % BUFS] = -1;
+    __syncthreads();
     const int G = a.n_head / a.n_kv, base = w.base, kv = w.kv;
-    const int rb = wv % RB, part = wv / RB;
-    const int row0 = w.row0 + kBlockRows * rb, row = row0 + l32, rowc = min(row, a.rows - 1), tok = rowc / G;
-    // the last position the wave's rows see
-    const int last = a.masks ? w.last : base + min(row0 + kBlockRows - 1, a.rows - 1) / G;
-    const int wsteps = RB * a.nsub, wbase = w.chunk * kUnit * a.nsub + part * wsteps * kStep;
-    const int nsteps = wbase > last || row0 >= a.rows ? 0 : min(wsteps, (last - wbase) / kStep + 1);
+    const int rb = wv % RB, part = wv / RB, tt = rb * 64 + lane;   // tt: thread within the part
+    const int row0 = w.row0 + kRowBlock * rb, row = row0 + l16, rowc = min(row, a.rows - 1), tok = rowc / G;
+    // the last position the wave's rows see (w.last: any of the workgroup's)
+    const int last = row0 >= a.rows ? -1 : a.masks ? w.last : base + min(row0 + kRowBlock - 1, a.rows - 1) / G;
+    const int psteps = kUnit * a.nsub / (kStep * PB), cbase = w.chunk * kUnit * a.nsub, pbase = cbase + part * psteps * kStep;
+    const int nsteps = min(psteps, (w.last - cbase) / kStep + 1);   // of the first part: the others run along
     uint64_t mask = 0;
     if (a.masks && row < a.rows) mask = a.masks[tok];
     const int lim = row >= a.rows ? -1 : a.masks ? base - 1 : base + tok;
 
-    half8 qh[NI][2], ql[NI][2];
-    float post;
+    const size_t kstride = KT == kKvF16 ? static_cast<size_t>(a.n_kv) * kKB : kKB;
+    const size_t vstride = VT == kKvF16 ? static_cast<size_t>(a.n_kv) * kVB : kVB;
+    const int unit = tt % NE, pos0 = tt / NE;   // of the thread's first unit; the next ones are 64 RB / NE positions further
+    const uint8_t* kp = a.kc + kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD).code + unit * (kKB / NE);
+    const uint8_t* vp = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).code + unit * (kVB / NE);
+    const uint8_t* ks = a.kc + kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD).scale + unit / 2;
+    const uint8_t* vs = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).scale + unit / 2;
+
+    Dims16<KT> kx[U];
+    Dims16<VT> vx[U];
+    uint32_t ksc[U], vsc[U];
+    auto load = [&](int sb) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (kUnits < 64 * RB && tt >= kUnits) break;
+            const size_t p = min(sb + pos0 + u * (64 * RB / NE), w.last);   // rows past the last are masked
+            kx[u] = load_k16<KT>(kp + p * kstride);
+            vx[u] = load_k16<VT>(vp + p * vstride);
+            if constexpr (KT != kKvF16) ksc[u] = ks[p * NB];
+            if constexpr (VT != kKvF16) vsc[u] = vs[p * NB];
+        }
+    };
+    uint8_t* tiles = pool + part * (BUFS * Pool::kBytes);
+    auto store = [&](int buf, int st) {
+        const bool tail = pbase + (st + 1) * kStep > base;   // uniform in the part
+        uint8_t* kt = tiles + buf * Pool::kBytes + unit * 32;
+        uint8_t* vt = kt + kStep * Pool::kKRow;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (kUnits < 64 * RB && tt >= kUnits) break;
+            const int p = pos0 + u * (64 * RB / NE);
+            half2v sk = {}, sv = {};
+            if constexpr (KT != kKvF16) sk = scale2(ksc[u], ksc[u]);
+            if constexpr (VT != kKvF16) sv = scale2(vsc[u], vsc[u]);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                *reinterpret_cast<half8*>(kt + p * Pool::kKRow + 16 * hf) = k_operand<KT>(kx[u], hf, sk);
+                u32x4 v = __builtin_bit_cast(u32x4, k_operand<VT>(vx[u], hf, sv));
+                if (tail && !(finite16(v[0]) && finite16(v[1]) && finite16(v[2]) && finite16(v[3]))) {
+                    v = u32x4{zero_odd(v[0]), zero_odd(v[1]), zero_odd(v[2]), zero_odd(v[3])};
+                    odd_step[part][buf] = st;   // every writer stores the same
+                }
+                *reinterpret_cast<u32x4*>(vt + p * Pool::kVRow + 16 * hf) = v;
+            }
+        }
+    };
+    load(pbase);
+
+    half8 qh[NC], ql[NC];
+    float post;   // score = product * post, in base 2
     {
-        const float* qr = a.q + (static_cast<size_t>(tok) * a.n_head + kv * G + (rowc - tok * G)) * HD + 16 * h;
-        float4 u[NI][4];
+        const float* qr = a.q + (static_cast<size_t>(tok) * a.n_head + kv * G + (rowc - tok * G)) * HD + 8 * g4;
+        float4 u[NC][2];
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int f = 0; f < 4; ++f) u[i][f] = reinterpret_cast<const float4*>(qr + 32 * i)[f];
+            for (int f = 0; f < 2; ++f) u[c][f] = reinterpret_cast<const float4*>(qr + 32 * c)[f];
         float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int f = 0; f < 4; ++f)
-                m = fmaxf(m, fmaxf(fmaxf(fabsf(u[i][f].x), fabsf(u[i][f].y)), fmaxf(fabsf(u[i][f].z), fabsf(u[i][f].w))));
+            for (int f = 0; f < 2; ++f)
+                m = fmaxf(m, fmaxf(fmaxf(fabsf(u[c][f].x), fabsf(u[c][f].y)), fmaxf(fabsf(u[c][f].z), fabsf(u[c][f].w))));
+        m = fmaxf(m, xor_lane<16>(m));
         m = fmaxf(m, xor_lane<32>(m));
         const int sh = q_shift(m);
         const float f = ldexpf(1.0f, sh);
         post = a.scale * 1.44269504088896340736f * ldexpf(1.0f, -sh);
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const float4 b = u[i][2 * hf], c = u[i][2 * hf + 1];
-                const float x[8] = {b.x * f, b.y * f, b.z * f, b.w * f, c.x * f, c.y * f, c.z * f, c.w * f};
-                split8(x, qh[i][hf], ql[i][hf]);
-            }
-    }
-
-    const size_t kstride = KT == kKvF16 ? static_cast<size_t>(a.n_kv) * kKB : kKB;
-    const size_t vstride = VT == kKvF16 ? static_cast<size_t>(a.n_kv) * kVB : kVB;
-    const uint8_t* kp = a.kc + kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD).code + h * (kKB / (HD / 16));
-    const uint8_t* vp = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).code + v_offset<VT, VD>(l32);
-    const uint8_t* ks = a.kc + kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD).scale;
-    const uint8_t* vs = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).scale + VD * l32 / kKvBlock;
-
-    Dims16<KT> kx[NI];
-    uint32_t ksc[2];
-    DimsV<VT, VD> vx[16];
-    uint32_t vsc[16];
-    auto load_k = [&](int sb) {
-        const size_t p = min(sb + l32, last);
-#pragma unroll
-        for (int i = 0; i < NI; ++i) kx[i] = load_k16<KT>(kp + p * kstride + i * (kKB / NI));
-        if constexpr (KT != kKvF16) {
-            if constexpr (NB == 8) {
-                const uint2 s = *reinterpret_cast<const uint2*>(ks + p * NB);
-                ksc[0] = s.x, ksc[1] = s.y;
-            } else {
-                ksc[0] = *reinterpret_cast<const uint32_t*>(ks + p * NB);
-            }
+        for (int c = 0; c < NC; ++c) {
+            const float x[8] = {u[c][0].x * f, u[c][0].y * f, u[c][0].z * f, u[c][0].w * f,
+                                u[c][1].x * f, u[c][1].y * f, u[c][1].z * f, u[c][1].w * f};
+            split8(x, qh[c], ql[c]);
         }
-    };
-    auto slot = [&](int j) { return 8 * (j >> 2) + 4 * h + (j & 3); };   // the position of score register j in its step
-    auto load_vs = [&](int sb) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const size_t p = min(sb + slot(j), last);
-            vx[j] = load_v<VT, VD>(vp + p * vstride, l32);
-            if constexpr (VT != kKvF16) vsc[j] = vs[p * NB];
-        }
-    };
-    floatx16 o[VD];
-#pragma unroll
-    for (int e = 0; e < VD; ++e)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[e][r] = 0.0f;
-    float m_run = -INFINITY, l_run = 0.0f;
-
-    if (nsteps > 0) {
-        load_k(wbase);
-        load_vs(wbase);
     }
+    floatx4 o[NE];
+#pragma unroll
+    for (int e = 0; e < NE; ++e) o[e] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m_run = -INFINITY, l_run = 0.0f;   // l_run: this lane's positions only
+
+    store(0, 0);
+    __syncthreads();
     for (int st = 0; st < nsteps; ++st) {
-        const int sb = wbase + st * kStep;
-        floatx16 sc;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            half2v s = {};
-            if constexpr (KT != kKvF16) {   // block i
-                const uint32_t b = (ksc[i >> 2] >> (8 * (i & 3))) & 0xffu;
-                s = scale2(b, b);
-            }
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const half8 kk = k_operand<KT>(kx[i], hf, s);
-                sc = mfma(kk, qh[i][hf], sc);
-                sc = mfma(kk, ql[i][hf], sc);
-            }
-        }
+        const int sb = pbase + st * kStep, buf = BUFS == 2 ? st & 1 : 0;
         const bool more = st + 1 < nsteps;
-        if (more) load_k(sb + kStep);
-        const bool tail = sb + kStep > base;   // uniform
-        uint32_t seen = 0xffffu;
+        if (more) load(sb + kStep);
+        if (sb <= last) {   // uniform in the wave
+            const uint8_t* kt = tiles + buf * Pool::kBytes + l16 * Pool::kKRow + 16 * g4;
+            float sc[8];   // j: position sb + 4 g4 + j, or 16 + 4 g4 + j - 4 further
+            floatx4 dh[2], dl[2];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sc[j] *= post;
-        if (tail || row >= a.rows) {
-            seen = 0;
+            for (int t = 0; t < 2; ++t) {
+                dh[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                dl[t] = dh[t];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                if (sees(sb + slot(j), lim, mask, base, a.ntok)) seen |= 1u << j;
-                else sc[j] = -INFINITY;
+                for (int c = 0; c < NC; ++c) {
+                    const half8 kk = *reinterpret_cast<const half8*>(kt + 16 * t * Pool::kKRow + 64 * c);
+                    dh[t] = mfma(kk, qh[c], dh[t]);
+                    dl[t] = mfma(kk, ql[c], dl[t]);
+                }
             }
-        }
-        float mloc = sc[0];
+            interleave<2 * NC, 1, 2, 4>();
 #pragma unroll
-        for (int j = 1; j < 16; ++j) mloc = fmaxf(mloc, sc[j]);
-        mloc = fmaxf(mloc, xor_lane<32>(mloc));
-        const float m_new = mloc > m_run + kLazy ? mloc : m_run;
-        const float m_ref = m_new == -INFINITY ? 0.0f : m_new;
-        const float alpha = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_ref);
-        float p[16], lsum = 0.0f;
+            for (int j = 0; j < 8; ++j) sc[j] = (dh[j >> 2][j & 3] + dl[j >> 2][j & 3]) * post;
+            const bool tail = sb + kStep > base;   // uniform: the step reaches into the draft
+            uint32_t seen = 0xffu;
+            if (tail || row >= a.rows) {
+                seen = 0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(sc[j] - m_ref + kPScale);
-            lsum += p[j];
-        }
-        l_run = l_run * alpha + lsum;
-        m_run = m_new;
-        if (__ballot(alpha != 1.0f)) {
-            float al[16];
+                for (int j = 0; j < 8; ++j) {
+                    if (sees(sb + 4 * g4 + (j < 4 ? j : 12 + j), lim, mask, base, a.ntok)) seen |= 1u << j;
+                    else sc[j] = -INFINITY;
+                }
+            }
+            float mloc = sc[0];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) al[r] = __shfl(alpha, slot(r), 64);
-#pragma unroll
-            for (int e = 0; e < VD; ++e)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[e][r] *= al[r];
-        }
-        half8 ph[2], pl[2];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const float x[8] = {p[8 * m], p[8 * m + 1], p[8 * m + 2], p[8 * m + 3], p[8 * m + 4], p[8 * m + 5], p[8 * m + 6], p[8 * m + 7]};
-            split8(x, ph[m], pl[m]);
-        }
-        half2v vsp[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if constexpr (VT != kKvF16) vsp[j] = scale2(vsc[2 * j], vsc[2 * j + 1]);
-            else vsp[j] = half2v{};
-        }
-        if (tail) {
-            bool odd = false;
+            for (int j = 1; j < 8; ++j) mloc = fmaxf(mloc, sc[j]);
+            mloc = fmaxf(mloc, xor_lane<16>(mloc));
+            mloc = fmaxf(mloc, xor_lane<32>(mloc));
+            const float m_new = mloc > m_run + kLazy ? mloc : m_run;
+            const float m_ref = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: exp2(-inf) = 0, no NaN
+            const float alpha = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_ref);
+            float p[8], lsum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if constexpr (VT != kKvF16) {
-                    odd = odd || !finite16(u2(vsp[j]));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < VD / 2; ++e) odd = odd || !finite16(vx[2 * j].w[e]) || !finite16(vx[2 * j + 1].w[e]);
-                }
+                p[j] = __builtin_amdgcn_exp2f(sc[j] - m_ref + kPScale);
+                lsum += p[j];
             }
-            if (__ballot(odd)) {
-                float(*pw)[kStep] = reinterpret_cast<float(*)[kStep]>(&slab[wv][0][0]);   // [row][position], -1: not seen
+            l_run = l_run * alpha + lsum;
+            m_run = m_new;
+            if (__ballot(alpha != 1.0f)) {   // uniform: some row's maximum moved
+                float al[4];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) pw[l32][slot(j)] = seen >> j & 1 ? p[j] : -1.0f;
+                for (int r = 0; r < 4; ++r) al[r] = __shfl(alpha, 4 * g4 + r, 64);
+#pragma unroll
+                for (int e = 0; e < NE; ++e)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[e][r] *= al[r];
+            }
+            half8 ph, pl;
+            split8(p, ph, pl);
+            // the lane's address of the transposed reads: position 4 g4 + l16 / 4, dims 4 (l16 % 4) ..
+            const uint8_t* vr = tiles + buf * Pool::kBytes + kStep * Pool::kKRow + (4 * g4 + (l16 >> 2)) * Pool::kVRow + 8 * (l16 & 3);
+            auto column = [&](int e) {   // dims 16 e + l16 of the lane's eight positions
+                const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*) (vr + 32 * e));
+                const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*) (vr + 16 * Pool::kVRow + 32 * e));
+                const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
+                return h8(x.x, x.y, y.x, y.y);
+            };
+            if (tail && odd_step[part][buf] == st) {   // uniform: some V is not finite (zero in the tile)
+                float(*pw)[kStep] = pb[wv];   // [row][position], -1: not seen
+#pragma unroll
+                for (int j = 0; j < 8; ++j) pw[l16][4 * g4 + (j < 4 ? j : 12 + j)] = seen >> j & 1 ? p[j] : -1.0f;
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 for (int pp = 0; pp < kStep; ++pp) {
-                    const size_t p1 = min(sb + pp, last);
+                    float x[4];
 #pragma unroll
-                    for (int e = 0; e < VD; ++e) {
+                    for (int r = 0; r < 4; ++r) x[r] = pw[4 * g4 + r][pp];
+                    const KvRow<VT> vrow = kv_row<VT>(min(sb + pp, w.last), kv, a.n_kv, a.max_ctx, HD);
+#pragma unroll
+                    for (int e = 0; e < NE; ++e) {
+                        const int d = 16 * e + l16;
                         float v;
-                        if constexpr (VT == kKvF16) v = half_bits_to_float(reinterpret_cast<const uint16_t*>(vp + p1 * vstride)[e]);
-                        else v = kv_scale_value(vs[p1 * NB]);
+                        if constexpr (VT == kKvF16) v = half_bits_to_float(reinterpret_cast<const uint16_t*>(a.vc + vrow.code)[d]);
+                        else v = kv_scale_value(a.vc[vrow.scale + d / kKvBlock]);   // NaN: every value of the block
                         if (fabsf(v) <= FLT_MAX) continue;
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const float x = pw[slot(r)][pp];
-                            if (!(x < 0.0f)) o[e][r] = __builtin_fmaf(x, v, o[e][r]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    if constexpr (VT == kKvF16) {
-#pragma unroll
-                        for (int e = 0; e < VD / 2; ++e) vx[j].w[e] = zero_odd(vx[j].w[e]);
-                    } else if ((j & 1) == 0) {
-                        vsp[j >> 1] = h2(zero_odd(u2(vsp[j >> 1])));
+                        for (int r = 0; r < 4; ++r)
+                            if (!(x[r] < 0.0f)) o[e][r] = __builtin_fmaf(x[r], v, o[e][r]);
                     }
                 }
             }
+#pragma unroll
+            for (int e = 0; e < NE; e += 2) {
+                const half8 v0 = column(e), v1 = column(e + 1);
+                o[e] = mfma(ph, v0, o[e]);
+                o[e + 1] = mfma(ph, v1, o[e + 1]);
+                o[e] = mfma(pl, v0, o[e]);
+                o[e + 1] = mfma(pl, v1, o[e + 1]);
+            }
+            interleave<NE / 2, 4, 4, 2>();
         }
-#pragma unroll
-        for (int e = 0; e < VD / 2; ++e)
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                uint32_t ev[4], od[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v_pair<VT, VD>(vx[8 * m + 2 * j], vx[8 * m + 2 * j + 1], e, vsp[4 * m + j], ev[j], od[j]);
-                const half8 b0 = h8(ev[0], ev[1], ev[2], ev[3]), b1 = h8(od[0], od[1], od[2], od[3]);
-                o[2 * e] = mfma(ph[m], b0, o[2 * e]);
-                o[2 * e + 1] = mfma(ph[m], b1, o[2 * e + 1]);
-                o[2 * e] = mfma(pl[m], b0, o[2 * e]);
-                o[2 * e + 1] = mfma(pl[m], b1, o[2 * e + 1]);
-            }
-        if (more) load_vs(sb + kStep);
+        if (BUFS == 1) __syncthreads();   // the tile is read
+        if (more) store(BUFS == 2 ? buf ^ 1 : 0, st + 1);
+        __syncthreads();
     }
 
+    l_run += xor_lane<16>(l_run);
     l_run += xor_lane<32>(l_run);
-    if (h == 0) {
-        stat[wv][0][l32] = m_run;
-        stat[wv][1][l32] = l_run;
+    if (g4 == 0) {
+        stat[wv][0][l16] = m_run;
+        stat[wv][1][l16] = l_run;
     }
     __syncthreads();
-    join_stats<RB, kBlockRows>(stat, fac, top, sum);
+    join_stats<kTileWaves, RB, kRowBlock>(stat, fac, top, sum);
+    auto& slab = *reinterpret_cast<float(*)[kTileWaves][kOct][HD]>(pool);
 #pragma unroll
-    for (int oct = 0; oct < kBlockRows / kOct; ++oct) {
+    for (int oct = 0; oct < kRowBlock / kOct; ++oct) {
+        if ((g4 >> 1) == oct) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int e = 0; e < VD; e += 4)
-                *reinterpret_cast<float4*>(&slab[wv][4 * h + r][VD * l32 + e]) =
-                    make_float4(o[e][4 * oct + r], o[e + 1][4 * oct + r], o[e + 2][4 * oct + r], o[e + 3][4 * oct + r]);
+                for (int e = 0; e < NE; ++e) slab[wv][4 * (g4 & 1) + r][16 * e + l16] = o[e][r];
+        }
         __syncthreads();
-        join_rows<HD, RB, kBlockRows>(a, w, slab, fac, top, sum, oct);
+        join_rows<HD, kTileWaves, RB, kRowBlock>(a, w, slab, fac, top, sum, oct);
         __syncthreads();
     }
 }
@@ -850,12 +878,81 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeArgs a) {
     if (a.q8) q8_1_store_lane(v, a.q8 + static_cast<size_t>(t) * a.q8_stride + (h * (HD / 32) + d / 32) * kQ8_1Bytes);
 }
 
+// The same for a few chunks, where the work is a pass over the records: HD / 4 lanes a row, four dims a lane, no LDS.
+constexpr int kFlatChunks = 8;
+
+template <int HD>
+__global__ __launch_bounds__(kThreads) void tree_merge_flat_kernel(TreeArgs a) {
+    constexpr int L4 = HD / 4;
+    const int i = blockIdx.x * (kThreads / L4) + static_cast<int>(threadIdx.x) / L4, d = 4 * (static_cast<int>(threadIdx.x) % L4);
+    if (i >= a.ntok * a.n_head) return;
+    const int t = i / a.n_head, h = i - t * a.n_head;
+    const int G = a.n_head / a.n_kv, kv = h / G, row = t * G + (h - kv * G);
+    float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (a.gate) {   // 4-byte aligned
+        const float* p = a.gate + static_cast<size_t>(t) * a.gate_stride + h * 2 * HD + HD + d;
+        g = make_float4(p[0], p[1], p[2], p[3]);
+    }
+    const int base = a.pos[0];
+    if (base < 0 || base > a.max_ctx - a.ntok) return;   // uniform: a slot outside the cache
+    const int nchunk = (base + (a.masks ? a.ntok - 1 : t)) / (kUnit * a.nsub) + 1;
+    const size_t cstride = static_cast<size_t>(a.n_kv) * a.rows_pad, r0 = static_cast<size_t>(kv) * a.rows_pad + row;
+    const float2* ml = reinterpret_cast<const float2*>(a.wml) + r0;
+    const float* ro = a.wo + r0 * HD + d;
+    float m = -INFINITY, l = 0.0f;
+    for (int c = 0; c < nchunk; ++c) m = fmaxf(m, ml[c * cstride].x);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < nchunk; ++c) {
+        const float2 x = ml[c * cstride];
+        const float4 v = *reinterpret_cast<const float4*>(ro + c * cstride * HD);
+        const float w = __builtin_amdgcn_exp2f(x.x - ref);
+        l = __builtin_fmaf(x.y, w, l);
+        o[0] = __builtin_fmaf(w, v.x, o[0]);
+        o[1] = __builtin_fmaf(w, v.y, o[1]);
+        o[2] = __builtin_fmaf(w, v.z, o[2]);
+        o[3] = __builtin_fmaf(w, v.w, o[3]);
+    }
+    const float gs[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        o[k] = m == -INFINITY ? 0.0f : o[k] / l;
+        if (a.gate) o[k] *= 1.0f / (1.0f + expf(-gs[k]));
+    }
+    if (a.y) {
+        float* y = a.y + static_cast<size_t>(t) * a.y_stride + h * HD + d;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = o[k];
+    }
+    if (a.q8) {   // q8_1_store_lane's block and bits: its lane's element is 4 (lane % 8) + k here
+        float amax = fmaxf(fmaxf(fabsf(o[0]), fabsf(o[1])), fmaxf(fabsf(o[2]), fabsf(o[3])));
+        amax = fmaxf(amax, xor_lane<4>(amax));
+        amax = fmaxf(amax, xor_lane<2>(amax));
+        amax = fmaxf(amax, xor_lane<1>(amax));
+        float s[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            s[k] = o[k] + xor_lane<4>(o[k]);
+            s[k] += xor_lane<2>(s[k]);
+            s[k] += xor_lane<1>(s[k]);
+        }
+        const float total = (s[0] + s[2]) + (s[1] + s[3]), dq = amax / 127.0f;
+        uint32_t w = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            w |= (static_cast<uint32_t>(amax == 0.0f ? 0 : static_cast<int>(roundf(o[k] / dq))) & 0xffu) << (8 * k);
+        uint8_t* block = a.q8 + static_cast<size_t>(t) * a.q8_stride + (h * (HD / 32) + d / 32) * kQ8_1Bytes;
+        *reinterpret_cast<uint32_t*>(block + 4 + (d & 31)) = w;
+        if ((d & 31) == 0) *reinterpret_cast<uint32_t*>(block) = float_to_half_sat(dq) | (float_to_half_sat(total) << 16);
+    }
+}
+
 bool tree_shape_ok(int max_ctx, int n_head, int n_kv, int head_dim, int ntok) {
     return kv_shape_ok(max_ctx, n_kv, head_dim) && n_head > 0 && n_head <= 65535 && n_head % n_kv == 0 && n_head / n_kv <= 64 &&
            ntok >= 1 && ntok <= kMaxChain;
 }
 
-// the form of a call: query rows per KV head, row blocks side by side in a workgroup (0: the 16 x 16 form), rows a
+// the form of a call: query rows per KV head, 16-row blocks side by side in a workgroup (0: the form of few rows), rows a
 // workgroup holds, workgroups per (chunk, KV head)
 struct Form {
     int rows, rb, held, groups;
@@ -863,8 +960,8 @@ struct Form {
 Form tree_form(int n_head, int n_kv, int ntok) {
     Form f;
     f.rows = ntok * (n_head / n_kv);
-    f.rb = f.rows <= kFewRows ? 0 : f.rows <= kBlockRows ? 1 : f.rows <= 2 * kBlockRows ? 2 : 4;
-    f.held = f.rb ? kBlockRows * f.rb : kFewRows;
+    f.rb = f.rows <= kFewRows ? 0 : f.rows <= 32 ? 2 : f.rows <= 64 ? 4 : 8;
+    f.held = f.rb ? kRowBlock * f.rb : kFewRows;
     f.groups = (f.rows + f.held - 1) / f.held;
     return f;
 }
@@ -875,11 +972,11 @@ long long tree_chunks(int max_ctx, int nsub) {
 
 template <int KT, int VT, int HD>
 void launch_partial(const TreeArgs& a, int rb, unsigned blocks, hipStream_t s) {
-    auto go = [&](auto* kernel) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, s, a); };
-    if (rb == 0) go(&tree_few_kernel<KT, VT, HD>);
-    else if (rb == 1) go(&tree_rows_kernel<KT, VT, HD, 1>);
-    else if (rb == 2) go(&tree_rows_kernel<KT, VT, HD, 2>);
-    else go(&tree_rows_kernel<KT, VT, HD, 4>);
+    auto go = [&](auto* kernel, int threads) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, s, a); };
+    if (rb == 0) go(&tree_few_kernel<KT, VT, HD>, kThreads);
+    else if (rb == 2) go(&tree_tile_kernel<KT, VT, HD, 2>, kTileThreads);
+    else if (rb == 4) go(&tree_tile_kernel<KT, VT, HD, 4>, kTileThreads);
+    else go(&tree_tile_kernel<KT, VT, HD, 8>, kTileThreads);
 }
 
 template <int HD>
@@ -888,7 +985,10 @@ void launch_tree(const TreeArgs& a, int ktype, int vtype, int rb, unsigned block
     else if (ktype == kKvI4) launch_partial<kKvI4, kKvI4, HD>(a, rb, blocks, s);
     else if (vtype == kKvI8) launch_partial<kKvI8, kKvI8, HD>(a, rb, blocks, s);
     else launch_partial<kKvI8, kKvI4, HD>(a, rb, blocks, s);
-    if (!a.direct) hipLaunchKernelGGL((tree_merge_kernel<HD>), dim3(a.ntok, a.n_head, HD / kMergeDims), dim3(kThreads), 0, s, a);
+    if (a.npairs / a.n_kv > kFlatChunks)
+        hipLaunchKernelGGL((tree_merge_kernel<HD>), dim3(a.ntok, a.n_head, HD / kMergeDims), dim3(kThreads), 0, s, a);
+    else if (!a.direct)
+        hipLaunchKernelGGL((tree_merge_flat_kernel<HD>), dim3((a.ntok * a.n_head + 1024 / HD - 1) / (1024 / HD)), dim3(kThreads), 0, s, a);
 }
 
 }  // namespace
