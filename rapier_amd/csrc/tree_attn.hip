@@ -59,105 +59,117 @@ __device__ __forceinline__ half8 h8(uint32_t a, uint32_t b, uint32_t c, uint32_t
     return __builtin_bit_cast(half8, u32x4{a, b, c, d});
 }
 
-constexpr uint32_t kMagic = 0x64646464u;   // high byte of the fp16 numbers 1024 + 0..255
-__device__ __forceinline__ half2v bias2(int type) {
-    const _Float16 b = static_cast<_Float16>(1024 + kv_bias(type));
-    return half2v{b, b};
-}
-// two scales (bytes 0 and 1 of w, spread to the halves) as fp16
-__device__ __forceinline__ half2v scale2(uint32_t lo, uint32_t hi) { return h2((lo << 7) | (hi << 23)); }
+// Codes become fp16 by one fused multiply-add a pair: the code is put into the mantissa of a power of two (I8: 1024 + u,
+// I4: 64 + u), and fma(x, s / 16, -bias s / 16) is code * s / 16 exactly (u is code + 128 or code + 8; a sixteenth keeps the
+// addend an fp16 number up to the largest scale, and every value above fp16's smallest step).  The sixteenths come out of
+// the scores' factor and the joined rows' weights.
+template <int T>
+constexpr float kSixteen = T == kKvF16 ? 1.0f : 16.0f;
 
-// 16 neighbouring dims of one position's K
+struct Scale2 {
+    half2v s, c;
+};
+// the scales of a pair's two values, from their scale bytes (I8 and I4)
+template <int T>
+__device__ __forceinline__ Scale2 scale2(uint32_t lo, uint32_t hi) {
+    constexpr _Float16 kBias = static_cast<_Float16>(T == kKvI8 ? -1152.0f : -72.0f), kPart = static_cast<_Float16>(0.0625f);
+    Scale2 r;
+    r.s = h2((lo << 7) | (hi << 23)) * half2v{kPart, kPart};
+    r.c = r.s * half2v{kBias, kBias};
+    return r;
+}
+__device__ __forceinline__ uint32_t fma2(uint32_t x, const Scale2& s) { return u2(__builtin_elementwise_fma(h2(x), s.s, s.c)); }
+
+// (w & mask) | magic in one instruction: with both as literals the compiler takes two
+__device__ __forceinline__ uint32_t nibbles(uint32_t w) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(0x00f000f0u), "v"(0x54005400u));
+    return r;
+}
+// pair k of a word of eight I4 codes, at bits 4..7 of both halves
+__device__ __forceinline__ uint32_t nibble_pair(uint32_t w, int k) { return nibbles(k == 0 ? w << 4 : w >> (4 * (k - 1))); }
+constexpr uint32_t kMagic8 = 0x64646464u;   // high byte of the fp16 numbers 1024 + 0..255
+
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+// `rows` rows from p as a buffer: a row past them reads as zeros, so a step past the last position loads nothing
+__device__ __forceinline__ Rsrc rows_buffer(const uint8_t* p, int rows, size_t stride) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, static_cast<int>(max(rows, 0) * stride), 0x00027000);
+}
+
+// 16 neighbouring dims of a position
 template <int T>
 struct Dims16 {
     uint32_t w[T == kKvF16 ? 8 : T == kKvI8 ? 4 : 2];
 };
 template <int T>
-__device__ __forceinline__ Dims16<T> load_k16(const uint8_t* p) {
+__device__ __forceinline__ Dims16<T> load16(Rsrc r, int lane_at, int at) {
     Dims16<T> x;
     if constexpr (T == kKvI4) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        x.w[0] = v.x, x.w[1] = v.y;
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, lane_at, at, 0);
+        x.w[0] = v[0], x.w[1] = v[1];
     } else {
 #pragma unroll
         for (int i = 0; i < (T == kKvF16 ? 2 : 1); ++i) {
-            const uint4 v = reinterpret_cast<const uint4*>(p)[i];
-            x.w[4 * i] = v.x, x.w[4 * i + 1] = v.y, x.w[4 * i + 2] = v.z, x.w[4 * i + 3] = v.w;
+            const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, lane_at + 16 * i, at, 0);
+            x.w[4 * i] = v[0], x.w[4 * i + 1] = v[1], x.w[4 * i + 2] = v[2], x.w[4 * i + 3] = v[3];
         }
     }
     return x;
 }
 // dims 8 hf + 0..7 of them as an MFMA operand
 template <int T>
-__device__ __forceinline__ half8 k_operand(const Dims16<T>& x, int hf, half2v s) {
+__device__ __forceinline__ half8 operand(const Dims16<T>& x, int hf, const Scale2& s) {
     if constexpr (T == kKvF16) {
         return h8(x.w[4 * hf], x.w[4 * hf + 1], x.w[4 * hf + 2], x.w[4 * hf + 3]);
-    } else if constexpr (T == kKvI8) {
-        uint32_t r[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t c = perm(kMagic, x.w[2 * hf + (i >> 1)], i & 1 ? 0x04030402u : 0x04010400u);
-            r[i] = u2((h2(c) - bias2(T)) * s);
-        }
-        return h8(r[0], r[1], r[2], r[3]);
     } else {
         uint32_t r[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t c = ((x.w[hf] >> (4 * i)) & 0x000f000fu) | 0x64006400u;
-            r[i] = u2((h2(c) - bias2(T)) * s);
+            if constexpr (T == kKvI8) r[i] = fma2(perm(kMagic8, x.w[2 * hf + (i >> 1)], i & 1 ? 0x04030402u : 0x04010400u), s);
+            else r[i] = fma2(nibble_pair(x.w[hf], i), s);
         }
         return h8(r[0], r[1], r[2], r[3]);
     }
 }
 
-// VD neighbouring dims of one position's V (I4 at VD = 4: half the dims of a word, brought down to the bits of the first)
+// VD neighbouring dims of a position
 template <int T, int VD>
 struct DimsV {
     static constexpr int kBytes = T == kKvF16 ? 2 * VD : T == kKvI8 ? VD : VD / 2;
-    uint32_t w[kBytes <= 4 ? 1 : kBytes / 4];
+    uint32_t w[kBytes / 4];
 };
-// the lane's first byte in a row (lane index n)
 template <int T, int VD>
-__device__ __forceinline__ int v_offset(int n) {
-    constexpr int kB = DimsV<T, VD>::kBytes;
-    return kB == 2 ? 4 * (n >> 1) : kB * n;
-}
-template <int T, int VD>
-__device__ __forceinline__ DimsV<T, VD> load_v(const uint8_t* p, int n) {
+__device__ __forceinline__ DimsV<T, VD> load_dims(Rsrc r, int lane_at, int at) {
     DimsV<T, VD> x;
     constexpr int kB = DimsV<T, VD>::kBytes;
     if constexpr (kB >= 16) {
 #pragma unroll
         for (int i = 0; i < kB / 16; ++i) {
-            const uint4 v = reinterpret_cast<const uint4*>(p)[i];
-            x.w[4 * i] = v.x, x.w[4 * i + 1] = v.y, x.w[4 * i + 2] = v.z, x.w[4 * i + 3] = v.w;
+            const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, lane_at + 16 * i, at, 0);
+            x.w[4 * i] = v[0], x.w[4 * i + 1] = v[1], x.w[4 * i + 2] = v[2], x.w[4 * i + 3] = v[3];
         }
     } else if constexpr (kB == 8) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        x.w[0] = v.x, x.w[1] = v.y;
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, lane_at, at, 0);
+        x.w[0] = v[0], x.w[1] = v[1];
     } else {
-        x.w[0] = *reinterpret_cast<const uint32_t*>(p);
-        if constexpr (kB == 2) x.w[0] >>= 8 * (n & 1);
+        x.w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane_at, at, 0);
     }
     return x;
 }
-// dims 2 e and 2 e + 1 of two positions a, b as halves (a, b), scaled by s = (scale of a, scale of b)
+// dims 2 e and 2 e + 1 of two positions a, b as halves (a, b), scaled by s = the scales of a and b
 template <int T, int VD>
-__device__ __forceinline__ void v_pair(const DimsV<T, VD>& a, const DimsV<T, VD>& b, int e, half2v s, uint32_t& even, uint32_t& odd) {
+__device__ __forceinline__ void v_pair(const DimsV<T, VD>& a, const DimsV<T, VD>& b, int e, const Scale2& s, uint32_t& even, uint32_t& odd) {
     if constexpr (T == kKvF16) {
         even = perm(b.w[e], a.w[e], 0x05040100u);
         odd = perm(b.w[e], a.w[e], 0x07060302u);
     } else if constexpr (T == kKvI8) {
         const uint32_t m = perm(b.w[e >> 1], a.w[e >> 1], e & 1 ? 0x07030602u : 0x05010400u);   // a0 b0 a1 b1
-        even = u2((h2(perm(kMagic, m, 0x04010400u)) - bias2(T)) * s);
-        odd = u2((h2(perm(kMagic, m, 0x04030402u)) - bias2(T)) * s);
+        even = fma2(perm(kMagic8, m, 0x04010400u), s);
+        odd = fma2(perm(kMagic8, m, 0x04030402u), s);
     } else {
         // even dims are in a word's low half, odd ones in the high half
-        const uint32_t lo = perm(b.w[e >> 2], a.w[e >> 2], 0x05040100u), hi = perm(b.w[e >> 2], a.w[e >> 2], 0x07060302u);
-        const int k = 4 * (e & 3);
-        even = u2((h2(((lo >> k) & 0x000f000fu) | 0x64006400u) - bias2(T)) * s);
-        odd = u2((h2(((hi >> k) & 0x000f000fu) | 0x64006400u) - bias2(T)) * s);
+        even = fma2(nibble_pair(perm(b.w[e >> 2], a.w[e >> 2], 0x05040100u), e & 3), s);
+        odd = fma2(nibble_pair(perm(b.w[e >> 2], a.w[e >> 2], 0x07060302u), e & 3), s);
     }
 }
 
@@ -194,7 +206,7 @@ struct Work {
     int chunk, kv, row0, base, last;   // row0: its first row, last: the last position any of its rows sees
 };
 template <int ROWS>
-__device__ __forceinline__ bool tree_work(const TreeArgs& a, Work& w) {
+__device__ __forceinline__ bool tree_share(const TreeArgs& a, Work& w) {
     // the groups of a (chunk, head) pair are consecutive workgroups of one XCD (workgroups go to the XCDs round robin),
     // so the pair's rows come from HBM once
     const int k8 = static_cast<int>(blockIdx.x >> 3), q8 = k8 / a.groups;
@@ -203,6 +215,10 @@ __device__ __forceinline__ bool tree_work(const TreeArgs& a, Work& w) {
     w.chunk = pair / a.n_kv;
     w.kv = pair - w.chunk * a.n_kv;
     w.row0 = ROWS * (k8 - q8 * a.groups);
+    return true;
+}
+template <int ROWS>
+__device__ __forceinline__ bool tree_reach(const TreeArgs& a, Work& w) {
     w.base = a.pos[0];
     if (w.base < 0 || w.base > a.max_ctx - a.ntok) return false;   // a slot outside the cache
     const int G = a.n_head / a.n_kv;
@@ -215,6 +231,49 @@ __device__ __forceinline__ bool sees(int p, int lim, uint64_t mask, int base, in
     return p <= lim || (mask && p >= base && p - base < ntok && ((mask >> (p - base)) & 1));
 }
 
+// Four dims of a row's result from its joined sums (m the maximum, -inf: nothing seen): gate, fp32, Q8_1.  The lanes of a
+// row's 32-dim block are eight neighbours.
+template <int HD>
+__device__ __forceinline__ void finish4(const TreeArgs& a, int t, int h, int d, float (&o)[4], float m, float l, const float (&gate)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        o[k] = m == -INFINITY ? 0.0f : o[k] / l;
+        if (a.gate) o[k] *= 1.0f / (1.0f + expf(-gate[k]));
+    }
+    if (a.y) {   // 4-byte aligned
+        float* y = a.y + static_cast<size_t>(t) * a.y_stride + h * HD + d;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = o[k];
+    }
+    if (a.q8) {   // q8_1_store_lane's block and bits: its lane's element is 4 (lane % 8) + k here
+        float amax = fmaxf(fmaxf(fabsf(o[0]), fabsf(o[1])), fmaxf(fabsf(o[2]), fabsf(o[3])));
+        amax = fmaxf(amax, xor_lane<4>(amax));
+        amax = fmaxf(amax, xor_lane<2>(amax));
+        amax = fmaxf(amax, xor_lane<1>(amax));
+        float s[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            s[k] = o[k] + xor_lane<4>(o[k]);
+            s[k] += xor_lane<2>(s[k]);
+            s[k] += xor_lane<1>(s[k]);
+        }
+        const float total = (s[0] + s[2]) + (s[1] + s[3]), dq = amax / 127.0f;
+        uint32_t w = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            w |= (static_cast<uint32_t>(amax == 0.0f ? 0 : static_cast<int>(roundf(o[k] / dq))) & 0xffu) << (8 * k);
+        uint8_t* block = a.q8 + static_cast<size_t>(t) * a.q8_stride + (h * (HD / 32) + d / 32) * kQ8_1Bytes;
+        *reinterpret_cast<uint32_t*>(block + 4 + (d & 31)) = w;
+        if ((d & 31) == 0) *reinterpret_cast<uint32_t*>(block) = float_to_half_sat(dq) | (float_to_half_sat(total) << 16);
+    }
+}
+template <int HD>
+__device__ __forceinline__ void load_gate(const TreeArgs& a, int t, int h, int d, float (&g)[4]) {
+    const float* p = a.gate ? a.gate + static_cast<size_t>(t) * a.gate_stride + h * 2 * HD + HD + d : nullptr;   // 4-byte aligned
+#pragma unroll
+    for (int k = 0; k < 4; ++k) g[k] = p ? p[k] : 0.0f;
+}
+
 // Joins the waves' parts of 8 * RB rows (rows 8 oct .. of each of RB row blocks) from their LDS slabs [wave][8][HD] and
 // either writes records or, for a call of one chunk, the result: fac[wave][row of the block] is a part's weight, sum[row]
 // the joined l.  Wave w holds part w / RB of row block w % RB.
@@ -224,30 +283,36 @@ __device__ __forceinline__ void join_rows(const TreeArgs& a, const Work& w, cons
                                           const float (&sum)[RB][BLOCK], int oct) {
     constexpr int PB = WAVES / RB;
     const int G = a.n_head / a.n_kv;
+    for (int i = 4 * static_cast<int>(threadIdx.x); i < RB * kOct * HD; i += 4 * 64 * WAVES) {
+        const int d = i % HD, r8 = i / HD, rb = r8 / kOct, rr = r8 % kOct, rk = kOct * oct + rr, row = w.row0 + BLOCK * rb + rk;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < RB * kOct * HD / (64 * WAVES); ++i) {
-        const int e = static_cast<int>(threadIdx.x) + 64 * WAVES * i, d = e % HD, r8 = e / HD;   // r8: uniform in a wave
-        const int rb = r8 / kOct, rr = r8 % kOct, rk = kOct * oct + rr, row = w.row0 + BLOCK * rb + rk;
-        float v = slab[rb][rr][d] * fac[rb][rk];
-#pragma unroll
-        for (int p = 1; p < PB; ++p) v = __builtin_fmaf(slab[rb + RB * p][rr][d], fac[rb + RB * p][rk], v);
-        if (row < a.rows && !a.direct) {
-            const size_t rec = (static_cast<size_t>(w.chunk) * a.n_kv + w.kv) * a.rows_pad + row;
-            a.wo[rec * HD + d] = v;
-            if (d == 0) *reinterpret_cast<float2*>(a.wml + 2 * rec) = make_float2(top[rb][rk], sum[rb][rk]);
-        } else if (row < a.rows) {
+        for (int p = 0; p < PB; ++p) {
+            const float4 x = *reinterpret_cast<const float4*>(&slab[rb + RB * p][rr][d]);
+            const float f = fac[rb + RB * p][rk];
+            v[0] = __builtin_fmaf(x.x, f, v[0]);
+            v[1] = __builtin_fmaf(x.y, f, v[1]);
+            v[2] = __builtin_fmaf(x.z, f, v[2]);
+            v[3] = __builtin_fmaf(x.w, f, v[3]);
+        }
+        if (row >= a.rows) continue;
+        if (a.direct) {
             const int t = row / G, h = w.kv * G + row - t * G;
-            v = top[rb][rk] == -INFINITY ? 0.0f : v / sum[rb][rk];
-            if (a.gate) v *= 1.0f / (1.0f + expf(-a.gate[static_cast<size_t>(t) * a.gate_stride + h * 2 * HD + HD + d]));
-            if (a.y) a.y[static_cast<size_t>(t) * a.y_stride + h * HD + d] = v;
-            if (a.q8) q8_1_store_lane(v, a.q8 + static_cast<size_t>(t) * a.q8_stride + (h * (HD / 32) + d / 32) * kQ8_1Bytes);
+            float g[4];
+            load_gate<HD>(a, t, h, d, g);
+            finish4<HD>(a, t, h, d, v, top[rb][rk], sum[rb][rk], g);
+        } else {
+            const size_t rec = (static_cast<size_t>(w.chunk) * a.n_kv + w.kv) * a.rows_pad + row;
+            *reinterpret_cast<float4*>(a.wo + rec * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
+            if (d == 0) *reinterpret_cast<float2*>(a.wml + 2 * rec) = make_float2(top[rb][rk], sum[rb][rk]);
         }
     }
 }
 
 // the parts' weights and the joined sum of every row, from stat[wave][m, l][row of the block]
+// (times `unit`, what the parts' o is short of)
 template <int WAVES, int RB, int BLOCK>
-__device__ __forceinline__ void join_stats(const float (&stat)[WAVES][2][BLOCK], float (&fac)[WAVES][BLOCK], float (&top)[RB][BLOCK],
+__device__ __forceinline__ void join_stats(float unit, const float (&stat)[WAVES][2][BLOCK], float (&fac)[WAVES][BLOCK], float (&top)[RB][BLOCK],
                                            float (&sum)[RB][BLOCK]) {
     constexpr int PB = WAVES / RB;
     const int i = threadIdx.x;
@@ -261,7 +326,7 @@ __device__ __forceinline__ void join_stats(const float (&stat)[WAVES][2][BLOCK],
 #pragma unroll
     for (int p = 0; p < PB; ++p) {
         const float f = __builtin_amdgcn_exp2f(stat[rb + RB * p][0][r] - ref);
-        fac[rb + RB * p][r] = f;
+        fac[rb + RB * p][r] = f * unit;
         l = __builtin_fmaf(stat[rb + RB * p][1][r], f, l);
     }
     top[rb][r] = m;
@@ -288,11 +353,12 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
     __shared__ float stat[kWaves][2][kFewRows], fac[kWaves][kFewRows], top[1][kFewRows], sum[1][kFewRows];
 
     Work w;
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l16 = lane & 15, g4 = lane >> 4;
-    if (!tree_work<kFewRows>(a, w)) return;
-    const int G = a.n_head / a.n_kv, base = w.base, last = w.last, kv = w.kv;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
+    if (!tree_share<kFewRows>(a, w)) return;
+    const int G = a.n_head / a.n_kv, kv = w.kv;
     const int row = l16 & 7, rowc = min(row, a.rows - 1), tok = rowc / G;
     const bool low = l16 >= 8;
+    // the query rows and masks do not depend on the position: in flight together with it
     const float* qr = a.q + (static_cast<size_t>(tok) * a.n_head + kv * G + (rowc - tok * G)) * HD + 16 * g4;
     float qx[NI][16];
 #pragma unroll
@@ -302,46 +368,52 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
             const float4 u = reinterpret_cast<const float4*>(qr + 64 * i)[f];
             qx[i][4 * f] = u.x, qx[i][4 * f + 1] = u.y, qx[i][4 * f + 2] = u.z, qx[i][4 * f + 3] = u.w;
         }
-    const int wlen = kStep * a.nsub, wbase = (w.chunk * kWaves + wv) * wlen;
-    const int nsteps = wbase > last ? 0 : min(a.nsub, (last - wbase) / kStep + 1);
     uint64_t mask = 0;   // of the row's token: bit j = draft slot base + j
     if (a.masks && row < a.rows) mask = a.masks[tok];
+    if (!tree_reach<kFewRows>(a, w)) return;
+    const int base = w.base, last = w.last;
+    const int wlen = kStep * a.nsub, wbase = (w.chunk * kWaves + wv) * wlen;
+    const int nsteps = wbase > last ? 0 : min(a.nsub, (last - wbase) / kStep + 1);
     const int lim = row >= a.rows ? -1 : a.masks ? base - 1 : base + tok;   // the row sees every position up to here
 
-    // the head's rows: position p at kp + p * kstride
+    // the head's rows, kstride apart; a lane's place in a step's
     const size_t kstride = KT == kKvF16 ? static_cast<size_t>(a.n_kv) * kKB : kKB;
     const size_t vstride = VT == kKvF16 ? static_cast<size_t>(a.n_kv) * kVB : kVB;
-    const uint8_t* kp = a.kc + kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD).code + g4 * (kKB / (HD / 16));
-    const uint8_t* vp = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).code + v_offset<VT, VD>(l16);
-    const uint8_t* ks = a.kc + kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD).scale;
-    const uint8_t* vs = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).scale + VD * l16 / kKvBlock;
+    const KvRow<KT> k0 = kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD);
+    const KvRow<VT> v0 = kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD);
+    const uint8_t *kp = a.kc + k0.code, *ks = a.kc + k0.scale, *vp = a.vc + v0.code, *vs = a.vc + v0.scale;
+    const int kat = static_cast<int>(l16 * kstride) + g4 * (kKB / (HD / 16)), vat = static_cast<int>(4 * g4 * vstride) + l16 * DimsV<VT, VD>::kBytes;
+    const int vsat = 4 * g4 * NB + VD * l16 / kKvBlock;
 
     Dims16<KT> kx[2][NI];
     uint32_t ksc[2][2];
     DimsV<VT, VD> vx[8];
     uint32_t vsc[8];
-    auto load_k = [&](int sb) {
+    auto load_k = [&](int sb) {   // rows past the last read as zeros
+        const Rsrc r = rows_buffer(kp + sb * kstride, min(last + 1 - sb, kStep), kstride);
+        const Rsrc rs = rows_buffer(ks + static_cast<size_t>(sb) * NB, min(last + 1 - sb, kStep), NB);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const size_t p = min(sb + 16 * t + l16, last);   // rows past the last are masked
 #pragma unroll
-            for (int i = 0; i < NI; ++i) kx[t][i] = load_k16<KT>(kp + p * kstride + i * (kKB / NI));
+            for (int i = 0; i < NI; ++i) kx[t][i] = load16<KT>(r, kat + i * (kKB / NI), static_cast<int>(16 * t * kstride));
             if constexpr (KT != kKvF16) {
                 if constexpr (NB == 8) {
-                    const uint2 s = *reinterpret_cast<const uint2*>(ks + p * NB);
-                    ksc[t][0] = s.x, ksc[t][1] = s.y;
+                    const auto s = __builtin_amdgcn_raw_buffer_load_b64(rs, l16 * NB, 16 * t * NB, 0);
+                    ksc[t][0] = s[0], ksc[t][1] = s[1];
                 } else {
-                    ksc[t][0] = *reinterpret_cast<const uint32_t*>(ks + p * NB);
+                    ksc[t][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, l16 * NB, 16 * t * NB, 0);
                 }
             }
         }
     };
     auto load_vs = [&](int sb) {
+        const Rsrc r = rows_buffer(vp + sb * vstride, min(last + 1 - sb, kStep), vstride);
+        const Rsrc rs = rows_buffer(vs + static_cast<size_t>(sb) * NB, min(last + 1 - sb, kStep), NB);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const size_t p = min(sb + 4 * g4 + (j < 4 ? j : 12 + j), last);
-            vx[j] = load_v<VT, VD>(vp + p * vstride, l16);
-            if constexpr (VT != kKvF16) vsc[j] = vs[p * NB];
+            const int p = j < 4 ? j : 12 + j;
+            vx[j] = load_dims<VT, VD>(r, vat, static_cast<int>(p * vstride));
+            if constexpr (VT != kKvF16) vsc[j] = __builtin_amdgcn_raw_buffer_load_b8(rs, vsat + p * NB, 0, 0);
         }
     };
     if (nsteps > 0) {
@@ -361,7 +433,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
         m = fmaxf(m, xor_lane<32>(m));
         const int sh = q_shift(m);
         const float f = ldexpf(1.0f, sh);
-        post = a.scale * 1.44269504088896340736f * ldexpf(1.0f, -sh);
+        post = a.scale * (1.44269504088896340736f * kSixteen<KT>) * ldexpf(1.0f, -sh);
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -387,13 +459,13 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
             floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                half2v s = {};
+                Scale2 s = {};
                 if constexpr (KT != kKvF16) {   // block 2 i + g4 / 2
                     const uint32_t b = (ksc[t][i >> 1] >> (16 * (i & 1) + 8 * (g4 >> 1))) & 0xffu;
-                    s = scale2(b, b);
+                    s = scale2<KT>(b, b);
                 }
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) acc = mfma(k_operand<KT>(kx[t][i], hf, s), qb[i][hf], acc);
+                for (int hf = 0; hf < 2; ++hf) acc = mfma(operand<KT>(kx[t][i], hf, s), qb[i][hf], acc);
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) sc[4 * t + r] = (acc[r] + xor_lane<8>(acc[r])) * post;
@@ -441,18 +513,18 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
             const _Float16 h = static_cast<_Float16>(p[j]);
             pa[j] = low ? static_cast<_Float16>(p[j] - static_cast<float>(h)) : h;
         }
-        half2v vsp[4];
+        Scale2 vsp[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if constexpr (VT != kKvF16) vsp[j] = scale2(vsc[2 * j], vsc[2 * j + 1]);
-            else vsp[j] = half2v{};
+            if constexpr (VT != kKvF16) vsp[j] = scale2<VT>(vsc[2 * j], vsc[2 * j + 1]);
+            else vsp[j] = Scale2{};
         }
         if (tail) {
             bool odd = false;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (VT != kKvF16) {
-                    odd = odd || !finite16(u2(vsp[j]));
+                    odd = odd || !finite16(u2(vsp[j].s));
                 } else {
 #pragma unroll
                     for (int e = 0; e < VD / 2; ++e) odd = odd || !finite16(vx[2 * j].w[e]) || !finite16(vx[2 * j + 1].w[e]);
@@ -469,8 +541,8 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
 #pragma unroll
                     for (int e = 0; e < VD; ++e) {
                         float v;
-                        if constexpr (VT == kKvF16) v = half_bits_to_float(reinterpret_cast<const uint16_t*>(vp + p1 * vstride)[e]);
-                        else v = kv_scale_value(vs[p1 * NB]);   // NaN: every value of the block
+                        if constexpr (VT == kKvF16) v = half_bits_to_float(reinterpret_cast<const uint16_t*>(vp + p1 * vstride)[VD * l16 + e]);
+                        else v = kv_scale_value(vs[p1 * NB + VD * l16 / kKvBlock]);   // NaN: every value of the block
                         if (fabsf(v) <= FLT_MAX) continue;
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
@@ -485,7 +557,8 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
 #pragma unroll
                         for (int e = 0; e < VD / 2; ++e) vx[j].w[e] = zero_odd(vx[j].w[e]);
                     } else if ((j & 1) == 0) {
-                        vsp[j >> 1] = h2(zero_odd(u2(vsp[j >> 1])));
+                        vsp[j >> 1].s = h2(zero_odd(u2(vsp[j >> 1].s)));
+                        vsp[j >> 1].c = h2(zero_odd(u2(vsp[j >> 1].c)));
                     }
                 }
             }
@@ -520,7 +593,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
                 *reinterpret_cast<float4*>(&slab[wv][4 * g4 + r][VD * l16 + e]) = make_float4(o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]);
     }
     __syncthreads();
-    join_stats<kWaves, 1, kFewRows>(stat, fac, top, sum);
+    join_stats<kWaves, 1, kFewRows>(kSixteen<VT>, stat, fac, top, sum);
     __syncthreads();
     join_rows<HD, kWaves, 1, kFewRows>(a, w, slab, fac, top, sum, 0);
 }
@@ -581,41 +654,55 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
     __shared__ float stat[kTileWaves][2][kRowBlock], fac[kTileWaves][kRowBlock], top[RB][kRowBlock], sum[RB][kRowBlock];
 
     Work w;
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l16 = lane & 15, g4 = lane >> 4;
-    if (!tree_work<kRowBlock * RB>(a, w)) return;
-    if (threadIdx.x < PB * BUFS) odd_step[threadIdx.x / BUFS][threadIdx.x % BUFS] = -1;
-    __syncthreads();
-    const int G = a.n_head / a.n_kv, base = w.base, kv = w.kv;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
+    if (!tree_share<kRowBlock * RB>(a, w)) return;
+    const int G = a.n_head / a.n_kv, kv = w.kv;
     const int rb = wv % RB, part = wv / RB, tt = rb * 64 + lane;   // tt: thread within the part
     const int row0 = w.row0 + kRowBlock * rb, row = row0 + l16, rowc = min(row, a.rows - 1), tok = rowc / G;
+    // the query rows and masks do not depend on the position: in flight together with it
+    const float* qr = a.q + (static_cast<size_t>(tok) * a.n_head + kv * G + (rowc - tok * G)) * HD + 8 * g4;
+    float4 qx[NC][2];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) qx[c][f] = reinterpret_cast<const float4*>(qr + 32 * c)[f];
+    uint64_t mask = 0;
+    if (a.masks && row < a.rows) mask = a.masks[tok];
+    if (!tree_reach<kRowBlock * RB>(a, w)) return;
+    if (threadIdx.x < PB * BUFS) odd_step[threadIdx.x / BUFS][threadIdx.x % BUFS] = -1;
+    __syncthreads();
+    const int base = w.base;
     // the last position the wave's rows see (w.last: any of the workgroup's)
     const int last = row0 >= a.rows ? -1 : a.masks ? w.last : base + min(row0 + kRowBlock - 1, a.rows - 1) / G;
     const int psteps = kUnit * a.nsub / (kStep * PB), cbase = w.chunk * kUnit * a.nsub, pbase = cbase + part * psteps * kStep;
     const int nsteps = min(psteps, (w.last - cbase) / kStep + 1);   // of the first part: the others run along
-    uint64_t mask = 0;
-    if (a.masks && row < a.rows) mask = a.masks[tok];
     const int lim = row >= a.rows ? -1 : a.masks ? base - 1 : base + tok;
 
     const size_t kstride = KT == kKvF16 ? static_cast<size_t>(a.n_kv) * kKB : kKB;
     const size_t vstride = VT == kKvF16 ? static_cast<size_t>(a.n_kv) * kVB : kVB;
-    const int unit = tt % NE, pos0 = tt / NE;   // of the thread's first unit; the next ones are 64 RB / NE positions further
-    const uint8_t* kp = a.kc + kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD).code + unit * (kKB / NE);
-    const uint8_t* vp = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).code + unit * (kVB / NE);
-    const uint8_t* ks = a.kc + kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD).scale + unit / 2;
-    const uint8_t* vs = a.vc + kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD).scale + unit / 2;
+    const KvRow<KT> k0 = kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD);
+    const KvRow<VT> v0 = kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD);
+    const uint8_t *kp = a.kc + k0.code, *ks = a.kc + k0.scale, *vp = a.vc + v0.code, *vs = a.vc + v0.scale;
+    // the thread's first unit; the next ones are kUp positions further
+    constexpr int kUp = 64 * RB / NE;
+    const int unit = tt % NE, pos0 = tt / NE;
+    const int kat = static_cast<int>(pos0 * kstride) + unit * (kKB / NE), vat = static_cast<int>(pos0 * vstride) + unit * (kVB / NE);
+    const int sat = pos0 * NB + unit / 2;
 
     Dims16<KT> kx[U];
     Dims16<VT> vx[U];
     uint32_t ksc[U], vsc[U];
-    auto load = [&](int sb) {
+    auto load = [&](int sb) {   // rows past the last read as zeros
+        const int n = min(w.last + 1 - sb, kStep);
+        const Rsrc rk = rows_buffer(kp + sb * kstride, n, kstride), rks = rows_buffer(ks + static_cast<size_t>(sb) * NB, n, NB);
+        const Rsrc rv = rows_buffer(vp + sb * vstride, n, vstride), rvs = rows_buffer(vs + static_cast<size_t>(sb) * NB, n, NB);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (kUnits < 64 * RB && tt >= kUnits) break;
-            const size_t p = min(sb + pos0 + u * (64 * RB / NE), w.last);   // rows past the last are masked
-            kx[u] = load_k16<KT>(kp + p * kstride);
-            vx[u] = load_k16<VT>(vp + p * vstride);
-            if constexpr (KT != kKvF16) ksc[u] = ks[p * NB];
-            if constexpr (VT != kKvF16) vsc[u] = vs[p * NB];
+            kx[u] = load16<KT>(rk, kat, static_cast<int>(u * kUp * kstride));
+            vx[u] = load16<VT>(rv, vat, static_cast<int>(u * kUp * vstride));
+            if constexpr (KT != kKvF16) ksc[u] = __builtin_amdgcn_raw_buffer_load_b8(rks, sat + u * kUp * NB, 0, 0);
+            if constexpr (VT != kKvF16) vsc[u] = __builtin_amdgcn_raw_buffer_load_b8(rvs, sat + u * kUp * NB, 0, 0);
         }
     };
     uint8_t* tiles = pool + part * (BUFS * Pool::kBytes);
@@ -626,14 +713,14 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (kUnits < 64 * RB && tt >= kUnits) break;
-            const int p = pos0 + u * (64 * RB / NE);
-            half2v sk = {}, sv = {};
-            if constexpr (KT != kKvF16) sk = scale2(ksc[u], ksc[u]);
-            if constexpr (VT != kKvF16) sv = scale2(vsc[u], vsc[u]);
+            const int p = pos0 + u * kUp;
+            Scale2 sk = {}, sv = {};
+            if constexpr (KT != kKvF16) sk = scale2<KT>(ksc[u], ksc[u]);
+            if constexpr (VT != kKvF16) sv = scale2<VT>(vsc[u], vsc[u]);
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-                *reinterpret_cast<half8*>(kt + p * Pool::kKRow + 16 * hf) = k_operand<KT>(kx[u], hf, sk);
-                u32x4 v = __builtin_bit_cast(u32x4, k_operand<VT>(vx[u], hf, sv));
+                *reinterpret_cast<half8*>(kt + p * Pool::kKRow + 16 * hf) = operand<KT>(kx[u], hf, sk);
+                u32x4 v = __builtin_bit_cast(u32x4, operand<VT>(vx[u], hf, sv));
                 if (tail && !(finite16(v[0]) && finite16(v[1]) && finite16(v[2]) && finite16(v[3]))) {
                     v = u32x4{zero_odd(v[0]), zero_odd(v[1]), zero_odd(v[2]), zero_odd(v[3])};
                     odd_step[part][buf] = st;   // every writer stores the same
@@ -647,27 +734,21 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
     half8 qh[NC], ql[NC];
     float post;   // score = product * post, in base 2
     {
-        const float* qr = a.q + (static_cast<size_t>(tok) * a.n_head + kv * G + (rowc - tok * G)) * HD + 8 * g4;
-        float4 u[NC][2];
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int f = 0; f < 2; ++f) u[c][f] = reinterpret_cast<const float4*>(qr + 32 * c)[f];
         float m = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int f = 0; f < 2; ++f)
-                m = fmaxf(m, fmaxf(fmaxf(fabsf(u[c][f].x), fabsf(u[c][f].y)), fmaxf(fabsf(u[c][f].z), fabsf(u[c][f].w))));
+                m = fmaxf(m, fmaxf(fmaxf(fabsf(qx[c][f].x), fabsf(qx[c][f].y)), fmaxf(fabsf(qx[c][f].z), fabsf(qx[c][f].w))));
         m = fmaxf(m, xor_lane<16>(m));
         m = fmaxf(m, xor_lane<32>(m));
         const int sh = q_shift(m);
         const float f = ldexpf(1.0f, sh);
-        post = a.scale * 1.44269504088896340736f * ldexpf(1.0f, -sh);
+        post = a.scale * (1.44269504088896340736f * kSixteen<KT>) * ldexpf(1.0f, -sh);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const float x[8] = {u[c][0].x * f, u[c][0].y * f, u[c][0].z * f, u[c][0].w * f,
-                                u[c][1].x * f, u[c][1].y * f, u[c][1].z * f, u[c][1].w * f};
+            const float x[8] = {qx[c][0].x * f, qx[c][0].y * f, qx[c][0].z * f, qx[c][0].w * f,
+                                qx[c][1].x * f, qx[c][1].y * f, qx[c][1].z * f, qx[c][1].w * f};
             split8(x, qh[c], ql[c]);
         }
     }
@@ -790,7 +871,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
         stat[wv][1][l16] = l_run;
     }
     __syncthreads();
-    join_stats<kTileWaves, RB, kRowBlock>(stat, fac, top, sum);
+    join_stats<kTileWaves, RB, kRowBlock>(kSixteen<VT>, stat, fac, top, sum);
     auto& slab = *reinterpret_cast<float(*)[kTileWaves][kOct][HD]>(pool);
 #pragma unroll
     for (int oct = 0; oct < kRowBlock / kOct; ++oct) {
@@ -820,19 +901,22 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeArgs a) {
     const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, g = tid >> 6;
     const int d = kMergeDims * blockIdx.z + lane;
     const int G = a.n_head / a.n_kv, kv = h / G, row = t * G + (h - kv * G);
+    // the first records and o values do not wait for the position: every chunk of the cache has a place (what a chunk past
+    // the last position holds is not used), and indexes are clamped (a load under a branch gets a wait of its own)
+    const int all = a.npairs / a.n_kv;
+    const size_t cstride = static_cast<size_t>(a.n_kv) * a.rows_pad, r0 = static_cast<size_t>(kv) * a.rows_pad + row;
+    const float2* ml = reinterpret_cast<const float2*>(a.wml) + r0;
+    const float* ro = a.wo + r0 * HD + d;
+    const float2 first = ml[min(tid, all - 1) * cstride];
+    float oa[kMergeBatch];   // chunks g + 4 k
+#pragma unroll
+    for (int k = 0; k < kMergeBatch; ++k) oa[k] = ro[min(g + 4 * k, all - 1) * cstride * HD];
     float gate = 0.0f;
     if (a.gate) gate = a.gate[static_cast<size_t>(t) * a.gate_stride + h * 2 * HD + HD + d];
     const int base = a.pos[0];
     if (base < 0 || base > a.max_ctx - a.ntok) return;   // uniform: a slot outside the cache
     const int nchunk = (base + (a.masks ? a.ntok - 1 : t)) / (kUnit * a.nsub) + 1;
-    const size_t cstride = static_cast<size_t>(a.n_kv) * a.rows_pad, r0 = static_cast<size_t>(kv) * a.rows_pad + row;
-    const float2* ml = reinterpret_cast<const float2*>(a.wml) + r0;
-    const float* ro = a.wo + r0 * HD + d;
-    const float2 first = ml[min(tid, nchunk - 1) * cstride];
-    float oa[kMergeBatch];   // chunks g + 4 k, clamped (a load under a branch gets a wait of its own)
-#pragma unroll
-    for (int k = 0; k < kMergeBatch; ++k) oa[k] = ro[min(g + 4 * k, nchunk - 1) * cstride * HD];
-    float m = first.x;
+    float m = tid < nchunk ? first.x : -INFINITY;
     for (int c = tid + kThreads; c < nchunk; c += kThreads) m = fmaxf(m, ml[c * cstride].x);
     m = group_max<64>(m);
     if (lane == 0) red[0][g] = m;
@@ -888,11 +972,8 @@ __global__ __launch_bounds__(kThreads) void tree_merge_flat_kernel(TreeArgs a) {
     if (i >= a.ntok * a.n_head) return;
     const int t = i / a.n_head, h = i - t * a.n_head;
     const int G = a.n_head / a.n_kv, kv = h / G, row = t * G + (h - kv * G);
-    float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (a.gate) {   // 4-byte aligned
-        const float* p = a.gate + static_cast<size_t>(t) * a.gate_stride + h * 2 * HD + HD + d;
-        g = make_float4(p[0], p[1], p[2], p[3]);
-    }
+    float g[4];
+    load_gate<HD>(a, t, h, d, g);
     const int base = a.pos[0];
     if (base < 0 || base > a.max_ctx - a.ntok) return;   // uniform: a slot outside the cache
     const int nchunk = (base + (a.masks ? a.ntok - 1 : t)) / (kUnit * a.nsub) + 1;
@@ -913,38 +994,7 @@ __global__ __launch_bounds__(kThreads) void tree_merge_flat_kernel(TreeArgs a) {
         o[2] = __builtin_fmaf(w, v.z, o[2]);
         o[3] = __builtin_fmaf(w, v.w, o[3]);
     }
-    const float gs[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        o[k] = m == -INFINITY ? 0.0f : o[k] / l;
-        if (a.gate) o[k] *= 1.0f / (1.0f + expf(-gs[k]));
-    }
-    if (a.y) {
-        float* y = a.y + static_cast<size_t>(t) * a.y_stride + h * HD + d;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] = o[k];
-    }
-    if (a.q8) {   // q8_1_store_lane's block and bits: its lane's element is 4 (lane % 8) + k here
-        float amax = fmaxf(fmaxf(fabsf(o[0]), fabsf(o[1])), fmaxf(fabsf(o[2]), fabsf(o[3])));
-        amax = fmaxf(amax, xor_lane<4>(amax));
-        amax = fmaxf(amax, xor_lane<2>(amax));
-        amax = fmaxf(amax, xor_lane<1>(amax));
-        float s[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            s[k] = o[k] + xor_lane<4>(o[k]);
-            s[k] += xor_lane<2>(s[k]);
-            s[k] += xor_lane<1>(s[k]);
-        }
-        const float total = (s[0] + s[2]) + (s[1] + s[3]), dq = amax / 127.0f;
-        uint32_t w = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            w |= (static_cast<uint32_t>(amax == 0.0f ? 0 : static_cast<int>(roundf(o[k] / dq))) & 0xffu) << (8 * k);
-        uint8_t* block = a.q8 + static_cast<size_t>(t) * a.q8_stride + (h * (HD / 32) + d / 32) * kQ8_1Bytes;
-        *reinterpret_cast<uint32_t*>(block + 4 + (d & 31)) = w;
-        if ((d & 31) == 0) *reinterpret_cast<uint32_t*>(block) = float_to_half_sat(dq) | (float_to_half_sat(total) << 16);
-    }
+    finish4<HD>(a, t, h, d, o, m, l, g);
 }
 
 bool tree_shape_ok(int max_ctx, int n_head, int n_kv, int head_dim, int ntok) {
