@@ -27,6 +27,7 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));   // rows of a caller's stride
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
@@ -34,8 +35,6 @@ constexpr int kStep = 32;          // positions of a step
 constexpr int kUnit = kWaves * kStep;
 constexpr int kMaxChunks = 2048;
 constexpr int kMaxTree = 64, kMaxChain = 1024;
-constexpr int kOct = 8;            // rows joined at a time
-constexpr int kFewRows = 8;        // query rows per KV head of the form without a tile
 constexpr float kPScale = 8.0f;    // p goes as 2^8 p
 constexpr float kLazy = 7.0f;      // a maximum moves once a score passes it by more than 2^7 (2^15 p is an fp16 number)
 
@@ -188,6 +187,11 @@ __device__ __forceinline__ void split8(const float (&x)[8], half8& hi, half8& lo
 __device__ __forceinline__ bool finite16(uint32_t w) {   // both halves
     return (w & 0x7c00u) != 0x7c00u && (w & 0x7c000000u) != 0x7c000000u;
 }
+// the larger magnitudes of two words of fp16, half by half, as bits
+__device__ __forceinline__ uint32_t max_magnitude(uint32_t m, uint32_t w) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+}
 // a word of fp16 V without its infinities and NaN
 __device__ __forceinline__ uint32_t zero_odd(uint32_t w) {
     if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
@@ -207,6 +211,7 @@ struct Work {
 };
 template <int ROWS>
 __device__ __forceinline__ bool tree_share(const TreeArgs& a, Work& w) {
+    w.base = a.pos[0];   // in flight over what does not depend on it
     // the groups of a (chunk, head) pair are consecutive workgroups of one XCD (workgroups go to the XCDs round robin),
     // so the pair's rows come from HBM once
     const int k8 = static_cast<int>(blockIdx.x >> 3), q8 = k8 / a.groups;
@@ -219,7 +224,6 @@ __device__ __forceinline__ bool tree_share(const TreeArgs& a, Work& w) {
 }
 template <int ROWS>
 __device__ __forceinline__ bool tree_reach(const TreeArgs& a, Work& w) {
-    w.base = a.pos[0];
     if (w.base < 0 || w.base > a.max_ctx - a.ntok) return false;   // a slot outside the cache
     const int G = a.n_head / a.n_kv;
     w.last = w.base + (a.masks ? a.ntok - 1 : min(w.row0 + ROWS - 1, a.rows - 1) / G);
@@ -240,11 +244,7 @@ __device__ __forceinline__ void finish4(const TreeArgs& a, int t, int h, int d, 
         o[k] = m == -INFINITY ? 0.0f : o[k] / l;
         if (a.gate) o[k] *= 1.0f / (1.0f + expf(-gate[k]));
     }
-    if (a.y) {   // 4-byte aligned
-        float* y = a.y + static_cast<size_t>(t) * a.y_stride + h * HD + d;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] = o[k];
-    }
+    if (a.y) *reinterpret_cast<float4u*>(a.y + static_cast<size_t>(t) * a.y_stride + h * HD + d) = float4u{o[0], o[1], o[2], o[3]};
     if (a.q8) {   // q8_1_store_lane's block and bits: its lane's element is 4 (lane % 8) + k here
         float amax = fmaxf(fmaxf(fabsf(o[0]), fabsf(o[1])), fmaxf(fabsf(o[2]), fabsf(o[3])));
         amax = fmaxf(amax, xor_lane<4>(amax));
@@ -269,42 +269,53 @@ __device__ __forceinline__ void finish4(const TreeArgs& a, int t, int h, int d, 
 }
 template <int HD>
 __device__ __forceinline__ void load_gate(const TreeArgs& a, int t, int h, int d, float (&g)[4]) {
-    const float* p = a.gate ? a.gate + static_cast<size_t>(t) * a.gate_stride + h * 2 * HD + HD + d : nullptr;   // 4-byte aligned
+    float4u x = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (a.gate) x = *reinterpret_cast<const float4u*>(a.gate + static_cast<size_t>(t) * a.gate_stride + h * 2 * HD + HD + d);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) g[k] = p ? p[k] : 0.0f;
+    for (int k = 0; k < 4; ++k) g[k] = x[k];
 }
 
-// Joins the waves' parts of 8 * RB rows (rows 8 oct .. of each of RB row blocks) from their LDS slabs [wave][8][HD] and
-// either writes records or, for a call of one chunk, the result: fac[wave][row of the block] is a part's weight, sum[row]
-// the joined l.  Wave w holds part w / RB of row block w % RB.
+// Joins the waves' parts of RB row blocks from their LDS slabs [wave][row of the block][HD] and either writes records or,
+// for a call of one chunk, the result: fac[wave][row] is a part's weight, top[row] and sum[row] the joined m and l.  Wave w
+// holds part w / RB of row block w % RB.
 template <int HD, int WAVES, int RB, int BLOCK>
-__device__ __forceinline__ void join_rows(const TreeArgs& a, const Work& w, const float (&slab)[WAVES][kOct][HD],
+__device__ __forceinline__ void join_rows(const TreeArgs& a, const Work& w, const float (&slab)[WAVES][BLOCK][HD],
                                           const float (&fac)[WAVES][BLOCK], const float (&top)[RB][BLOCK],
-                                          const float (&sum)[RB][BLOCK], int oct) {
-    constexpr int PB = WAVES / RB;
+                                          const float (&sum)[RB][BLOCK]) {
+    constexpr int PB = WAVES / RB, N = RB * BLOCK * HD / (4 * 64 * WAVES);   // N rounds of four dims a lane
     const int G = a.n_head / a.n_kv;
-    for (int i = 4 * static_cast<int>(threadIdx.x); i < RB * kOct * HD; i += 4 * 64 * WAVES) {
-        const int d = i % HD, r8 = i / HD, rb = r8 / kOct, rr = r8 % kOct, rk = kOct * oct + rr, row = w.row0 + BLOCK * rb + rk;
+    const int d = 4 * (static_cast<int>(threadIdx.x) % (HD / 4)), r0 = static_cast<int>(threadIdx.x) / (HD / 4);
+    constexpr int kUp = 4 * 64 * WAVES / HD;   // rows a round is further
+    float g[N][4];
+    if (a.direct && a.gate) {   // all gates in flight together
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int row = min(w.row0 + r0 + i * kUp, a.rows - 1), t = row / G;
+            load_gate<HD>(a, t, w.kv * G + row - t * G, d, g[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int r = r0 + i * kUp, rb = r / BLOCK, rk = r % BLOCK, row = w.row0 + r;
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int p = 0; p < PB; ++p) {
-            const float4 x = *reinterpret_cast<const float4*>(&slab[rb + RB * p][rr][d]);
+            const float4 x = *reinterpret_cast<const float4*>(&slab[rb + RB * p][rk][d]);
             const float f = fac[rb + RB * p][rk];
             v[0] = __builtin_fmaf(x.x, f, v[0]);
             v[1] = __builtin_fmaf(x.y, f, v[1]);
             v[2] = __builtin_fmaf(x.z, f, v[2]);
             v[3] = __builtin_fmaf(x.w, f, v[3]);
         }
-        if (row >= a.rows) continue;
-        if (a.direct) {
-            const int t = row / G, h = w.kv * G + row - t * G;
-            float g[4];
-            load_gate<HD>(a, t, h, d, g);
-            finish4<HD>(a, t, h, d, v, top[rb][rk], sum[rb][rk], g);
-        } else {
-            const size_t rec = (static_cast<size_t>(w.chunk) * a.n_kv + w.kv) * a.rows_pad + row;
-            *reinterpret_cast<float4*>(a.wo + rec * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
-            if (d == 0) *reinterpret_cast<float2*>(a.wml + 2 * rec) = make_float2(top[rb][rk], sum[rb][rk]);
+        if (row < a.rows) {
+            if (a.direct) {
+                const int t = row / G;
+                finish4<HD>(a, t, w.kv * G + row - t * G, d, v, top[rb][rk], sum[rb][rk], g[i]);
+            } else {
+                const size_t rec = (static_cast<size_t>(w.chunk) * a.n_kv + w.kv) * a.rows_pad + row;
+                *reinterpret_cast<float4*>(a.wo + rec * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
+                if (d == 0) *reinterpret_cast<float2*>(a.wml + 2 * rec) = make_float2(top[rb][rk], sum[rb][rk]);
+            }
         }
     }
 }
@@ -333,31 +344,37 @@ __device__ __forceinline__ void join_stats(float unit, const float (&stat)[WAVES
     sum[rb][r] = l;
 }
 
-// ---- up to 8 query rows: v_mfma_f32_16x16x32_f16 -------------------------------------------------------------------------
+// ---- few query rows: v_mfma_f32_16x16x32_f16 from the cache ---------------------------------------------------------------
 // Lane: l16 = l % 16, g4 = l / 16; A rows, B and D columns are l16; A and B hold k = 8 g4 + 0..7; D rows are 4 g4 + 0..3.
-//   scores    D[position][n] += K[position][dims] . q_n[dims]: column n < 8 is the high part of row n, column n >= 8 the low
-//             part of row n - 8, so one chain gives both.  Lane (l16, g4) takes 16 neighbouring dims of position l16 at a
+//   scores    D[position][n] += K[position][dims] . q_n[dims]; lane (l16, g4) takes 16 neighbouring dims of position l16 at a
 //             time, 64 i + 16 g4 + [0, 16), as two operands of eight, straight from the cache.
-//   P V       D[m][dim] += P_m[positions] V[positions][dim], rows m split the same way.  The score lane (row, positions
-//             4 g4 + r of two tiles) holds P in the A layout already, k slot j being position 4 g4 + j or 16 + 4 g4 + j - 4.
-//             V comes by lane (l16, g4) as HD / 16 neighbouring dims of those eight positions; operand e gathers dim e.
+//   P V       D[m][dim] += P_m[positions] V[positions][dim].  The score lane (row, positions 4 g4 + r of two tiles) holds P in
+//             the A layout already, k slot j being position 4 g4 + j or 16 + 4 g4 + j - 4.  V comes by lane (l16, g4) as
+//             HD / 16 neighbouring dims of those eight positions; operand e gathers dim e.
+// Up to 8 rows, column (row) n < 8 is the high part of row n and n >= 8 the low part of row n - 8: one product gives both.  Up
+// to 16 rows the parts are two products, with q's operands in LDS (the registers hold o and the step's K and V).
 // The waves take quarters of the chunk.  K of the next step is loaded when this step's scores are done, V when its product is:
 // each has half a step to arrive.
-template <int KT, int VT, int HD>
+template <int KT, int VT, int HD, int ROWS>
 __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kernel(TreeArgs a) {
+    constexpr bool PACKED = ROWS == 8;
     constexpr int NI = HD / 64;        // K: 16-dim pieces a lane takes of a position
     constexpr int VD = HD / 16;        // V: dims a lane takes of a position
     constexpr int NB = HD / kKvBlock;  // scale bytes of a row
     constexpr int kKB = kv_row_bytes(KT, HD), kVB = kv_row_bytes(VT, HD);
-    __shared__ __attribute__((aligned(16))) float slab[kWaves][kOct][HD];
-    __shared__ float stat[kWaves][2][kFewRows], fac[kWaves][kFewRows], top[1][kFewRows], sum[1][kFewRows];
+    __shared__ __attribute__((aligned(16))) float slab[kWaves][ROWS][HD];   // the rows that are joined
+    // until then q's operands [piece][half][part][lane]
+    auto& qs = *reinterpret_cast<half8(*)[NI][2][2][64]>(&slab[0][0][0]);
+    static_assert(PACKED || sizeof(qs) <= sizeof(slab), "q's operands fit");
+    __shared__ float pb[kWaves][ROWS][kStep];   // a step's p where a V is not finite
+    __shared__ float stat[kWaves][2][ROWS], fac[kWaves][ROWS], top[1][ROWS], sum[1][ROWS];
 
     Work w;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
-    if (!tree_share<kFewRows>(a, w)) return;
+    if (!tree_share<ROWS>(a, w)) return;
     const int G = a.n_head / a.n_kv, kv = w.kv;
-    const int row = l16 & 7, rowc = min(row, a.rows - 1), tok = rowc / G;
-    const bool low = l16 >= 8;
+    const int slot = PACKED ? l16 & 7 : l16, row = w.row0 + slot, rowc = min(row, a.rows - 1), tok = rowc / G;
+    const bool low = PACKED && l16 >= 8;
     // the query rows and masks do not depend on the position: in flight together with it
     const float* qr = a.q + (static_cast<size_t>(tok) * a.n_head + kv * G + (rowc - tok * G)) * HD + 16 * g4;
     float qx[NI][16];
@@ -370,7 +387,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
         }
     uint64_t mask = 0;   // of the row's token: bit j = draft slot base + j
     if (a.masks && row < a.rows) mask = a.masks[tok];
-    if (!tree_reach<kFewRows>(a, w)) return;
+    if (!tree_reach<ROWS>(a, w)) return;
     const int base = w.base, last = w.last;
     const int wlen = kStep * a.nsub, wbase = (w.chunk * kWaves + wv) * wlen;
     const int nsteps = wbase > last ? 0 : min(a.nsub, (last - wbase) / kStep + 1);
@@ -421,7 +438,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
         load_vs(wbase);
     }
 
-    half8 qb[NI][2];
+    half8 qb[PACKED ? NI : 1][2];
     float post;   // score = product * post, in base 2
     {
         float m = 0.0f;
@@ -438,14 +455,27 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
         for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf)
+            {
+                float x[8];
+                half8 hi, lo;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float x = qx[i][8 * hf + e] * f;
-                    const _Float16 h = static_cast<_Float16>(x);
-                    qb[i][hf][e] = low ? static_cast<_Float16>(x - static_cast<float>(h)) : h;
+                for (int e = 0; e < 8; ++e) x[e] = qx[i][8 * hf + e] * f;
+                split8(x, hi, lo);
+                if constexpr (PACKED) {
+                    qb[i][hf] = low ? lo : hi;
+                } else if (i == wv) {   // every wave has the group's rows: each writes a piece
+                    qs[i][hf][0][lane] = hi;
+                    qs[i][hf][1][lane] = lo;
                 }
+            }
     }
 
+    if constexpr (!PACKED) {
+        static_assert(PACKED || NI <= kWaves, "a piece a wave");
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();   // __syncthreads would also wait for the first K and V
+        asm volatile("" ::: "memory");
+    }
     floatx4 o[VD];
 #pragma unroll
     for (int e = 0; e < VD; ++e) o[e] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -456,7 +486,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
         float sc[8];   // j: position sb + 4 g4 + j, or 16 + 4 g4 + j - 4 further
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f}, acl = acc;
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 Scale2 s = {};
@@ -465,10 +495,18 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
                     s = scale2<KT>(b, b);
                 }
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) acc = mfma(operand<KT>(kx[t][i], hf, s), qb[i][hf], acc);
+                for (int hf = 0; hf < 2; ++hf) {
+                    const half8 kk = operand<KT>(kx[t][i], hf, s);
+                    if constexpr (PACKED) {
+                        acc = mfma(kk, qb[i][hf], acc);
+                    } else {
+                        acc = mfma(kk, qs[i][hf][0][lane], acc);
+                        acl = mfma(kk, qs[i][hf][1][lane], acl);
+                    }
+                }
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sc[4 * t + r] = (acc[r] + xor_lane<8>(acc[r])) * post;
+            for (int r = 0; r < 4; ++r) sc[4 * t + r] = (acc[r] + (PACKED ? xor_lane<8>(acc[r]) : acl[r])) * post;
         }
         const bool more = st + 1 < nsteps;
         if (more) load_k(sb + kStep);
@@ -501,18 +539,15 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
         if (__ballot(alpha != 1.0f)) {   // uniform: some row's maximum moved
             float al[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) al[r] = __shfl(alpha, 4 * (g4 & 1) + r, 64);
+            for (int r = 0; r < 4; ++r) al[r] = __shfl(alpha, PACKED ? 4 * (g4 & 1) + r : 4 * g4 + r, 64);
 #pragma unroll
             for (int e = 0; e < VD; ++e)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[e][r] *= al[r];
         }
-        half8 pa;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const _Float16 h = static_cast<_Float16>(p[j]);
-            pa[j] = low ? static_cast<_Float16>(p[j] - static_cast<float>(h)) : h;
-        }
+        half8 ph, pl;
+        split8(p, ph, pl);
+        if (low) ph = pl;
         Scale2 vsp[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -520,21 +555,21 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
             else vsp[j] = Scale2{};
         }
         if (tail) {
-            bool odd = false;
+            uint32_t big = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (VT != kKvF16) {
-                    odd = odd || !finite16(u2(vsp[j].s));
+                    big = max_magnitude(big, u2(vsp[j].s));
                 } else {
 #pragma unroll
-                    for (int e = 0; e < VD / 2; ++e) odd = odd || !finite16(vx[2 * j].w[e]) || !finite16(vx[2 * j + 1].w[e]);
+                    for (int e = 0; e < VD / 2; ++e) big = max_magnitude(max_magnitude(big, vx[2 * j].w[e]), vx[2 * j + 1].w[e]);
                 }
             }
-            if (__ballot(odd)) {
-                float(*pw)[kStep] = reinterpret_cast<float(*)[kStep]>(&slab[wv][0][0]);   // [row][position], -1: not seen
+            if (__ballot(!finite16(big))) {
+                float(*pw)[kStep] = pb[wv];   // [row][position], -1: not seen
                 if (!low)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) pw[row][4 * g4 + (j < 4 ? j : 12 + j)] = seen >> j & 1 ? p[j] : -1.0f;
+                    for (int j = 0; j < 8; ++j) pw[slot][4 * g4 + (j < 4 ? j : 12 + j)] = seen >> j & 1 ? p[j] : -1.0f;
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 for (int pp = 0; pp < kStep; ++pp) {
                     const size_t p1 = min(sb + pp, last);
@@ -546,7 +581,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
                         if (fabsf(v) <= FLT_MAX) continue;
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const float x = g4 < 2 ? pw[4 * (g4 & 1) + r][pp] : -1.0f;
+                            const float x = !PACKED ? pw[4 * g4 + r][pp] : g4 < 2 ? pw[4 * (g4 & 1) + r][pp] : -1.0f;   // the high rows
                             if (!(x < 0.0f)) o[e][r] = __builtin_fmaf(x, v, o[e][r]);
                         }
                     }
@@ -568,8 +603,13 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
             uint32_t ev[4], od[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) v_pair<VT, VD>(vx[2 * j], vx[2 * j + 1], e, vsp[j], ev[j], od[j]);
-            o[2 * e] = mfma(pa, h8(ev[0], ev[1], ev[2], ev[3]), o[2 * e]);
-            o[2 * e + 1] = mfma(pa, h8(od[0], od[1], od[2], od[3]), o[2 * e + 1]);
+            const half8 b0 = h8(ev[0], ev[1], ev[2], ev[3]), b1 = h8(od[0], od[1], od[2], od[3]);
+            o[2 * e] = mfma(ph, b0, o[2 * e]);
+            o[2 * e + 1] = mfma(ph, b1, o[2 * e + 1]);
+            if constexpr (!PACKED) {
+                o[2 * e] = mfma(pl, b0, o[2 * e]);
+                o[2 * e + 1] = mfma(pl, b1, o[2 * e + 1]);
+            }
         }
         if (more) load_vs(sb + kStep);
     }
@@ -577,15 +617,17 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
     l_run += xor_lane<16>(l_run);
     l_run += xor_lane<32>(l_run);
     if (g4 == 0 && !low) {
-        stat[wv][0][row] = m_run;
-        stat[wv][1][row] = l_run;
+        stat[wv][0][slot] = m_run;
+        stat[wv][1][slot] = l_run;
     }
-    // high rows + low rows: lanes g4 < 2 end with o[row 4 g4 + r]
+    if constexpr (!PACKED) __syncthreads();   // q's operands are read
+    if constexpr (PACKED) {   // high rows + low rows: lanes g4 < 2 end with o[row 4 g4 + r]
 #pragma unroll
-    for (int e = 0; e < VD; ++e)
+        for (int e = 0; e < VD; ++e)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[e][r] += xor_lane<32>(o[e][r]);
-    if (g4 < 2) {
+            for (int r = 0; r < 4; ++r) o[e][r] += xor_lane<32>(o[e][r]);
+    }
+    if (!PACKED || g4 < 2) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -593,9 +635,9 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
                 *reinterpret_cast<float4*>(&slab[wv][4 * g4 + r][VD * l16 + e]) = make_float4(o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]);
     }
     __syncthreads();
-    join_stats<kWaves, 1, kFewRows>(kSixteen<VT>, stat, fac, top, sum);
+    join_stats<kWaves, 1, ROWS>(kSixteen<VT>, stat, fac, top, sum);
     __syncthreads();
-    join_rows<HD, kWaves, 1, kFewRows>(a, w, slab, fac, top, sum, 0);
+    join_rows<HD, kWaves, 1, ROWS>(a, w, slab, fac, top, sum);
 }
 
 // ---- more rows: the tile in LDS ---------------------------------------------------------------------------------------------
@@ -620,8 +662,8 @@ struct TilePool {
     static constexpr int kKRow = 2 * HD + 16, kVRow = 2 * HD + 32;     // bytes
     static constexpr int kBytes = kStep * (kKRow + kVRow);             // one tile
     static constexpr int kBufs = kParts == 4 ? 1 : 2;                  // two tiles a part where they fit
-    static constexpr int kSlab = kTileWaves * kOct * HD * 4;           // the rows that are joined, after the last step
-    static constexpr int kPool = kParts * kBufs * kBytes > kSlab ? kParts * kBufs * kBytes : kSlab;
+    static constexpr int kPool = kParts * kBufs * kBytes;
+    static_assert(kParts == 1 || kPool >= kTileWaves * kRowBlock * HD * 4, "the parts' rows are joined in the tiles' place");
 };
 
 // The order of N groups of R LDS reads and M products in a block: AHEAD groups' reads, then a group's reads for a group's
@@ -651,7 +693,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
     __shared__ __attribute__((aligned(16))) uint8_t pool[Pool::kPool];
     __shared__ float pb[kTileWaves][kRowBlock][kStep];           // a step's p where a V is not finite
     __shared__ int odd_step[PB][BUFS];                           // the last step whose V had one
-    __shared__ float stat[kTileWaves][2][kRowBlock], fac[kTileWaves][kRowBlock], top[RB][kRowBlock], sum[RB][kRowBlock];
+    __shared__ float stat[kTileWaves][2][kRowBlock], fac[kTileWaves][kRowBlock], top[RB][kRowBlock], sum[RB][kRowBlock];   // PB > 1
 
     Work w;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
@@ -670,7 +712,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
     if (a.masks && row < a.rows) mask = a.masks[tok];
     if (!tree_reach<kRowBlock * RB>(a, w)) return;
     if (threadIdx.x < PB * BUFS) odd_step[threadIdx.x / BUFS][threadIdx.x % BUFS] = -1;
-    __syncthreads();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();   // __syncthreads would also wait for the query rows
     const int base = w.base;
     // the last position the wave's rows see (w.last: any of the workgroup's)
     const int last = row0 >= a.rows ? -1 : a.masks ? w.last : base + min(row0 + kRowBlock - 1, a.rows - 1) / G;
@@ -866,24 +909,58 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
 
     l_run += xor_lane<16>(l_run);
     l_run += xor_lane<32>(l_run);
-    if (g4 == 0) {
-        stat[wv][0][l16] = m_run;
-        stat[wv][1][l16] = l_run;
-    }
-    __syncthreads();
-    join_stats<kTileWaves, RB, kRowBlock>(kSixteen<VT>, stat, fac, top, sum);
-    auto& slab = *reinterpret_cast<float(*)[kTileWaves][kOct][HD]>(pool);
-#pragma unroll
-    for (int oct = 0; oct < kRowBlock / kOct; ++oct) {
-        if ((g4 >> 1) == oct) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int e = 0; e < NE; ++e) slab[wv][4 * (g4 & 1) + r][16 * e + l16] = o[e][r];
+    if constexpr (PB > 1) {
+        if (g4 == 0) {
+            stat[wv][0][l16] = m_run;
+            stat[wv][1][l16] = l_run;
         }
+        auto& slab = *reinterpret_cast<float(*)[kTileWaves][kRowBlock][HD]>(pool);   // the tiles are read
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < NE; ++e) slab[wv][4 * g4 + r][16 * e + l16] = o[e][r];
         __syncthreads();
-        join_rows<HD, kTileWaves, RB, kRowBlock>(a, w, slab, fac, top, sum, oct);
+        join_stats<kTileWaves, RB, kRowBlock>(kSixteen<VT>, stat, fac, top, sum);
         __syncthreads();
+        join_rows<HD, kTileWaves, RB, kRowBlock>(a, w, slab, fac, top, sum);
+    } else {
+        // one part: the wave's rows straight from its registers, 16 dims of four rows an instruction
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int rw = row0 + 4 * g4 + r, t = min(rw, a.rows - 1) / G, h = kv * G + min(rw, a.rows - 1) - t * G;
+            const float m = __shfl(m_run, 4 * g4 + r, 64), l = __shfl(l_run, 4 * g4 + r, 64);
+            if (!a.direct) {
+                const size_t rec = (static_cast<size_t>(w.chunk) * a.n_kv + kv) * a.rows_pad + rw;
+                if (rw < a.rows) {
+#pragma unroll
+                    for (int e = 0; e < NE; ++e) a.wo[rec * HD + 16 * e + l16] = o[e][r] * kSixteen<VT>;
+                    if (l16 == 0) *reinterpret_cast<float2*>(a.wml + 2 * rec) = make_float2(m, l);
+                }
+                continue;
+            }
+            float g[NE];
+#pragma unroll
+            for (int e = 0; e < NE; ++e) g[e] = a.gate ? a.gate[static_cast<size_t>(t) * a.gate_stride + h * 2 * HD + HD + 16 * e + l16] : 0.0f;
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+                float v = m == -INFINITY ? 0.0f : o[e][r] * kSixteen<VT> / l;
+                if (a.gate) v *= 1.0f / (1.0f + expf(-g[e]));
+                o[e][r] = v;
+                if (a.y && rw < a.rows) a.y[static_cast<size_t>(t) * a.y_stride + h * HD + 16 * e + l16] = v;
+            }
+            if (!a.q8) continue;
+#pragma unroll
+            for (int e = 0; e < NE; e += 2) {   // q8_1_store_lane's block and bits: its lane's element is 16 (e % 2) + l16 here
+                const float u = o[e][r], v = o[e + 1][r];
+                const float amax = group_max<16>(fmaxf(fabsf(u), fabsf(v))), total = group_sum<16>(u + v), dq = amax / 127.0f;
+                uint8_t* block = a.q8 + static_cast<size_t>(t) * a.q8_stride + (h * (HD / 32) + e / 2) * kQ8_1Bytes;
+                if (rw < a.rows) {
+                    block[4 + l16] = static_cast<uint8_t>(static_cast<int8_t>(amax == 0.0f ? 0 : static_cast<int>(roundf(u / dq))));
+                    block[20 + l16] = static_cast<uint8_t>(static_cast<int8_t>(amax == 0.0f ? 0 : static_cast<int>(roundf(v / dq))));
+                    if (l16 == 0) *reinterpret_cast<uint32_t*>(block) = float_to_half_sat(dq) | (float_to_half_sat(total) << 16);
+                }
+            }
+        }
     }
 }
 
@@ -1003,15 +1080,18 @@ bool tree_shape_ok(int max_ctx, int n_head, int n_kv, int head_dim, int ntok) {
 }
 
 // the form of a call: query rows per KV head, 16-row blocks side by side in a workgroup (0: the form of few rows), rows a
-// workgroup holds, workgroups per (chunk, KV head)
+// workgroup holds, workgroups per (chunk, KV head).  17 to 32 rows are two groups of few rows, which begin and end sooner,
+// or over long chunks a tile, which turns K and V to fp16 once: I8, 8 tokens x 4 heads behind 4K 14.4 / 17.6 us, 32K
+// 31.7 / 30.7, 64K 50.7 / 47.4 (F16 84 / 64).
+constexpr int kLongSub = 6;
 struct Form {
     int rows, rb, held, groups;
 };
-Form tree_form(int n_head, int n_kv, int ntok) {
+Form tree_form(int n_head, int n_kv, int ntok, long long nsub) {
     Form f;
     f.rows = ntok * (n_head / n_kv);
-    f.rb = f.rows <= kFewRows ? 0 : f.rows <= 32 ? 2 : f.rows <= 64 ? 4 : 8;
-    f.held = f.rb ? kRowBlock * f.rb : kFewRows;
+    f.rb = f.rows <= 16 ? 0 : f.rows <= 32 ? (nsub >= kLongSub ? 2 : 0) : f.rows <= 64 ? 4 : 8;
+    f.held = f.rb ? kRowBlock * f.rb : f.rows <= 8 ? 8 : 16;
     f.groups = (f.rows + f.held - 1) / f.held;
     return f;
 }
@@ -1021,20 +1101,21 @@ long long tree_chunks(int max_ctx, int nsub) {
 }
 
 template <int KT, int VT, int HD>
-void launch_partial(const TreeArgs& a, int rb, unsigned blocks, hipStream_t s) {
+void launch_partial(const TreeArgs& a, const Form& f, unsigned blocks, hipStream_t s) {
     auto go = [&](auto* kernel, int threads) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, s, a); };
-    if (rb == 0) go(&tree_few_kernel<KT, VT, HD>, kThreads);
-    else if (rb == 2) go(&tree_tile_kernel<KT, VT, HD, 2>, kTileThreads);
-    else if (rb == 4) go(&tree_tile_kernel<KT, VT, HD, 4>, kTileThreads);
+    if (f.held == 8) go(&tree_few_kernel<KT, VT, HD, 8>, kThreads);
+    else if (f.held == 16) go(&tree_few_kernel<KT, VT, HD, 16>, kThreads);
+    else if (f.rb == 2) go(&tree_tile_kernel<KT, VT, HD, 2>, kTileThreads);
+    else if (f.rb == 4) go(&tree_tile_kernel<KT, VT, HD, 4>, kTileThreads);
     else go(&tree_tile_kernel<KT, VT, HD, 8>, kTileThreads);
 }
 
 template <int HD>
-void launch_tree(const TreeArgs& a, int ktype, int vtype, int rb, unsigned blocks, hipStream_t s) {
-    if (ktype == kKvF16) launch_partial<kKvF16, kKvF16, HD>(a, rb, blocks, s);
-    else if (ktype == kKvI4) launch_partial<kKvI4, kKvI4, HD>(a, rb, blocks, s);
-    else if (vtype == kKvI8) launch_partial<kKvI8, kKvI8, HD>(a, rb, blocks, s);
-    else launch_partial<kKvI8, kKvI4, HD>(a, rb, blocks, s);
+void launch_tree(const TreeArgs& a, int ktype, int vtype, const Form& f, unsigned blocks, hipStream_t s) {
+    if (ktype == kKvF16) launch_partial<kKvF16, kKvF16, HD>(a, f, blocks, s);
+    else if (ktype == kKvI4) launch_partial<kKvI4, kKvI4, HD>(a, f, blocks, s);
+    else if (vtype == kKvI8) launch_partial<kKvI8, kKvI8, HD>(a, f, blocks, s);
+    else launch_partial<kKvI8, kKvI4, HD>(a, f, blocks, s);
     if (a.npairs / a.n_kv > kFlatChunks)
         hipLaunchKernelGGL((tree_merge_kernel<HD>), dim3(a.ntok, a.n_head, HD / kMergeDims), dim3(kThreads), 0, s, a);
     else if (!a.direct)
@@ -1051,10 +1132,19 @@ extern "C" int rmi_gqa_tree_nsub(int ctx, int n_head, int n_kv, int head_dim, in
         set_error("gqa_tree_nsub: invalid shape");
         return 0;
     }
-    // a workgroup a compute unit
-    const long long groups = tree_form(n_head, n_kv, ntok).groups, units = (ctx + kUnit - 1) / kUnit;
-    const long long want = (units * n_kv * groups + 255) / 256;
-    return static_cast<int>(std::max(std::max(1LL, (units + kMaxChunks - 1) / kMaxChunks), std::min(units, want)));
+    // At least a workgroup for each of 256 compute units, from chunks as long as that leaves; long contexts of the form of few
+    // rows two (they hide each other's waits), but not at less than four steps a wave, where a workgroup's own beginning and
+    // end weigh more.  I8, 1 / 8 tokens at 16 heads: 64K at 512 / 256 workgroups 35.4 / 38.6 and 50.7 / 57.1 us, 16K (8
+    // tokens) 24.0 / 21.9 us; 4K at 128 / 64 workgroups of the one and two steps 12.6 / 14.7 us.
+    const long long units = (ctx + kUnit - 1) / kUnit;
+    auto split = [&](const Form& f) {
+        const long long work = units * n_kv * f.groups, want = (work + 255) / 256;
+        return std::min(units, f.rb ? want : std::max((work + 511) / 512, std::min(want, 4LL)));
+    };
+    long long nsub = split(tree_form(n_head, n_kv, ntok, 1));
+    const Form f = tree_form(n_head, n_kv, ntok, nsub);
+    if (f.rb == 2) nsub = std::max<long long>(kLongSub, split(f));
+    return static_cast<int>(std::max({1LL, (units + kMaxChunks - 1) / kMaxChunks, nsub}));
 }
 
 extern "C" size_t rmi_gqa_tree_workspace_bytes(int max_ctx, int n_head, int n_kv, int head_dim, int ntok, int nsub) {
@@ -1062,7 +1152,7 @@ extern "C" size_t rmi_gqa_tree_workspace_bytes(int max_ctx, int n_head, int n_kv
         set_error("gqa_tree_workspace_bytes: invalid shape");
         return 0;
     }
-    const Form f = tree_form(n_head, n_kv, ntok);
+    const Form f = tree_form(n_head, n_kv, ntok, nsub);
     return static_cast<size_t>(tree_chunks(max_ctx, nsub)) * n_kv * (static_cast<size_t>(f.groups) * f.held) * (head_dim + 2) * sizeof(float);
 }
 
@@ -1079,7 +1169,7 @@ extern "C" int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache
         (masks && (reinterpret_cast<uintptr_t>(masks) & 7u)) || (gate_src && !aligned4(gate_src)) || (!y && !q8) ||
         (y && !aligned4(y)) || (q8 && (!aligned4(q8) || q8_stride % 4)))
         return fail(RMI_ERR_POINTER, "gqa_tree_decode: null or misaligned pointer");
-    const Form f = tree_form(n_head, n_kv, ntok);
+    const Form f = tree_form(n_head, n_kv, ntok, nsub);
     TreeArgs a{};
     a.q = q;
     a.kc = static_cast<const uint8_t*>(kcache);
@@ -1108,7 +1198,7 @@ extern "C" int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache
     a.wo = static_cast<float*>(workspace);
     a.wml = a.wo + static_cast<size_t>(pairs) * a.rows_pad * head_dim;
     auto* s = static_cast<hipStream_t>(stream);
-    if (head_dim == 256) launch_tree<256>(a, ktype, vtype, f.rb, static_cast<unsigned>(blocks), s);
-    else launch_tree<128>(a, ktype, vtype, f.rb, static_cast<unsigned>(blocks), s);
+    if (head_dim == 256) launch_tree<256>(a, ktype, vtype, f, static_cast<unsigned>(blocks), s);
+    else launch_tree<128>(a, ktype, vtype, f, static_cast<unsigned>(blocks), s);
     return launch_status("gqa_tree_decode");
 }

@@ -86,7 +86,7 @@ def test_trees(rmi, types, nh, nkv, hd, ntok, base):
 
 
 @pytest.mark.parametrize("types", PAIRS, ids=IDS)
-@pytest.mark.parametrize("ntok,base,nsub", [(1, 0, 1), (1, 999, 1), (2, 1023, 2), (7, 255, 1), (33, 100, 1), (64, 64, 3), (65, 0, 1), (130, 515, 2)])
+@pytest.mark.parametrize("ntok,base,nsub", [(5, 1700, 6), (8, 1500, 7), (1, 0, 1), (1, 999, 1), (2, 1023, 2), (7, 255, 1), (33, 100, 1), (64, 64, 3), (65, 0, 1), (130, 515, 2)])
 def test_chains(rmi, types, ntok, base, nsub):
     Call(rmi, types, 8, 2, 256, ntok, base, None, seed=ntok, nsub=nsub).check()
 
