@@ -527,7 +527,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
         mloc = fmaxf(mloc, xor_lane<32>(mloc));
         const float m_new = mloc > m_run + kLazy ? mloc : m_run;
         const float m_ref = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: exp2(-inf) = 0, no NaN
-        const float alpha = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_ref);
+        const float alpha = m_run == m_new || m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_ref);   // -inf: o is 0
         float p[8], lsum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -621,13 +621,22 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
         stat[wv][1][slot] = l_run;
     }
     if constexpr (!PACKED) __syncthreads();   // q's operands are read
-    if constexpr (PACKED) {   // high rows + low rows: lanes g4 < 2 end with o[row 4 g4 + r]
+    if constexpr (PACKED) {
+        // high rows + low rows, two registers at a time: a swap of a's upper and b's lower lanes, then one add, leaves a's sums
+        // in the lower lanes (row 4 g4 + r) and b's in the upper (row 4 (g4 - 2) + r + 1)
 #pragma unroll
-        for (int e = 0; e < VD; ++e)
+        for (int r = 0; r < 4; r += 2) {
+            float v[VD];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[e][r] += xor_lane<32>(o[e][r]);
-    }
-    if (!PACKED || g4 < 2) {
+            for (int e = 0; e < VD; ++e) {
+                const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[e][r]), __float_as_uint(o[e][r + 1]), false, false);
+                v[e] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+            }
+            float* to = &slab[wv][4 * (g4 & 1) + r + (g4 >> 1)][VD * l16];
+#pragma unroll
+            for (int e = 0; e < VD; e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+        }
+    } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -841,7 +850,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
             mloc = fmaxf(mloc, xor_lane<32>(mloc));
             const float m_new = mloc > m_run + kLazy ? mloc : m_run;
             const float m_ref = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: exp2(-inf) = 0, no NaN
-            const float alpha = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_ref);
+            const float alpha = m_run == m_new || m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_ref);   // -inf: o is 0
             float p[8], lsum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
