@@ -174,12 +174,23 @@ def _p(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+_raw_stream = None   # torch's current stream handle, once its GPU state exists
+
+
+def _current_stream():
+    global _raw_stream
+    import torch
+    s = torch.cuda.current_stream().cuda_stream
+    if torch.cuda.is_initialized() and hasattr(torch._C, "_cuda_getCurrentRawStream"):
+        # the handle itself: current_stream() builds a Stream object for it at every call, 3 us
+        device, raw = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
+        _raw_stream = lambda: raw(device())  # noqa: E731
+    return s
+
+
 def _stream(stream):
     if stream is None:
-        import torch
-        if torch.cuda.is_initialized():   # the raw handle: current_stream() builds a Stream object for it, 3 us
-            return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
-        return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        return ctypes.c_void_p(_raw_stream() if _raw_stream else _current_stream())
     if isinstance(stream, int):
         return ctypes.c_void_p(stream)
     return ctypes.c_void_p(stream.cuda_stream)

@@ -70,17 +70,25 @@ __device__ __forceinline__ uint32_t kv_scale_byte(uint32_t amax_bits) {
     return b;
 }
 
-// x / s to the nearest integer, half to even, as if divided exactly: the candidate from the reciprocal is off by at most
-// one next to a border, and the remainder x - k s is exact (k s has eleven bits, and the difference is a multiple of x's
-// last place no larger than x, or x itself at k = 0).
-template <int T>
-__device__ __forceinline__ int kv_code(float x, float s, float inv) {
+// 1 / s in two parts (inv + rest, exact to 2^-46)
+__device__ __forceinline__ float kv_inverse_rest(float s, float inv) { return __builtin_fmaf(-inv, s, 1.0f) * inv; }
+
+// code + bias, in the result's low byte: x / s to the nearest integer, half to even, as if divided exactly.  The two-part
+// inverse gives x / s rounded to fp32 once, y.  Where y is no half-integer, rounding y is rounding x / s; where it is one, the
+// remainder x - y s (exact: y s has 12 bits) tells whether x / s is.  For x that are fp16 numbers (X16) it always is: x / s is
+// a multiple of 2^-12 of itself over a divisor of at most 15, so nothing but a tie comes near one.
+template <int T, bool X16 = false>
+__device__ __forceinline__ uint32_t kv_code(float x, float s, float inv, float rest) {
     constexpr float kQ = static_cast<float>(kv_qmax(T));
-    if (!(s > 0.0f)) return 0;   // an empty block, or a NaN scale
-    float k = fminf(fmaxf(__builtin_rintf(x * inv), -kQ), kQ);
-    const float r = __builtin_fmaf(-k, s, x), a = fabsf(r), half = 0.5f * s;
-    if (a > half || (a == half && (static_cast<int>(k) & 1))) k += r > 0.0f ? 1.0f : -1.0f;
-    return static_cast<int>(fminf(fmaxf(k, -kQ), kQ));
+    float y = __builtin_fmaf(x, inv, x * rest);
+    if constexpr (!X16) {
+        if (__builtin_amdgcn_fractf(fabsf(y)) == 0.5f) {
+            const float r = __builtin_fmaf(-y, s, x);
+            y += r > 0.0f ? 0.25f : r < 0.0f ? -0.25f : 0.0f;
+        }
+    }
+    const float k = __builtin_amdgcn_fmed3f(y, -kQ, kQ) + (8388608.0f + kv_bias(T));   // rounds to an integer, half to even
+    return s > 0.0f ? __float_as_uint(k) : static_cast<uint32_t>(kv_bias(T));          // an empty block, or a NaN scale: 0
 }
 
 // where code + bias of dim d goes in the word of its eight dims (I4)

@@ -7,6 +7,7 @@
 #include "kv_cache.h"
 #include "rope.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace rmi {
@@ -81,56 +82,73 @@ __device__ __forceinline__ void store8(void* out, size_t e, const F8& x) {
 
 constexpr int kRowThreads = 256;
 
-template <int T, bool SRC16, bool VEC>
-__global__ __launch_bounds__(kRowThreads) void kv_write_kernel(const void* __restrict__ src, int src_stride,
-                                                               uint8_t* __restrict__ cache, int first, size_t units,
-                                                               int n_kv, int head_dim, int max_ctx) {
-    const size_t u = static_cast<size_t>(blockIdx.x) * kRowThreads + threadIdx.x;
-    if (u >= units) return;   // units is a multiple of 16 (a row): the lanes of a block stay or go together
-    const int per = head_dim >> 3;                       // units per (position, head) row
-    const size_t hr = u / per;
-    const int g = static_cast<int>(u - hr * per);        // eight dims 8 g ..
-    const int row = static_cast<int>(hr / n_kv), kv = static_cast<int>(hr - static_cast<size_t>(row) * n_kv);
-    const F8 x = load8<SRC16, VEC>(src, static_cast<size_t>(row) * src_stride + kv * head_dim + 8 * g);
-    const KvRow<T> at = kv_row<T>(first + row, kv, n_kv, max_ctx, head_dim);
+// eight dims x to unit (row, kv, g) of the cache; the lanes of a row's 16 neighbouring units call together
+template <int T, bool SRC16>
+__device__ __forceinline__ void write_unit(uint8_t* __restrict__ cache, const F8& x, int p, int kv, int g, int n_kv, int head_dim, int max_ctx) {
+    const KvRow<T> at = kv_row<T>(p, kv, n_kv, max_ctx, head_dim);
     if constexpr (T == kKvF16) {
         store8<true, true>(cache + at.code, 8 * g, x);
-        return;
-    }
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x.v[i]) & 0x7fffffffu);
-    m = max(m, xor_lane<1>(m));
-    m = max(m, xor_lane<2>(m));
-    const uint32_t sb = kv_scale_byte<T>(m);
-    const float s = kv_scale_value(sb), inv = 1.0f / s;
-    uint32_t c[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = static_cast<uint32_t>(kv_code<T>(x.v[i], s, inv) + kv_bias(T));
-    if constexpr (T == kKvI8) {
-        *reinterpret_cast<uint2*>(cache + at.code + 8 * g) =
-            make_uint2(c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24), c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24));
     } else {
-        uint32_t w = 0;
+        uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w |= c[i] << kv_i4_shift(i);
-        *reinterpret_cast<uint32_t*>(cache + at.code + 4 * g) = w;
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x.v[i]) & 0x7fffffffu);
+        m = max(m, xor_lane<1>(m));
+        m = max(m, xor_lane<2>(m));
+        const uint32_t sb = kv_scale_byte<T>(m);
+        const float s = kv_scale_value(sb), inv = 1.0f / s;
+        const float rest = kv_inverse_rest(s, inv);
+        uint32_t c[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = kv_code<T, SRC16>(x.v[i], s, inv, rest);
+        if constexpr (T == kKvI8) {
+            // the low bytes of four words: pairs, then pairs of pairs
+            auto pack = [](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                return __builtin_amdgcn_perm(__builtin_amdgcn_perm(a3, a2, 0x0c0c0400u), __builtin_amdgcn_perm(a1, a0, 0x0c0c0400u), 0x05040100u);
+            };
+            *reinterpret_cast<uint2*>(cache + at.code + 8 * g) = make_uint2(pack(c[0], c[1], c[2], c[3]), pack(c[4], c[5], c[6], c[7]));
+        } else {
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w |= (c[i] & 15u) << kv_i4_shift(i);
+            *reinterpret_cast<uint32_t*>(cache + at.code + 4 * g) = w;
+        }
+        uint32_t w = sb | (xor_lane<4>(sb) << 8);   // in the lanes of block 0 of four
+        w |= xor_lane<8>(w) << 16;
+        if ((g & 15) == 0) *reinterpret_cast<uint32_t*>(cache + at.scale + (g >> 2)) = w;
     }
-    uint32_t w = sb | (xor_lane<4>(sb) << 8);   // in the lanes of block 0 of four
-    w |= xor_lane<8>(w) << 16;
-    if ((g & 15) == 0) *reinterpret_cast<uint32_t*>(cache + at.scale + (g >> 2)) = w;
+}
+
+// Workgroup (rows, KV head), a row's heads side by side (together they read whole rows): the head's rows are neighbours in
+// the cache, and no lane divides.  A lane takes units of two rows, both loads out before the first is used.  fp16 to I4, 65501 rows of 1024 dims: 44 us, 3.9 TB/s (the rows read
+// back: 27 us).
+constexpr int kWriteUnits = 2;
+
+template <int T, bool SRC16, bool VEC>
+__global__ __launch_bounds__(kRowThreads) void kv_write_kernel(const void* __restrict__ src, int src_stride,
+                                                               uint8_t* __restrict__ cache, int first, int n, int n_kv,
+                                                               int head_dim, int max_ctx) {
+    const int shift = head_dim == 256 ? 5 : 4, up = kRowThreads >> shift;   // units per row 2^shift, rows a unit of the lane is further
+    const int rows = blockIdx.x / n_kv, kv = blockIdx.x - rows * n_kv;
+    const int g = static_cast<int>(threadIdx.x) & ((1 << shift) - 1);   // eight dims 8 g ..
+    const int row0 = rows * (kWriteUnits * up) + (static_cast<int>(threadIdx.x) >> shift);
+    F8 x[kWriteUnits];
+#pragma unroll
+    for (int k = 0; k < kWriteUnits; ++k)
+        x[k] = load8<SRC16, VEC>(src, static_cast<size_t>(min(row0 + k * up, n - 1)) * src_stride + kv * head_dim + 8 * g);
+#pragma unroll
+    for (int k = 0; k < kWriteUnits; ++k)   // a row's lanes stay or go together
+        if (row0 + k * up < n) write_unit<T, SRC16>(cache, x[k], first + row0 + k * up, kv, g, n_kv, head_dim, max_ctx);
 }
 
 template <int T, bool OUT16, bool VEC>
 __global__ __launch_bounds__(kRowThreads) void kv_read_kernel(const uint8_t* __restrict__ cache, void* __restrict__ out,
-                                                              int out_stride, int first, size_t units, int n_kv,
-                                                              int head_dim, int max_ctx) {
-    const size_t u = static_cast<size_t>(blockIdx.x) * kRowThreads + threadIdx.x;
-    if (u >= units) return;
-    const int per = head_dim >> 3;
-    const size_t hr = u / per;
-    const int g = static_cast<int>(u - hr * per);
-    const int row = static_cast<int>(hr / n_kv), kv = static_cast<int>(hr - static_cast<size_t>(row) * n_kv);
+                                                              int out_stride, int first, int n, int n_kv, int head_dim,
+                                                              int max_ctx) {
+    const int shift = head_dim == 256 ? 5 : 4;
+    const int rows = blockIdx.x / n_kv, kv = blockIdx.x - rows * n_kv;
+    const int g = static_cast<int>(threadIdx.x) & ((1 << shift) - 1);
+    const int row = rows * (kRowThreads >> shift) + (static_cast<int>(threadIdx.x) >> shift);
+    if (row >= n) return;
     const KvRow<T> at = kv_row<T>(first + row, kv, n_kv, max_ctx, head_dim);
     F8 x;
     if constexpr (T == kKvF16) {
@@ -207,11 +225,10 @@ __global__ __launch_bounds__(256) void kv_compact_kernel(CachePtrs caches, const
 }
 
 // ---- norm, rotation, cache write ------------------------------------------------------------------------------------------
-// Workgroup (token, part): the token's (cos, sin) per pair once into LDS, then a wave per head row, lane l holding dims
-// l + 64 k: the norm is attn_prep's tree (a 64-lane butterfly per 64 dims, summed in order), the rotation's partner comes
-// through the wave's LDS row.  K rows that are quantised go through the same steps in fp64.  A scale block is 32 lanes at
-// one k.  `per_wave` rows a wave: one for few tokens (latency), all of the token's rows on four waves for many, where the
-// fp64 angles of a workgroup are then shared by all heads.
+// Workgroup (token, part): the token's (cos, sin) per pair once into LDS, then a wave per head row, a lane HD / 64 neighbouring
+// dims; a row's loads go out before the work on the row before it.  q: attn_prep's arithmetic and bits.  K: the same steps in
+// fp64, rounded to fp32 once, so what the cache holds does not hang on the order of a sum.  The rotation's partner comes
+// through the wave's LDS row; a scale block is 8 (HD 256) or 16 lanes.
 constexpr int kPrepWaves = 4;
 
 struct PrepArgs {
@@ -244,37 +261,81 @@ __device__ __forceinline__ double group_sum64(double v) {
     return v;
 }
 
-// the wave's row (lane: dims lane + 64 k) into position p of a cache
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));   // rows of a caller's stride
+typedef float float2u __attribute__((ext_vector_type(2), aligned(4)));
+
+template <int N>
+__device__ __forceinline__ void load_dims(float (&x)[N], const float* p) {
+    if constexpr (N == 4) {
+        const float4u v = *reinterpret_cast<const float4u*>(p);
+        x[0] = v[0], x[1] = v[1], x[2] = v[2], x[3] = v[3];
+    } else {
+        const float2u v = *reinterpret_cast<const float2u*>(p);
+        x[0] = v[0], x[1] = v[1];
+    }
+}
+
+// the sum of the squares of a row, as attn_prep takes it: per 64 dims a butterfly over the dim's bits from 32 down (its first
+// step contracted: fma(x_d, x_d, x_{d + 32}^2) for d < 32), the 64-dim sums in order.  A dim's low bits are its place in
+// the lane.
+template <int N>
+__device__ __forceinline__ float square_sum(const float (&x)[N]) {
+    constexpr int L = 32 / N;   // lanes between d and d + 32
+    float v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = __builtin_fmaf(x[j], x[j], xor_lane<L>(x[j] * x[j]));
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        if constexpr (L > 8) v[j] += xor_lane<8>(v[j]);
+        if constexpr (L > 4) v[j] += xor_lane<4>(v[j]);
+        v[j] += xor_lane<2>(v[j]);
+        v[j] += xor_lane<1>(v[j]);
+    }
+    const float s = N == 4 ? (v[0] + v[2]) + (v[1] + v[N - 1]) : v[0] + v[1];
+    float t = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 64 / (2 * L); ++k) t += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s), 2 * L * k));
+    return t;
+}
+
+// the wave's row (lane: dims N lane + 0 .. N - 1) into position p of a cache
 template <int T, int HD>
 __device__ __forceinline__ void store_row(const float (&x)[HD / 64], uint8_t* cache, int p, int kv, int n_kv, int max_ctx,
                                           int lane) {
+    constexpr int N = HD / 64;
     const KvRow<T> at = kv_row<T>(p, kv, n_kv, max_ctx, HD);
+    const int d = N * lane;
+    if constexpr (T == kKvF16) {
+        uint32_t w[N / 2];
 #pragma unroll
-    for (int k = 0; k < HD / 64; ++k) {
-        const int d = lane + 64 * k;
-        if constexpr (T == kKvF16) {
-            reinterpret_cast<uint16_t*>(cache + at.code)[d] = static_cast<uint16_t>(half_bits(x[k]));
-        } else {
-            uint32_t m = __float_as_uint(x[k]) & 0x7fffffffu;
-            m = max(m, xor_lane<16>(m));
-            m = max(m, xor_lane<8>(m));
-            m = max(m, xor_lane<4>(m));
-            m = max(m, xor_lane<2>(m));
-            m = max(m, xor_lane<1>(m));
-            const uint32_t sb = kv_scale_byte<T>(m);
-            const float s = kv_scale_value(sb);
-            const uint32_t c = static_cast<uint32_t>(kv_code<T>(x[k], s, 1.0f / s) + kv_bias(T));
-            if constexpr (T == kKvI8) {
-                cache[at.code + d] = static_cast<uint8_t>(c);
-            } else {
-                uint32_t w = c << kv_i4_shift(d);
-                w |= xor_lane<1>(w);
-                w |= xor_lane<2>(w);
-                w |= xor_lane<4>(w);
-                if ((d & 7) == 0) *reinterpret_cast<uint32_t*>(cache + at.code + d / 2) = w;
-            }
-            if ((d & 31) == 0) cache[at.scale + d / 32] = static_cast<uint8_t>(sb);
+        for (int j = 0; j < N; j += 2) w[j / 2] = half_bits(x[j]) | (half_bits(x[j + 1]) << 16);
+        if constexpr (N == 4) *reinterpret_cast<uint2*>(cache + at.code + 2 * d) = make_uint2(w[0], w[N / 2 - 1]);
+        else *reinterpret_cast<uint32_t*>(cache + at.code + 2 * d) = w[0];
+    } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+        if constexpr (N == 2) m = max(m, xor_lane<8>(m));
+        m = max(m, xor_lane<4>(m));
+        m = max(m, xor_lane<2>(m));
+        m = max(m, xor_lane<1>(m));
+        const uint32_t sb = kv_scale_byte<T>(m);
+        const float s = kv_scale_value(sb), inv = 1.0f / s, rest = kv_inverse_rest(s, inv);
+        uint32_t w = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t c = kv_code<T>(x[j], s, inv, rest) & (T == kKvI8 ? 0xffu : 0xfu);
+            w |= c << (T == kKvI8 ? 8 * j : kv_i4_shift(d + j));
         }
+        if constexpr (T == kKvI8) {
+            if constexpr (N == 4) *reinterpret_cast<uint32_t*>(cache + at.code + d) = w;
+            else *reinterpret_cast<uint16_t*>(cache + at.code + d) = static_cast<uint16_t>(w);
+        } else {
+            w |= xor_lane<1>(w);
+            if constexpr (N == 2) w |= xor_lane<2>(w);
+            if ((d & 7) == 0) *reinterpret_cast<uint32_t*>(cache + at.code + d / 2) = w;
+        }
+        if ((d & 31) == 0) cache[at.scale + d / 32] = static_cast<uint8_t>(sb);
     }
 }
 
@@ -282,83 +343,86 @@ template <int KT, int VT, int HD>
 __global__ __launch_bounds__(64 * kPrepWaves) void prep_axes_kernel(PrepArgs a) {
     constexpr int N = HD / 64;
     __shared__ double cs[HD / 2][2];
-    __shared__ double rows[kPrepWaves][HD];
-    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    __shared__ float2 csf[HD / 2];   // rounded, for q
+    __shared__ __attribute__((aligned(16))) double rows[kPrepWaves][HD];
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), d0 = N * lane;
     const int base = a.pos[0], half = a.n_rot / 2;
+    const float* src = a.q3 + static_cast<size_t>(t) * a.q3_stride;
+    const int items = a.n_head + 2 * a.n_kv, first = (blockIdx.y * kPrepWaves + wv) * a.per_wave;
+    const int end = min(first + a.per_wave, items);
+    float nx[N], wq[N], wk[N];   // nx: the next row
+    auto load = [&](int it) {
+        it = min(it, items - 1);
+        load_dims(nx, (it < a.n_head ? src + it * 2 * HD : src + 2 * a.n_head * HD + (it - a.n_head) * HD) + d0);   // [q | gate] .., k, v
+    };
+    load(first);
+    load_dims(wq, a.qn + d0);
+    load_dims(wk, a.kn + d0);
     if (base < -t || base >= a.max_ctx - t) return;   // uniform: a slot outside the cache stores nothing
     const int p = base + t;
     if (tid < half) {
         const int ap = a.axis_pos ? a.axis_pos[static_cast<size_t>(rope_axis(a.axes, tid)) * a.ntok + t] : p;
-        rope_cos_sin_d(ap, rope_freq(tid, a.n_rot, a.theta), tid, a.yarn, &cs[tid][0], &cs[tid][1]);
+        double c, s;
+        rope_cos_sin_d(ap, rope_freq(tid, a.n_rot, a.theta), tid, a.yarn, &c, &s);
+        cs[tid][0] = c;
+        cs[tid][1] = s;
+        csf[tid] = make_float2(static_cast<float>(c), static_cast<float>(s));
     }
     __syncthreads();
-    const float* src = a.q3 + static_cast<size_t>(t) * a.q3_stride;
-    const int items = a.n_head + 2 * a.n_kv, first = (blockIdx.y * kPrepWaves + wv) * a.per_wave;
-    for (int it = first; it < min(first + a.per_wave, items); ++it) {
-        const bool is_q = it < a.n_head, is_v = it >= a.n_head + a.n_kv;
-        const int kv = is_v ? it - a.n_head - a.n_kv : it - a.n_head;
-        const float* row = is_q ? src + it * 2 * HD : src + 2 * a.n_head * HD + ((is_v ? a.n_kv : 0) + kv) * HD;
+    for (int it = first; it < end; ++it) {
         float x[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) x[k] = row[lane + 64 * k];
-        if (is_v) {
-            store_row<VT, HD>(x, a.vc, p, kv, a.n_kv, a.max_ctx, lane);
-            continue;
-        }
-        const float* w = is_q ? a.qn : a.kn;
-        if (is_q || KT == kKvF16) {
+        for (int j = 0; j < N; ++j) x[j] = nx[j];
+        if (it + 1 < end) load(it + 1);
+        if (it >= a.n_head + a.n_kv) {
+            store_row<VT, HD>(x, a.vc, p, it - a.n_head - a.n_kv, a.n_kv, a.max_ctx, lane);
+        } else if (it < a.n_head) {
             float* xs = reinterpret_cast<float*>(rows[wv]);
-            float ss = 0.0f;
+            const float inv = rsqrtf(square_sum<N>(x) / static_cast<float>(HD) + a.eps);
 #pragma unroll
-            for (int k = 0; k < N; ++k)   // lane 0's sum, as attn_prep takes it
-                ss += __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(group_sum<64>(x[k] * x[k]))));
-            const float inv = rsqrtf(ss / static_cast<float>(HD) + a.eps);
-#pragma unroll
-            for (int k = 0; k < N; ++k) {
-                x[k] = x[k] * inv * w[lane + 64 * k];
-                xs[lane + 64 * k] = x[k];
+            for (int j = 0; j < N; ++j) {
+                x[j] = x[j] * inv * wq[j];
+                xs[d0 + j] = x[j];
             }
             wave_lds_sync();
+            if (d0 < a.n_rot) {
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
-                const int d = lane + 64 * k;
-                if (d < a.n_rot) {
-                    const int i = d < half ? d : d - half;
-                    const float c = static_cast<float>(cs[i][0]), s = static_cast<float>(cs[i][1]);
-                    x[k] = d < half ? rope_lo(x[k], xs[d + half], c, s) : rope_hi(xs[d - half], x[k], c, s);
+                for (int j = 0; j < N; ++j) {
+                    const int d = d0 + j;
+                    if (d >= a.n_rot) break;
+                    const float2 e = csf[d < half ? d : d - half];
+                    x[j] = d < half ? rope_lo(x[j], xs[d + half], e.x, e.y) : rope_hi(xs[d - half], x[j], e.x, e.y);
                 }
             }
             wave_lds_sync();   // the next row overwrites the exchange
-            if (is_q) {
-#pragma unroll
-                for (int k = 0; k < N; ++k)
-                    a.qout[(static_cast<size_t>(t) * a.n_head + it) * HD + lane + 64 * k] = x[k];
-            } else {
-                store_row<KT, HD>(x, a.kc, p, kv, a.n_kv, a.max_ctx, lane);
-            }
+            float* to = a.qout + (static_cast<size_t>(t) * a.n_head + it) * HD + d0;
+            if constexpr (N == 4) *reinterpret_cast<float4u*>(to) = float4u{x[0], x[1], x[2], x[N - 1]};
+            else *reinterpret_cast<float2u*>(to) = float2u{x[0], x[1]};
         } else {
             double* xs = rows[wv];
             double y[N], ss = 0.0;
 #pragma unroll
-            for (int k = 0; k < N; ++k) ss += static_cast<double>(x[k]) * static_cast<double>(x[k]);
+            for (int j = 0; j < N; ++j) ss += static_cast<double>(x[j]) * static_cast<double>(x[j]);
             const double inv = 1.0 / sqrt(group_sum64(ss) / HD + static_cast<double>(a.eps));
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
-                y[k] = static_cast<double>(x[k]) * inv * static_cast<double>(w[lane + 64 * k]);
-                xs[lane + 64 * k] = y[k];
+            for (int j = 0; j < N; ++j) {
+                y[j] = static_cast<double>(x[j]) * inv * static_cast<double>(wk[j]);
+                xs[d0 + j] = y[j];
             }
             wave_lds_sync();
+            if (d0 < a.n_rot) {
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
-                const int d = lane + 64 * k;
-                if (d < a.n_rot) {
+                for (int j = 0; j < N; ++j) {
+                    const int d = d0 + j;
+                    if (d >= a.n_rot) break;
                     const int i = d < half ? d : d - half;
-                    y[k] = d < half ? y[k] * cs[i][0] - xs[d + half] * cs[i][1] : xs[d - half] * cs[i][1] + y[k] * cs[i][0];
+                    y[j] = d < half ? y[j] * cs[i][0] - xs[d + half] * cs[i][1] : xs[d - half] * cs[i][1] + y[j] * cs[i][0];
                 }
-                x[k] = static_cast<float>(y[k]);
             }
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[j] = static_cast<float>(y[j]);
             wave_lds_sync();
-            store_row<KT, HD>(x, a.kc, p, kv, a.n_kv, a.max_ctx, lane);
+            store_row<KT, HD>(x, a.kc, p, it - a.n_head, a.n_kv, a.max_ctx, lane);
         }
     }
 }
@@ -401,15 +465,15 @@ extern "C" int rmi_kv_write(int type, const void* src, int src_f16, int src_stri
                             int n_kv, int head_dim, int max_ctx, void* stream) {
     RMI_TRY(row_args("kv_write: invalid arguments", type, cache, src, src_f16, src_stride, first, n, n_kv, head_dim, max_ctx));
     if (n == 0) return RMI_OK;
-    const size_t units = static_cast<size_t>(n) * n_kv * (head_dim / 8);
-    const size_t blocks = (units + kRowThreads - 1) / kRowThreads;
-    if (blocks > 0x7fffffffu) return fail(RMI_ERR_SHAPE, "kv_write: too many rows for one call");
+    const int per = kWriteUnits * kRowThreads / (head_dim / 8);   // rows a workgroup
+    const long long blocks = (static_cast<long long>(n) + per - 1) / per * n_kv;
+    if (blocks > 0x7fffffffLL) return fail(RMI_ERR_SHAPE, "kv_write: too many rows for one call");
     const bool vec = aligned16(src) && src_stride % (src_f16 ? 8 : 4) == 0;   // 16-byte loads, else one by one
     auto* out = static_cast<uint8_t*>(cache);
     return with_type(type, [&](auto t) {
         auto go = [&](auto* kernel) {
-            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRowThreads), 0, static_cast<hipStream_t>(stream),
-                               src, src_stride, out, first, units, n_kv, head_dim, max_ctx);
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRowThreads), 0, static_cast<hipStream_t>(stream), src,
+                               src_stride, out, first, n, n_kv, head_dim, max_ctx);
             return launch_status("kv_write");
         };
         constexpr int T = decltype(t)::value;
@@ -422,15 +486,15 @@ extern "C" int rmi_kv_read(int type, const void* cache, void* out, int out_f16, 
                            int n_kv, int head_dim, int max_ctx, void* stream) {
     RMI_TRY(row_args("kv_read: invalid arguments", type, cache, out, out_f16, out_stride, first, n, n_kv, head_dim, max_ctx));
     if (n == 0) return RMI_OK;
-    const size_t units = static_cast<size_t>(n) * n_kv * (head_dim / 8);
-    const size_t blocks = (units + kRowThreads - 1) / kRowThreads;
-    if (blocks > 0x7fffffffu) return fail(RMI_ERR_SHAPE, "kv_read: too many rows for one call");
+    const int per = kRowThreads / (head_dim / 8);
+    const long long blocks = (static_cast<long long>(n) + per - 1) / per * n_kv;
+    if (blocks > 0x7fffffffLL) return fail(RMI_ERR_SHAPE, "kv_read: too many rows for one call");
     const bool vec = aligned16(out) && out_stride % (out_f16 ? 8 : 4) == 0;
     const auto* in = static_cast<const uint8_t*>(cache);
     return with_type(type, [&](auto t) {
         auto go = [&](auto* kernel) {
-            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRowThreads), 0, static_cast<hipStream_t>(stream),
-                               in, out, out_stride, first, units, n_kv, head_dim, max_ctx);
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRowThreads), 0, static_cast<hipStream_t>(stream), in,
+                               out, out_stride, first, n, n_kv, head_dim, max_ctx);
             return launch_status("kv_read");
         };
         constexpr int T = decltype(t)::value;
@@ -498,8 +562,9 @@ extern "C" int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* q
     a.eps = eps;
     a.axes = *axes;
     const int items = n_head + 2 * n_kv;
-    // a row per wave up to 64 tokens, then a token per workgroup
-    a.per_wave = ntok <= 64 ? 1 : (items + kPrepWaves - 1) / kPrepWaves;
+    // rows a wave: as many as leave about a thousand workgroups (they share a token's angles), one for few tokens (latency).
+    // 999 tokens, 24 rows each: 1 / 3 / 6 rows a wave 19.6 / 15.9 / 14.4 us
+    a.per_wave = std::min((items + kPrepWaves - 1) / kPrepWaves, static_cast<int>((static_cast<long long>(items) * ntok + 4095) / 4096));
     const int parts = (items + kPrepWaves * a.per_wave - 1) / (kPrepWaves * a.per_wave);
     return with_type(ktype, [&](auto k) {
         return with_type(vtype, [&](auto v) {

@@ -5,7 +5,9 @@
 // One launch, no workspace: a workgroup owns 1024 neighbouring logits and counts the history's tokens among them in LDS
 // (integer adds, so the order does not matter).  A column's text is the shared history plus its path in the draft, and a
 // window that reaches over the path's tokens drops as many of the history's oldest: both are at most 64 single tokens per
-// column, kept as a short list of those in the slice and added to the counts for that column alone.
+// column, kept as a short list of those in the slice and added to the counts for that column alone.  Every workgroup reads
+// the whole history (four ids a lane and load, from the L2): one column of 248320 logits takes 4.8 us behind 4001 tokens and
+// 8.1 behind 20001, bound by the chain length - ids - counts - logits at the first and by those reads at the second.
 #include "rmi_common.h"
 
 #include <cmath>
@@ -16,6 +18,8 @@ namespace {
 constexpr int kSlice = 1024;
 constexpr int kThreads = 256;   // four neighbouring logits each
 constexpr int kMaxDraft = 64;
+
+typedef int int4u __attribute__((ext_vector_type(4), aligned(4)));   // a window begins anywhere
 
 struct LogitsArgs {
     const float* logits;
@@ -42,6 +46,21 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
     __shared__ int any;
     const int tid = threadIdx.x, v0 = blockIdx.x * kSlice, o0 = 4 * tid, v = v0 + o0;
     const int c0 = blockIdx.y * a.per_wg, c1 = min(c0 + a.per_wg, a.ncols);
+    // a column's four logits and the grammar's word, a column ahead
+    float nx[4];
+    uint32_t nok = 0xfu;
+    auto load = [&](int c) {
+        const float* in = a.logits + static_cast<size_t>(c) * a.col_stride + v;
+        if (VEC && v + 3 < a.n) {
+            const float4 f = *reinterpret_cast<const float4*>(in);
+            nx[0] = f.x, nx[1] = f.y, nx[2] = f.z, nx[3] = f.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nx[i] = v + i < a.n ? in[i] : 0.0f;
+        }
+        if (a.allow && v < a.n) nok = a.allow[static_cast<size_t>(c) * a.allow_stride + (v >> 5)] >> (v & 31);
+    };
+    load(c0);
     *reinterpret_cast<int4*>(cnt + o0) = make_int4(0, 0, 0, 0);
     *reinterpret_cast<int4*>(bidx + o0) = make_int4(-1, -1, -1, -1);
     if (tid == 0) any = 0;
@@ -60,10 +79,21 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
         adj[tid] = in ? off : -1;
         if (in) any = 1;   // every writer stores the same value
     }
-    for (int i = start + tid; i < len; i += kThreads) {
-        const unsigned off = static_cast<unsigned>(a.history[i]) - static_cast<unsigned>(v0);
+    auto count = [&](int id) {
+        const unsigned off = static_cast<unsigned>(id) - static_cast<unsigned>(v0);
         if (off < kSlice) atomicAdd(&cnt[off], 1);
+    };
+    const int* hist = a.history + start;
+    const int nh = len - start, whole = nh & ~3;
+#pragma unroll 4
+    for (int i = 4 * tid; i < whole; i += 4 * kThreads) {
+        const int4u h = *reinterpret_cast<const int4u*>(hist + i);
+        count(h[0]);
+        count(h[1]);
+        count(h[2]);
+        count(h[3]);
     }
+    if (tid < nh - whole) count(hist[whole + tid]);
     for (int i = tid; i < a.n_bias; i += kThreads) {
         const unsigned off = static_cast<unsigned>(a.bias_ids[i]) - static_cast<unsigned>(v0);
         if (off < kSlice) atomicMax(&bidx[off], i);
@@ -78,18 +108,9 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
     const bool biased[4] = {bi.x >= 0, bi.y >= 0, bi.z >= 0, bi.w >= 0};
     const bool adjust = any != 0;   // uniform
     for (int c = c0; c < c1; ++c) {
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const float* in = a.logits + static_cast<size_t>(c) * a.col_stride + v;
-        if (VEC && v + 3 < a.n) {
-            const float4 f = *reinterpret_cast<const float4*>(in);
-            x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (v + i < a.n) x[i] = in[i];
-        }
-        uint32_t ok = 0xfu;
-        if (a.allow && v < a.n) ok = a.allow[static_cast<size_t>(c) * a.allow_stride + (v >> 5)] >> (v & 31);
+        float x[4] = {nx[0], nx[1], nx[2], nx[3]};
+        const uint32_t ok = nok;
+        if (c + 1 < c1) load(c + 1);
         int delta = 0, doff = -1;
         if (adjust) {
             if (tid < 2 * kMaxDraft) {
@@ -175,10 +196,15 @@ extern "C" int rmi_logits_process(const float* logits, int n, int ncols, int col
     a.n_bias = n_bias;
     a.allow = allow;
     a.allow_stride = allow_stride;
-    a.per_wg = 4;
+    // columns a workgroup: they share its counts, but about 2000 workgroups are needed to hide a column's latency.  248320
+    // logits, history 1999, 1 / 2 / 4 / 8 columns a workgroup: 16 columns 11.9 / 9.7 / 10.6 / 14.1 us (3.3 TB/s at the
+    // rule's 2), 64 columns 43.8 / 34.8 / 31.1 / 29.7 (4.3 TB/s at 8)
+    const int slices = (n + kSlice - 1) / kSlice;
+    a.per_wg = static_cast<int>((static_cast<long long>(ncols) * slices + 2047) / 2048);
+    a.per_wg = a.per_wg < ncols ? a.per_wg : ncols;
     const bool vec = aligned16(logits) && aligned16(out) && (ncols == 1 || (col_stride % 4 == 0 && out_stride % 4 == 0));
     auto go = [&](auto* kernel) {
-        hipLaunchKernelGGL(kernel, dim3((n + kSlice - 1) / kSlice, (ncols + a.per_wg - 1) / a.per_wg), dim3(kThreads), 0,
+        hipLaunchKernelGGL(kernel, dim3(slices, (ncols + a.per_wg - 1) / a.per_wg), dim3(kThreads), 0,
                            static_cast<hipStream_t>(stream), a);
         return launch_status("logits_process");
     };

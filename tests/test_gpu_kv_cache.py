@@ -177,10 +177,7 @@ def test_prep_axes(rmi, ktype, vtype, nh, nkv, hd, n_rot, sections, inter, ntok,
     assert np.abs(host(qo).reshape(want.shape) - want).max() <= (128 + 8) * 2.0 ** -24 * np.abs(want).max()
     kr = prep_ref(kx, kn, *args).astype(np.float32)
     got = ref.decode(host(k[1]), ktype, max_ctx, nkv, hd)[p0:p0 + ntok]
-    if ktype == ref.F16:   # half a step of fp16 besides the fp32 error
-        assert np.abs(got - kr).max() <= (2.0 ** -11 + 136 * 2.0 ** -24) * np.abs(kr).max()
-    else:
-        assert np.array_equal(got, ref.held(kr, ktype))
+    assert np.array_equal(got, ref.held(kr, ktype))
     assert np.array_equal(ref.decode(host(v[1]), vtype, max_ctx, nkv, hd)[p0:p0 + ntok], ref.held(vx, vtype))
     for (whole, c), b, t in ((k, kb, ktype), (v, vb, vtype)):
         assert changed_positions(b, host(c), t, max_ctx, nkv, hd) <= set(range(p0, p0 + ntok))
@@ -188,7 +185,8 @@ def test_prep_axes(rmi, ktype, vtype, nh, nkv, hd, n_rot, sections, inter, ntok,
 
 
 @pytest.mark.parametrize("factor", [1.0, 4.0])
-def test_prep_axes_text_positions_give_attn_preps_bits(rmi, factor):
+def test_prep_axes_text_positions_give_attn_preps_rows(rmi, factor):
+    """q and V bit for bit; K within one fp16 step (fp64 before the rounding here, fp32 there), nearly always equal"""
     rng = np.random.default_rng(6)
     nh, nkv, hd, ntok, max_ctx, p0 = 16, 4, 256, 7, 128, 40
     width = 2 * nh * hd + 2 * nkv * hd
@@ -205,8 +203,10 @@ def test_prep_axes_text_positions_give_attn_preps_bits(rmi, factor):
         else:
             rmi.attn_prep_rope(q3, width, qn, kn, k, v, pos, qo, nh, nkv, hd, 64, 1e7, factor, 32768.0, 1e-6, ntok, max_ctx)
         outs.append([host(x).copy() for x in (qo, k, v)])
-    for a, b in zip(*outs):
-        assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+    (q0, k0, v0), (q1, k1, v1) = outs
+    assert np.array_equal(q0.view(np.uint32), q1.view(np.uint32)) and np.array_equal(v0, v1)
+    bits = [np.where(k.view(np.int16) < 0, -32768 - k.view(np.int16).astype(np.int32), k.view(np.int16)) for k in (k0, k1)]   # in order
+    assert np.abs(bits[0] - bits[1]).max() <= 1 and (bits[0] != bits[1]).mean() < 0.01
 
 
 @pytest.mark.parametrize("p0", [-1, 30, 2000000000])
