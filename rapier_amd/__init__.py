@@ -558,6 +558,19 @@ def gqa_flash_decode_noalloc(q, kcache, vcache, pos, gate_src, gate_stride, y, y
 
 # ---- K/V caches in 16, 8 or 4 bits, attention for drafted trees over them, logits of a tree's nodes ---------------------
 
+# Short calls of many arguments: addresses go as plain integers (an argument of a declared c_void_p takes one; building the
+# c_void_p objects first costs 0.1 us each).
+
+def _a(t):
+    return None if t is None else t.data_ptr()
+
+
+def _s(stream):
+    if stream is None:
+        return _raw_stream() if _raw_stream else _current_stream()
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
 def kv_cache_bytes(type_, max_ctx, n_kv, head_dim) -> int:
     n = lib().rmi_kv_cache_bytes(type_, max_ctx, n_kv, head_dim)
     if n == 0:
@@ -572,21 +585,21 @@ def _is_f16(t):
 
 def kv_write(type_, src, src_stride, cache, first, n, n_kv, head_dim, max_ctx, stream=None):
     """n rows [n_kv x head_dim] of float32 or float16, src_stride elements apart, to positions [first, first + n)"""
-    _call("rmi_kv_write", type_, _p(src), _is_f16(src), src_stride, _p(cache), first, n, n_kv, head_dim, max_ctx,
-          _stream(stream))
+    _call("rmi_kv_write", type_, _a(src), _is_f16(src), src_stride, _a(cache), first, n, n_kv, head_dim, max_ctx,
+          _s(stream))
 
 
 def kv_read(type_, cache, out, out_stride, first, n, n_kv, head_dim, max_ctx, stream=None):
     """positions [first, first + n) of a cache back to float32 or float16 rows"""
-    _call("rmi_kv_read", type_, _p(cache), _p(out), _is_f16(out), out_stride, first, n, n_kv, head_dim, max_ctx,
-          _stream(stream))
+    _call("rmi_kv_read", type_, _a(cache), _a(out), _is_f16(out), out_stride, first, n, n_kv, head_dim, max_ctx,
+          _s(stream))
 
 
 def kv_compact(type_, caches, pos, path, count, max_path, n_kv, head_dim, max_ctx, stream=None):
     """rows pos[0] + path[i] -> pos[0] + i, i < min(count[0], max_path), in each of the caches (a list of tensors)"""
     ptrs = (ctypes.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches])
-    _call("rmi_kv_compact", type_, ptrs, len(caches), _p(pos), _p(path), _p(count), max_path, n_kv, head_dim, max_ctx,
-          _stream(stream))
+    _call("rmi_kv_compact", type_, ptrs, len(caches), _a(pos), _a(path), _a(count), max_path, n_kv, head_dim, max_ctx,
+          _s(stream))
 
 
 class RopeAxes(ctypes.Structure):
@@ -600,9 +613,9 @@ def attn_prep_axes(q3, q3_stride, qn, kn, ktype, kcache, vtype, vcache, pos, axi
     """per-head norm, rotation at axis_pos ([3][ntok]; None: the slots) and the cache write at slots pos[0] + t"""
     rope = RopeParams(freq_base, factor, orig_ctx, ext_factor, attn_factor, beta_fast, beta_slow)
     axes = RopeAxes((ctypes.c_int * 3)(*sections), int(interleaved))
-    _call("rmi_attn_prep_axes", _p(q3), q3_stride, _p(qn), _p(kn), ktype, _p(kcache), vtype, _p(vcache), _p(pos),
-          _p(axis_pos), _p(qout), n_head, n_kv, head_dim, n_rot, ctypes.byref(rope), ctypes.byref(axes), eps, ntok,
-          max_ctx, _stream(stream))
+    _call("rmi_attn_prep_axes", _a(q3), q3_stride, _a(qn), _a(kn), ktype, _a(kcache), vtype, _a(vcache), _a(pos),
+          _a(axis_pos), _a(qout), n_head, n_kv, head_dim, n_rot, ctypes.byref(rope), ctypes.byref(axes), eps, ntok,
+          max_ctx, _s(stream))
 
 
 def gqa_tree_nsub(ctx, n_head, n_kv, head_dim, ntok) -> int:
@@ -624,9 +637,9 @@ def gqa_tree_decode(q, ktype, kcache, vtype, vcache, pos, masks, gate_src, gate_
                     workspace, n_head, n_kv, head_dim, ntok, max_ctx, nsub, scale, stream=None):
     """attention of ntok drafted tokens at slots pos[0] + t: all of the context before them, and of each other what
     masks[t] (int64 bit patterns) says; masks None: the chain j <= t"""
-    _call("rmi_gqa_tree_decode", _p(q), ktype, _p(kcache), vtype, _p(vcache), _p(pos), _p(masks), _p(gate_src),
-          gate_stride, _p(y), y_stride, _p(q8), q8_stride, _p(workspace), n_head, n_kv, head_dim, ntok, max_ctx, nsub,
-          scale, _stream(stream))
+    _call("rmi_gqa_tree_decode", _a(q), ktype, _a(kcache), vtype, _a(vcache), _a(pos), _a(masks), _a(gate_src),
+          gate_stride, _a(y), y_stride, _a(q8), q8_stride, _a(workspace), n_head, n_kv, head_dim, ntok, max_ctx, nsub,
+          scale, _s(stream))
 
 
 class Penalties(ctypes.Structure):
@@ -640,6 +653,6 @@ def logits_process(logits, n, ncols, col_stride, out, out_stride, history, histo
                    bias_vals=None, n_bias=0, allow=None, allow_stride=0, stream=None):
     """biases, penalties over history (+ the draft path of each column's mask) and grammar masks, before argmax / topk"""
     pen = Penalties(repetition, presence, frequency, window)
-    _call("rmi_logits_process", _p(logits), n, ncols, col_stride, _p(out), out_stride, _p(history), _p(history_len),
-          max_history, _p(draft), _p(masks), ndraft, ctypes.byref(pen), _p(bias_ids), _p(bias_vals), n_bias, _p(allow),
-          allow_stride, _stream(stream))
+    _call("rmi_logits_process", _a(logits), n, ncols, col_stride, _a(out), out_stride, _a(history), _a(history_len),
+          max_history, _a(draft), _a(masks), ndraft, ctypes.byref(pen), _a(bias_ids), _a(bias_vals), n_bias, _a(allow),
+          allow_stride, _s(stream))
