@@ -379,8 +379,9 @@ int rmi_kv_read(int type, const void* cache, void* out, int out_f16, int out_str
                 int head_dim, int max_ctx, void* stream);
 /* Moves rows pos[0] + path[i] to pos[0] + i for i < min(count[0], max_path) in each of n_caches (1..64) caches of one
  * type: the accepted path of a drafted tree becomes the context's next rows.  `caches` is a host array of device
- * pointers, read during the call; pos, path and count are device words.  All rows are read before any is written.  A
- * move from or to a position outside [0, max_ctx) is left out.  max_path <= 64. */
+ * pointers to caches that do not overlap, read during the call; pos, path and count are device words.  All rows are read
+ * before any is written, so a path may name a row twice or in any order.  A move from or to a position outside
+ * [0, max_ctx) is left out.  max_path <= 64. */
 int rmi_kv_compact(int type, void* const* caches, int n_caches, const int* pos, const int* path, const int* count,
                    int max_path, int n_kv, int head_dim, int max_ctx, void* stream);
 
@@ -395,7 +396,7 @@ typedef struct rmi_rope_axes {
  * pos[0] + t (nothing is written for a slot outside [0, max_ctx)) and its rotation is at axis_pos[a * ntok + t] of axis a
  * (null: the slot, on every axis).  With a null axis_pos q and V are bitwise rmi_attn_prep_rope's; K rows are normed and
  * rotated in fp64 and rounded to fp32 once (what the cache holds then does not hang on the order of a sum), so an F16 K may
- * differ from rmi_attn_prep_rope's by one step where its fp32 lies at a border.  ntok >= 1. */
+ * differ from rmi_attn_prep_rope's by one step where its fp32 lies at a border.  ntok >= 1; the caches do not overlap. */
 int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* qn, const float* kn, int ktype, void* kcache,
                        int vtype, void* vcache, const int* pos, const int* axis_pos, float* qout, int n_head, int n_kv,
                        int head_dim, int n_rot, const rmi_rope_params* rope, const rmi_rope_axes* axes, float eps,
@@ -406,12 +407,14 @@ int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* qn, const fl
  * 64; a token that sees nothing gives zeros), or with null masks the chain j <= t (ntok <= 1024: decode, verify and
  * prompt chunks).  q is [ntok][n_head][head_dim]; kcache / vcache types: both F16, both I8, both I4, or I8 and I4;
  * sigmoid gate as rmi_gqa_flash_decode's (gate of head h at + h * 2 * head_dim + head_dim; null: no gate); fp32 y
- * (nullable) and Q8_1 (nullable).  Rows a token does not see have no part in its result, whatever they hold.  If a slot
- * lies outside [0, max_ctx) nothing is written.
+ * (nullable; rows y_stride elements apart) and Q8_1 (nullable; q8_stride bytes).  Rows a token does not see have no part
+ * in its result, whatever they hold; a NaN or an infinity in q or in a row that it sees makes the result NaN or infinite.
+ * If a slot lies outside [0, max_ctx) nothing is written.
  * The context is split into chunks of 128 * nsub positions; rmi_gqa_tree_nsub gives the split for a context of `ctx`
  * positions, to be settled once (results differ in the last bits between splits).  workspace holds
  * rmi_gqa_tree_workspace_bytes(...) bytes, 16-byte aligned, and needs no initial state; calls that may overlap need one
- * each.  Same inputs, same bits; I8 and I4 caches give the bits of an F16 cache that holds their values. */
+ * each.  Same inputs, same bits; I8 and I4 caches give the bits of an F16 cache that holds their values; and while
+ * ntok * n_head / n_kv <= 8, each token of a chain has the bits of a call of its own at the same nsub. */
 int rmi_gqa_tree_nsub(int ctx, int n_head, int n_kv, int head_dim, int ntok);
 size_t rmi_gqa_tree_workspace_bytes(int max_ctx, int n_head, int n_kv, int head_dim, int ntok, int nsub);
 int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache, int vtype, const void* vcache, const int* pos,

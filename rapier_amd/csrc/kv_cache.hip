@@ -429,6 +429,12 @@ __global__ __launch_bounds__(64 * kPrepWaves) void prep_axes_kernel(PrepArgs a) 
 
 bool aligned_to(const void* p, size_t n) { return p && (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+// whether two caches of these sizes share bytes
+bool overlap(const void* p, size_t p_bytes, const void* q, size_t q_bytes) {
+    const auto a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+    return a < b ? b - a < p_bytes : a - b < q_bytes;
+}
+
 // calls f with the type as a constant
 template <typename F>
 int with_type(int type, F&& f) {
@@ -511,9 +517,13 @@ extern "C" int rmi_kv_compact(int type, void* const* caches, int n_caches, const
     if (!caches || !aligned4(pos) || !aligned4(path) || !aligned4(count))
         return fail(RMI_ERR_POINTER, "kv_compact: invalid arguments");
     CachePtrs ptrs{};
+    const size_t bytes = rmi_kv_cache_bytes(type, max_ctx, n_kv, head_dim);
     for (int i = 0; i < n_caches; ++i) {
         if (!aligned16(caches[i])) return fail(RMI_ERR_POINTER, "kv_compact: null or misaligned cache");
         ptrs.p[i] = static_cast<uint8_t*>(caches[i]);
+        for (int j = 0; j < i; ++j)   // two workgroups would move the same rows
+            if (overlap(caches[i], bytes, caches[j], bytes))
+                return fail(RMI_ERR_POINTER, "kv_compact: caches overlap");
     }
     return with_type(type, [&](auto t) {
         hipLaunchKernelGGL((kv_compact_kernel<decltype(t)::value>), dim3(n_caches, n_kv), dim3(256), 0,
@@ -542,6 +552,8 @@ extern "C" int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* q
     if (!aligned4(q3) || !aligned4(qn) || !aligned4(kn) || !aligned16(kcache) || !aligned16(vcache) || !aligned4(pos) ||
         (axis_pos && !aligned4(axis_pos)) || !aligned4(qout))
         return fail(RMI_ERR_POINTER, what);
+    if (overlap(kcache, rmi_kv_cache_bytes(ktype, max_ctx, n_kv, head_dim), vcache, rmi_kv_cache_bytes(vtype, max_ctx, n_kv, head_dim)))
+        return fail(RMI_ERR_POINTER, "attn_prep_axes: the caches overlap");
     PrepArgs a{};
     if (!yarn_setup(*rope, n_rot, &a.yarn)) return fail(RMI_ERR_SHAPE, "attn_prep_axes: invalid YaRN parameters");
     a.q3 = q3;

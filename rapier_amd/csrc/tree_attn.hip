@@ -235,13 +235,20 @@ __device__ __forceinline__ bool sees(int p, int lim, uint64_t mask, int base, in
     return p <= lim || (mask && p >= base && p - base < ntok && ((mask >> (p - base)) & 1));
 }
 
-// Four dims of a row's result from its joined sums (m the maximum, -inf: nothing seen): gate, fp32, Q8_1.  The lanes of a
-// row's 32-dim block are eight neighbours.
+// A row's o / l; zero where its token sees nothing.  A maximum of -inf alone does not say so: seen scores that are all NaN or
+// -inf leave it too, and those rows are NaN (l is NaN, or 0 / 0).
+__device__ __forceinline__ float normed(const TreeArgs& a, int t, float o, float m, float l) {
+    if (m == -INFINITY && a.masks && a.pos[0] == 0 && !(a.masks[t] & (~0ull >> (64 - a.ntok)))) return 0.0f;
+    return o / l;
+}
+
+// Four dims of a row's result from its joined sums: gate, fp32, Q8_1.  The lanes of a row's 32-dim block are eight
+// neighbours.
 template <int HD>
 __device__ __forceinline__ void finish4(const TreeArgs& a, int t, int h, int d, float (&o)[4], float m, float l, const float (&gate)[4]) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        o[k] = m == -INFINITY ? 0.0f : o[k] / l;
+        o[k] = normed(a, t, o[k], m, l);
         if (a.gate) o[k] *= 1.0f / (1.0f + expf(-gate[k]));
     }
     if (a.y) *reinterpret_cast<float4u*>(a.y + static_cast<size_t>(t) * a.y_stride + h * HD + d) = float4u{o[0], o[1], o[2], o[3]};
@@ -952,7 +959,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
             for (int e = 0; e < NE; ++e) g[e] = a.gate ? a.gate[static_cast<size_t>(t) * a.gate_stride + h * 2 * HD + HD + 16 * e + l16] : 0.0f;
 #pragma unroll
             for (int e = 0; e < NE; ++e) {
-                float v = m == -INFINITY ? 0.0f : o[e][r] * kSixteen<VT> / l;
+                float v = normed(a, t, o[e][r] * kSixteen<VT>, m, l);
                 if (a.gate) v *= 1.0f / (1.0f + expf(-g[e]));
                 o[e][r] = v;
                 if (a.y && rw < a.rows) a.y[static_cast<size_t>(t) * a.y_stride + h * HD + 16 * e + l16] = v;
@@ -975,8 +982,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
 
 // ---- merge -------------------------------------------------------------------------------------------------------------
 // Workgroup (token, head, 64 dims): every lane has the (m, l) of a chunk and its group's first o in flight together; weights
-// 2^(m - M) to LDS, wave g sums chunks g, g + 4, ... in order, then the four waves in order; gate, fp32, Q8_1.  A row that
-// sees nothing has M = -inf.
+// 2^(m - M) to LDS, wave g sums chunks g, g + 4, ... in order, then the four waves in order; gate, fp32, Q8_1.
 constexpr int kMergeDims = 64, kMergeBatch = 16;
 
 template <int HD>
@@ -1042,7 +1048,7 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeArgs a) {
     __syncthreads();
     if (g != 0) return;
     float v = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
-    v = m == -INFINITY ? 0.0f : v / l;
+    v = normed(a, t, v, m, l);
     if (a.gate) v *= 1.0f / (1.0f + expf(-gate));
     if (a.y) a.y[static_cast<size_t>(t) * a.y_stride + h * HD + d] = v;
     if (a.q8) q8_1_store_lane(v, a.q8 + static_cast<size_t>(t) * a.q8_stride + (h * (HD / 32) + d / 32) * kQ8_1Bytes);
@@ -1178,6 +1184,9 @@ extern "C" int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache
         (masks && (reinterpret_cast<uintptr_t>(masks) & 7u)) || (gate_src && !aligned4(gate_src)) || (!y && !q8) ||
         (y && !aligned4(y)) || (q8 && (!aligned4(q8) || q8_stride % 4)))
         return fail(RMI_ERR_POINTER, "gqa_tree_decode: null or misaligned pointer");
+    const int width = n_head * head_dim;
+    if (ntok > 1 && ((y && y_stride < width) || (q8 && q8_stride < width / 32 * static_cast<int>(kQ8_1Bytes))))
+        return fail(RMI_ERR_SHAPE, "gqa_tree_decode: output rows overlap");
     const Form f = tree_form(n_head, n_kv, ntok, nsub);
     TreeArgs a{};
     a.q = q;

@@ -140,6 +140,31 @@ def test_unseen_rows_hold_anything(rmi, types, bad, what):
         assert np.array_equal(y[t][~fin & ~np.isnan(want[t])], want[t][~fin & ~np.isnan(want[t])])
 
 
+@pytest.mark.parametrize("types", PAIRS, ids=IDS)
+@pytest.mark.parametrize("ntok", [1, 3, 6, 20, 40])
+def test_a_result_that_is_not_a_number_is_not_zero(rmi, types, ntok):
+    """a NaN in q, or scores of a row that are all NaN or -infinity, is no row that sees nothing"""
+    masks = [1 << i for i in range(ntok)]
+    masks[0] |= 2 if ntok == 3 else 0
+    c = Call(rmi, types, 8, 2, 256, ntok, 0, masks, nsub=1)
+    for m in (masks, None):
+        c.masks = m
+        for what in ("q", "k", "-inf"):
+            q, raw = c.q.copy(), c.raw
+            c.q, t = np.abs(c.q) + 0.5, ntok - 1
+            if what == "q":
+                c.q[t, 3, 17] = np.nan
+            else:   # the rows of the last token: with masks it sees them alone
+                k = c.values()[0].astype(np.float32)
+                k[:ntok, :, :] = np.nan if what == "k" else -np.inf
+                c.raw = [ref.encode(k, types[0]), raw[1]]
+            y = c.run()
+            c.q, c.raw = q, raw
+            assert np.isnan(y[t, 3]).all()
+            if what == "q":
+                assert np.isfinite(np.delete(y, 3, 1)).all() and np.isfinite(y[:t, 3]).all()
+
+
 @pytest.mark.parametrize("types", PAIRS[1:], ids=IDS[1:])
 @pytest.mark.parametrize("ntok,base", [(1, 700), (6, 333), (40, 500)])
 def test_quantised_caches_give_the_bits_of_an_fp16_cache_of_their_values(rmi, types, ntok, base):

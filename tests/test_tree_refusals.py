@@ -6,6 +6,7 @@ import pytest
 FAKE = ctypes.c_void_p(1 << 20)
 OFF8 = ctypes.c_void_p((1 << 20) + 8)
 OFF4 = ctypes.c_void_p((1 << 20) + 4)
+FAR = ctypes.c_void_p(1 << 30)
 ODD = ctypes.c_void_p((1 << 20) + 1)
 
 
@@ -50,13 +51,14 @@ def test_compact(rmi):
 
     for bad in ({"type_": 7}, {"n": 0}, {"ptrs": (1 << 20,) * 65}, {"max_path": 0}, {"max_path": 65}, {"n_kv": 0}, {"hd": 64}, {"max_ctx": 0},
                 {"null": True}, {"pos": None}, {"path": None}, {"count": None}, {"pos": ODD}, {"ptrs": (1 << 20, None)},
+                {"ptrs": (1 << 20, 1 << 22, 1 << 20)}, {"ptrs": ((1 << 20) + 16, 1 << 20)},
                 {"ptrs": ((1 << 20) + 8,)}):
         with pytest.raises(ValueError, match="kv_compact"):
             call(**bad)
 
 
 def test_prep_axes(rmi):
-    def call(q3=FAKE, qn=FAKE, kn=FAKE, ktype=1, k=FAKE, vtype=1, v=FAKE, pos=FAKE, axis=FAKE, qout=FAKE, nh=16, nkv=4, hd=256, n_rot=64,
+    def call(q3=FAKE, qn=FAKE, kn=FAKE, ktype=1, k=FAKE, vtype=1, v=FAR, pos=FAKE, axis=FAKE, qout=FAKE, nh=16, nkv=4, hd=256, n_rot=64,
              base=1e7, factor=1.0, orig=0.0, sec=(12, 10, 10), inter=1, ntok=1, max_ctx=100, rope=True, axes=True):
         r = rmi.RopeParams(base, factor, orig, 1.0, 1.0, 32.0, 1.0)
         x = rmi.RopeAxes((ctypes.c_int * 3)(*sec), inter)
@@ -66,22 +68,23 @@ def test_prep_axes(rmi):
     for bad in ({"ktype": 3}, {"vtype": -1}, {"nh": 15}, {"nh": 0}, {"nkv": 0}, {"hd": 192}, {"n_rot": 63}, {"n_rot": 258}, {"n_rot": -2},
                 {"base": 1.0}, {"base": float("nan")}, {"factor": 2.0}, {"sec": (11, 10, 10)}, {"sec": (34, -1, -1)}, {"sec": (2 ** 31 - 1, 0, 0)},
                 {"sec": (8, 12, 12)}, {"sec": (10, 10, 12)}, {"ntok": 0}, {"ntok": 101}, {"max_ctx": 0}, {"rope": False}, {"axes": False},
-                {"q3": None}, {"qn": None}, {"kn": None}, {"k": None}, {"v": OFF4}, {"pos": None}, {"axis": ODD}, {"qout": None}):
+                {"q3": None}, {"qn": None}, {"kn": None}, {"k": None}, {"v": OFF4}, {"pos": None}, {"axis": ODD}, {"qout": None},
+                {"v": FAKE}, {"k": FAR, "v": ctypes.c_void_p((1 << 30) + 1600)}):
         with pytest.raises(ValueError, match="attn_prep_axes"):
             call(**bad)
 
 
 def test_tree_attention(rmi):
-    def call(q=FAKE, ktype=1, k=FAKE, vtype=1, v=FAKE, pos=FAKE, masks=FAKE, gate=FAKE, y=FAKE, q8=FAKE, q8s=36, ws=FAKE, nh=16, nkv=4, hd=256,
+    def call(q=FAKE, ktype=1, k=FAKE, vtype=1, v=FAKE, pos=FAKE, masks=FAKE, gate=FAKE, y=FAKE, ys=4096, q8=FAKE, q8s=4608, ws=FAKE, nh=16, nkv=4, hd=256,
              ntok=8, max_ctx=1000, nsub=1):
-        rmi._call("rmi_gqa_tree_decode", q, ktype, k, vtype, v, pos, masks, gate, 10240, y, 4096, q8, q8s, ws, nh, nkv, hd, ntok, max_ctx, nsub,
+        rmi._call("rmi_gqa_tree_decode", q, ktype, k, vtype, v, pos, masks, gate, 10240, y, ys, q8, q8s, ws, nh, nkv, hd, ntok, max_ctx, nsub,
                   0.0625, None)
 
     for bad in ({"ktype": 3}, {"vtype": 9}, {"ktype": 0}, {"vtype": 0}, {"ktype": 2, "vtype": 1}, {"nh": 15}, {"nh": 0}, {"nkv": 0},
                 {"nh": 260}, {"hd": 64}, {"ntok": 0}, {"ntok": 65}, {"ntok": 1025, "masks": None, "max_ctx": 5000}, {"ntok": 9, "max_ctx": 8},
                 {"max_ctx": 0}, {"nsub": 0}, {"nsub": -1}, {"nsub": 1, "max_ctx": 128 * 2048 + 1}, {"q": None}, {"q": OFF8}, {"k": None},
-                {"v": OFF4}, {"pos": None}, {"masks": OFF4}, {"gate": ODD}, {"y": None, "q8": None}, {"y": ODD}, {"q8": ODD}, {"q8s": 37},
-                {"ws": None}, {"ws": OFF8}):
+                {"v": OFF4}, {"pos": None}, {"masks": OFF4}, {"gate": ODD}, {"y": None, "q8": None}, {"y": ODD}, {"q8": ODD}, {"q8s": 4609},
+                {"ys": 4095}, {"ys": -4096}, {"q8s": 4604}, {"ws": None}, {"ws": OFF8}):
         with pytest.raises(ValueError, match="gqa_tree_decode"):
             call(**bad)
 
