@@ -90,9 +90,11 @@ __device__ __forceinline__ uint32_t nibble_pair(uint32_t w, int k) { return nibb
 constexpr uint32_t kMagic8 = 0x64646464u;   // high byte of the fp16 numbers 1024 + 0..255
 
 typedef __amdgpu_buffer_rsrc_t Rsrc;
-// `rows` rows from p as a buffer: a row past them reads as zeros, so a step past the last position loads nothing
+// `rows` rows from p as a buffer: a row past them reads as zeros, so a step past the last position loads nothing.  The length
+// is told to be scalar: clamping takes a vector instruction, and each load would loop over its lanes' descriptors.
 __device__ __forceinline__ Rsrc rows_buffer(const uint8_t* p, int rows, size_t stride) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, static_cast<int>(max(rows, 0) * stride), 0x00027000);
+    const int n = __builtin_amdgcn_readfirstlane(min(max(rows, 0), kStep));
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, static_cast<int>(n * stride), 0x00027000);
 }
 
 // 16 neighbouring dims of a position
@@ -414,8 +416,8 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
     DimsV<VT, VD> vx[8];
     uint32_t vsc[8];
     auto load_k = [&](int sb) {   // rows past the last read as zeros
-        const Rsrc r = rows_buffer(kp + sb * kstride, min(last + 1 - sb, kStep), kstride);
-        const Rsrc rs = rows_buffer(ks + static_cast<size_t>(sb) * NB, min(last + 1 - sb, kStep), NB);
+        const Rsrc r = rows_buffer(kp + sb * kstride, last + 1 - sb, kstride);
+        const Rsrc rs = rows_buffer(ks + static_cast<size_t>(sb) * NB, last + 1 - sb, NB);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -431,8 +433,8 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
         }
     };
     auto load_vs = [&](int sb) {
-        const Rsrc r = rows_buffer(vp + sb * vstride, min(last + 1 - sb, kStep), vstride);
-        const Rsrc rs = rows_buffer(vs + static_cast<size_t>(sb) * NB, min(last + 1 - sb, kStep), NB);
+        const Rsrc r = rows_buffer(vp + sb * vstride, last + 1 - sb, vstride);
+        const Rsrc rs = rows_buffer(vs + static_cast<size_t>(sb) * NB, last + 1 - sb, NB);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int p = j < 4 ? j : 12 + j;
@@ -752,7 +754,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
     Dims16<VT> vx[U];
     uint32_t ksc[U], vsc[U];
     auto load = [&](int sb) {   // rows past the last read as zeros
-        const int n = min(w.last + 1 - sb, kStep);
+        const int n = w.last + 1 - sb;
         const Rsrc rk = rows_buffer(kp + sb * kstride, n, kstride), rks = rows_buffer(ks + static_cast<size_t>(sb) * NB, n, NB);
         const Rsrc rv = rows_buffer(vp + sb * vstride, n, vstride), rvs = rows_buffer(vs + static_cast<size_t>(sb) * NB, n, NB);
 #pragma unroll
