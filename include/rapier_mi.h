@@ -411,10 +411,13 @@ int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* qn, const fl
  * in its result, whatever they hold; a NaN or an infinity in q or in a row that it sees makes the result NaN or infinite.
  * If a slot lies outside [0, max_ctx) nothing is written.
  * The context is split into chunks of 128 * nsub positions; rmi_gqa_tree_nsub gives the split for a context of `ctx`
- * positions, to be settled once (results differ in the last bits between splits).  workspace holds
+ * positions, to be settled once (results differ in the last bits between splits).  With RMI_TREE_SHORT added, more than 16
+ * query rows per KV head are worked on 16 at a time, which pays over short chunks.  workspace holds
  * rmi_gqa_tree_workspace_bytes(...) bytes, 16-byte aligned, and needs no initial state; calls that may overlap need one
- * each.  Same inputs, same bits; I8 and I4 caches give the bits of an F16 cache that holds their values; and while
- * ntok * n_head / n_kv <= 8, each token of a chain has the bits of a call of its own at the same nsub. */
+ * each.  Same inputs, same bits; I8 and I4 caches give the bits of an F16 cache that holds their values (but for 17 to 32
+ * query rows at nsub >= 6 without RMI_TREE_SHORT); and while ntok * n_head / n_kv <= 8, each token of a chain has the
+ * bits of a call of its own at the same nsub. */
+enum { RMI_TREE_SHORT = 1 << 24 };
 int rmi_gqa_tree_nsub(int ctx, int n_head, int n_kv, int head_dim, int ntok);
 size_t rmi_gqa_tree_workspace_bytes(int max_ctx, int n_head, int n_kv, int head_dim, int ntok, int nsub);
 int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache, int vtype, const void* vcache, const int* pos,

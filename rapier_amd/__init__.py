@@ -19,6 +19,7 @@ CSRC = os.path.join(_HERE, "csrc")
 RMI_OK, RMI_ERR_SHAPE, RMI_ERR_POINTER, RMI_ERR_STREAM, RMI_ERR_LAUNCH, RMI_ERR_UNSUPPORTED, RMI_ERR_STATE = range(7)
 GGML_Q8_0, GGML_Q6_K = 8, 14
 KV_F16, KV_I8, KV_I4 = range(3)   # K/V cache types
+TREE_SHORT = 1 << 24              # a split's flag (gqa_tree_nsub)
 Q6K_BYTES, Q8_0_BYTES, Q8_1_BYTES = 210, 34, 36
 
 _lib = None
@@ -619,7 +620,7 @@ def attn_prep_axes(q3, q3_stride, qn, kn, ktype, kcache, vtype, vcache, pos, axi
 
 
 def gqa_tree_nsub(ctx, n_head, n_kv, head_dim, ntok) -> int:
-    """the split of a context of ctx positions (chunks of 128 * nsub)"""
+    """the split of a context of ctx positions: chunks of 128 * nsub, with TREE_SHORT added where groups of 16 rows pay"""
     n = lib().rmi_gqa_tree_nsub(ctx, n_head, n_kv, head_dim, ntok)
     if n == 0:
         raise ValueError(last_error())

@@ -385,13 +385,13 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
     const int slot = PACKED ? l16 & 7 : l16, row = w.row0 + slot, rowc = min(row, a.rows - 1), tok = rowc / G;
     const bool low = PACKED && l16 >= 8;
     // the query rows and masks do not depend on the position: in flight together with it
-    const float* qr = a.q + (static_cast<size_t>(tok) * a.n_head + kv * G + (rowc - tok * G)) * HD + 16 * g4;
+    const float* qr = a.q + (static_cast<size_t>(tok) * a.n_head + kv * G + (rowc - tok * G)) * HD + 32 * g4;
     float qx[NI][16];
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
-            const float4 u = reinterpret_cast<const float4*>(qr + 64 * i)[f];
+            const float4 u = reinterpret_cast<const float4*>(qr + 128 * (i >> 1) + 16 * (i & 1))[f];
             qx[i][4 * f] = u.x, qx[i][4 * f + 1] = u.y, qx[i][4 * f + 2] = u.z, qx[i][4 * f + 3] = u.w;
         }
     uint64_t mask = 0;   // of the row's token: bit j = draft slot base + j
@@ -408,20 +408,29 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
     const KvRow<KT> k0 = kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD);
     const KvRow<VT> v0 = kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD);
     const uint8_t *kp = a.kc + k0.code, *ks = a.kc + k0.scale, *vp = a.vc + v0.code, *vs = a.vc + v0.scale;
-    const int kat = static_cast<int>(l16 * kstride) + g4 * (kKB / (HD / 16)), vat = static_cast<int>(4 * g4 * vstride) + l16 * DimsV<VT, VD>::kBytes;
+    const int kat = static_cast<int>(l16 * kstride) + g4 * (kKB / (HD / 32)), vat = static_cast<int>(4 * g4 * vstride) + l16 * DimsV<VT, VD>::kBytes;
     const int vsat = 4 * g4 * NB + VD * l16 / kKvBlock;
 
     Dims16<KT> kx[2][NI];
     uint32_t ksc[2][2];
     DimsV<VT, VD> vx[8];
     uint32_t vsc[8];
-    auto load_k = [&](int sb) {   // rows past the last read as zeros
-        const Rsrc r = rows_buffer(kp + sb * kstride, last + 1 - sb, kstride);
-        const Rsrc rs = rows_buffer(ks + static_cast<size_t>(sb) * NB, last + 1 - sb, NB);
+    auto load_k = [&](int sb, bool wanted) {   // rows past the last read as zeros
+        const int n = wanted ? last + 1 - sb : 0;
+        const Rsrc r = rows_buffer(kp + sb * kstride, n, kstride);
+        const Rsrc rs = rows_buffer(ks + static_cast<size_t>(sb) * NB, n, NB);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
-            for (int i = 0; i < NI; ++i) kx[t][i] = load16<KT>(r, kat + i * (kKB / NI), static_cast<int>(16 * t * kstride));
+            for (int i = 0; i < NI; i += 2) {
+                if constexpr (KT == kKvI4) {
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, kat + i * (kKB / NI), static_cast<int>(16 * t * kstride), 0);
+                    kx[t][i].w[0] = v[0], kx[t][i].w[1] = v[1], kx[t][i + 1].w[0] = v[2], kx[t][i + 1].w[1] = v[3];
+                } else {
+                    kx[t][i] = load16<KT>(r, kat + i * (kKB / NI), static_cast<int>(16 * t * kstride));
+                    kx[t][i + 1] = load16<KT>(r, kat + i * (kKB / NI) + kKB / (HD / 16), static_cast<int>(16 * t * kstride));
+                }
+            }
             if constexpr (KT != kKvF16) {
                 if constexpr (NB == 8) {
                     const auto s = __builtin_amdgcn_raw_buffer_load_b64(rs, l16 * NB, 16 * t * NB, 0);
@@ -432,9 +441,10 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
             }
         }
     };
-    auto load_vs = [&](int sb) {
-        const Rsrc r = rows_buffer(vp + sb * vstride, last + 1 - sb, vstride);
-        const Rsrc rs = rows_buffer(vs + static_cast<size_t>(sb) * NB, last + 1 - sb, NB);
+    auto load_vs = [&](int sb, bool wanted) {
+        const int n = wanted ? last + 1 - sb : 0;
+        const Rsrc r = rows_buffer(vp + sb * vstride, n, vstride);
+        const Rsrc rs = rows_buffer(vs + static_cast<size_t>(sb) * NB, n, NB);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int p = j < 4 ? j : 12 + j;
@@ -442,10 +452,9 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
             if constexpr (VT != kKvF16) vsc[j] = __builtin_amdgcn_raw_buffer_load_b8(rs, vsat + p * NB, 0, 0);
         }
     };
-    if (nsteps > 0) {
-        load_k(wbase);
-        load_vs(wbase);
-    }
+    load_k(wbase, nsteps > 0);
+    __builtin_amdgcn_sched_barrier(0);   // in this order, as in the loop: a wait for K then leaves V in flight
+    load_vs(wbase, nsteps > 0);
 
     half8 qb[PACKED ? NI : 1][2];
     float post;   // score = product * post, in base 2
@@ -499,8 +508,8 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 Scale2 s = {};
-                if constexpr (KT != kKvF16) {   // block 2 i + g4 / 2
-                    const uint32_t b = (ksc[t][i >> 1] >> (16 * (i & 1) + 8 * (g4 >> 1))) & 0xffu;
+                if constexpr (KT != kKvF16) {   // block 4 (i / 2) + g4
+                    const uint32_t b = (ksc[t][i >> 1] >> (8 * g4)) & 0xffu;
                     s = scale2<KT>(b, b);
                 }
 #pragma unroll
@@ -517,8 +526,9 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
 #pragma unroll
             for (int r = 0; r < 4; ++r) sc[4 * t + r] = (acc[r] + (PACKED ? xor_lane<8>(acc[r]) : acl[r])) * post;
         }
+        // the loads are not under a branch: behind one, every wait would be for all that might be out
         const bool more = st + 1 < nsteps;
-        if (more) load_k(sb + kStep);
+        load_k(sb + kStep, more);
         const bool tail = sb + kStep > base;   // uniform: the step reaches into the draft
         uint32_t seen = 0xffu;
         if (tail || row >= a.rows) {
@@ -620,7 +630,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
                 o[2 * e + 1] = mfma(pl, b1, o[2 * e + 1]);
             }
         }
-        if (more) load_vs(sb + kStep);
+        load_vs(sb + kStep, more);
     }
 
     l_run += xor_lane<16>(l_run);
@@ -1096,22 +1106,26 @@ bool tree_shape_ok(int max_ctx, int n_head, int n_kv, int head_dim, int ntok) {
            ntok >= 1 && ntok <= kMaxChain;
 }
 
-// the form of a call: query rows per KV head, 16-row blocks side by side in a workgroup (0: the form of few rows), rows a
-// workgroup holds, workgroups per (chunk, KV head).  17 to 32 rows are two groups of few rows, which begin and end sooner,
-// or over long chunks a tile, which turns K and V to fp16 once: I8, 8 tokens x 4 heads behind 4K 14.4 / 17.6 us, 32K
-// 31.7 / 30.7, 64K 50.7 / 47.4 (F16 84 / 64).
+// The form of a call: query rows per KV head, 16-row blocks side by side in a workgroup (0: the form of few rows), rows a
+// workgroup holds, workgroups per (chunk, KV head).  Up to 16 rows the form of few rows; more rows are groups of it where the
+// split asks for that (RMI_TREE_SHORT: rmi_gqa_tree_nsub), else tiles, which turn K and V to fp16 once for all of a workgroup's
+// rows.  17 to 32 rows of I8 and I4 stay groups of few (64K, 8 tokens x 4 heads: 45.7 / 38.9 us, tiles 47.3 / 40.2), F16 takes
+// tiles over long chunks (61 us, groups of few 83: they load K and V twice).
 constexpr int kLongSub = 6;
+constexpr int kShort = RMI_TREE_SHORT;
 struct Form {
     int rows, rb, held, groups;
 };
-Form tree_form(int n_head, int n_kv, int ntok, long long nsub) {
+Form tree_form(int n_head, int n_kv, int ntok, int split, bool f16) {
     Form f;
     f.rows = ntok * (n_head / n_kv);
-    f.rb = f.rows <= 16 ? 0 : f.rows <= 32 ? (nsub >= kLongSub ? 2 : 0) : f.rows <= 64 ? 4 : 8;
+    f.rb = f.rows <= 16 || (split & kShort) ? 0 : f.rows <= 32 ? (f16 && split >= kLongSub ? 2 : 0) : f.rows <= 64 ? 4 : 8;
     f.held = f.rb ? kRowBlock * f.rb : f.rows <= 8 ? 8 : 16;
     f.groups = (f.rows + f.held - 1) / f.held;
     return f;
 }
+// the chunk's length in a split, in units; 0: not one
+int split_nsub(int split) { return split < 1 || split >= 2 * kShort ? 0 : split & (kShort - 1); }
 long long tree_chunks(int max_ctx, int nsub) {
     const long long len = static_cast<long long>(kUnit) * nsub;
     return (max_ctx + len - 1) / len;
@@ -1122,8 +1136,9 @@ void launch_partial(const TreeArgs& a, const Form& f, unsigned blocks, hipStream
     auto go = [&](auto* kernel, int threads) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, s, a); };
     if (f.held == 8) go(&tree_few_kernel<KT, VT, HD, 8>, kThreads);
     else if (f.held == 16) go(&tree_few_kernel<KT, VT, HD, 16>, kThreads);
-    else if (f.rb == 2) go(&tree_tile_kernel<KT, VT, HD, 2>, kTileThreads);
-    else if (f.rb == 4) go(&tree_tile_kernel<KT, VT, HD, 4>, kTileThreads);
+    else if (f.rb == 2) {
+        if constexpr (KT == kKvF16) go(&tree_tile_kernel<KT, VT, HD, 2>, kTileThreads);
+    } else if (f.rb == 4) go(&tree_tile_kernel<KT, VT, HD, 4>, kTileThreads);
     else go(&tree_tile_kernel<KT, VT, HD, 8>, kTileThreads);
 }
 
@@ -1149,27 +1164,35 @@ extern "C" int rmi_gqa_tree_nsub(int ctx, int n_head, int n_kv, int head_dim, in
         set_error("gqa_tree_nsub: invalid shape");
         return 0;
     }
-    // At least a workgroup for each of 256 compute units, from chunks as long as that leaves; long contexts of the form of few
-    // rows two (they hide each other's waits), but not at less than four steps a wave, where a workgroup's own beginning and
-    // end weigh more.  I8, 1 / 8 tokens at 16 heads: 64K at 512 / 256 workgroups 35.4 / 38.6 and 50.7 / 57.1 us, 16K (8
-    // tokens) 24.0 / 21.9 us; 4K at 128 / 64 workgroups of the one and two steps 12.6 / 14.7 us.
+    // One workgroup for each of 256 compute units: as many chunks as leave an XCD's 32 units a (chunk, head, group) each, since
+    // a 33rd doubles the launch's time.  I8, 12 tokens x 4 heads behind 16K: 33 an XCD 32.0 us, 27 28.9, 24 23.7; 1 token at
+    // 64K with two workgroups a unit 32.8 us, one 32.8 (I4 23.7 / 22.9, F16 55 / 51).
     const long long units = (ctx + kUnit - 1) / kUnit;
-    auto split = [&](const Form& f) {
-        const long long work = units * n_kv * f.groups, want = (work + 255) / 256;
-        return std::min(units, f.rb ? want : std::max((work + 511) / 512, std::min(want, 4LL)));
+    auto nsub_for = [&](int groups) {
+        const int pairs = 8 * std::max(1, 32 / groups), chunks = std::max(1, pairs / n_kv);
+        return (units + chunks - 1) / chunks;
     };
-    long long nsub = split(tree_form(n_head, n_kv, ntok, 1));
-    const Form f = tree_form(n_head, n_kv, ntok, nsub);
-    if (f.rb == 2) nsub = std::max<long long>(kLongSub, split(f));
-    return static_cast<int>(std::max({1LL, (units + kMaxChunks - 1) / kMaxChunks, nsub}));
+    // More than 16 rows as groups of few while a wave of theirs has at most 8 steps, where a workgroup's beginning and end
+    // and the records of many chunks weigh more than turning K and V to fp16 once: 16 tokens x 4 heads, groups / tiles: I8 4K
+    // 16.5 / 19.9 us, 8K 20.0 / 22.6, 16K 24.6 / 25.8; 64 tokens 4K 26.4 / 32.9, 32 tokens 16K (16 steps) 40 / 36.5;
+    // F16 16 tokens 4K 17.5 / 18.8, 16K 32.6 / 27.2.
+    constexpr int kFewSteps = 8;
+    const Form few = tree_form(n_head, n_kv, ntok, kShort + 1, false), tile = tree_form(n_head, n_kv, ntok, kLongSub, true);
+    long long nsub = nsub_for(few.groups);
+    const bool in_groups = few.rows > 16 && few.groups <= 32 && nsub <= kFewSteps;
+    if (few.rows > 16 && !in_groups) nsub = std::max<long long>(tile.rb == 2 ? kLongSub : 1, nsub_for(tile.groups));
+    nsub = std::max({1LL, (units + kMaxChunks - 1) / kMaxChunks, nsub});
+    return static_cast<int>(nsub) | (in_groups ? kShort : 0);
 }
 
 extern "C" size_t rmi_gqa_tree_workspace_bytes(int max_ctx, int n_head, int n_kv, int head_dim, int ntok, int nsub) {
+    const int split = nsub;
+    nsub = split_nsub(split);
     if (!tree_shape_ok(max_ctx, n_head, n_kv, head_dim, ntok) || nsub < 1 || tree_chunks(max_ctx, nsub) > kMaxChunks) {
         set_error("gqa_tree_workspace_bytes: invalid shape");
         return 0;
     }
-    const Form f = tree_form(n_head, n_kv, ntok, nsub);
+    const Form f = tree_form(n_head, n_kv, ntok, split, false);   // 17 to 32 rows take the same space in both forms
     return static_cast<size_t>(tree_chunks(max_ctx, nsub)) * n_kv * (static_cast<size_t>(f.groups) * f.held) * (head_dim + 2) * sizeof(float);
 }
 
@@ -1179,6 +1202,8 @@ extern "C" int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache
                                    int head_dim, int ntok, int max_ctx, int nsub, float scale, void* stream) {
     if (!kv_type_ok(ktype) || !kv_type_ok(vtype) || (ktype != vtype && !(ktype == kKvI8 && vtype == kKvI4)))
         return fail(RMI_ERR_UNSUPPORTED, "gqa_tree_decode: cache types F16 / F16, I8 / I8, I4 / I4 or I8 / I4");
+    const int split = nsub;
+    nsub = split_nsub(split);
     if (!tree_shape_ok(max_ctx, n_head, n_kv, head_dim, ntok) || ntok > max_ctx || (masks && ntok > kMaxTree) || nsub < 1 ||
         tree_chunks(max_ctx, nsub) > kMaxChunks)
         return fail(RMI_ERR_SHAPE, "gqa_tree_decode: invalid arguments");
@@ -1189,7 +1214,7 @@ extern "C" int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache
     const int width = n_head * head_dim;
     if (ntok > 1 && ((y && y_stride < width) || (q8 && q8_stride < width / 32 * static_cast<int>(kQ8_1Bytes))))
         return fail(RMI_ERR_SHAPE, "gqa_tree_decode: output rows overlap");
-    const Form f = tree_form(n_head, n_kv, ntok, nsub);
+    const Form f = tree_form(n_head, n_kv, ntok, split, ktype == kKvF16);
     TreeArgs a{};
     a.q = q;
     a.kc = static_cast<const uint8_t*>(kcache);

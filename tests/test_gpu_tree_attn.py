@@ -91,6 +91,14 @@ def test_chains(rmi, types, ntok, base, nsub):
     Call(rmi, types, 8, 2, 256, ntok, base, None, seed=ntok, nsub=nsub).check()
 
 
+@pytest.mark.parametrize("types", PAIRS, ids=IDS)
+@pytest.mark.parametrize("ntok,base,nsub,masked", [(5, 1700, 6, True), (5, 200, 1, False), (17, 0, 1, True), (33, 700, 2, True), (64, 1100, 3, True),
+                                                   (64, 3, 9, True), (130, 515, 2, False), (300, 1, 1, False)])
+def test_groups_of_sixteen_rows(rmi, types, ntok, base, nsub, masked):
+    masks = ref.tree_masks(np.random.default_rng(ntok), ntok, reach=9)[0] if masked else None
+    Call(rmi, types, 8, 2, 128 if ntok % 2 else 256, ntok, base, masks, seed=ntok, nsub=nsub + rmi.TREE_SHORT).check()
+
+
 @pytest.mark.parametrize("ntok", [17, 40, 64])
 @pytest.mark.parametrize("types", PAIRS, ids=IDS)
 def test_wide_trees_over_many_chunks(rmi, types, ntok):
@@ -170,10 +178,13 @@ def test_a_result_that_is_not_a_number_is_not_zero(rmi, types, ntok):
 def test_quantised_caches_give_the_bits_of_an_fp16_cache_of_their_values(rmi, types, ntok, base):
     masks, _ = ref.tree_masks(np.random.default_rng(2), ntok)
     c = Call(rmi, types, 16, 4, 256, ntok, base, masks, nsub=1)
-    y = c.run()
-    c.raw = [ref.encode(x, ref.F16) for x in c.values()]
-    c.types = (ref.F16, ref.F16)
-    assert np.array_equal(y.view(np.uint32), c.run().view(np.uint32))
+    raw = c.raw
+    for nsub in (1, 2 + rmi.TREE_SHORT):
+        c.types, c.raw, c.nsub = types, raw, nsub
+        y = c.run()
+        c.raw = [ref.encode(x, ref.F16) for x in c.values()]
+        c.types = (ref.F16, ref.F16)
+        assert np.array_equal(y.view(np.uint32), c.run().view(np.uint32))
 
 
 @pytest.mark.parametrize("types", PAIRS, ids=IDS)

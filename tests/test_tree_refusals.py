@@ -82,7 +82,7 @@ def test_tree_attention(rmi):
 
     for bad in ({"ktype": 3}, {"vtype": 9}, {"ktype": 0}, {"vtype": 0}, {"ktype": 2, "vtype": 1}, {"nh": 15}, {"nh": 0}, {"nkv": 0},
                 {"nh": 260}, {"hd": 64}, {"ntok": 0}, {"ntok": 65}, {"ntok": 1025, "masks": None, "max_ctx": 5000}, {"ntok": 9, "max_ctx": 8},
-                {"max_ctx": 0}, {"nsub": 0}, {"nsub": -1}, {"nsub": 1, "max_ctx": 128 * 2048 + 1}, {"q": None}, {"q": OFF8}, {"k": None},
+                {"max_ctx": 0}, {"nsub": 0}, {"nsub": -1}, {"nsub": 1 << 24}, {"nsub": 1 << 25}, {"nsub": (1 << 25) + 1}, {"nsub": 1, "max_ctx": 128 * 2048 + 1}, {"q": None}, {"q": OFF8}, {"k": None},
                 {"v": OFF4}, {"pos": None}, {"masks": OFF4}, {"gate": ODD}, {"y": None, "q8": None}, {"y": ODD}, {"q8": ODD}, {"q8s": 4609},
                 {"ys": 4095}, {"ys": -4096}, {"q8s": 4604}, {"ws": None}, {"ws": OFF8}):
         with pytest.raises(ValueError, match="gqa_tree_decode"):
@@ -92,9 +92,11 @@ def test_tree_attention(rmi):
 def test_tree_plan(rmi):
     for ctx in (1, 127, 128, 5000, 65536, 1 << 20):
         for ntok in (1, 8, 64, 999):
-            nsub = rmi.gqa_tree_nsub(ctx, 16, 4, 256, ntok)
-            assert 1 <= nsub <= -(-ctx // 128) and -(-ctx // (128 * nsub)) <= 2048
-            assert rmi.gqa_tree_workspace_bytes(ctx, 16, 4, 256, ntok, nsub) > 0
+            split = rmi.gqa_tree_nsub(ctx, 16, 4, 256, ntok)
+            nsub = split & (rmi.TREE_SHORT - 1)
+            assert split == nsub or split == nsub + rmi.TREE_SHORT
+            assert 1 <= nsub <= max(6, -(-ctx // 128)) and -(-ctx // (128 * nsub)) <= 2048
+            assert rmi.gqa_tree_workspace_bytes(ctx, 16, 4, 256, ntok, split) > 0
     for bad in ((0, 16, 4, 256, 1), (100, 15, 4, 256, 1), (100, 16, 4, 64, 1), (100, 16, 4, 256, 0), (100, 16, 4, 256, 1025)):
         with pytest.raises(ValueError):
             rmi.gqa_tree_nsub(*bad)
@@ -102,8 +104,13 @@ def test_tree_plan(rmi):
             rmi.gqa_tree_workspace_bytes(*bad, 1)
     with pytest.raises(ValueError):
         rmi.gqa_tree_workspace_bytes(100, 16, 4, 256, 1, 0)
+    for bad in (rmi.TREE_SHORT, 2 * rmi.TREE_SHORT, 2 * rmi.TREE_SHORT + 1, 2 ** 31 - 1):
+        with pytest.raises(ValueError):
+            rmi.gqa_tree_workspace_bytes(100, 16, 4, 256, 1, bad)
     with pytest.raises(ValueError):
         rmi.gqa_tree_workspace_bytes(128 * 2048 + 1, 16, 4, 256, 1, 1)
+    with pytest.raises(ValueError):
+        rmi.gqa_tree_workspace_bytes(128 * 2048 + 1, 16, 4, 256, 1, 1 + rmi.TREE_SHORT)
 
 
 def test_logits(rmi):
