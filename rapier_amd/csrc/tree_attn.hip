@@ -133,10 +133,13 @@ __device__ __forceinline__ half8 operand(const Dims16<T>& x, int hf, const Scale
     }
 }
 
-// VD neighbouring dims of a position
+// A lane's VD dims of a position: in runs of 16 bytes at most, lane l's k-th run at byte kRun * (16 k + l), so that 16 lanes
+// read whole lines
 template <int T, int VD>
 struct DimsV {
-    static constexpr int kBytes = T == kKvF16 ? 2 * VD : T == kKvI8 ? VD : VD / 2;
+    static constexpr int kBytes = T == kKvF16 ? 2 * VD : T == kKvI8 ? VD : VD / 2, kRun = kBytes < 16 ? kBytes : 16;
+    static constexpr int kRunDims = VD * kRun / kBytes;
+    static __device__ __forceinline__ int dim(int l16, int e) { return kRunDims * (16 * (e / kRunDims) + l16) + e % kRunDims; }
     uint32_t w[kBytes / 4];
 };
 template <int T, int VD>
@@ -146,7 +149,7 @@ __device__ __forceinline__ DimsV<T, VD> load_dims(Rsrc r, int lane_at, int at) {
     if constexpr (kB >= 16) {
 #pragma unroll
         for (int i = 0; i < kB / 16; ++i) {
-            const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, lane_at + 16 * i, at, 0);
+            const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, lane_at + 256 * i, at, 0);
             x.w[4 * i] = v[0], x.w[4 * i + 1] = v[1], x.w[4 * i + 2] = v[2], x.w[4 * i + 3] = v[3];
         }
     } else if constexpr (kB == 8) {
@@ -355,19 +358,23 @@ __device__ __forceinline__ void join_stats(float unit, const float (&stat)[WAVES
 
 // ---- few query rows: v_mfma_f32_16x16x32_f16 from the cache ---------------------------------------------------------------
 // Lane: l16 = l % 16, g4 = l / 16; A rows, B and D columns are l16; A and B hold k = 8 g4 + 0..7; D rows are 4 g4 + 0..3.
-//   scores    D[position][n] += K[position][dims] . q_n[dims]; lane (l16, g4) takes 16 neighbouring dims of position l16 at a
-//             time, 64 i + 16 g4 + [0, 16), as two operands of eight, straight from the cache.
+//   scores    D[position][n] += K[position][dims] . q_n[dims]; lane (l16, g4) takes 32 neighbouring dims of position l16,
+//             128 k + 32 g4 + [0, 32), as four operands of eight, straight from the cache: one load and one scale of I4.
+//             (F16 would read in whole lines with other dims, 5 % over 64K, but then its bits would not be the others'.)
 //   P V       D[m][dim] += P_m[positions] V[positions][dim].  The score lane (row, positions 4 g4 + r of two tiles) holds P in
 //             the A layout already, k slot j being position 4 g4 + j or 16 + 4 g4 + j - 4.  V comes by lane (l16, g4) as
-//             HD / 16 neighbouring dims of those eight positions; operand e gathers dim e.
+//             HD / 16 dims of those eight positions (DimsV); operand e gathers the lane's dim e.
 // Up to 8 rows, column (row) n < 8 is the high part of row n and n >= 8 the low part of row n - 8: one product gives both.  Up
 // to 16 rows the parts are two products, with q's operands in LDS (the registers hold o and the step's K and V).
 // The waves take quarters of the chunk.  K of the next step is loaded when this step's scores are done, V when its product is:
-// each has half a step to arrive.
+// each has half a step to arrive.  (Two steps ahead, in alternating registers, cost more than it hid: 30 us for 23.)
+// One token of 16 heads behind 65501 positions: F16 50 us with its join (5.3 TB/s), I8 33 (4.2), I4 23 (3.1).  Seven of them
+// are the beginning (position, first loads, q's parts) and the end; past that F16 and I8 are bound by the memory, I4 by
+// waiting on it with one wave a SIMD: its codes' 570 vector instructions a step take half the time.
 template <int KT, int VT, int HD, int ROWS>
 __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kernel(TreeArgs a) {
     constexpr bool PACKED = ROWS == 8;
-    constexpr int NI = HD / 64;        // K: 16-dim pieces a lane takes of a position
+    constexpr int NI = HD / 64;        // K: 16-dim pieces a lane takes of a position, two to a 32-dim run
     constexpr int VD = HD / 16;        // V: dims a lane takes of a position
     constexpr int NB = HD / kKvBlock;  // scale bytes of a row
     constexpr int kKB = kv_row_bytes(KT, HD), kVB = kv_row_bytes(VT, HD);
@@ -408,7 +415,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
     const KvRow<KT> k0 = kv_row<KT>(0, kv, a.n_kv, a.max_ctx, HD);
     const KvRow<VT> v0 = kv_row<VT>(0, kv, a.n_kv, a.max_ctx, HD);
     const uint8_t *kp = a.kc + k0.code, *ks = a.kc + k0.scale, *vp = a.vc + v0.code, *vs = a.vc + v0.scale;
-    const int kat = static_cast<int>(l16 * kstride) + g4 * (kKB / (HD / 32)), vat = static_cast<int>(4 * g4 * vstride) + l16 * DimsV<VT, VD>::kBytes;
+    const int kat = static_cast<int>(l16 * kstride) + g4 * (kKB / (HD / 32)), vat = static_cast<int>(4 * g4 * vstride) + l16 * DimsV<VT, VD>::kRun;
     const int vsat = 4 * g4 * NB + VD * l16 / kKvBlock;
 
     Dims16<KT> kx[2][NI];
@@ -595,7 +602,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
 #pragma unroll
                     for (int e = 0; e < VD; ++e) {
                         float v;
-                        if constexpr (VT == kKvF16) v = half_bits_to_float(reinterpret_cast<const uint16_t*>(vp + p1 * vstride)[VD * l16 + e]);
+                        if constexpr (VT == kKvF16) v = half_bits_to_float(reinterpret_cast<const uint16_t*>(vp + p1 * vstride)[DimsV<VT, VD>::dim(l16, e)]);
                         else v = kv_scale_value(vs[p1 * NB + VD * l16 / kKvBlock]);   // NaN: every value of the block
                         if (fabsf(v) <= FLT_MAX) continue;
 #pragma unroll
@@ -651,16 +658,16 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
                 const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[e][r]), __float_as_uint(o[e][r + 1]), false, false);
                 v[e] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
             }
-            float* to = &slab[wv][4 * (g4 & 1) + r + (g4 >> 1)][VD * l16];
+            float* to = slab[wv][4 * (g4 & 1) + r + (g4 >> 1)];
 #pragma unroll
-            for (int e = 0; e < VD; e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            for (int e = 0; e < VD; e += 4) *reinterpret_cast<float4*>(to + DimsV<VT, VD>::dim(l16, e)) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
         }
     } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int e = 0; e < VD; e += 4)
-                *reinterpret_cast<float4*>(&slab[wv][4 * g4 + r][VD * l16 + e]) = make_float4(o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]);
+                *reinterpret_cast<float4*>(&slab[wv][4 * g4 + r][DimsV<VT, VD>::dim(l16, e)]) = make_float4(o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]);
     }
     __syncthreads();
     join_stats<kWaves, 1, ROWS>(kSixteen<VT>, stat, fac, top, sum);
