@@ -684,6 +684,8 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
 //   P V       A = P, B = V columns by transposed reads (ds_read_b64_tr_b16: the 16 lanes of a g4 give the addresses of four
 //             positions x 16 dims and get a dim's four positions each), k slots as above.
 // Row strides of 16 and 32 bytes past a power of two spread a read's rows over the banks.
+// 999 tokens x 16 heads behind 8001 positions, I8 / I4: 286 us with the join's 16, 278 GFLOP of the two products each at 83 % of
+// the rate of a large matrix product; 64 rows a workgroup in place of 128 362 us.
 constexpr int kTileWaves = 8;
 constexpr int kTileThreads = 64 * kTileWaves;
 constexpr int kRowBlock = 16;
@@ -1001,7 +1003,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
 
 // ---- merge -------------------------------------------------------------------------------------------------------------
 // Workgroup (token, head, 64 dims): every lane has the (m, l) of a chunk and its group's first o in flight together; weights
-// 2^(m - M) to LDS, wave g sums chunks g, g + 4, ... in order, then the four waves in order; gate, fp32, Q8_1.
+// 2^(m - M) to LDS, wave g sums chunks g, g + 4, ... in order, then the four waves in order; gate, fp32, Q8_1.  64 chunks of one
+// token 3.9 us, a chain of waits (position, records, two barriers); whole rows a workgroup instead of 64 dims: no faster.
 constexpr int kMergeDims = 64, kMergeBatch = 16;
 
 template <int HD>
@@ -1073,7 +1076,8 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeArgs a) {
     if (a.q8) q8_1_store_lane(v, a.q8 + static_cast<size_t>(t) * a.q8_stride + (h * (HD / 32) + d / 32) * kQ8_1Bytes);
 }
 
-// The same for a few chunks, where the work is a pass over the records: HD / 4 lanes a row, four dims a lane, no LDS.
+// The same for a few chunks, where the work is a pass over the records: HD / 4 lanes a row, four dims a lane, no LDS.  999 tokens,
+// two chunks: 16 us, 4.1 TB/s.
 constexpr int kFlatChunks = 8;
 
 template <int HD>
