@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
+import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "librapier_mi.so")
@@ -566,9 +567,22 @@ def _a(t):
     return None if t is None else t.data_ptr()
 
 
-def _s(stream):
+_gpu = None   # torch's current device and raw stream, without the checks (0.5 us each) around them
+
+
+def _s(stream, t):
+    """the stream's handle, for a call whose tensors are where t is: on the current GPU, whose kernels and streams these are"""
+    global _gpu
+    at = t.get_device()   # -1: host memory
+    if at < 0:
+        raise ValueError("a tensor that is not on the current GPU")
+    if _gpu is None:
+        c = sys.modules["torch"]._C
+        _gpu = c._cuda_getDevice, c._cuda_getCurrentRawStream
+    if at != _gpu[0]():
+        raise ValueError("a tensor that is not on the current GPU")
     if stream is None:
-        return _raw_stream() if _raw_stream else _current_stream()
+        return _gpu[1](at)
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
@@ -579,28 +593,36 @@ def kv_cache_bytes(type_, max_ctx, n_kv, head_dim) -> int:
     return n
 
 
+_ROWS = {}   # dtypes of rows -> whether they are 16-bit
+
+
 def _is_f16(t):
-    """1 for 16-bit rows (float16, or int16 / uint16 that hold its bits), 0 for float32"""
-    return 1 if t.element_size() == 2 else 0
+    """1 for float16 rows (or int16 / uint16 that hold their bits), 0 for float32"""
+    if not _ROWS:
+        torch = sys.modules["torch"]
+        _ROWS.update({torch.float32: 0, torch.float16: 1, torch.int16: 1, torch.uint16: 1})
+    if t.dtype not in _ROWS:
+        raise ValueError(f"rows of float32 or float16, not {t.dtype}")
+    return _ROWS[t.dtype]
 
 
 def kv_write(type_, src, src_stride, cache, first, n, n_kv, head_dim, max_ctx, stream=None):
     """n rows [n_kv x head_dim] of float32 or float16, src_stride elements apart, to positions [first, first + n)"""
     _call("rmi_kv_write", type_, _a(src), _is_f16(src), src_stride, _a(cache), first, n, n_kv, head_dim, max_ctx,
-          _s(stream))
+          _s(stream, cache))
 
 
 def kv_read(type_, cache, out, out_stride, first, n, n_kv, head_dim, max_ctx, stream=None):
     """positions [first, first + n) of a cache back to float32 or float16 rows"""
     _call("rmi_kv_read", type_, _a(cache), _a(out), _is_f16(out), out_stride, first, n, n_kv, head_dim, max_ctx,
-          _s(stream))
+          _s(stream, cache))
 
 
 def kv_compact(type_, caches, pos, path, count, max_path, n_kv, head_dim, max_ctx, stream=None):
     """rows pos[0] + path[i] -> pos[0] + i, i < min(count[0], max_path), in each of the caches (a list of tensors)"""
     ptrs = (ctypes.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches])
     _call("rmi_kv_compact", type_, ptrs, len(caches), _a(pos), _a(path), _a(count), max_path, n_kv, head_dim, max_ctx,
-          _s(stream))
+          _s(stream, pos))
 
 
 class RopeAxes(ctypes.Structure):
@@ -616,7 +638,7 @@ def attn_prep_axes(q3, q3_stride, qn, kn, ktype, kcache, vtype, vcache, pos, axi
     axes = RopeAxes((ctypes.c_int * 3)(*sections), int(interleaved))
     _call("rmi_attn_prep_axes", _a(q3), q3_stride, _a(qn), _a(kn), ktype, _a(kcache), vtype, _a(vcache), _a(pos),
           _a(axis_pos), _a(qout), n_head, n_kv, head_dim, n_rot, ctypes.byref(rope), ctypes.byref(axes), eps, ntok,
-          max_ctx, _s(stream))
+          max_ctx, _s(stream, kcache))
 
 
 def gqa_tree_nsub(ctx, n_head, n_kv, head_dim, ntok) -> int:
@@ -640,7 +662,7 @@ def gqa_tree_decode(q, ktype, kcache, vtype, vcache, pos, masks, gate_src, gate_
     masks[t] (int64 bit patterns) says; masks None: the chain j <= t"""
     _call("rmi_gqa_tree_decode", _a(q), ktype, _a(kcache), vtype, _a(vcache), _a(pos), _a(masks), _a(gate_src),
           gate_stride, _a(y), y_stride, _a(q8), q8_stride, _a(workspace), n_head, n_kv, head_dim, ntok, max_ctx, nsub,
-          scale, _s(stream))
+          scale, _s(stream, q))
 
 
 class Penalties(ctypes.Structure):
@@ -656,4 +678,4 @@ def logits_process(logits, n, ncols, col_stride, out, out_stride, history, histo
     pen = Penalties(repetition, presence, frequency, window)
     _call("rmi_logits_process", _a(logits), n, ncols, col_stride, _a(out), out_stride, _a(history), _a(history_len),
           max_history, _a(draft), _a(masks), ndraft, ctypes.byref(pen), _a(bias_ids), _a(bias_vals), n_bias, _a(allow),
-          allow_stride, _s(stream))
+          allow_stride, _s(stream, logits))

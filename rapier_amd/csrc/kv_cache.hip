@@ -428,6 +428,9 @@ __global__ __launch_bounds__(64 * kPrepWaves) void prep_axes_kernel(PrepArgs a) 
     }
 }
 
+constexpr long long kMaxBlocks = 0xffffffffLL / kRowThreads;   // a launch's work-items along an axis are a 32-bit number
+static_assert(kRowThreads == 64 * kPrepWaves);
+
 bool aligned_to(const void* p, size_t n) { return p && (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // whether two caches of these sizes share bytes
@@ -474,7 +477,7 @@ extern "C" int rmi_kv_write(int type, const void* src, int src_f16, int src_stri
     if (n == 0) return RMI_OK;
     const int per = kWriteUnits * kRowThreads / (head_dim / 8);   // rows a workgroup
     const long long blocks = (static_cast<long long>(n) + per - 1) / per * n_kv;
-    if (blocks > 0x7fffffffLL) return fail(RMI_ERR_SHAPE, "kv_write: too many rows for one call");
+    if (blocks > kMaxBlocks) return fail(RMI_ERR_SHAPE, "kv_write: too many rows for one call");
     const bool vec = aligned16(src) && src_stride % (src_f16 ? 8 : 4) == 0;   // 16-byte loads, else one by one
     auto* out = static_cast<uint8_t*>(cache);
     return with_type(type, [&](auto t) {
@@ -495,7 +498,7 @@ extern "C" int rmi_kv_read(int type, const void* cache, void* out, int out_f16, 
     if (n == 0) return RMI_OK;
     const int per = kRowThreads / (head_dim / 8);
     const long long blocks = (static_cast<long long>(n) + per - 1) / per * n_kv;
-    if (blocks > 0x7fffffffLL) return fail(RMI_ERR_SHAPE, "kv_read: too many rows for one call");
+    if (blocks > kMaxBlocks) return fail(RMI_ERR_SHAPE, "kv_read: too many rows for one call");
     const bool vec = aligned16(out) && out_stride % (out_f16 ? 8 : 4) == 0;
     const auto* in = static_cast<const uint8_t*>(cache);
     return with_type(type, [&](auto t) {
@@ -540,7 +543,7 @@ extern "C" int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* q
     const char* what = "attn_prep_axes: invalid arguments";
     if (!kv_type_ok(ktype) || !kv_type_ok(vtype)) return fail(RMI_ERR_UNSUPPORTED, "attn_prep_axes: unknown cache type");
     if (!kv_shape_ok(max_ctx, n_kv, head_dim) || n_head <= 0 || n_head > 65535 || n_head % n_kv || n_rot < 0 || n_rot > head_dim || n_rot % 2 ||
-        ntok < 1 || ntok > max_ctx || !rope || !(rope->freq_base > 1.0f) || !axes ||
+        ntok < 1 || ntok > max_ctx || ntok > kMaxBlocks || !rope || !(rope->freq_base > 1.0f) || !axes ||
         2LL * n_head * head_dim + 2LL * n_kv * head_dim > 0x7fffffffLL)
         return fail(RMI_ERR_SHAPE, what);
     const int* s = axes->section;

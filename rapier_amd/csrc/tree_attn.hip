@@ -1248,7 +1248,7 @@ extern "C" int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache
     a.q8_stride = q8_stride;
     a.scale = scale;
     const long long chunks = tree_chunks(max_ctx, nsub), pairs = chunks * n_kv, blocks = (pairs + 7) / 8 * 8 * f.groups;
-    if (blocks > 0x7fffffffLL) return fail(RMI_ERR_SHAPE, "gqa_tree_decode: too many workgroups");
+    if (blocks > 0xffffffffLL / kTileThreads) return fail(RMI_ERR_SHAPE, "gqa_tree_decode: too many workgroups");
     a.npairs = static_cast<int>(pairs);
     a.direct = chunks == 1;
     a.wo = static_cast<float*>(workspace);

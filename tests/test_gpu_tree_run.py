@@ -228,3 +228,48 @@ def test_two_calls_at_once(rmi):
     t.cuda.synchronize()
     for i in range(2):
         assert np.array_equal(host(ys[i]).view(np.uint32), want[i].view(np.uint32))
+
+
+@pytest.mark.parametrize("type_,ntok", [(ref.F16, 3), (ref.F16, 70), (ref.I8, 3), (ref.I8, 40), (ref.I4, 5)])
+def test_a_cache_beyond_32_bit_offsets(rmi, type_, ntok):
+    """2.3 million positions x 8 heads x 256: rows at the far end written, seen, moved and read back; the others are zero, so the
+    softmax has a closed form"""
+    t = torch()
+    nkv, hd, ctx = 8, 256, 2300000
+    rng = np.random.default_rng(ntok)
+    caches = [t.zeros(rmi.kv_cache_bytes(type_, ctx, nkv, hd), dtype=t.uint8, device="cuda:0") for _ in range(2)]
+    n, base = ntok + 4, ctx - ntok          # four rows of the context, then the draft, which ends with the cache
+    rows = [rng.standard_normal((n, nkv, hd)).astype(np.float32) for _ in range(2)]
+    for c, x in zip(caches, rows):
+        rmi.kv_write(type_, dev(x), nkv * hd, c, base - 4, n, nkv, hd, ctx)
+    held = [ref.held(x, type_) for x in rows]
+    q = rng.standard_normal((ntok, nkv, hd)).astype(np.float32)
+    pos = dev(np.array([base], np.int32))
+    nsub = rmi.gqa_tree_nsub(ctx, nkv, nkv, hd, ntok)
+    ws, y = empty(rmi.gqa_tree_workspace_bytes(ctx, nkv, nkv, hd, ntok, nsub), "uint8"), empty(ntok * nkv * hd)
+    scale = 0.75   # scores of about +-12: the few rows weigh as much as the zeros
+    rmi.gqa_tree_decode(dev(q), type_, caches[0], type_, caches[1], pos, None, None, 0, y, nkv * hd, None, 0, ws, nkv, nkv, hd, ntok, ctx, nsub,
+                        scale)
+    got = host(y).reshape(ntok, nkv, hd)
+    for i in range(ntok):
+        m = 4 + i + 1
+        s = np.einsum("hd,phd->hp", q[i].astype(np.float64), held[0][:m]) * scale
+        top = np.maximum(s.max(1, keepdims=True), 0)
+        w = np.exp(s - top)
+        total = w.sum(1) + (base - 4) * np.exp(-top[:, 0])
+        want = np.einsum("hp,phd->hd", w, held[1][:m]) / total[:, None]
+        # a weight's relative error: its score's ((hd + 8) roundings of the sum of |q k|), the exponent's and the sum's (a lane
+        # adds once per step of 32 positions, a chunk's wave has nsub of them)
+        a = np.einsum("hd,phd->hp", np.abs(q[i]).astype(np.float64), np.abs(held[0][:m])).max(1) * scale
+        rel = 2 * (hd + 8) * 2.0 ** -24 * a + 2.0 ** -18 + (m + (nsub & (rmi.TREE_SHORT - 1))) * 2.0 ** -24
+        assert (np.abs(got[i] - want) <= (rel * (w @ np.ones(m)) / total * np.abs(held[1]).max())[:, None]).all()
+    path = [1, ntok - 1]
+    rmi.kv_compact(type_, caches, pos, dev(np.array(path, np.int32)), dev(np.array([2], np.int32)), 2, nkv, hd, ctx)
+    out = empty(n * nkv * hd)
+    for c, h in zip(caches, held):
+        rmi.kv_read(type_, c, out, nkv * hd, base - 4, n, nkv, hd, ctx)
+        want = h.copy()
+        want[4], want[5] = h[4 + path[0]], h[4 + path[1]]
+        assert np.array_equal(host(out).reshape(n, nkv, hd).astype(np.float64), want)
+    del caches
+    t.cuda.empty_cache()

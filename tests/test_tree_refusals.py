@@ -126,3 +126,34 @@ def test_logits(rmi):
                 {"ids": None}, {"vals": None}, {"allow": ODD}):
         with pytest.raises(ValueError, match="logits_process"):
             call(**bad)
+
+
+def test_bindings_refuse_host_tensors_and_other_types(rmi):
+    import torch
+    x, i = torch.zeros(4096), torch.zeros(4, dtype=torch.int32)
+    b = torch.zeros(1 << 20, dtype=torch.uint8)
+    for f in (lambda: rmi.kv_write(rmi.KV_I8, x, 1024, b, 0, 1, 4, 256, 100),
+              lambda: rmi.kv_read(rmi.KV_I8, b, x, 1024, 0, 1, 4, 256, 100),
+              lambda: rmi.kv_compact(rmi.KV_I8, [b], i, i, i, 1, 4, 256, 100),
+              lambda: rmi.gqa_tree_decode(x, 1, b, 1, b, i, None, None, 0, x, 4096, None, 0, b, 16, 4, 256, 1, 100, 1, 0.06),
+              lambda: rmi.attn_prep_axes(x, 6144, x, x, 1, b, 1, b, i, None, x, 16, 4, 256, 64, 1e6, 1.0, 0.0, (12, 10, 10), True, 1e-6, 1, 100),
+              lambda: rmi.logits_process(x, 100, 1, 100, x, 100, None, None, 0),
+              lambda: rmi.logits_process(x, 100, 1, 100, x, 100, None, None, 0, stream=1)):
+        with pytest.raises(ValueError, match="current GPU"):
+            f()
+    for t in (torch.bfloat16, torch.float64, torch.uint8):
+        with pytest.raises(ValueError, match="float32 or float16"):
+            rmi.kv_write(rmi.KV_I8, x.to(t), 1024, b, 0, 1, 4, 256, 100)
+        with pytest.raises(ValueError, match="float32 or float16"):
+            rmi.kv_read(rmi.KV_I8, b, x.to(t), 1024, 0, 1, 4, 256, 100)
+
+
+def test_launches_stay_in_32_bit_work_items(rmi):
+    with pytest.raises(ValueError, match="too many rows"):
+        rmi._call("rmi_kv_read", 2, FAKE, FAR, 1, 64 * 256, 0, 1 << 22, 64, 256, 1 << 22, None)
+    with pytest.raises(ValueError, match="too many rows"):
+        rmi._call("rmi_kv_write", 2, FAKE, 1, 128 * 256, FAR, 0, 1 << 22, 128, 256, 1 << 22, None)
+    p, a = rmi.RopeParams(1e6, 1.0, 0.0, 1.0, 1.0, 32.0, 1.0), rmi.RopeAxes((ctypes.c_int * 3)(32, 0, 0), 0)
+    with pytest.raises(ValueError, match="attn_prep_axes"):
+        rmi._call("rmi_attn_prep_axes", FAKE, 512, FAKE, FAKE, 1, FAKE, 1, ctypes.c_void_p(1 << 45), FAKE, None, FAKE, 1, 1, 128, 64,
+                  ctypes.byref(p), ctypes.byref(a), 1e-6, 1 << 25, 1 << 26, None)
