@@ -9,6 +9,7 @@ here computes on the CPU.  A missing library is an ``ImportError``-style failure
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import subprocess
 import sys
@@ -167,8 +168,16 @@ def _check(rc):
         raise RapierError(msg)
 
 
+_entries = {}   # entry points by name
+
+
 def _call(name, *args):
-    _check(getattr(lib(), name)(*args))
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(lib(), name)
+    rc = fn(*args)
+    if rc:
+        _check(rc)
 
 
 def _p(t):
@@ -630,12 +639,18 @@ class RopeAxes(ctypes.Structure):
     _fields_ = [("section", ctypes.c_int * 3), ("interleaved", ctypes.c_int)]
 
 
+@functools.lru_cache(maxsize=64)
+def _rope_args(sections, interleaved, *rope):
+    """the argument blocks of these values, which the library only reads (building them costs as much as the call)"""
+    return RopeParams(*rope), RopeAxes((ctypes.c_int * 3)(*sections), interleaved)
+
+
 def attn_prep_axes(q3, q3_stride, qn, kn, ktype, kcache, vtype, vcache, pos, axis_pos, qout, n_head, n_kv, head_dim,
                    n_rot, freq_base, factor, orig_ctx, sections, interleaved, eps, ntok, max_ctx, ext_factor=1.0,
                    attn_factor=1.0, beta_fast=32.0, beta_slow=1.0, stream=None):
     """per-head norm, rotation at axis_pos ([3][ntok]; None: the slots) and the cache write at slots pos[0] + t"""
-    rope = RopeParams(freq_base, factor, orig_ctx, ext_factor, attn_factor, beta_fast, beta_slow)
-    axes = RopeAxes((ctypes.c_int * 3)(*sections), int(interleaved))
+    rope, axes = _rope_args(tuple(sections), int(interleaved), freq_base, factor, orig_ctx, ext_factor, attn_factor,
+                            beta_fast, beta_slow)
     _call("rmi_attn_prep_axes", _a(q3), q3_stride, _a(qn), _a(kn), ktype, _a(kcache), vtype, _a(vcache), _a(pos),
           _a(axis_pos), _a(qout), n_head, n_kv, head_dim, n_rot, ctypes.byref(rope), ctypes.byref(axes), eps, ntok,
           max_ctx, _s(stream, kcache))

@@ -1004,7 +1004,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
 // ---- merge -------------------------------------------------------------------------------------------------------------
 // Workgroup (token, head, 64 dims): every lane has the (m, l) of a chunk and its group's first o in flight together; weights
 // 2^(m - M) to LDS, wave g sums chunks g, g + 4, ... in order, then the four waves in order; gate, fp32, Q8_1.  64 chunks of one
-// token 3.9 us, a chain of waits (position, records, two barriers); whole rows a workgroup instead of 64 dims: no faster.
+// token 3.9 us, a chain of waits (position, records, two barriers).  A whole row a workgroup: 10.6 us in place of 11.2 for 32 chunks of 64 tokens,
+// which are joined in groups of 16 rows, over few chunks, instead.
 constexpr int kMergeDims = 64, kMergeBatch = 16;
 
 template <int HD>
@@ -1176,7 +1177,7 @@ extern "C" int rmi_gqa_tree_nsub(int ctx, int n_head, int n_kv, int head_dim, in
         return 0;
     }
     // One workgroup for each of 256 compute units: as many chunks as leave an XCD's 32 units a (chunk, head, group) each, since
-    // a 33rd doubles the launch's time.  I8, 12 tokens x 4 heads behind 16K: 33 an XCD 32.0 us, 27 28.9, 24 23.7; 1 token at
+    // a 33rd is done after or beside another.  I8, 12 tokens x 4 heads behind 16K: 33 an XCD 32.0 us, 24 23.7; 1 token at
     // 64K with two workgroups a unit 32.8 us, one 32.8 (I4 23.7 / 22.9, F16 55 / 51).
     const long long units = (ctx + kUnit - 1) / kUnit;
     auto nsub_for = [&](int groups) {
@@ -1186,7 +1187,7 @@ extern "C" int rmi_gqa_tree_nsub(int ctx, int n_head, int n_kv, int head_dim, in
     // More than 16 rows as groups of few while a wave of theirs has at most 8 steps, where a workgroup's beginning and end
     // and the records of many chunks weigh more than turning K and V to fp16 once: 16 tokens x 4 heads, groups / tiles: I8 4K
     // 16.5 / 19.9 us, 8K 20.0 / 22.6, 16K 24.6 / 25.8; 64 tokens 4K 26.4 / 32.9, 32 tokens 16K (16 steps) 40 / 36.5;
-    // F16 16 tokens 4K 17.5 / 18.8, 16K 32.6 / 27.2.
+    // F16 16 tokens 4K 17.5 / 18.8, 16K 32.6 / 27.2, 64 tokens 4K 33.3 / 32.9.
     constexpr int kFewSteps = 8;
     const Form few = tree_form(n_head, n_kv, ntok, kShort + 1, false), tile = tree_form(n_head, n_kv, ntok, kLongSub, true);
     long long nsub = nsub_for(few.groups);
