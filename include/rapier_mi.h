@@ -365,7 +365,8 @@ int rmi_gqa_flash_decode_noalloc(const float* q, const uint16_t* kcache, const u
  * A block of 32 dims shares the scale s: a scale byte b is the fp16 number with the bits b << 7 (five exponent and three
  * mantissa bits).  s is the smallest such number with Q s >= max|x| (Q = 127 / 7, at most 512 / 8192: larger values
  * saturate), code = x / s rounded to the nearest integer (half to even), |code| <= Q, and the cache holds code * s, which
- * is an fp16 number exactly.  A block with an infinity or a NaN gets s = NaN and reads back as NaN. */
+ * is an fp16 number exactly.  A block with an infinity or a NaN gets s = NaN and reads back as NaN.  No call writes another
+ * scale byte above that of 512 / 8192; the attention takes those of 960 / 15360 and more as NaN. */
 enum { RMI_KV_F16 = 0, RMI_KV_I8 = 1, RMI_KV_I4 = 2 };
 
 /* bytes of one cache; 0 on a bad type or shape */

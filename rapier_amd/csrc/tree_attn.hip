@@ -77,6 +77,13 @@ __device__ __forceinline__ Scale2 scale2(uint32_t lo, uint32_t hi) {
     r.c = r.s * half2v{kBias, kBias};
     return r;
 }
+// The first scale byte whose addend is past fp16's largest number (199 for I8, 231 for I4): a block with it or a larger one has
+// no finite value here.  The quantiser writes none but 255, the NaN's; unwritten memory holds any.
+template <int T>
+constexpr uint32_t kOddScale = kv_top_scale(T) + 7;
+// what every value of such a block is (NaN); zero for the others
+template <int T>
+__device__ __forceinline__ float odd_value(uint32_t byte) { return byte < kOddScale<T> ? 0.0f : __builtin_nanf(""); }
 __device__ __forceinline__ uint32_t fma2(uint32_t x, const Scale2& s) { return u2(__builtin_elementwise_fma(h2(x), s.s, s.c)); }
 
 // (w & mask) | magic in one instruction: with both as literals the compiler takes two
@@ -197,12 +204,12 @@ __device__ __forceinline__ uint32_t max_magnitude(uint32_t m, uint32_t w) {
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
 }
-// a word of fp16 V without its infinities and NaN
-__device__ __forceinline__ uint32_t zero_odd(uint32_t w) {
-    if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
-    if ((w & 0x7c000000u) == 0x7c000000u) w &= 0xffffu;
-    return w;
+// a mask of the halves of a word that are finite
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
+    return ((w & 0x7c00u) != 0x7c00u ? 0xffffu : 0u) | ((w & 0x7c000000u) != 0x7c000000u ? 0xffff0000u : 0u);
 }
+// a word of fp16 V without its infinities and NaN
+__device__ __forceinline__ uint32_t zero_odd(uint32_t w) { return w & finite_halves(w); }
 
 // the power of two that brings a row's largest |q| to [2^13, 2^14), as its exponent
 __device__ __forceinline__ int q_shift(float amax) {
@@ -585,7 +592,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (VT != kKvF16) {
-                    big = max_magnitude(big, u2(vsp[j].s));
+                    big = max_magnitude(big, u2(vsp[j].c));   // not finite wherever s is not
                 } else {
 #pragma unroll
                     for (int e = 0; e < VD / 2; ++e) big = max_magnitude(max_magnitude(big, vx[2 * j].w[e]), vx[2 * j + 1].w[e]);
@@ -603,7 +610,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
                     for (int e = 0; e < VD; ++e) {
                         float v;
                         if constexpr (VT == kKvF16) v = half_bits_to_float(reinterpret_cast<const uint16_t*>(vp + p1 * vstride)[DimsV<VT, VD>::dim(l16, e)]);
-                        else v = kv_scale_value(vs[p1 * NB + VD * l16 / kKvBlock]);   // NaN: every value of the block
+                        else v = odd_value<VT>(vs[p1 * NB + VD * l16 / kKvBlock]);
                         if (fabsf(v) <= FLT_MAX) continue;
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
@@ -618,8 +625,9 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
 #pragma unroll
                         for (int e = 0; e < VD / 2; ++e) vx[j].w[e] = zero_odd(vx[j].w[e]);
                     } else if ((j & 1) == 0) {
-                        vsp[j >> 1].s = h2(zero_odd(u2(vsp[j >> 1].s)));
-                        vsp[j >> 1].c = h2(zero_odd(u2(vsp[j >> 1].c)));
+                        const uint32_t c = u2(vsp[j >> 1].c);
+                        vsp[j >> 1].s = h2(u2(vsp[j >> 1].s) & finite_halves(c));
+                        vsp[j >> 1].c = h2(c & finite_halves(c));
                     }
                 }
             }
@@ -921,7 +929,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tree_tile_kernel(TreeArgs a) 
                         const int d = 16 * e + l16;
                         float v;
                         if constexpr (VT == kKvF16) v = half_bits_to_float(reinterpret_cast<const uint16_t*>(a.vc + vrow.code)[d]);
-                        else v = kv_scale_value(a.vc[vrow.scale + d / kKvBlock]);   // NaN: every value of the block
+                        else v = odd_value<VT>(a.vc[vrow.scale + d / kKvBlock]);
                         if (fabsf(v) <= FLT_MAX) continue;
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
