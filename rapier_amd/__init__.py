@@ -579,10 +579,14 @@ def _a(t):
 _gpu = None   # torch's current device and raw stream, without the checks (0.5 us each) around them
 
 
-def _s(stream, t):
-    """the stream's handle, for a call whose tensors are where t is: on the current GPU, whose kernels and streams these are"""
+def _s(stream, at, *tensors):
+    """the stream's handle, for a call on the tensor `at` and these (None: an argument left out): all on the current GPU, whose
+    kernels and streams these are"""
     global _gpu
-    at = t.get_device()   # -1: host memory
+    at = at.get_device()   # -1: host memory
+    for t in tensors:
+        if t is not None and t.get_device() != at:
+            raise ValueError("a tensor that is not on the current GPU")
     if at < 0:
         raise ValueError("a tensor that is not on the current GPU")
     if _gpu is None:
@@ -592,7 +596,11 @@ def _s(stream, t):
         raise ValueError("a tensor that is not on the current GPU")
     if stream is None:
         return _gpu[1](at)
-    return stream if isinstance(stream, int) else stream.cuda_stream
+    if isinstance(stream, int):
+        return stream
+    if getattr(stream, "device_index", at) != at:
+        raise ValueError("a stream that is not the current GPU's")
+    return stream.cuda_stream
 
 
 def kv_cache_bytes(type_, max_ctx, n_kv, head_dim) -> int:
@@ -618,20 +626,20 @@ def _is_f16(t):
 def kv_write(type_, src, src_stride, cache, first, n, n_kv, head_dim, max_ctx, stream=None):
     """n rows [n_kv x head_dim] of float32 or float16, src_stride elements apart, to positions [first, first + n)"""
     _call("rmi_kv_write", type_, _a(src), _is_f16(src), src_stride, _a(cache), first, n, n_kv, head_dim, max_ctx,
-          _s(stream, cache))
+          _s(stream, cache, src))
 
 
 def kv_read(type_, cache, out, out_stride, first, n, n_kv, head_dim, max_ctx, stream=None):
     """positions [first, first + n) of a cache back to float32 or float16 rows"""
     _call("rmi_kv_read", type_, _a(cache), _a(out), _is_f16(out), out_stride, first, n, n_kv, head_dim, max_ctx,
-          _s(stream, cache))
+          _s(stream, cache, out))
 
 
 def kv_compact(type_, caches, pos, path, count, max_path, n_kv, head_dim, max_ctx, stream=None):
     """rows pos[0] + path[i] -> pos[0] + i, i < min(count[0], max_path), in each of the caches (a list of tensors)"""
     ptrs = (ctypes.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches])
     _call("rmi_kv_compact", type_, ptrs, len(caches), _a(pos), _a(path), _a(count), max_path, n_kv, head_dim, max_ctx,
-          _s(stream, pos))
+          _s(stream, pos, path, count, *caches))
 
 
 class RopeAxes(ctypes.Structure):
@@ -653,7 +661,7 @@ def attn_prep_axes(q3, q3_stride, qn, kn, ktype, kcache, vtype, vcache, pos, axi
                             beta_fast, beta_slow)
     _call("rmi_attn_prep_axes", _a(q3), q3_stride, _a(qn), _a(kn), ktype, _a(kcache), vtype, _a(vcache), _a(pos),
           _a(axis_pos), _a(qout), n_head, n_kv, head_dim, n_rot, ctypes.byref(rope), ctypes.byref(axes), eps, ntok,
-          max_ctx, _s(stream, kcache))
+          max_ctx, _s(stream, kcache, vcache, q3, qn, kn, pos, axis_pos, qout))
 
 
 def gqa_tree_nsub(ctx, n_head, n_kv, head_dim, ntok) -> int:
@@ -677,7 +685,7 @@ def gqa_tree_decode(q, ktype, kcache, vtype, vcache, pos, masks, gate_src, gate_
     masks[t] (int64 bit patterns) says; masks None: the chain j <= t"""
     _call("rmi_gqa_tree_decode", _a(q), ktype, _a(kcache), vtype, _a(vcache), _a(pos), _a(masks), _a(gate_src),
           gate_stride, _a(y), y_stride, _a(q8), q8_stride, _a(workspace), n_head, n_kv, head_dim, ntok, max_ctx, nsub,
-          scale, _s(stream, q))
+          scale, _s(stream, q, kcache, vcache, pos, masks, gate_src, y, q8, workspace))
 
 
 class Penalties(ctypes.Structure):
@@ -693,4 +701,4 @@ def logits_process(logits, n, ncols, col_stride, out, out_stride, history, histo
     pen = Penalties(repetition, presence, frequency, window)
     _call("rmi_logits_process", _a(logits), n, ncols, col_stride, _a(out), out_stride, _a(history), _a(history_len),
           max_history, _a(draft), _a(masks), ndraft, ctypes.byref(pen), _a(bias_ids), _a(bias_vals), n_bias, _a(allow),
-          allow_stride, _s(stream, logits))
+          allow_stride, _s(stream, logits, out, history, history_len, draft, masks, bias_ids, bias_vals, allow))
