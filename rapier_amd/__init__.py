@@ -576,17 +576,35 @@ def _a(t):
     return None if t is None else t.data_ptr()
 
 
-_gpu = None   # torch's current device and raw stream, without the checks (0.5 us each) around them
+_gpu = None     # torch's current device and raw stream, without the checks (0.5 us each) around them
+_kinds = None   # what float, int and mask arguments may be
 
 
-def _s(stream, at, *tensors):
-    """the stream's handle, for a call on the tensor `at` and these (None: an argument left out): all on the current GPU, whose
-    kernels and streams these are"""
+_NAMES = ("float32", "int32", "int64")
+
+
+def _argument_kinds():
+    global _kinds
+    torch = sys.modules["torch"]   # uint8: raw memory
+    _kinds = ({torch.float32, torch.uint8}, {torch.int32, torch.uint32, torch.uint8}, {torch.int64, torch.uint64, torch.uint8})
+    return _kinds
+
+
+def _s(stream, at, raw=(), f32=(), i32=(), i64=()):
+    """the stream's handle, for a call on the tensor `at` and these (None: an argument left out), which are on the current GPU,
+    whose kernels and streams these are, and of the element types that the library takes"""
     global _gpu
     at = at.get_device()   # -1: host memory
-    for t in tensors:
+    for t in raw:
         if t is not None and t.get_device() != at:
             raise ValueError("a tensor that is not on the current GPU")
+    for kind, tensors in zip(_kinds or _argument_kinds(), (f32, i32, i64)):
+        for t in tensors:
+            if t is not None:
+                if t.get_device() != at:
+                    raise ValueError("a tensor that is not on the current GPU")
+                if t.dtype not in kind:
+                    raise ValueError(f"a tensor of {t.dtype} where the library takes {_NAMES[_kinds.index(kind)]}")
     if at < 0:
         raise ValueError("a tensor that is not on the current GPU")
     if _gpu is None:
@@ -626,20 +644,20 @@ def _is_f16(t):
 def kv_write(type_, src, src_stride, cache, first, n, n_kv, head_dim, max_ctx, stream=None):
     """n rows [n_kv x head_dim] of float32 or float16, src_stride elements apart, to positions [first, first + n)"""
     _call("rmi_kv_write", type_, _a(src), _is_f16(src), src_stride, _a(cache), first, n, n_kv, head_dim, max_ctx,
-          _s(stream, cache, src))
+          _s(stream, cache, (src,)))
 
 
 def kv_read(type_, cache, out, out_stride, first, n, n_kv, head_dim, max_ctx, stream=None):
     """positions [first, first + n) of a cache back to float32 or float16 rows"""
     _call("rmi_kv_read", type_, _a(cache), _a(out), _is_f16(out), out_stride, first, n, n_kv, head_dim, max_ctx,
-          _s(stream, cache, out))
+          _s(stream, cache, (out,)))
 
 
 def kv_compact(type_, caches, pos, path, count, max_path, n_kv, head_dim, max_ctx, stream=None):
     """rows pos[0] + path[i] -> pos[0] + i, i < min(count[0], max_path), in each of the caches (a list of tensors)"""
     ptrs = (ctypes.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches])
     _call("rmi_kv_compact", type_, ptrs, len(caches), _a(pos), _a(path), _a(count), max_path, n_kv, head_dim, max_ctx,
-          _s(stream, pos, path, count, *caches))
+          _s(stream, pos, caches, (), (pos, path, count)))
 
 
 class RopeAxes(ctypes.Structure):
@@ -661,7 +679,7 @@ def attn_prep_axes(q3, q3_stride, qn, kn, ktype, kcache, vtype, vcache, pos, axi
                             beta_fast, beta_slow)
     _call("rmi_attn_prep_axes", _a(q3), q3_stride, _a(qn), _a(kn), ktype, _a(kcache), vtype, _a(vcache), _a(pos),
           _a(axis_pos), _a(qout), n_head, n_kv, head_dim, n_rot, ctypes.byref(rope), ctypes.byref(axes), eps, ntok,
-          max_ctx, _s(stream, kcache, vcache, q3, qn, kn, pos, axis_pos, qout))
+          max_ctx, _s(stream, kcache, (vcache,), (q3, qn, kn, qout), (pos, axis_pos)))
 
 
 def gqa_tree_nsub(ctx, n_head, n_kv, head_dim, ntok) -> int:
@@ -685,7 +703,7 @@ def gqa_tree_decode(q, ktype, kcache, vtype, vcache, pos, masks, gate_src, gate_
     masks[t] (int64 bit patterns) says; masks None: the chain j <= t"""
     _call("rmi_gqa_tree_decode", _a(q), ktype, _a(kcache), vtype, _a(vcache), _a(pos), _a(masks), _a(gate_src),
           gate_stride, _a(y), y_stride, _a(q8), q8_stride, _a(workspace), n_head, n_kv, head_dim, ntok, max_ctx, nsub,
-          scale, _s(stream, q, kcache, vcache, pos, masks, gate_src, y, q8, workspace))
+          scale, _s(stream, q, (kcache, vcache, q8, workspace), (q, gate_src, y), (pos,), (masks,)))
 
 
 class Penalties(ctypes.Structure):
@@ -701,4 +719,4 @@ def logits_process(logits, n, ncols, col_stride, out, out_stride, history, histo
     pen = Penalties(repetition, presence, frequency, window)
     _call("rmi_logits_process", _a(logits), n, ncols, col_stride, _a(out), out_stride, _a(history), _a(history_len),
           max_history, _a(draft), _a(masks), ndraft, ctypes.byref(pen), _a(bias_ids), _a(bias_vals), n_bias, _a(allow),
-          allow_stride, _s(stream, logits, out, history, history_len, draft, masks, bias_ids, bias_vals, allow))
+          allow_stride, _s(stream, logits, (), (logits, out, bias_vals), (history, history_len, draft, bias_ids, allow), (masks,)))

@@ -108,3 +108,27 @@ def test_another_gpu_than_the_current_one(entered, f):
     with pytest.raises(ValueError, match="stream"):
         f(tensors(f), stream=Stream(1))
     assert not entered
+
+
+@pytest.mark.parametrize("f,name", [p for p in EACH if p.values[0] not in (kv_write, kv_read) and CALLS[p.values[0]][p.values[1]] is not U8])
+def test_each_tensor_has_to_be_of_its_type(entered, f, name):
+    """a narrower tensor would be read or written past its end"""
+    t = tensors(f)
+    right = t[name].dtype
+    for wrong in {F32, I32, I64, torch.float16, torch.bfloat16, torch.float64, torch.int16, torch.int8, torch.bool} - {right}:
+        t[name].dtype = wrong
+        with pytest.raises(ValueError, match="where the library takes"):
+            f(t)
+    assert not entered
+    for same in {F32: (U8,), I32: (torch.uint32, U8), I64: (torch.uint64, U8)}[right]:   # U8: raw memory
+        t[name].dtype = same
+        f(t)
+
+
+@pytest.mark.parametrize("f,name", [(kv_write, "cache"), (kv_read, "cache"), (kv_compact, "second"), (prep, "k"), (tree, "v"), (tree, "workspace")])
+def test_caches_and_workspaces_are_memory_of_any_type(entered, f, name):
+    for dtype in (torch.float16, torch.int16, F32, I64):
+        t = tensors(f)
+        t[name].dtype = dtype
+        f(t)
+    assert len(entered) == 4
