@@ -641,15 +641,20 @@ def _is_f16(t):
     return _ROWS[t.dtype]
 
 
+def _rows(t, n, cache):
+    """the rows' address; no rows (an empty tensor has no address) are as well anywhere"""
+    return t.data_ptr() or (cache.data_ptr() if n == 0 else None)
+
+
 def kv_write(type_, src, src_stride, cache, first, n, n_kv, head_dim, max_ctx, stream=None):
     """n rows [n_kv x head_dim] of float32 or float16, src_stride elements apart, to positions [first, first + n)"""
-    _call("rmi_kv_write", type_, _a(src), _is_f16(src), src_stride, _a(cache), first, n, n_kv, head_dim, max_ctx,
+    _call("rmi_kv_write", type_, _rows(src, n, cache), _is_f16(src), src_stride, _a(cache), first, n, n_kv, head_dim, max_ctx,
           _s(stream, cache, (src,)))
 
 
 def kv_read(type_, cache, out, out_stride, first, n, n_kv, head_dim, max_ctx, stream=None):
     """positions [first, first + n) of a cache back to float32 or float16 rows"""
-    _call("rmi_kv_read", type_, _a(cache), _a(out), _is_f16(out), out_stride, first, n, n_kv, head_dim, max_ctx,
+    _call("rmi_kv_read", type_, _a(cache), _rows(out, n, cache), _is_f16(out), out_stride, first, n, n_kv, head_dim, max_ctx,
           _s(stream, cache, (out,)))
 
 

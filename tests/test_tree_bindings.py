@@ -132,3 +132,18 @@ def test_caches_and_workspaces_are_memory_of_any_type(entered, f, name):
         t[name].dtype = dtype
         f(t)
     assert len(entered) == 4
+
+
+@pytest.mark.parametrize("call,name", [(rmi.kv_write, "src"), (rmi.kv_read, "out")], ids=["kv_write", "kv_read"])
+@pytest.mark.parametrize("dtype", [F32, torch.float16])
+def test_no_rows_of_an_empty_tensor(monkeypatch, call, name, dtype):
+    """torch's empty tensors have no address; through the library itself, which launches nothing for no rows"""
+    monkeypatch.setattr(rmi, "_gpu", (lambda: 0, lambda at: 55))
+    rows, cache = Tensor(dtype, numel=0), Tensor(U8)
+    args = (rows, 1024, cache) if name == "src" else (cache, rows, 1024)
+    for first in (0, 100):
+        call(rmi.KV_I8, *args, first, 0, 4, 256, 100)
+    with pytest.raises(ValueError, match="invalid"):
+        call(rmi.KV_I8, *args, 0, 1, 4, 256, 100)
+    with pytest.raises(ValueError, match="invalid"):
+        call(rmi.KV_I8, *args, 101, 0, 4, 256, 100)
