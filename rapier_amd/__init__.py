@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 import os
 import subprocess
 import sys
@@ -680,8 +681,9 @@ def attn_prep_axes(q3, q3_stride, qn, kn, ktype, kcache, vtype, vcache, pos, axi
                    n_rot, freq_base, factor, orig_ctx, sections, interleaved, eps, ntok, max_ctx, ext_factor=1.0,
                    attn_factor=1.0, beta_fast=32.0, beta_slow=1.0, stream=None):
     """per-head norm, rotation at axis_pos ([3][ntok]; None: the slots) and the cache write at slots pos[0] + t"""
-    rope, axes = _rope_args(tuple(sections), int(interleaved), freq_base, factor, orig_ctx, ext_factor, attn_factor,
-                            beta_fast, beta_slow)
+    # by value: a tensor's element would be kept by its identity, whatever it holds later
+    rope, axes = _rope_args(tuple(map(operator.index, sections)), bool(interleaved), *map(
+        float, (freq_base, factor, orig_ctx, ext_factor, attn_factor, beta_fast, beta_slow)))
     _call("rmi_attn_prep_axes", _a(q3), q3_stride, _a(qn), _a(kn), ktype, _a(kcache), vtype, _a(vcache), _a(pos),
           _a(axis_pos), _a(qout), n_head, n_kv, head_dim, n_rot, ctypes.byref(rope), ctypes.byref(axes), eps, ntok,
           max_ctx, _s(stream, kcache, (vcache,), (q3, qn, kn, qout), (pos, axis_pos)))

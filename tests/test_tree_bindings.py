@@ -147,3 +147,22 @@ def test_no_rows_of_an_empty_tensor(monkeypatch, call, name, dtype):
         call(rmi.KV_I8, *args, 0, 1, 4, 256, 100)
     with pytest.raises(ValueError, match="invalid"):
         call(rmi.KV_I8, *args, 101, 0, 4, 256, 100)
+
+
+def test_rotary_values_that_change_in_place(entered):
+    """elements of tensors as base, factor and sections: every call has what they hold at that call"""
+    base, factor, sections = torch.tensor(1e4), torch.tensor(2.0), torch.tensor([12, 10, 10])
+    views = [sections[i] for i in range(3)]
+    t = tensors(prep)
+    for new in ((1e4, 2.0, (12, 10, 10)), (1e6, 4.0, (10, 11, 11)), (5e5, 8.0, (32, 0, 0))):
+        base.fill_(new[0])
+        factor.fill_(new[1])
+        sections.copy_(torch.tensor(new[2]))
+        rmi.attn_prep_axes(t["q3"], 10240, t["qn"], t["kn"], 1, t["k"], 1, t["v"], t["pos"], t["axis_pos"], t["qout"], 16, 4, 256, 64, base,
+                           factor, 32768.0, views, False, 1e-6, 1, 100)
+        blocks = [a._obj for a in entered[-1] if hasattr(a, "_obj")]
+        assert (blocks[0].freq_base, blocks[0].factor) == new[:2]
+        assert tuple(blocks[1].section) == new[2]
+    with pytest.raises(TypeError):
+        rmi.attn_prep_axes(t["q3"], 10240, t["qn"], t["kn"], 1, t["k"], 1, t["v"], t["pos"], t["axis_pos"], t["qout"], 16, 4, 256, 64, 1e4,
+                           1.0, 0.0, (12.5, 9.5, 10.0), False, 1e-6, 1, 100)
