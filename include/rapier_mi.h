@@ -372,7 +372,8 @@ enum { RMI_KV_F16 = 0, RMI_KV_I8 = 1, RMI_KV_I4 = 2 };
 /* bytes of one cache; 0 on a bad type or shape */
 size_t rmi_kv_cache_bytes(int type, int max_ctx, int n_kv, int head_dim);
 /* n rows [n_kv x head_dim] of fp32 (src_f16 = 0) or fp16 (1), src_stride elements apart, to positions [first, first + n)
- * of the cache; n = 0 does nothing (its arguments are checked).  The source may not overlap the cache. */
+ * of the cache; n = 0 does nothing (its arguments are checked).  The source may not lie on the rows it goes to, nor
+ * (rmi_kv_read) the output on those it comes from. */
 int rmi_kv_write(int type, const void* src, int src_f16, int src_stride, void* cache, int first, int n, int n_kv,
                  int head_dim, int max_ctx, void* stream);
 /* positions [first, first + n) back to rows of fp32 or fp16 (both exact for I8 and I4), out_stride elements apart */

@@ -5,6 +5,7 @@
 //   prep_axes    per-head RMSNorm, rotary embedding with three position axes, and the K / V write of new tokens
 // No counterpart in the reference, whose cache is fp16 (store_kv2_kernel, qw:340-345) and whose draft is one token.
 #include "kv_cache.h"
+#include "overlap.h"
 #include "rope.h"
 
 #include <algorithm>
@@ -433,10 +434,14 @@ static_assert(kRowThreads == 64 * kPrepWaves);
 
 bool aligned_to(const void* p, size_t n) { return p && (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-// whether two caches of these sizes share bytes
-bool overlap(const void* p, size_t p_bytes, const void* q, size_t q_bytes) {
-    const auto a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
-    return a < b ? b - a < p_bytes : a - b < q_bytes;
+// whether rows outside share bytes with the cache's of positions [first, first + n)
+bool on_cache_rows(int type, const void* rows, int rows16, int stride, const void* cache, int first, int n, int n_kv, int head_dim, int max_ctx) {
+    const long long el = rows16 ? 2 : 4, per = kv_row_bytes(type, head_dim), sper = head_dim / kKvBlock;
+    const RowSet out{rows, n, stride * el, n_kv * head_dim * el};
+    const auto* c = static_cast<const uint8_t*>(cache);
+    if (type == kKvF16) return rows_overlap(out, block_of(c + first * n_kv * per, n * n_kv * per));
+    return rows_overlap(out, {c + first * per, n_kv, max_ctx * per, n * per}) ||
+           rows_overlap(out, {c + n_kv * max_ctx * per + first * sper, n_kv, max_ctx * sper, n * sper});
 }
 
 // calls f with the type as a constant
@@ -478,6 +483,8 @@ extern "C" int rmi_kv_write(int type, const void* src, int src_f16, int src_stri
     const int per = kWriteUnits * kRowThreads / (head_dim / 8);   // rows a workgroup
     const long long blocks = (static_cast<long long>(n) + per - 1) / per * n_kv;
     if (blocks > kMaxBlocks) return fail(RMI_ERR_SHAPE, "kv_write: too many rows for one call");
+    if (on_cache_rows(type, src, src_f16, src_stride, cache, first, n, n_kv, head_dim, max_ctx))
+        return fail(RMI_ERR_POINTER, "kv_write: the source lies on the rows it goes to");
     const bool vec = aligned16(src) && src_stride % (src_f16 ? 8 : 4) == 0;   // 16-byte loads, else one by one
     auto* out = static_cast<uint8_t*>(cache);
     return with_type(type, [&](auto t) {
@@ -499,6 +506,8 @@ extern "C" int rmi_kv_read(int type, const void* cache, void* out, int out_f16, 
     const int per = kRowThreads / (head_dim / 8);
     const long long blocks = (static_cast<long long>(n) + per - 1) / per * n_kv;
     if (blocks > kMaxBlocks) return fail(RMI_ERR_SHAPE, "kv_read: too many rows for one call");
+    if (on_cache_rows(type, out, out_f16, out_stride, cache, first, n, n_kv, head_dim, max_ctx))
+        return fail(RMI_ERR_POINTER, "kv_read: the output lies on the rows it comes from");
     const bool vec = aligned16(out) && out_stride % (out_f16 ? 8 : 4) == 0;
     const auto* in = static_cast<const uint8_t*>(cache);
     return with_type(type, [&](auto t) {
@@ -526,7 +535,7 @@ extern "C" int rmi_kv_compact(int type, void* const* caches, int n_caches, const
         if (!aligned16(caches[i])) return fail(RMI_ERR_POINTER, "kv_compact: null or misaligned cache");
         ptrs.p[i] = static_cast<uint8_t*>(caches[i]);
         for (int j = 0; j < i; ++j)   // two workgroups would move the same rows
-            if (overlap(caches[i], bytes, caches[j], bytes))
+            if (rows_overlap(block_of(caches[i], bytes), block_of(caches[j], bytes)))
                 return fail(RMI_ERR_POINTER, "kv_compact: caches overlap");
     }
     return with_type(type, [&](auto t) {
@@ -556,7 +565,8 @@ extern "C" int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* q
     if (!aligned4(q3) || !aligned4(qn) || !aligned4(kn) || !aligned16(kcache) || !aligned16(vcache) || !aligned4(pos) ||
         (axis_pos && !aligned4(axis_pos)) || !aligned4(qout))
         return fail(RMI_ERR_POINTER, what);
-    if (overlap(kcache, rmi_kv_cache_bytes(ktype, max_ctx, n_kv, head_dim), vcache, rmi_kv_cache_bytes(vtype, max_ctx, n_kv, head_dim)))
+    if (rows_overlap(block_of(kcache, rmi_kv_cache_bytes(ktype, max_ctx, n_kv, head_dim)),
+                     block_of(vcache, rmi_kv_cache_bytes(vtype, max_ctx, n_kv, head_dim))))
         return fail(RMI_ERR_POINTER, "attn_prep_axes: the caches overlap");
     PrepArgs a{};
     if (!yarn_setup(*rope, n_rot, &a.yarn)) return fail(RMI_ERR_SHAPE, "attn_prep_axes: invalid YaRN parameters");

@@ -1,0 +1,77 @@
+"""Calls whose outputs lie on their inputs are refused before any device work (CPU); the test of strided rows itself against
+all bytes, in a small program."""
+import ctypes
+import os
+import shutil
+import subprocess
+import textwrap
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+PROGRAM = textwrap.dedent(r"""
+    #include "overlap.h"
+    #include <cstdio>
+    #include <set>
+    #include <random>
+    int main() {
+        std::mt19937 rng(1);
+        auto draw = [&](int lo, int hi) { return lo + static_cast<int>(rng() % (hi - lo + 1)); };
+        int shared = 0;
+        for (int i = 0; i < 200000; ++i) {
+            rmi::RowSet s[2];
+            std::set<long long> bytes[2];
+            for (int k = 0; k < 2; ++k) {
+                long long p = 1000 + draw(0, 60);
+                s[k] = {reinterpret_cast<const void*>(p), draw(1, 7), draw(-25, 25), draw(1, 12)};
+                for (long long r = 0; r < s[k].n; ++r)
+                    for (long long b = 0; b < s[k].bytes; ++b) bytes[k].insert(p + r * s[k].stride + b);
+            }
+            bool want = false;
+            for (long long b : bytes[0]) want = want || bytes[1].count(b);
+            shared += want;
+            if (rmi::rows_overlap(s[0], s[1]) != want) {
+                for (auto& x : s) std::printf("%p %lld %lld %lld\n", x.p, x.n, x.stride, x.bytes);
+                return 1;
+            }
+        }
+        std::printf("%d\n", shared);
+        return shared > 50000 && shared < 190000 ? 0 : 2;
+    }
+""")
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not available")
+def test_strided_rows_against_all_bytes(tmp_path):
+    src, exe = tmp_path / "overlap.cpp", tmp_path / "overlap"
+    src.write_text(PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", os.path.join(ROOT, "rapier_amd", "csrc"), str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.fixture(scope="module")
+def rmi():
+    import rapier_amd
+    rapier_amd.lib()
+    return rapier_amd
+
+
+BASE = 1 << 30
+
+
+def at(offset):
+    return ctypes.c_void_p(BASE + offset)
+
+
+# a cache of 100 positions x 4 heads x 256 at BASE, positions 10 .. 14; rows outside: five of 4 KB (fp32) or 2 KB
+@pytest.mark.parametrize("name", ["rmi_kv_write", "rmi_kv_read"])
+@pytest.mark.parametrize("type_,rows,f16,stride", [
+    (0, 10 * 2048, 1, 1024), (0, 15 * 2048 - 4, 0, 1024), (0, 10 * 2048 - 5 * 2048 + 2, 1, 1024), (0, 10 * 2048 - 4096 - 8192 * 2 + 4, 0, 2048),
+    (1, 10 * 256, 0, 1024), (1, (2 * 100 + 14) * 256 + 252, 0, 1024), (1, 4 * 100 * 256 + (3 * 100 + 14) * 8 + 4, 0, 1024),
+    (1, 4 * 100 * 256 + 10 * 8 - 5 * 2048 + 2, 1, 1024), (2, (100 + 10) * 128, 1, 1024), (2, 4 * 100 * 128 + (100 + 12) * 8, 1, 1024)])
+def test_rows_on_their_own_cache_rows(rmi, name, type_, rows, f16, stride):
+    a = (at(rows), f16, stride, at(0)) if name == "rmi_kv_write" else (at(0), at(rows), f16, stride)
+    with pytest.raises(ValueError, match="lies on"):
+        rmi._call(name, type_, *a, 10, 5, 4, 256, 100, None)
