@@ -434,7 +434,7 @@ int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache, int vtype
  *   x = logits[v] + bias of v (bias_ids / bias_vals, n_bias entries; of entries with one id the last counts)
  *   m > 0:  x = x > 0 ? x / repetition : x * repetition;   x -= m * frequency + presence
  *   bit v % 32 of allow[c * allow_stride + v / 32] clear:  x = -infinity     (null allow: every token)
- * out may be logits (with the same stride).  repetition > 0. */
+ * out may be logits (with the same stride); else the two share no element.  repetition > 0. */
 typedef struct rmi_penalties {
     float repetition, presence, frequency;
     int window;

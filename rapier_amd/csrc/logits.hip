@@ -8,6 +8,7 @@
 // column, kept as a short list of those in the slice and added to the counts for that column alone.  Every workgroup reads
 // the whole history (four ids a lane and load, from the L2): one column of 248320 logits takes 4.8 us behind 4001 tokens and
 // 8.1 behind 20001, bound by the chain length - ids - counts - logits at the first and by those reads at the second.
+#include "overlap.h"
 #include "rmi_common.h"
 
 #include <cmath>
@@ -177,6 +178,8 @@ extern "C" int rmi_logits_process(const float* logits, int n, int ncols, int col
         (ndraft > 0 && (!aligned4(draft) || !masks || (reinterpret_cast<uintptr_t>(masks) & 7u))) ||
         (n_bias > 0 && (!aligned4(bias_ids) || !aligned4(bias_vals))) || (allow && !aligned4(allow)))
         return fail(RMI_ERR_POINTER, "logits_process: null or misaligned pointer");
+    if (out != logits && rows_overlap({logits, ncols, 4LL * col_stride, 4LL * n}, {out, ncols, 4LL * out_stride, 4LL * n}))
+        return fail(RMI_ERR_POINTER, "logits_process: the output lies on other logits' places");
     LogitsArgs a{};
     a.logits = logits;
     a.out = out;

@@ -75,3 +75,13 @@ def test_rows_on_their_own_cache_rows(rmi, name, type_, rows, f16, stride):
     a = (at(rows), f16, stride, at(0)) if name == "rmi_kv_write" else (at(0), at(rows), f16, stride)
     with pytest.raises(ValueError, match="lies on"):
         rmi._call(name, type_, *a, 10, 5, 4, 256, 100, None)
+
+
+@pytest.mark.parametrize("out,ncols,col_stride,out_stride", [
+    (4, 1, 1000, 1000), (-4, 1, 1000, 1000), (3996, 1, 1000, 1000), (4000, 2, 1000, 1000), (-4 * 1004, 3, 1004, 1004), (4, 64, 1000, 1000),
+    (3996, 2, 2000, 2000), (4 * 2000, 3, 2000, 1000), (4 * 63 * 2000 + 4 * 999, 64, 2000, 2000), (-4 * 63 * 3001 + 400, 64, 2000, 3001)])
+def test_logits_on_other_logits(rmi, out, ncols, col_stride, out_stride):
+    p = rmi.Penalties(1.0, 0.0, 0.0, 0)
+    with pytest.raises(ValueError, match="lies on"):
+        rmi._call("rmi_logits_process", at(0), 1000, ncols, col_stride, at(out), out_stride, None, None, 0, None, None, 0, ctypes.byref(p), None,
+                  None, 0, None, 0, None)
