@@ -412,6 +412,7 @@ int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* qn, const fl
  * (nullable; rows y_stride elements apart) and Q8_1 (nullable; q8_stride bytes).  Rows a token does not see have no part
  * in its result, whatever they hold; a NaN or an infinity in q or in a row that it sees makes the result NaN or infinite.
  * If a slot lies outside [0, max_ctx) nothing is written.
+ * y may be q (rows n_head * head_dim apart); else outputs and workspace share no byte with each other or with what is read.
  * The context is split into chunks of 128 * nsub positions; rmi_gqa_tree_nsub gives the split for a context of `ctx`
  * positions, to be settled once (results differ in the last bits between splits).  With RMI_TREE_SHORT added, more than 16
  * query rows per KV head are worked on 16 at a time, which pays over short chunks.  workspace holds

@@ -3,7 +3,8 @@ import numpy as np
 import pytest
 
 from tests import kv_ref as ref
-from tests.gpu_util import dev, host
+from tests.gpu_util import dev, empty, host
+from tests.test_gpu_tree_attn import Call, as_masks
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +43,37 @@ def test_logits_between_the_columns(rmi):
     got = host(d).reshape(ncols, 2 * n)
     want = np.where(np.bincount(hist, minlength=n) > 0, x - np.float32(0.5), x)
     assert np.array_equal(got[:, :n], x) and np.array_equal(got[:, n:], want)
+
+
+@pytest.mark.parametrize("types", [(ref.F16, ref.F16), (ref.I8, ref.I4)], ids=["f16", "i8_i4"])
+@pytest.mark.parametrize("nh,nkv,hd,ntok,base,nsub", [(16, 4, 256, 1, 300, 1), (4, 2, 128, 3, 20, 1), (4, 2, 256, 6, 1300, 1), (4, 2, 256, 6, 20, 1),
+                                                      (8, 2, 256, 6, 20, 7), (8, 2, 128, 6, 1000, 6), (4, 2, 256, 20, 20, 1), (4, 2, 128, 30, 90, 1),
+                                                      (4, 2, 256, 40, 20, 1), (4, 1, 256, 33, 400, 1)])
+def test_tree_results_in_the_queries_place(rmi, types, nh, nkv, hd, ntok, base, nsub):
+    """y is q: every form, one chunk and several, rows that do not fill a group"""
+    masks, _ = ref.tree_masks(np.random.default_rng(ntok), ntok)
+    for m in (masks, None):
+        c = Call(rmi, types, nh, nkv, hd, ntok, base, m, nsub=nsub)
+        want = c.run()
+        q = dev(c.q)
+        ws = empty(rmi.gqa_tree_workspace_bytes(c.max_ctx, nh, nkv, hd, ntok, nsub), "uint8")
+        rmi.gqa_tree_decode(q, types[0], dev(c.raw[0]), types[1], dev(c.raw[1]), dev(np.array([base], np.int32)), as_masks(m), dev(c.q3), c.width, q,
+                            nh * hd, None, 0, ws, nh, nkv, hd, ntok, c.max_ctx, nsub, c.scale)
+        assert np.array_equal(host(q).reshape(want.shape).view(np.uint32), want.view(np.uint32))
+
+
+def test_tree_results_beside_the_gates(rmi):
+    """y in the columns behind a buffer's gates"""
+    nh, nkv, hd, ntok, base = 4, 2, 256, 9, 130
+    c = Call(rmi, (ref.I8, ref.I8), nh, nkv, hd, ntok, base, None, nsub=1)
+    want = c.run()
+    width = 2 * nh * hd + nh * hd
+    buf = np.zeros((ntok, width), np.float32)
+    buf[:, :2 * nh * hd] = c.q3[:, :2 * nh * hd]
+    d = dev(buf.reshape(-1))
+    ws = empty(rmi.gqa_tree_workspace_bytes(c.max_ctx, nh, nkv, hd, ntok, 1), "uint8")
+    rmi.gqa_tree_decode(dev(c.q), ref.I8, dev(c.raw[0]), ref.I8, dev(c.raw[1]), dev(np.array([base], np.int32)), None, d, width, d[2 * nh * hd:], width,
+                        None, 0, ws, nh, nkv, hd, ntok, c.max_ctx, 1, c.scale)
+    got = host(d).reshape(ntok, width)
+    assert np.array_equal(got[:, 2 * nh * hd:].reshape(want.shape).view(np.uint32), want.view(np.uint32))
+    assert np.array_equal(got[:, :2 * nh * hd], buf[:, :2 * nh * hd])

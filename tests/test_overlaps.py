@@ -85,3 +85,20 @@ def test_logits_on_other_logits(rmi, out, ncols, col_stride, out_stride):
     with pytest.raises(ValueError, match="lies on"):
         rmi._call("rmi_logits_process", at(0), 1000, ncols, col_stride, at(out), out_stride, None, None, 0, None, None, 0, ctypes.byref(p), None,
                   None, 0, None, 0, None)
+
+
+# 16 heads on 4 KV heads of 256, 8 tokens: q 128 KB, y the same, q8 36 KB, caches of 1000 positions, 1 MB each as I8
+TREE = {"q": 0, "k": 1 << 24, "v": 1 << 25, "gate": 1 << 26, "y": 1 << 20, "q8": 1 << 21, "ws": 1 << 27}
+
+
+@pytest.mark.parametrize("moved,to,extra", [
+    ("y", 16, {}), ("y", (1 << 17) - 4, {}), ("y", 0, {"ys": 4100}), ("y", -4 * 4096, {"ys": 4100}), ("y", (1 << 24) + 64, {}), ("y", (1 << 25) - 64, {}),
+    ("y", 1 << 26, {}), ("y", (1 << 26) + 4 * 256, {"ys": 10240}), ("y", (1 << 26) + 4 * 8188, {"ys": 10240}), ("y", (1 << 27) + 400000, {}),
+    ("y", (1 << 21) + 8 * 4608 - 4, {}), ("q8", 0, {}), ("q8", (1 << 24) + 1000000, {}), ("q8", (1 << 26) + 4 * 10240 * 7 + 4 * 256, {}),
+    ("ws", 1 << 16, {}), ("ws", (1 << 24) + 4096, {}), ("ws", (1 << 25) - 4096, {}), ("ws", 1 << 20, {}), ("ws", (1 << 21) - 16, {}),
+    ("ws", (1 << 26) + 4096, {})])
+def test_tree_outputs_on_inputs(rmi, moved, to, extra):
+    p = {k: at(v) for k, v in {**TREE, moved: to}.items()}
+    with pytest.raises(ValueError, match="lies on"):
+        rmi._call("rmi_gqa_tree_decode", p["q"], 1, p["k"], 1, p["v"], at(1 << 28), None, p["gate"], 10240, p["y"], extra.get("ys", 4096), p["q8"], 4608,
+                  p["ws"], 16, 4, 256, 8, 1000, 1, 0.0625, None)
