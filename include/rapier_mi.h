@@ -398,7 +398,8 @@ typedef struct rmi_rope_axes {
  * pos[0] + t (nothing is written for a slot outside [0, max_ctx)) and its rotation is at axis_pos[a * ntok + t] of axis a
  * (null: the slot, on every axis).  With a null axis_pos q and V are bitwise rmi_attn_prep_rope's; K rows are normed and
  * rotated in fp64 and rounded to fp32 once (what the cache holds then does not hang on the order of a sum), so an F16 K may
- * differ from rmi_attn_prep_rope's by one step where its fp32 lies at a border.  ntok >= 1; the caches do not overlap. */
+ * differ from rmi_attn_prep_rope's by one step where its fp32 lies at a border.  ntok >= 1; q3's rows, qout and the
+ * caches share no byte. */
 int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* qn, const float* kn, int ktype, void* kcache,
                        int vtype, void* vcache, const int* pos, const int* axis_pos, float* qout, int n_head, int n_kv,
                        int head_dim, int n_rot, const rmi_rope_params* rope, const rmi_rope_axes* axes, float eps,

@@ -565,9 +565,15 @@ extern "C" int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* q
     if (!aligned4(q3) || !aligned4(qn) || !aligned4(kn) || !aligned16(kcache) || !aligned16(vcache) || !aligned4(pos) ||
         (axis_pos && !aligned4(axis_pos)) || !aligned4(qout))
         return fail(RMI_ERR_POINTER, what);
-    if (rows_overlap(block_of(kcache, rmi_kv_cache_bytes(ktype, max_ctx, n_kv, head_dim)),
-                     block_of(vcache, rmi_kv_cache_bytes(vtype, max_ctx, n_kv, head_dim))))
-        return fail(RMI_ERR_POINTER, "attn_prep_axes: the caches overlap");
+    const RowSet read{q3, ntok, 4LL * q3_stride, 4LL * (2 * n_head + 2 * n_kv) * head_dim};
+    const RowSet written[] = {block_of(kcache, rmi_kv_cache_bytes(ktype, max_ctx, n_kv, head_dim)),
+                              block_of(vcache, rmi_kv_cache_bytes(vtype, max_ctx, n_kv, head_dim)),
+                              block_of(qout, static_cast<size_t>(ntok) * n_head * head_dim * 4)};
+    if (rows_overlap(written[0], written[1])) return fail(RMI_ERR_POINTER, "attn_prep_axes: the caches overlap");
+    if (rows_overlap(written[2], written[0]) || rows_overlap(written[2], written[1]))
+        return fail(RMI_ERR_POINTER, "attn_prep_axes: qout lies on a cache");
+    for (const RowSet& w : written)
+        if (rows_overlap(read, w)) return fail(RMI_ERR_POINTER, "attn_prep_axes: qout or a cache lies on the rows of q3");
     PrepArgs a{};
     if (!yarn_setup(*rope, n_rot, &a.yarn)) return fail(RMI_ERR_SHAPE, "attn_prep_axes: invalid YaRN parameters");
     a.q3 = q3;

@@ -102,3 +102,14 @@ def test_tree_outputs_on_inputs(rmi, moved, to, extra):
     with pytest.raises(ValueError, match="lies on"):
         rmi._call("rmi_gqa_tree_decode", p["q"], 1, p["k"], 1, p["v"], at(1 << 28), None, p["gate"], 10240, p["y"], extra.get("ys", 4096), p["q8"], 4608,
                   p["ws"], 16, 4, 256, 8, 1000, 1, 0.0625, None)
+
+
+@pytest.mark.parametrize("qout,k,v", [(0, 1 << 24, 1 << 25), (4 * 10240 * 5 - 4, 1 << 24, 1 << 25), (-4 * 4096 * 5 + 4, 1 << 24, 1 << 25),
+                                      (4 * 256, 1 << 24, 1 << 25), ((1 << 24) + 64, 1 << 24, 1 << 25), ((1 << 25) - 64, 1 << 24, 1 << 25),
+                                      (1 << 26, 4 * 10240 * 4, 1 << 25), (1 << 26, 1 << 24, -1024), (1 << 26, 1 << 24, (1 << 24) + 4096)])
+def test_prep_outputs_on_inputs(rmi, qout, k, v):
+    """five tokens of 16 + 4 heads of 256, I8 caches of 100 positions"""
+    p, a = rmi.RopeParams(1e6, 1.0, 0.0, 1.0, 1.0, 32.0, 1.0), rmi.RopeAxes((ctypes.c_int * 3)(32, 0, 0), 0)
+    with pytest.raises(ValueError, match="lies on|overlap"):
+        rmi._call("rmi_attn_prep_axes", at(0), 10240, at(1 << 28), at(1 << 28), 1, at(k), 1, at(v), at(1 << 28), None, at(qout), 16, 4, 256, 64,
+                  ctypes.byref(p), ctypes.byref(a), 1e-6, 5, 100, None)
