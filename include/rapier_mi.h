@@ -415,10 +415,11 @@ int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* qn, const fl
  * If a slot lies outside [0, max_ctx) nothing is written.
  * y may be q (rows n_head * head_dim apart); else outputs and workspace share no byte with each other or with what is read.
  * The context is split into chunks of 128 * nsub positions; rmi_gqa_tree_nsub gives the split for a context of `ctx`
- * positions, to be settled once (results differ in the last bits between splits).  With RMI_TREE_SHORT added, more than 16
- * query rows per KV head are worked on 16 at a time, which pays over short chunks.  workspace holds
- * rmi_gqa_tree_workspace_bytes(...) bytes, 16-byte aligned, and needs no initial state; calls that may overlap need one
- * each.  Same inputs, same bits; I8 and I4 caches give the bits of an F16 cache that holds their values (but for 17 to 32
+ * positions, to be settled once (results differ in the last bits between splits).  The whole cache may have 2048 chunks: nsub
+ * at least max_ctx / 262144, rounded up, which over a cache of more than 262144 positions can be more than a short text's
+ * split.  With RMI_TREE_SHORT added, more than 16 query rows per KV head are worked on 16 at a time, which pays over short
+ * chunks.  workspace holds rmi_gqa_tree_workspace_bytes(...) bytes, 16-byte aligned, and needs no initial state; calls that
+ * may overlap need one each.  Same inputs, same bits; I8 and I4 caches give the bits of an F16 cache that holds their values (but for 17 to 32
  * query rows at nsub >= 6 without RMI_TREE_SHORT); and while ntok * n_head / n_kv <= 8, each token of a chain has the
  * bits of a call of its own at the same nsub. */
 enum { RMI_TREE_SHORT = 1 << 24 };

@@ -34,7 +34,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kStep = 32;          // positions of a step
 constexpr int kUnit = kWaves * kStep;
-constexpr int kMaxChunks = 2048;
+constexpr int kMaxChunks = 2048;   // a chunk's weight in the merge's LDS; named in the messages
 constexpr int kMaxTree = 64, kMaxChain = 1024;
 constexpr float kPScale = 8.0f;    // p goes as 2^8 p
 constexpr float kLazy = 7.0f;      // a maximum moves once a score passes it by more than 2^7 (2^15 p is an fp16 number)
@@ -1209,8 +1209,12 @@ extern "C" int rmi_gqa_tree_nsub(int ctx, int n_head, int n_kv, int head_dim, in
 extern "C" size_t rmi_gqa_tree_workspace_bytes(int max_ctx, int n_head, int n_kv, int head_dim, int ntok, int nsub) {
     const int split = nsub;
     nsub = split_nsub(split);
-    if (!tree_shape_ok(max_ctx, n_head, n_kv, head_dim, ntok) || nsub < 1 || tree_chunks(max_ctx, nsub) > kMaxChunks) {
+    if (!tree_shape_ok(max_ctx, n_head, n_kv, head_dim, ntok) || nsub < 1) {
         set_error("gqa_tree_workspace_bytes: invalid shape");
+        return 0;
+    }
+    if (tree_chunks(max_ctx, nsub) > kMaxChunks) {
+        set_error("gqa_tree_workspace_bytes: more than 2048 chunks of 128 nsub positions in max_ctx: a larger nsub");
         return 0;
     }
     const Form f = tree_form(n_head, n_kv, ntok, split, false);   // 17 to 32 rows take the same space in both forms
@@ -1225,9 +1229,10 @@ extern "C" int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache
         return fail(RMI_ERR_UNSUPPORTED, "gqa_tree_decode: cache types F16 / F16, I8 / I8, I4 / I4 or I8 / I4");
     const int split = nsub;
     nsub = split_nsub(split);
-    if (!tree_shape_ok(max_ctx, n_head, n_kv, head_dim, ntok) || ntok > max_ctx || (masks && ntok > kMaxTree) || nsub < 1 ||
-        tree_chunks(max_ctx, nsub) > kMaxChunks)
+    if (!tree_shape_ok(max_ctx, n_head, n_kv, head_dim, ntok) || ntok > max_ctx || (masks && ntok > kMaxTree) || nsub < 1)
         return fail(RMI_ERR_SHAPE, "gqa_tree_decode: invalid arguments");
+    if (tree_chunks(max_ctx, nsub) > kMaxChunks)
+        return fail(RMI_ERR_SHAPE, "gqa_tree_decode: more than 2048 chunks of 128 nsub positions in max_ctx: a larger nsub");
     if (!aligned16(q) || !aligned16(kcache) || !aligned16(vcache) || !aligned4(pos) || !aligned16(workspace) ||
         (masks && (reinterpret_cast<uintptr_t>(masks) & 7u)) || (gate_src && !aligned4(gate_src)) || (!y && !q8) ||
         (y && !aligned4(y)) || (q8 && (!aligned4(q8) || q8_stride % 4)))
