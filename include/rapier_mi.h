@@ -431,9 +431,9 @@ int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache, int vtype
                         int max_ctx, int nsub, float scale, void* stream);
 
 /* What a sampler wants done to ncols (1..64) columns of n logits before rmi_argmax / rmi_topk.  Column c's text is
- * history[0 .. min(history_len[0], max_history)) (device words; null: empty) and then, with a draft of ndraft <= 64
- * tokens, those draft[j] whose bit j of masks[c] is set, in ascending order (the path to a tree's node); ids outside
- * [0, n) count for nothing.  m = how often v stands in the text's last `window` tokens (window <= 0: in all of it).
+ * history[0 .. min(history_len[0], max_history)) (device words; max_history 0: none, both may be null) and then, with a
+ * draft of ndraft <= 64 tokens, those draft[j] whose bit j of masks[c] is set, in ascending order (the path to a tree's
+ * node); ids outside [0, n) take their places and count for nothing.  m = how often v stands in the text's last `window` tokens (window <= 0: in all of it).
  *   x = logits[v] + bias of v (bias_ids / bias_vals, n_bias entries; of entries with one id the last counts)
  *   m > 0:  x = x > 0 ? x / repetition : x * repetition;   x -= m * frequency + presence
  *   bit v % 32 of allow[c * allow_stride + v / 32] clear:  x = -infinity     (null allow: every token)
