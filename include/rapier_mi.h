@@ -399,7 +399,7 @@ typedef struct rmi_rope_axes {
  * (null: the slot, on every axis).  With a null axis_pos q and V are bitwise rmi_attn_prep_rope's; K rows are normed and
  * rotated in fp64 and rounded to fp32 once (what the cache holds then does not hang on the order of a sum), so an F16 K may
  * differ from rmi_attn_prep_rope's by one step where its fp32 lies at a border.  ntok >= 1; q3's rows, qout and the
- * caches share no byte. */
+ * caches share no byte.  Every pair of types is written; rmi_gqa_tree_decode reads those it names, rmi_kv_read all. */
 int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* qn, const float* kn, int ktype, void* kcache,
                        int vtype, void* vcache, const int* pos, const int* axis_pos, float* qout, int n_head, int n_kv,
                        int head_dim, int n_rot, const rmi_rope_params* rope, const rmi_rope_axes* axes, float eps,
