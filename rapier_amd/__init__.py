@@ -8,6 +8,7 @@ here computes on the CPU.  A missing library is an ``ImportError``-style failure
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import operator
@@ -577,35 +578,17 @@ def _a(t):
     return None if t is None else t.data_ptr()
 
 
-_gpu = None     # torch's current device and raw stream, without the checks (0.5 us each) around them
-_kinds = None   # what float, int and mask arguments may be
+_gpu = None   # torch's current device and raw stream, without the checks (0.5 us each) around them
 
 
-_NAMES = ("float32", "int32", "int64")
-
-
-def _argument_kinds():
-    global _kinds
-    torch = sys.modules["torch"]   # uint8: raw memory
-    _kinds = ({torch.float32, torch.uint8}, {torch.int32, torch.uint32, torch.uint8}, {torch.int64, torch.uint64, torch.uint8})
-    return _kinds
-
-
-def _s(stream, at, raw=(), f32=(), i32=(), i64=()):
-    """the stream's handle, for a call on the tensor `at` and these (None: an argument left out), which are on the current GPU,
-    whose kernels and streams these are, and of the element types that the library takes"""
+def _s(stream, at, *tensors):
+    """the stream's handle, for a call on the tensor `at` and these (None: an argument left out): all on the current GPU, whose
+    kernels and streams these are"""
     global _gpu
     at = at.get_device()   # -1: host memory
-    for t in raw:
+    for t in tensors:
         if t is not None and t.get_device() != at:
             raise ValueError("a tensor that is not on the current GPU")
-    for kind, tensors in zip(_kinds or _argument_kinds(), (f32, i32, i64)):
-        for t in tensors:
-            if t is not None:
-                if t.get_device() != at:
-                    raise ValueError("a tensor that is not on the current GPU")
-                if t.dtype not in kind:
-                    raise ValueError(f"a tensor of {t.dtype} where the library takes {_NAMES[_kinds.index(kind)]}")
     if at < 0:
         raise ValueError("a tensor that is not on the current GPU")
     if _gpu is None:
@@ -622,6 +605,46 @@ def _s(stream, at, raw=(), f32=(), i32=(), i64=()):
     return stream.cuda_stream
 
 
+# element types that an argument may have (filled when torch is known to be there); uint8: raw memory
+_F32, _I32, _I64 = {}, {}, {}
+
+
+def _another_type(kind, t):
+    """an argument whose type is not in `kind`: the first one of all, or an error"""
+    if not kind:
+        torch = sys.modules["torch"]
+        for k, names in ((_F32, ("float32", "uint8")), (_I32, ("int32", "uint32", "uint8")), (_I64, ("int64", "uint64", "uint8"))):
+            k.update((getattr(torch, name), names[0]) for name in names)
+    if t.dtype not in kind:
+        raise ValueError(f"a tensor of {t.dtype} where the library takes {next(iter(kind.values()))}")
+
+
+# addresses of such arguments (None: left out)
+
+def _f32(t):
+    if t is None:
+        return None
+    if t.dtype not in _F32:
+        _another_type(_F32, t)
+    return t.data_ptr()
+
+
+def _i32(t):
+    if t is None:
+        return None
+    if t.dtype not in _I32:
+        _another_type(_I32, t)
+    return t.data_ptr()
+
+
+def _i64(t):
+    if t is None:
+        return None
+    if t.dtype not in _I64:
+        _another_type(_I64, t)
+    return t.data_ptr()
+
+
 def kv_cache_bytes(type_, max_ctx, n_kv, head_dim) -> int:
     n = lib().rmi_kv_cache_bytes(type_, max_ctx, n_kv, head_dim)
     if n == 0:
@@ -634,12 +657,14 @@ _ROWS = {}   # dtypes of rows -> whether they are 16-bit
 
 def _is_f16(t):
     """1 for float16 rows (or int16 / uint16 that hold their bits), 0 for float32"""
-    if not _ROWS:
+    f16 = _ROWS.get(t.dtype)
+    if f16 is None:
         torch = sys.modules["torch"]
         _ROWS.update({torch.float32: 0, torch.float16: 1, torch.int16: 1, torch.uint16: 1})
-    if t.dtype not in _ROWS:
-        raise ValueError(f"rows of float32 or float16, not {t.dtype}")
-    return _ROWS[t.dtype]
+        f16 = _ROWS.get(t.dtype)
+        if f16 is None:
+            raise ValueError(f"rows of float32 or float16, not {t.dtype}")
+    return f16
 
 
 def _rows(t, n, cache):
@@ -650,20 +675,20 @@ def _rows(t, n, cache):
 def kv_write(type_, src, src_stride, cache, first, n, n_kv, head_dim, max_ctx, stream=None):
     """n rows [n_kv x head_dim] of float32 or float16, src_stride elements apart, to positions [first, first + n)"""
     _call("rmi_kv_write", type_, _rows(src, n, cache), _is_f16(src), src_stride, _a(cache), first, n, n_kv, head_dim, max_ctx,
-          _s(stream, cache, (src,)))
+          _s(stream, cache, src))
 
 
 def kv_read(type_, cache, out, out_stride, first, n, n_kv, head_dim, max_ctx, stream=None):
     """positions [first, first + n) of a cache back to float32 or float16 rows"""
     _call("rmi_kv_read", type_, _a(cache), _rows(out, n, cache), _is_f16(out), out_stride, first, n, n_kv, head_dim, max_ctx,
-          _s(stream, cache, (out,)))
+          _s(stream, cache, out))
 
 
 def kv_compact(type_, caches, pos, path, count, max_path, n_kv, head_dim, max_ctx, stream=None):
     """rows pos[0] + path[i] -> pos[0] + i, i < min(count[0], max_path), in each of the caches (a list of tensors)"""
-    ptrs = (ctypes.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches])
-    _call("rmi_kv_compact", type_, ptrs, len(caches), _a(pos), _a(path), _a(count), max_path, n_kv, head_dim, max_ctx,
-          _s(stream, pos, caches, (), (pos, path, count)))
+    ptrs = array.array("Q", [c.data_ptr() for c in caches] or [0])
+    _call("rmi_kv_compact", type_, ptrs.buffer_info()[0], len(caches), _i32(pos), _i32(path), _i32(count), max_path, n_kv,
+          head_dim, max_ctx, _s(stream, pos, path, count, *caches))
 
 
 class RopeAxes(ctypes.Structure):
@@ -671,22 +696,34 @@ class RopeAxes(ctypes.Structure):
     _fields_ = [("section", ctypes.c_int * 3), ("interleaved", ctypes.c_int)]
 
 
+class _NotAValue(Exception):
+    """an argument that is kept by its identity, whatever it holds later (a tensor's element)"""
+
+
+def _by_value(values):
+    if not all(isinstance(v, (int, float)) for v in values):
+        raise _NotAValue   # and nothing is kept
+
+
 @functools.lru_cache(maxsize=64)
 def _rope_args(sections, interleaved, *rope):
     """the argument blocks of these values, which the library only reads (building them costs as much as the call)"""
-    return RopeParams(*rope), RopeAxes((ctypes.c_int * 3)(*sections), interleaved)
+    _by_value(sections + rope)
+    return ctypes.byref(RopeParams(*rope)), ctypes.byref(RopeAxes((ctypes.c_int * 3)(*sections), interleaved))
 
 
 def attn_prep_axes(q3, q3_stride, qn, kn, ktype, kcache, vtype, vcache, pos, axis_pos, qout, n_head, n_kv, head_dim,
                    n_rot, freq_base, factor, orig_ctx, sections, interleaved, eps, ntok, max_ctx, ext_factor=1.0,
                    attn_factor=1.0, beta_fast=32.0, beta_slow=1.0, stream=None):
     """per-head norm, rotation at axis_pos ([3][ntok]; None: the slots) and the cache write at slots pos[0] + t"""
-    # by value: a tensor's element would be kept by its identity, whatever it holds later
-    rope, axes = _rope_args(tuple(map(operator.index, sections)), bool(interleaved), *map(
-        float, (freq_base, factor, orig_ctx, ext_factor, attn_factor, beta_fast, beta_slow)))
-    _call("rmi_attn_prep_axes", _a(q3), q3_stride, _a(qn), _a(kn), ktype, _a(kcache), vtype, _a(vcache), _a(pos),
-          _a(axis_pos), _a(qout), n_head, n_kv, head_dim, n_rot, ctypes.byref(rope), ctypes.byref(axes), eps, ntok,
-          max_ctx, _s(stream, kcache, (vcache,), (q3, qn, kn, qout), (pos, axis_pos)))
+    values = freq_base, factor, orig_ctx, ext_factor, attn_factor, beta_fast, beta_slow
+    try:
+        rope, axes = _rope_args(tuple(sections), bool(interleaved), *values)
+    except _NotAValue:
+        rope, axes = _rope_args(tuple(map(operator.index, sections)), bool(interleaved), *map(float, values))
+    _call("rmi_attn_prep_axes", _f32(q3), q3_stride, _f32(qn), _f32(kn), ktype, _a(kcache), vtype, _a(vcache),
+          _i32(pos), _i32(axis_pos), _f32(qout), n_head, n_kv, head_dim, n_rot, rope, axes, eps, ntok, max_ctx,
+          _s(stream, kcache, vcache, q3, qn, kn, pos, axis_pos, qout))
 
 
 def gqa_tree_nsub(ctx, n_head, n_kv, head_dim, ntok) -> int:
@@ -708,9 +745,9 @@ def gqa_tree_decode(q, ktype, kcache, vtype, vcache, pos, masks, gate_src, gate_
                     workspace, n_head, n_kv, head_dim, ntok, max_ctx, nsub, scale, stream=None):
     """attention of ntok drafted tokens at slots pos[0] + t: all of the context before them, and of each other what
     masks[t] (int64 bit patterns) says; masks None: the chain j <= t"""
-    _call("rmi_gqa_tree_decode", _a(q), ktype, _a(kcache), vtype, _a(vcache), _a(pos), _a(masks), _a(gate_src),
-          gate_stride, _a(y), y_stride, _a(q8), q8_stride, _a(workspace), n_head, n_kv, head_dim, ntok, max_ctx, nsub,
-          scale, _s(stream, q, (kcache, vcache, q8, workspace), (q, gate_src, y), (pos,), (masks,)))
+    _call("rmi_gqa_tree_decode", _f32(q), ktype, _a(kcache), vtype, _a(vcache), _i32(pos), _i64(masks), _f32(gate_src),
+          gate_stride, _f32(y), y_stride, _a(q8), q8_stride, _a(workspace), n_head, n_kv, head_dim, ntok, max_ctx, nsub,
+          scale, _s(stream, q, kcache, vcache, pos, masks, gate_src, y, q8, workspace))
 
 
 class Penalties(ctypes.Structure):
@@ -719,11 +756,21 @@ class Penalties(ctypes.Structure):
                 ("window", ctypes.c_int)]
 
 
+@functools.lru_cache(maxsize=64)
+def _penalties(*values):
+    """the argument block of these values"""
+    _by_value(values)
+    return ctypes.byref(Penalties(*values))
+
+
 def logits_process(logits, n, ncols, col_stride, out, out_stride, history, history_len, max_history, window=0,
                    draft=None, masks=None, ndraft=0, repetition=1.0, presence=0.0, frequency=0.0, bias_ids=None,
                    bias_vals=None, n_bias=0, allow=None, allow_stride=0, stream=None):
     """biases, penalties over history (+ the draft path of each column's mask) and grammar masks, before argmax / topk"""
-    pen = Penalties(repetition, presence, frequency, window)
-    _call("rmi_logits_process", _a(logits), n, ncols, col_stride, _a(out), out_stride, _a(history), _a(history_len),
-          max_history, _a(draft), _a(masks), ndraft, ctypes.byref(pen), _a(bias_ids), _a(bias_vals), n_bias, _a(allow),
-          allow_stride, _s(stream, logits, (), (logits, out, bias_vals), (history, history_len, draft, bias_ids, allow), (masks,)))
+    try:
+        pen = _penalties(repetition, presence, frequency, window)
+    except _NotAValue:
+        pen = _penalties(float(repetition), float(presence), float(frequency), operator.index(window))
+    _call("rmi_logits_process", _f32(logits), n, ncols, col_stride, _f32(out), out_stride, _i32(history), _i32(history_len),
+          max_history, _i32(draft), _i64(masks), ndraft, pen, _i32(bias_ids), _f32(bias_vals), n_bias, _i32(allow),
+          allow_stride, _s(stream, logits, out, history, history_len, draft, masks, bias_ids, bias_vals, allow))
