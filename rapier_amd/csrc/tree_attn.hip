@@ -205,12 +205,12 @@ __device__ __forceinline__ uint32_t max_magnitude(uint32_t m, uint32_t w) {
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
 }
-// a mask of the halves of a word that are finite
-__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
-    return ((w & 0x7c00u) != 0x7c00u ? 0xffffu : 0u) | ((w & 0x7c000000u) != 0x7c000000u ? 0xffff0000u : 0u);
-}
 // a word of fp16 V without its infinities and NaN
-__device__ __forceinline__ uint32_t zero_odd(uint32_t w) { return w & finite_halves(w); }
+__device__ __forceinline__ uint32_t zero_odd(uint32_t w) {
+    if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
+    if ((w & 0x7c000000u) == 0x7c000000u) w &= 0xffffu;
+    return w;
+}
 
 // the power of two that brings a row's largest |q| to [2^13, 2^14), as its exponent
 __device__ __forceinline__ int q_shift(float amax) {
@@ -626,9 +626,10 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kerne
 #pragma unroll
                         for (int e = 0; e < VD / 2; ++e) vx[j].w[e] = zero_odd(vx[j].w[e]);
                     } else if ((j & 1) == 0) {
-                        const uint32_t c = u2(vsp[j >> 1].c);
-                        vsp[j >> 1].s = h2(u2(vsp[j >> 1].s) & finite_halves(c));
-                        vsp[j >> 1].c = h2(c & finite_halves(c));
+                        uint32_t s = u2(vsp[j >> 1].s), c = u2(vsp[j >> 1].c);
+                        if ((c & 0x7c00u) == 0x7c00u) s &= 0xffff0000u, c &= 0xffff0000u;
+                        if ((c & 0x7c000000u) == 0x7c000000u) s &= 0xffffu, c &= 0xffffu;
+                        vsp[j >> 1] = {h2(s), h2(c)};
                     }
                 }
             }
