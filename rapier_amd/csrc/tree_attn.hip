@@ -377,8 +377,9 @@ __device__ __forceinline__ void join_stats(float unit, const float (&stat)[WAVES
 // The waves take quarters of the chunk.  K of the next step is loaded when this step's scores are done, V when its product is:
 // each has half a step to arrive.  (Two steps ahead, in alternating registers, cost more than it hid: 30 us for 23.)
 // One token of 16 heads behind 65501 positions: F16 50 us with its join (5.3 TB/s), I8 33 (4.2), I4 23 (3.1).  Seven of them
-// are the beginning (position, first loads, q's parts) and the end; past that F16 and I8 are bound by the memory, I4 by
-// waiting on it with one wave a SIMD: its codes' 570 vector instructions a step take half the time.
+// are the beginning (position, first loads, q's parts) and the end; past that F16 and I8 are bound by the memory.  I4 has one wave a SIMD,
+// whose vector units are busy for 51 % of its life (5928 instructions for eight steps, a beginning and an end) and which waits
+// 26 % of it; I8 keys with I4 values 25 us.
 template <int KT, int VT, int HD, int ROWS>
 __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void tree_few_kernel(TreeArgs a) {
     constexpr bool PACKED = ROWS == 8;
@@ -1131,8 +1132,8 @@ bool tree_shape_ok(int max_ctx, int n_head, int n_kv, int head_dim, int ntok) {
 // The form of a call: query rows per KV head, 16-row blocks side by side in a workgroup (0: the form of few rows), rows a
 // workgroup holds, workgroups per (chunk, KV head).  Up to 16 rows the form of few rows; more rows are groups of it where the
 // split asks for that (RMI_TREE_SHORT: rmi_gqa_tree_nsub), else tiles, which turn K and V to fp16 once for all of a workgroup's
-// rows.  17 to 32 rows of I8 and I4 stay groups of few (64K, 8 tokens x 4 heads: 45.7 / 38.9 us, tiles 47.3 / 40.2), F16 takes
-// tiles over long chunks (61 us, groups of few 83: they load K and V twice).
+// rows.  17 to 32 rows of I8 and I4 stay groups of few (64K, 8 tokens x 4 heads: 45.7 / 38.9 us, tiles 47.3 / 40.2; I8 / I4 41), F16 takes
+// tiles over long chunks (60 us, groups of few 83: they load K and V twice).
 constexpr int kLongSub = 6;
 constexpr int kShort = RMI_TREE_SHORT;
 struct Form {
@@ -1196,8 +1197,10 @@ extern "C" int rmi_gqa_tree_nsub(int ctx, int n_head, int n_kv, int head_dim, in
     };
     // More than 16 rows as groups of few while a wave of theirs has at most 8 steps, where a workgroup's beginning and end
     // and the records of many chunks weigh more than turning K and V to fp16 once: 16 tokens x 4 heads, groups / tiles: I8 4K
-    // 16.5 / 19.9 us, 8K 20.0 / 22.6, 16K 24.6 / 25.8; 64 tokens 4K 26.4 / 32.9, 32 tokens 16K (16 steps) 40 / 36.5;
-    // F16 16 tokens 4K 17.5 / 18.8, 16K 32.6 / 27.2, 64 tokens 4K 33.3 / 32.9.
+    // 16.9 / 21.3 us, 8K 20.0 / 22.6, 16K 24.9 / 25.8; 64 tokens 4K 26.5 / 33.7, 32 tokens 16K (16 steps) 40 / 36;
+    // F16 16 tokens 4K 18.1 / 21.2, 16K 32.1 / 27.0, 64 tokens 4K 32.6 / 32.0; I4 16 tokens 4K 16.5 / 21.3, 16K 25.8 / 29.0.
+    // The rule does not know the cache's type: 16 tokens of F16 behind 16K are a sixth faster with the tiles' split (2), which a
+    // caller may give.
     constexpr int kFewSteps = 8;
     const Form few = tree_form(n_head, n_kv, ntok, kShort + 1, false), tile = tree_form(n_head, n_kv, ntok, kLongSub, true);
     long long nsub = nsub_for(few.groups);

@@ -163,3 +163,14 @@ def test_as_many_chunks_as_there_may_be(rmi):
 def test_fp16_tiles_of_32_rows(rmi, nh, nkv, ntok, base, nsub, hd):
     for masked in (True, False):
         form_call(rmi, F16, nh, nkv, hd, ntok, base, nsub, 0, masked).check()
+
+
+@pytest.mark.parametrize("ntok,used", [(1, 448), (6, 512), (20, 448), (40, 441)])
+def test_an_fp16_cache_by_the_positions_in_use(rmi, ntok, used):
+    """its layout does not hang on max_ctx: a call may be given the part that holds the text"""
+    c = form_call(rmi, F16, 4, 2, 256, ntok, 401, 1, 0, max_ctx=5000)
+    c.check()
+    k, v = c.values()
+    c.max_ctx = used   # of the same buffers
+    c.values = lambda: (k[:used], v[:used])
+    c.check()
