@@ -436,12 +436,12 @@ bool aligned_to(const void* p, size_t n) { return p && (reinterpret_cast<uintptr
 
 // whether rows outside share bytes with the cache's of positions [first, first + n)
 bool on_cache_rows(int type, const void* rows, int rows16, int stride, const void* cache, int first, int n, int n_kv, int head_dim, int max_ctx) {
-    const long long el = rows16 ? 2 : 4, per = kv_row_bytes(type, head_dim), sper = head_dim / kKvBlock;
-    const RowSet out{rows, n, stride * el, n_kv * head_dim * el};
+    const long long el = rows16 ? 2 : 4, heads = n_kv, ctx = max_ctx, per = kv_row_bytes(type, head_dim), sper = head_dim / kKvBlock;
+    const RowSet out{rows, n, stride * el, heads * head_dim * el};
     const auto* c = static_cast<const uint8_t*>(cache);
-    if (type == kKvF16) return rows_overlap(out, block_of(c + first * n_kv * per, n * n_kv * per));
-    return rows_overlap(out, {c + first * per, n_kv, max_ctx * per, n * per}) ||
-           rows_overlap(out, {c + n_kv * max_ctx * per + first * sper, n_kv, max_ctx * sper, n * sper});
+    if (type == kKvF16) return rows_overlap(out, block_of(c + heads * per * first, heads * per * n));
+    return rows_overlap(out, {c + per * first, heads, ctx * per, per * n}) ||
+           rows_overlap(out, {c + heads * ctx * per + sper * first, heads, ctx * sper, sper * n});
 }
 
 // calls f with the type as a constant

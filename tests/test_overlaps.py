@@ -77,6 +77,21 @@ def test_rows_on_their_own_cache_rows(rmi, name, type_, rows, f16, stride):
         rmi._call(name, type_, *a, 10, 5, 4, 256, 100, None)
 
 
+# caches whose rows and bytes pass 32 bits: 2^26 positions x 64 heads x 256, the last five of them
+FIRST = (1 << 26) - 5
+HUGE = {0: [64 * FIRST * 512, 64 * FIRST * 512 + 5 * 64 * 512 - 4],
+        1: [FIRST * 256, 63 * (1 << 26) * 256 + FIRST * 256 + 1000, 64 * (1 << 26) * 256 + FIRST * 8, 64 * (1 << 26) * (256 + 8) - 4],
+        2: [FIRST * 128, 64 * (1 << 26) * 128 + (31 * (1 << 26) + FIRST) * 8]}
+
+
+@pytest.mark.parametrize("name", ["rmi_kv_write", "rmi_kv_read"])
+@pytest.mark.parametrize("type_,rows", [(t, r) for t in HUGE for r in HUGE[t]])
+def test_rows_on_their_own_rows_of_a_huge_cache(rmi, name, type_, rows):
+    a = (at(rows), 0, 64 * 256, at(0)) if name == "rmi_kv_write" else (at(0), at(rows), 0, 64 * 256)
+    with pytest.raises(ValueError, match="lies on"):
+        rmi._call(name, type_, *a, FIRST, 5, 64, 256, 1 << 26, None)
+
+
 @pytest.mark.parametrize("out,ncols,col_stride,out_stride", [
     (4, 1, 1000, 1000), (-4, 1, 1000, 1000), (3996, 1, 1000, 1000), (4000, 2, 1000, 1000), (-4 * 1004, 3, 1004, 1004), (4, 64, 1000, 1000),
     (3996, 2, 2000, 2000), (4 * 2000, 3, 2000, 1000), (4 * 63 * 2000 + 4 * 999, 64, 2000, 2000), (-4 * 63 * 3001 + 400, 64, 2000, 3001)])
