@@ -366,7 +366,7 @@ int rmi_gqa_flash_decode_noalloc(const float* q, const uint16_t* kcache, const u
  * mantissa bits).  s is the smallest such number with Q s >= max|x| (Q = 127 / 7, at most 512 / 8192: larger values
  * saturate), code = x / s rounded to the nearest integer (half to even), |code| <= Q, and the cache holds code * s, which
  * is an fp16 number exactly.  A block with an infinity or a NaN gets s = NaN and reads back as NaN.  No call writes another
- * scale byte above that of 512 / 8192; the attention takes those of 960 / 15360 and more as NaN. */
+ * scale byte above that of 512 / 8192; from 960 / 15360 on, a V is NaN to the attention and a score undefined. */
 enum { RMI_KV_F16 = 0, RMI_KV_I8 = 1, RMI_KV_I4 = 2 };
 
 /* bytes of one cache; 0 on a bad type or shape */
@@ -411,7 +411,8 @@ int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* qn, const fl
  * prompt chunks).  q is [ntok][n_head][head_dim]; kcache / vcache types: both F16, both I8, both I4, or I8 and I4;
  * sigmoid gate as rmi_gqa_flash_decode's (gate of head h at + h * 2 * head_dim + head_dim; null: no gate); fp32 y
  * (nullable; rows y_stride elements apart) and Q8_1 (nullable; q8_stride bytes).  Rows a token does not see have no part
- * in its result, whatever they hold; a NaN or an infinity in q or in a row that it sees makes the result NaN or infinite.
+ * in its result, whatever they hold.  A NaN in what it sees, or an infinity in its q or a V, makes the result NaN or
+ * infinite; an infinity in an F16 K makes it NaN, or what the formula gives (a score of -infinity has no weight).
  * If a slot lies outside [0, max_ctx) nothing is written.
  * y may be q (rows n_head * head_dim apart); else outputs and workspace share no byte with each other or with what is read.
  * The context is split into chunks of 128 * nsub positions; rmi_gqa_tree_nsub gives the split for a context of `ctx`

@@ -174,3 +174,22 @@ def test_an_fp16_cache_by_the_positions_in_use(rmi, ntok, used):
     c.max_ctx = used   # of the same buffers
     c.values = lambda: (k[:used], v[:used])
     c.check()
+
+
+@pytest.mark.parametrize("nh,nkv,hd,ntok,short", SHAPES)
+@pytest.mark.parametrize("bad", [np.inf, -np.inf])
+def test_an_infinity_in_a_key_that_is_seen(rmi, nh, nkv, hd, ntok, short, bad):
+    """in one dim of a row of the context: NaN, or the formula's result; where that is NaN (a score of infinity), NaN"""
+    base, rng = 70, np.random.default_rng(4)
+    kv = [rng.standard_normal((base + ntok + 5, nkv, hd)).astype(np.float32) for _ in range(2)]
+    kv[0][30, :, 7] = bad
+    c = Call(rmi, (ref.F16, ref.F16), nh, nkv, hd, ntok, base, None, nsub=1 + short * rmi.TREE_SHORT, kv=kv)
+    y = c.run()
+    with np.errstate(all="ignore"):
+        want, _ = c.expected()
+        c.raw[0] = c.raw[0].copy()
+        c.raw[0].view(np.float16).reshape(c.max_ctx, nkv, hd)[30, :, 7] = 0   # a bound without the infinity
+        bound = c.expected()[1]
+    nan = np.isnan(y).all(-1)
+    assert (nan | ~np.isnan(y).any(-1)).all() and nan[np.isnan(want).any(-1)].all()
+    assert (np.abs(y - want) <= bound)[~nan].all()
