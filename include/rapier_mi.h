@@ -420,9 +420,9 @@ int rmi_attn_prep_axes(const float* q3, int q3_stride, const float* qn, const fl
  * at least max_ctx / 262144, rounded up, which over a cache of more than 262144 positions can be more than a short text's
  * split.  With RMI_TREE_SHORT added, more than 16 query rows per KV head are worked on 16 at a time, which pays over short
  * chunks.  workspace holds rmi_gqa_tree_workspace_bytes(...) bytes, 16-byte aligned, and needs no initial state; calls that
- * may overlap need one each.  Same inputs, same bits; I8 and I4 caches give the bits of an F16 cache that holds their values (but for 17 to 32
- * query rows at nsub >= 6 without RMI_TREE_SHORT); and while ntok * n_head / n_kv <= 8, each token of a chain has the
- * bits of a call of its own at the same nsub. */
+ * may overlap need one each.  Same inputs, same bits; I8 and I4 caches give the bits of an F16 cache that holds their
+ * values (but for 17 to 32 query rows at nsub >= 6 without RMI_TREE_SHORT); and while ntok * n_head / n_kv <= 8, each token
+ * of a chain has the bits of a call of its own at the same nsub. */
 enum { RMI_TREE_SHORT = 1 << 24 };
 int rmi_gqa_tree_nsub(int ctx, int n_head, int n_kv, int head_dim, int ntok);
 size_t rmi_gqa_tree_workspace_bytes(int max_ctx, int n_head, int n_kv, int head_dim, int ntok, int nsub);
@@ -434,7 +434,8 @@ int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache, int vtype
 /* What a sampler wants done to ncols (1..64) columns of n logits before rmi_argmax / rmi_topk.  Column c's text is
  * history[0 .. min(history_len[0], max_history)) (device words; max_history 0: none, both may be null) and then, with a
  * draft of ndraft <= 64 tokens, those draft[j] whose bit j of masks[c] is set, in ascending order (the path to a tree's
- * node); ids outside [0, n) take their places and count for nothing.  m = how often v stands in the text's last `window` tokens (window <= 0: in all of it).
+ * node); ids outside [0, n) take their places and count for nothing.  m = how often v stands in the text's last `window`
+ * tokens (window <= 0: in all of it).
  *   x = logits[v] + bias of v (bias_ids / bias_vals, n_bias entries; of entries with one id the last counts)
  *   m > 0:  x = x > 0 ? x / repetition : x * repetition;   x -= m * frequency + presence
  *   bit v % 32 of allow[c * allow_stride + v / 32] clear:  x = -infinity     (null allow: every token)

@@ -1244,19 +1244,22 @@ extern "C" int rmi_gqa_tree_decode(const float* q, int ktype, const void* kcache
     const int width = n_head * head_dim;
     if (ntok > 1 && ((y && y_stride < width) || (q8 && q8_stride < width / 32 * static_cast<int>(kQ8_1Bytes))))
         return fail(RMI_ERR_SHAPE, "gqa_tree_decode: output rows overlap");
-    // y may be q itself: a row's workgroup alone reads its q, and before it writes.  The gates of a token: from the first to the
-    // last (no row of y or q8 fits between two)
+    // y may be q itself: a row's workgroup alone reads its q, and before it writes
     const RowSet in[] = {block_of(q, static_cast<size_t>(ntok) * width * 4), block_of(kcache, rmi_kv_cache_bytes(ktype, max_ctx, n_kv, head_dim)),
-                         block_of(vcache, rmi_kv_cache_bytes(vtype, max_ctx, n_kv, head_dim)),
-                         {gate_src ? gate_src + head_dim : nullptr, gate_src ? ntok : 0, 4LL * gate_stride, 4LL * (2 * width - head_dim)}};
+                         block_of(vcache, rmi_kv_cache_bytes(vtype, max_ctx, n_kv, head_dim))};
     const RowSet out[] = {block_of(workspace, rmi_gqa_tree_workspace_bytes(max_ctx, n_head, n_kv, head_dim, ntok, split)),
                           {q8, q8 ? ntok : 0, q8_stride, width / 32 * kQ8_1Bytes},
                           {y, y ? ntok : 0, 4LL * y_stride, 4LL * width}};
     const bool in_place = y == q && (ntok == 1 || y_stride == width);
     for (const RowSet& o : out) {
         for (const RowSet& i : in)
-            if (o.n && i.n && !(in_place && o.p == y && i.p == q) && rows_overlap(o, i))
+            if (o.n && !(in_place && o.p == y && i.p == q) && rows_overlap(o, i))
                 return fail(RMI_ERR_POINTER, "gqa_tree_decode: an output or the workspace lies on what the call reads");
+        // a token's gates from the first to the last, then head by head: a row of q8 may fit between two
+        if (gate_src && o.n && rows_overlap(o, {gate_src + head_dim, ntok, 4LL * gate_stride, 4LL * (2 * width - head_dim)}))
+            for (int h = 0; h < n_head; ++h)
+                if (rows_overlap(o, {gate_src + static_cast<size_t>(2 * h + 1) * head_dim, ntok, 4LL * gate_stride, 4LL * head_dim}))
+                    return fail(RMI_ERR_POINTER, "gqa_tree_decode: an output or the workspace lies on the gates");
         for (const RowSet* other = out; other != &o; ++other)
             if (o.n && other->n && rows_overlap(o, *other))
                 return fail(RMI_ERR_POINTER, "gqa_tree_decode: an output or the workspace lies on another");

@@ -62,6 +62,26 @@ def test_tree_results_in_the_queries_place(rmi, types, nh, nkv, hd, ntok, base, 
         assert np.array_equal(host(q).reshape(want.shape).view(np.uint32), want.view(np.uint32))
 
 
+@pytest.mark.parametrize("nh,ntok", [(2, 1), (2, 7), (3, 5)])
+def test_q8_rows_between_the_gates(rmi, orc, nh, ntok):
+    """rows of Q8_1 in the place of a head's spent q, between the gates of two heads"""
+    hd, base = 256, 130
+    c = Call(rmi, (ref.I8, ref.I8), nh, nh, hd, ntok, base, None, nsub=1)
+    want = np.stack([orc.quantize_q8_1(y.reshape(-1), nh * hd) for y in c.run()])
+    d = dev(c.q3.reshape(-1))
+    ws = empty(rmi.gqa_tree_workspace_bytes(c.max_ctx, nh, nh, hd, ntok, 1), "uint8")
+    rmi.gqa_tree_decode(dev(c.q), ref.I8, dev(c.raw[0]), ref.I8, dev(c.raw[1]), dev(np.array([base], np.int32)), None, d, c.width, None, 0, d[2 * hd:],
+                        4 * c.width, ws, nh, nh, hd, ntok, c.max_ctx, 1, c.scale)
+    got = host(d).reshape(ntok, c.width)
+    n = nh * hd // 32 * 9   # words of a row
+    assert np.array_equal(got[:, 2 * hd:2 * hd + n].copy().view(np.uint8).reshape(ntok, -1), want)
+    got[:, 2 * hd:2 * hd + n] = c.q3[:, 2 * hd:2 * hd + n]
+    assert np.array_equal(got, c.q3)
+    with pytest.raises(ValueError, match="gates"):
+        rmi.gqa_tree_decode(dev(c.q), ref.I8, dev(c.raw[0]), ref.I8, dev(c.raw[1]), dev(np.array([base], np.int32)), None, d, c.width, None, 0,
+                            d[3 * hd - 1:], 4 * c.width, ws, nh, nh, hd, ntok, c.max_ctx, 1, c.scale)
+
+
 def test_tree_results_beside_the_gates(rmi):
     """y in the columns behind a buffer's gates"""
     nh, nkv, hd, ntok, base = 4, 2, 256, 9, 130
