@@ -450,6 +450,91 @@ int rmi_logits_process(const float* logits, int n, int ncols, int col_stride, fl
                        const float* bias_vals, int n_bias, const uint32_t* allow, int allow_stride, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------------
+ * Several requests served at once: caches in pages of one pool, attention for a ragged batch (no counterpart in the
+ * reference, which serves one request)
+ * ------------------------------------------------------------------------------------------------------------- */
+
+/* A page is a cache (above) of page_size = 16, 32, 64, 128 or 256 positions, rmi_kv_cache_bytes(type, page_size, ...) bytes in
+ * the layout of that max_ctx; a pool is n_pages of them one after another, 16-byte aligned, n_pages * page_size < 2^31.  K and V
+ * of a layer are two pools under the same page ids.  Slot s is position s % page_size of page s / page_size.  A block table has
+ * a row of table_stride page ids for each of up to 4096 requests: position p of request i is in page
+ * table[i * table_stride + p / page_size].  Lengths, page ids and slots are device words and checked there: none leads outside a
+ * pool, a table or a call's rows.  No two pages of one table that are in use may be the same. */
+enum { RMI_PAGES_OK = 0, RMI_PAGES_BAD_LENGTH = 1, RMI_PAGES_NONE_LEFT = 2 };   /* status of a request in a plan */
+
+/* The plan of a round in which request i, of past[i] positions so far, gets count[i] >= 0 new tokens.
+ *   row_start[n_req + 1]  exclusive sums of count: request i's new tokens are rows row_start[i] .. row_start[i + 1] - 1
+ *   table                 the pages that it needs, ceil((past + count) / page_size) - ceil(past / page_size), behind those it has;
+ *                         in request order the first page taken is free_pages[n_free[0] - 1], the next the one before
+ *   kv_len[i], status[i]  past + count and RMI_PAGES_OK; or 0 and a reason, and the request gets no page: its lengths are
+ *                         negative, longer than the table's row or than 2^30, or its rows pass max_tok; or it needs pages and the
+ *                         sum of those needed up to and with it passes n_free
+ *   slot, pos [max_tok]   per row its token's slot (-1: refused, or behind the last request) and position (0 behind the last)
+ *   n_left                what is left of the free list, free_pages[0 .. n_left)
+ * free_pages holds n_pages words, max_tok <= 2^30.  Outputs share no byte with each other or with inputs (n_left is not n_free:
+ * rmi_page_trim leads back). */
+int rmi_page_plan(const int* past, const int* count, int n_req, int page_size, int n_pages, const int* free_pages,
+                  const int* n_free, int* table, int table_stride, int max_tok, int* row_start, int* kv_len, int* slot,
+                  int* pos, int* n_left, int* status, void* stream);
+/* Gives back the pages past the positions that requests keep: pages ceil(keep / page_size) .. ceil(len / page_size) - 1 of each,
+ * in the order of requests and positions, to free_pages[n_free[0]] on; n_out the new count.  keep = len gives back nothing (nor
+ * does keep < 0 or keep > len), keep = 0 all of a request.  Pages past n_pages free ones are dropped.  The table is left as
+ * it is.  Outputs share no byte with each other or with inputs. */
+int rmi_page_trim(const int* len, const int* keep, int n_req, int page_size, int n_pages, const int* table, int table_stride,
+                  const int* n_free, int* free_pages, int* n_out, void* stream);
+/* rmi_kv_read for rows at slots: rows of n_kv x head_dim in fp32 or fp16, out_stride elements apart, zeros for a slot outside
+ * the pool.  Rows are written by rmi_attn_prep_paged, or page by page by rmi_kv_write. */
+int rmi_kv_page_read(int type, const void* pool, const int* slot, void* out, int out_f16, int out_stride, int n, int n_kv,
+                     int head_dim, int page_size, int n_pages, void* stream);
+
+/* element types of 16-bit rows, and which dims of a row make pair i of n_rot / 2 */
+enum { RMI_ROWS_F16 = 0, RMI_ROWS_BF16 = 1 };
+enum { RMI_ROPE_HALF = 0, RMI_ROPE_NEIGHBOURS = 1 };   /* (i, i + n_rot / 2), or (2 i, 2 i + 1) */
+
+/* rmi_attn_prep_rope for a batch over pages: row t of q3 ([n_head x (q | gate) | k | v]) is at position pos[t], its K and V rows
+ * go to slot[t] of the pools, its q rows normed, rotated and rounded to qout[t][head][dim] of qtype.  A row whose slot is outside
+ * the pool is left out, its q rows too.  A null qn or kn leaves the norm of q or K out.  q is worked on in fp32, K in fp64 and
+ * rounded to fp32 once before it is stored (as in rmi_attn_prep_axes); angles are formed in fp64.  rope as in rmi_attn_prep_rope
+ * (ext_factor 0: all pairs by 1 / factor).  Slots of a call are distinct.  The pools, qout and what is read share no byte; qout
+ * 16-byte aligned. */
+int rmi_attn_prep_paged(const float* q3, int q3_stride, const float* qn, const float* kn, int ktype, void* kpool, int vtype,
+                        void* vpool, const int* slot, const int* pos, int qtype, void* qout, int n_head, int n_kv, int head_dim,
+                        int n_rot, const rmi_rope_params* rope, int pairs, float eps, int ntok, int page_size, int n_pages,
+                        void* stream);
+
+/* Attention of a batch's new tokens over their requests' pages: request i's rows row_start[i] .. row_start[i + 1] - 1 of q
+ * ([ntok][n_head][head_dim] of qtype) are its last positions, up to kv_len[i] - 1, and a token sees the positions up to its own.
+ * Any mix of single tokens, drafts and prompt chunks.  Cache types as rmi_gqa_tree_decode's; products on fp16 operands (bf16 q
+ * is brought to fp16 by a power of two a row, the weights are rounded to fp16), sums in fp32.  scale > 0.  Sigmoid gate, y (of
+ * qtype, 8-byte aligned, y_stride a multiple of 4) and Q8_1 as rmi_gqa_tree_decode's.
+ * Left as they are: rows behind the last request's, and rows of a request with more than max_new new tokens or more than max_ctx
+ * positions.  A token at a negative position (kv_len below the number of new tokens) gives zeros.  A token that sees a position
+ * whose page id is outside the pool or past the table's row gives NaN.  What a token does not see has no part in its result,
+ * whatever it holds; a NaN or an infinity in what it sees makes it NaN or infinite.
+ * The contexts are worked on in chunks of `split` positions, a multiple of 128 that leaves at most 1024 chunks of max_ctx;
+ * rmi_gqa_paged_split gives it for a batch of total_ctx positions in all, to be settled once (results differ in the last bits
+ * between splits).  workspace holds rmi_gqa_paged_workspace_bytes(...) bytes, 16-byte aligned (null where split >= max_ctx), and
+ * needs no initial state; calls that may overlap need one each.  ntok <= 2^24.  Outputs and workspace share no byte with each
+ * other or with what is read.  Same inputs, same bits. */
+int rmi_gqa_paged_split(long long total_ctx, int max_ctx, int n_req, int ntok, int max_new, int n_head, int n_kv, int head_dim);
+size_t rmi_gqa_paged_workspace_bytes(int ntok, int max_ctx, int n_head, int head_dim, int split);
+int rmi_gqa_paged_attn(int qtype, const void* q, int ktype, const void* kpool, int vtype, const void* vpool, const int* table,
+                       int table_stride, const int* row_start, const int* kv_len, const float* gate_src, int gate_stride,
+                       void* y, int y_stride, uint8_t* q8, int q8_stride, void* workspace, int n_req, int ntok, int max_new,
+                       int max_ctx, int n_head, int n_kv, int head_dim, int page_size, int n_pages, int split, float scale,
+                       void* stream);
+
+/* Causal attention over whole prompts packed row by row, without a cache: rows row_start[i] .. row_start[i + 1] - 1 of q
+ * ([n_head][head_dim]), k and v ([n_kv][head_dim]), all of one type, are request i's; row t of it sees its rows up to t.  Rows are
+ * q_stride, k_stride and v_stride elements apart (multiples of 8; q, k and v 16-byte aligned); an F16 cache's rows, contiguous or
+ * pages in order, can be k and v.  BF16 rows are multiplied as bf16, the weights rounded to it.  Requests of more than max_len
+ * rows are left out, rows behind the last request's are left as they are.  Gate, y, Q8_1 and what is not finite as above. */
+int rmi_gqa_prompt_attn(int type, const void* q, int q_stride, const void* k, int k_stride, const void* v, int v_stride,
+                        const int* row_start, const float* gate_src, int gate_stride, void* y, int y_stride, uint8_t* q8,
+                        int q8_stride, int n_req, int ntok, int max_len, int n_head, int n_kv, int head_dim, float scale,
+                        void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
  * Seeded synthetic tensors in HBM (stand-in for a GGUF file: random-init weights; no reference counterpart)
  * ------------------------------------------------------------------------------------------------------------- */
 int rmi_gen_q6_k(void* w, size_t nblocks, uint64_t seed, float d_std, void* stream);

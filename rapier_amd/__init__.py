@@ -24,6 +24,8 @@ RMI_OK, RMI_ERR_SHAPE, RMI_ERR_POINTER, RMI_ERR_STREAM, RMI_ERR_LAUNCH, RMI_ERR_
 GGML_Q8_0, GGML_Q6_K = 8, 14
 KV_F16, KV_I8, KV_I4 = range(3)   # K/V cache types
 TREE_SHORT = 1 << 24              # a split's flag (gqa_tree_nsub)
+ROPE_HALF, ROPE_NEIGHBOURS = range(2)                        # dims (i, i + n_rot / 2) or (2 i, 2 i + 1) of a pair
+PAGES_OK, PAGES_BAD_LENGTH, PAGES_NONE_LEFT = range(3)       # a request's status in a page plan
 Q6K_BYTES, Q8_0_BYTES, Q8_1_BYTES = 210, 34, 36
 
 _lib = None
@@ -120,6 +122,17 @@ SIGNATURES = {
     "rmi_gqa_tree_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
     "rmi_gqa_tree_decode": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i,
                                  _i, _f, _vp]),
+    "rmi_page_plan": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "rmi_page_trim": (_i, [_vp, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp]),
+    "rmi_kv_page_read": (_i, [_i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "rmi_attn_prep_paged": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp, _i, _f,
+                                 _i, _i, _i, _vp]),
+    "rmi_gqa_paged_split": (_i, [ctypes.c_longlong, _i, _i, _i, _i, _i, _i, _i]),
+    "rmi_gqa_paged_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "rmi_gqa_paged_attn": (_i, [_i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _i,
+                                _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp]),
+    "rmi_gqa_prompt_attn": (_i, [_i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i,
+                                 _f, _vp]),
     "rmi_logits_process": (_i, [_vp, _i, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i,
                                 _vp]),
 }
@@ -774,3 +787,102 @@ def logits_process(logits, n, ncols, col_stride, out, out_stride, history, histo
     _call("rmi_logits_process", _f32(logits), n, ncols, col_stride, _f32(out), out_stride, _i32(history), _i32(history_len),
           max_history, _i32(draft), _i64(masks), ndraft, pen, _i32(bias_ids), _f32(bias_vals), n_bias, _i32(allow),
           allow_stride, _s(stream, logits, out, history, history_len, draft, masks, bias_ids, bias_vals, allow))
+
+
+# ---- several requests at once: caches in pages, attention for a ragged batch --------------------------------------------
+
+def page_plan(past, count, n_req, page_size, n_pages, free_pages, n_free, table, table_stride, max_tok, row_start, kv_len, slot,
+              pos, n_left, status, stream=None):
+    """row starts, lengths, slots and positions of count[i] new tokens of each request, and the pages they need (int32 tensors)"""
+    _call("rmi_page_plan", _i32(past), _i32(count), n_req, page_size, n_pages, _i32(free_pages), _i32(n_free), _i32(table),
+          table_stride, max_tok, _i32(row_start), _i32(kv_len), _i32(slot), _i32(pos), _i32(n_left), _i32(status),
+          _s(stream, table, past, count, free_pages, n_free, row_start, kv_len, slot, pos, n_left, status))
+
+
+def page_trim(length, keep, n_req, page_size, n_pages, table, table_stride, n_free, free_pages, n_out, stream=None):
+    """the pages past the first keep[i] of length[i] positions of each request, back to the free list"""
+    _call("rmi_page_trim", _i32(length), _i32(keep), n_req, page_size, n_pages, _i32(table), table_stride, _i32(n_free),
+          _i32(free_pages), _i32(n_out), _s(stream, table, length, keep, n_free, free_pages, n_out))
+
+
+def kv_page_read(type_, pool, slot, out, out_stride, n, n_kv, head_dim, page_size, n_pages, stream=None):
+    """the rows of n slots of a pool to float32 or float16 rows"""
+    _call("rmi_kv_page_read", type_, _a(pool), _i32(slot), _rows(out, n, pool), _is_f16(out), out_stride, n, n_kv, head_dim,
+          page_size, n_pages, _s(stream, pool, slot, out))
+
+
+_ROWS16 = {}   # dtypes of 16-bit rows -> the library's name of them
+
+
+def _row_type(*tensors):
+    """RMI_ROWS_F16 or RMI_ROWS_BF16, the type of all of these (None: an argument left out)"""
+    kind = None
+    for t in tensors:
+        if t is None:
+            continue
+        k = _ROWS16.get(t.dtype)
+        if k is None:
+            torch = sys.modules["torch"]
+            _ROWS16.update({torch.float16: 0, torch.bfloat16: 1})
+            k = _ROWS16.get(t.dtype)
+            if k is None:
+                raise ValueError(f"rows of float16 or bfloat16, not {t.dtype}")
+        if kind is None:
+            kind = k
+        elif k != kind:
+            raise ValueError("rows of one type, float16 or bfloat16")
+    return kind
+
+
+@functools.lru_cache(maxsize=64)
+def _rope_values(*rope):
+    """the argument block of these values"""
+    _by_value(rope)
+    return ctypes.byref(RopeParams(*rope))
+
+
+def attn_prep_paged(q3, q3_stride, qn, kn, ktype, kpool, vtype, vpool, slot, pos, qout, n_head, n_kv, head_dim, n_rot, pairs,
+                    freq_base, eps, ntok, page_size, n_pages, factor=1.0, orig_ctx=0.0, ext_factor=1.0, attn_factor=1.0,
+                    beta_fast=32.0, beta_slow=1.0, stream=None):
+    """per-head norm (qn / kn None: none), rotation of row t at pos[t], q to float16 or bfloat16 rows, K and V to slot[t]"""
+    values = freq_base, factor, orig_ctx, ext_factor, attn_factor, beta_fast, beta_slow
+    try:
+        rope = _rope_values(*values)
+    except _NotAValue:
+        rope = _rope_values(*map(float, values))
+    _call("rmi_attn_prep_paged", _f32(q3), q3_stride, _f32(qn), _f32(kn), ktype, _a(kpool), vtype, _a(vpool), _i32(slot),
+          _i32(pos), _row_type(qout), _a(qout), n_head, n_kv, head_dim, n_rot, rope, pairs, eps, ntok, page_size, n_pages,
+          _s(stream, kpool, vpool, q3, qn, kn, slot, pos, qout))
+
+
+def gqa_paged_split(total_ctx, max_ctx, n_req, ntok, max_new, n_head, n_kv, head_dim) -> int:
+    """the positions of a chunk, for a batch of total_ctx positions and ntok new tokens in all"""
+    n = lib().rmi_gqa_paged_split(total_ctx, max_ctx, n_req, ntok, max_new, n_head, n_kv, head_dim)
+    if n == 0:
+        raise ValueError(last_error())
+    return n
+
+
+def gqa_paged_workspace_bytes(ntok, max_ctx, n_head, head_dim, split) -> int:
+    n = lib().rmi_gqa_paged_workspace_bytes(ntok, max_ctx, n_head, head_dim, split)
+    if n == 0:
+        raise ValueError(last_error())
+    return n
+
+
+def gqa_paged_attn(q, ktype, kpool, vtype, vpool, table, table_stride, row_start, kv_len, gate_src, gate_stride, y, y_stride, q8,
+                   q8_stride, workspace, n_req, ntok, max_new, max_ctx, n_head, n_kv, head_dim, page_size, n_pages, split, scale,
+                   stream=None):
+    """attention of each request's new tokens (rows row_start[i] .. of q) over its pages, up to position kv_len[i] - 1"""
+    _call("rmi_gqa_paged_attn", _row_type(q, y), _a(q), ktype, _a(kpool), vtype, _a(vpool), _i32(table), table_stride,
+          _i32(row_start), _i32(kv_len), _f32(gate_src), gate_stride, _a(y), y_stride, _a(q8), q8_stride, _a(workspace), n_req,
+          ntok, max_new, max_ctx, n_head, n_kv, head_dim, page_size, n_pages, split, scale,
+          _s(stream, q, kpool, vpool, table, row_start, kv_len, gate_src, y, q8, workspace))
+
+
+def gqa_prompt_attn(q, q_stride, k, k_stride, v, v_stride, row_start, gate_src, gate_stride, y, y_stride, q8, q8_stride, n_req,
+                    ntok, max_len, n_head, n_kv, head_dim, scale, stream=None):
+    """causal attention over whole prompts packed row by row (float16 or bfloat16)"""
+    _call("rmi_gqa_prompt_attn", _row_type(q, k, v, y), _a(q), q_stride, _a(k), k_stride, _a(v), v_stride, _i32(row_start),
+          _f32(gate_src), gate_stride, _a(y), y_stride, _a(q8), q8_stride, n_req, ntok, max_len, n_head, n_kv, head_dim, scale,
+          _s(stream, q, k, v, row_start, gate_src, y, q8))
