@@ -526,7 +526,7 @@ int rmi_gqa_paged_attn(int qtype, const void* q, int ktype, const void* kpool, i
 
 /* Causal attention over whole prompts packed row by row, without a cache: rows row_start[i] .. row_start[i + 1] - 1 of q
  * ([n_head][head_dim]), k and v ([n_kv][head_dim]), all of one type, are request i's; row t of it sees its rows up to t.  Rows are
- * q_stride, k_stride and v_stride elements apart (multiples of 8; q, k and v 16-byte aligned); an F16 cache's rows, contiguous or
+ * q_stride, k_stride and v_stride elements apart (multiples of 8, those of k and v up to 2^26; q, k and v 16-byte aligned); an F16 cache's rows, contiguous or
  * pages in order, can be k and v.  BF16 rows are multiplied as bf16, the weights rounded to it.  Requests of more than max_len
  * rows are left out, rows behind the last request's are left as they are.  Gate, y, Q8_1 and what is not finite as above. */
 int rmi_gqa_prompt_attn(int type, const void* q, int q_stride, const void* k, int k_stride, const void* v, int v_stride,

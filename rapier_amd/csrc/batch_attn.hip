@@ -76,17 +76,24 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
 
 // The workgroup's tile by its rank among all of the call.  A request's tile at `level` is its rows 128 level ..; tiles go by level,
 // the highest first, since the work grows with it (the prefix a tile sees): the longest start first and the short ones fill the
-// end.  tiles[i] in LDS: request i's number.  False: the call has no such tile.
-__device__ __forceinline__ bool tile_of_rank(const BatchArgs& a, const int* tiles, uint32_t rank, int* req, int* level) {
+// end.  count(i): request i's number of tiles, i < 64 ceil(n_req / 64).  False: the call has no such tile.
+template <typename F>
+__device__ __forceinline__ bool tile_of_rank(const BatchArgs& a, F&& count, uint32_t rank, int* req, int* level) {
     const int lane = threadIdx.x & 63;
     auto above = [&](int l) {   // tiles at level l and higher
         uint32_t s = 0;
-        for (int i = lane; i < a.n_req; i += 64) s += static_cast<uint32_t>(max(tiles[i] - l, 0));
+        for (int i = lane; i < a.n_req; i += 64) s += static_cast<uint32_t>(max(count(i) - l, 0));
         return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(wave_sum(s))));
     };
     if (rank >= above(0)) return false;
     int lo = 0, hi = a.levels;   // above(lo) > rank, above(hi) <= rank (nothing is at the bound)
     uint32_t below = 0;          // above(hi)
+    if (a.n_req == 1) {
+        const int n = __builtin_amdgcn_readfirstlane(count(0));
+        *req = 0;
+        *level = n - 1 - static_cast<int>(rank);
+        return true;
+    }
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         const uint32_t f = above(mid);
@@ -95,7 +102,7 @@ __device__ __forceinline__ bool tile_of_rank(const BatchArgs& a, const int* tile
     }
     uint32_t k = rank - below;   // which of the level's requests, in order
     for (int i0 = 0; i0 < a.n_req; i0 += 64) {
-        const uint64_t has = __ballot(i0 + lane < a.n_req && tiles[min(i0 + lane, a.n_req - 1)] > lo);
+        const uint64_t has = __ballot(i0 + lane < a.n_req && count(min(i0 + lane, a.n_req - 1)) > lo);
         const uint32_t n = __popcll(has);
         if (k < n) {
             uint64_t m = has;
@@ -129,7 +136,9 @@ __device__ __forceinline__ floatx16 mfma32(u32x4 a, u32x4 b, floatx16 c) {
 __device__ __forceinline__ floatx4 mfma16(half8 a, half8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 // ---- results ---------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float gated(float v, float g) { return v / (1.0f + expf(-g)); }
+constexpr float kLog2e = 1.44269504088896340736f;
+// v sigmoid(g): |g| 2^-23 relative from the exponent's rounding, two more roundings
+__device__ __forceinline__ float gated(float v, float g) { return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g)); }
 
 // the Q8_1 block and bits of q8_1_store_lane from a lane's four values of a 32-dim row block whose eight lanes are neighbours
 __device__ __forceinline__ void store_q8_quads(const float (&o)[4], uint8_t* block, int d) {
@@ -158,14 +167,18 @@ __device__ __forceinline__ void load_gate(const BatchArgs& a, int t, int h, int 
     for (int k = 0; k < 4; ++k) g[k] = x[k];
 }
 
-// four dims of a row's result; the lanes of a 32-dim block are eight neighbours.  `none`: the token sees nothing
-template <int HD>
-__device__ __forceinline__ void finish4(const BatchArgs& a, int t, int h, int d, float (&o)[4], float l, bool none, const float (&gate)[4]) {
+// a row's sums over its weights' sum; zeros where the token sees nothing
+__device__ __forceinline__ void normed4(float (&o)[4], float l, bool none) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        o[k] = none ? 0.0f : o[k] / l;
+    for (int k = 0; k < 4; ++k) o[k] = none ? 0.0f : o[k] / l;
+}
+
+// four dims of a row's result; the lanes of a 32-dim block are eight neighbours
+template <int HD>
+__device__ __forceinline__ void finish4(const BatchArgs& a, int t, int h, int d, float (&o)[4], const float (&gate)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
         if (a.gate) o[k] = gated(o[k], gate[k]);
-    }
     if (a.y)
         *reinterpret_cast<uint2*>(a.y + 2 * (static_cast<ptrdiff_t>(t) * a.y_stride + h * HD + d)) =
             make_uint2(pack16(a.bf16, o[0], o[1]), pack16(a.bf16, o[2], o[3]));
@@ -493,7 +506,8 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void batch_few_kern
             v[3] = __builtin_fmaf(x.w, f, v[3]);
         }
         if (a.chunks == 1) {
-            finish4<HD>(a, at, h, d, v, sum[1][r], base + t < 0, g);
+            normed4(v, sum[1][r], base + t < 0);
+            finish4<HD>(a, at, h, d, v, g);
         } else {
             const size_t rec = (static_cast<size_t>(chunk) * a.ntok + at) * a.n_head + h;
             *reinterpret_cast<float4*>(a.wo + rec * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
@@ -516,6 +530,34 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void batch_few_kern
 // K piece c of row p is at c ^ (p % 16), V piece c at c ^ {0, 3, 5, 6}[p % 4].
 constexpr int kPaged = 1, kRowsF16 = 2, kRowsBF16 = 3;   // where K and V come from
 
+// 16 bytes a lane from base + off into LDS: lane l's at `to` + 16 l (base and to uniform).  Written out because the compiler, where
+// it knows of such a load, waits for all of them before any read of LDS; the loop waits for its own, a step later.  Nothing else
+// here uses m0.
+__device__ __forceinline__ void load_lds(const uint8_t* base, uint32_t off, uint32_t to) {
+    const uint64_t b = reinterpret_cast<uintptr_t>(base);
+    const uint64_t u = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b))) |
+                       static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b >> 32)))) << 32;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(static_cast<int>(to))), "v"(off),
+                 "s"(u)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*) p));
+}
+
+// N products, product k of the operand that read(k) brings from LDS, with AHEAD operands on their way: left alone the compiler
+// reads an operand, waits for it and multiplies.  `ready` holds the first ones.
+template <int AHEAD, int N, typename READ, typename PRODUCT>
+__device__ __forceinline__ void stream(u32x4 (&ready)[AHEAD], READ&& read, PRODUCT&& product) {
+    static_assert(N >= AHEAD, "");
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        product(k, ready[k % AHEAD]);
+        if (k + AHEAD < N) ready[k % AHEAD] = read(k + AHEAD);
+        __builtin_amdgcn_sched_barrier(0x6);   // vector and scalar arithmetic alone may pass
+    }
+}
+
 __device__ __forceinline__ int v_swizzle(int p) { return (0x6530 >> (4 * (p & 3))) & 7; }
 
 template <int HD>
@@ -533,6 +575,8 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
     constexpr bool DIRECT_K = KT == kKvF16, DIRECT_V = VT == kKvF16;   // no codes to turn
     constexpr int STEP = S::kStep, ROW = S::kRow, NS = STEP / 32;      // 32-position pieces of a step
     constexpr int NK = HD / 16, ND = HD / 32;
+    constexpr int AHEAD = HD == 256 ? 2 : 4;         // operands from LDS on their way
+    constexpr bool V_EARLY = HD == 128;              // the first of V over the softmax
     constexpr int WR = STEP / kWaves;                // rows of a step that a wave loads
     constexpr int PER = 1024 / ROW, NL = WR / PER;   // rows a direct load, loads a wave
     constexpr int NG = STEP / 16;                    // 16-position pieces, each in one page
@@ -550,15 +594,22 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
     const uint32_t rank = blockIdx.x / a.n_kv / a.chunks;
     int i = 0, level = 0;
     {
-        int* tiles = reinterpret_cast<int*>(pool);
-        for (int k = tid; k < a.n_req; k += kThreads) {
+        auto tiles_of = [&](int k) {
             const int rows = request(a, k, a.row_start[k], a.row_start[k + 1]).n * G;
-            tiles[k] = a.skip_few && rows <= kFewRows ? 0 : (rows + kTileRows - 1) / kTileRows;
-        }
+            return a.skip_few && rows <= kFewRows ? 0 : (rows + kTileRows - 1) / kTileRows;
+        };
         if (tid < 2) odd[tid] = 0;
-        __syncthreads();
-        if (!tile_of_rank(a, tiles, rank, &i, &level)) return;   // uniform
-        __syncthreads();   // read before the first tile overwrites it
+        if (a.n_req <= 64) {   // a request a lane
+            const int mine = tiles_of(min(lane, a.n_req - 1));
+            if (!tile_of_rank(a, [&](int) { return mine; }, rank, &i, &level)) return;   // uniform
+        } else {
+            int* tiles = reinterpret_cast<int*>(pool);
+            for (int k = tid; k < a.n_req; k += kThreads) tiles[k] = tiles_of(k);
+            __syncthreads();
+            const bool has = tile_of_rank(a, [&](int k) { return tiles[k]; }, rank, &i, &level);
+            __syncthreads();   // read before the first tile overwrites it
+            if (!has) return;   // uniform
+        }
     }
     i = __builtin_amdgcn_readfirstlane(i);
     level = __builtin_amdgcn_readfirstlane(level);
@@ -620,9 +671,7 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
         for (int n = 0; n < NL; ++n) {
             const int r = n * PER + lr, p = p0 + r;
             const int piece = k ? c ^ (p & 15) : c ^ (v_swizzle(p) << 1);
-            const size_t off = static_cast<size_t>(min(r, most)) * stride + 16 * piece;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*) (from + off),
-                                             (__attribute__((address_space(3))) void*) (to + (p0 + n * PER) * ROW), 16, 0, 0);
+            load_lds(from, static_cast<uint32_t>(min(r, most)) * static_cast<uint32_t>(stride) + 16 * piece, lds_address(to + (p0 + n * PER) * ROW));
         }
     };
     // a thread's units of codes: unit = position and 16 dims of it
@@ -682,6 +731,12 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
         if constexpr (!DIRECT_V) put(vx, vsc, std::integral_constant<int, VT>{}, to + S::kHalf, false);
     };
 
+    find_pages(c0);
+    if (nsteps > 0) load(0, c0);
+    // q is here before the loop: inside it, a wait for q would be one for the tiles on their way
+#pragma unroll
+    for (int k = 0; k < NK; ++k) asm volatile("" : "+v"(q[k]));
+
     floatx16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -714,8 +769,6 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
         return (w & E) != E && (w & (E << 16)) != (E << 16);
     };
 
-    find_pages(c0);
-    if (nsteps > 0) load(0, c0);
     bad = next_bad;
     find_pages(c0 + STEP);
     turn(0);
@@ -761,13 +814,34 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
         if (sb <= wlast) {   // uniform in the wave
             floatx16 s[NS];
 #pragma unroll
-            for (int j = 0; j < NS; ++j) {
+            for (int j = 0; j < NS; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[j][r] = 0.0f;
+            auto k_piece = [&](int n) {   // dims 16 k .. of positions 32 j ..
+                const int j = n / NK, k = n % NK;
+                return *reinterpret_cast<const u32x4*>(tile + 32 * j * ROW + (kat ^ ((k & 7) << 5)) + (k >> 3) * 256);
+            };
+            const uint8_t* const vt = tile + S::kHalf;
+            auto v_piece = [&](int n) {   // 16 positions 16 k .. of dims 32 d ..
+                const int k = n / ND, d = n % ND;
+                typedef short s16x4 __attribute__((ext_vector_type(4)));
+                typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                const uint8_t* at = vt + 16 * k * ROW + (vat ^ ((d & 3) << 6)) + (d >> 2) * 256;
+                const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*) at));
+                const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*) (at + 8 * ROW)));
+                return u32x4{x.x, x.y, y.x, y.y};
+            };
+            u32x4 ready[AHEAD];
 #pragma unroll
-                for (int k = 0; k < NK; ++k)
-                    s[j] = mfma32<BF>(*reinterpret_cast<const u32x4*>(tile + 32 * j * ROW + (kat ^ ((k & 7) << 5)) + (k >> 3) * 256), q[k], s[j]);
-            }
+            for (int n = 0; n < AHEAD; ++n) ready[n] = k_piece(n);
+            __builtin_amdgcn_sched_barrier(0x6);
+            stream<AHEAD, NS * NK>(ready, k_piece, [&](int n, u32x4 x) { s[n / NK] = mfma32<BF>(x, q[n % NK], s[n / NK]); });
+            auto v_first = [&] {
+#pragma unroll
+                for (int n = 0; n < AHEAD; ++n) ready[n] = v_piece(n);
+                __builtin_amdgcn_sched_barrier(0x6);
+            };
+            if constexpr (V_EARLY) v_first();
             if (step_bad)
 #pragma unroll
                 for (int j = 0; j < NS; ++j)
@@ -809,7 +883,6 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
             }
-            const uint8_t* const vt = tile + S::kHalf;
             if (tail && odd[buf] == st + 1) {   // uniform
                 for (int pp = 0; pp < STEP; ++pp) {
                     const int at = sb + pp;
@@ -849,17 +922,8 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
                     }
                 }
             }
-#pragma unroll
-            for (int k = 0; k < 2 * NS; ++k)   // 16 positions
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    typedef short s16x4 __attribute__((ext_vector_type(4)));
-                    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-                    const uint8_t* at = vt + 16 * k * ROW + (vat ^ ((d & 3) << 6)) + (d >> 2) * 256;
-                    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*) at));
-                    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*) (at + 8 * ROW)));
-                    o[d] = mfma32<BF>(u32x4{x.x, x.y, y.x, y.y}, p[k], o[d]);
-                }
+            if constexpr (!V_EARLY) v_first();
+            stream<AHEAD, 2 * NS * ND>(ready, v_piece, [&](int n, u32x4 x) { o[n % ND] = mfma32<BF>(x, p[n / ND], o[n % ND]); });
         }
         if (more) turn(buf ^ 1);
     }
@@ -869,54 +933,70 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
     const int t = rq.start + tok;
     if (a.chunks > 1) {
         const size_t rec = (static_cast<size_t>(chunk) * a.ntok + t) * a.n_head + head;
+        float* const to = a.wo + rec * HD + 4 * h;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int r = 0; r < 16; r += 4)
-                *reinterpret_cast<float4*>(a.wo + rec * HD + 32 * d + 2 * r + 4 * h) =
+                *reinterpret_cast<float4*>(to + 32 * d + 2 * r) =
                     make_float4(o[d][r] * kSixteen<VT>, o[d][r + 1] * kSixteen<VT>, o[d][r + 2] * kSixteen<VT>, o[d][r + 3] * kSixteen<VT>);
         if (h == 0) *reinterpret_cast<float2*>(a.wml + 2 * rec) = make_float2(m_run, l_run);
         return;
     }
+    // the lane's half of its row, from its registers.  Gates four 32-dim blocks ahead: one block's at a time would wait for memory
+    // eight times over (3 us each way at a workgroup's end)
+    const float unit = kSixteen<VT> / l_run;
+    constexpr int BLOCKS = 4;
+    const float* const from = a.gate ? a.gate + static_cast<ptrdiff_t>(t) * a.gate_stride + head * 2 * HD + HD + 4 * h : nullptr;
+    float4u g[BLOCKS][4];
+    auto block = [&](int d) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[d % BLOCKS][e] = *reinterpret_cast<const float4u*>(from + 32 * d + 8 * e);
+    };
+    if (from) {
+#pragma unroll
+        for (int d = 0; d < BLOCKS; ++d) block(d);
+    }
+    uint16_t* const to = reinterpret_cast<uint16_t*>(a.y) + static_cast<ptrdiff_t>(t) * a.y_stride + head * HD + 4 * h;
+    uint8_t* const to8 = a.q8 + static_cast<ptrdiff_t>(t) * a.q8_stride + head * ND * kQ8_1Bytes;
+    const bool out_bf = PAGED ? a.bf16 : BF;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
         float v[16];
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            float g[4];
-            load_gate<HD>(a, t, head, 32 * d + 2 * r + 4 * h, g);
+        for (int r = 0; r < 16; ++r) v[r] = lim < 0 ? 0.0f : o[d][r] * unit;
+        if (from) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[r + e] = lim < 0 ? 0.0f : o[d][r + e] * kSixteen<VT> / l_run;
-                if (a.gate) v[r + e] = gated(v[r + e], g[e]);
-            }
-            if (a.y)
-                *reinterpret_cast<uint2*>(a.y + 2 * (static_cast<ptrdiff_t>(t) * a.y_stride + head * HD + 32 * d + 2 * r + 4 * h)) =
-                    make_uint2(pack16(PAGED ? a.bf16 : BF, v[r], v[r + 1]), pack16(PAGED ? a.bf16 : BF, v[r + 2], v[r + 3]));
+            for (int r = 0; r < 16; ++r) v[r] = gated(v[r], g[d % BLOCKS][r >> 2][r & 3]);
+            if (d + BLOCKS < ND) block(d + BLOCKS);
         }
+        if (a.y)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4)
+                *reinterpret_cast<uint2*>(to + 32 * d + 2 * r) = make_uint2(pack16(out_bf, v[r], v[r + 1]), pack16(out_bf, v[r + 2], v[r + 3]));
         if (a.q8) {   // q8_1_store_lane's block and bits: a lane has elements 8 (r / 4) + 4 h + r % 4
             float amax = 0.0f, s[8];
 #pragma unroll
             for (int r = 0; r < 16; ++r) amax = fmaxf(amax, fabsf(v[r]));
             amax = fmaxf(amax, xor_lane<32>(amax));
 #pragma unroll
-            for (int r = 0; r < 8; ++r) s[r] = v[r] + v[r + 8];   // lane ^ 16
+            for (int r = 0; r < 8; ++r) s[r] = v[r] + v[r + 8];   // element ^ 16
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 s[r] += s[r + 4];               // ^ 8
                 s[r] += xor_lane<32>(s[r]);     // ^ 4
             }
             const float total = (s[0] + s[2]) + (s[1] + s[3]), dq = amax / 127.0f;
-            uint8_t* block = a.q8 + static_cast<ptrdiff_t>(t) * a.q8_stride + (head * ND + d) * kQ8_1Bytes;
+            uint8_t* const blk = to8 + d * kQ8_1Bytes;
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 uint32_t w = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     w |= (static_cast<uint32_t>(amax == 0.0f ? 0 : static_cast<int>(roundf(v[r + e] / dq))) & 0xffu) << (8 * e);
-                *reinterpret_cast<uint32_t*>(block + 4 + 2 * r + 4 * h) = w;
+                *reinterpret_cast<uint32_t*>(blk + 4 + 2 * r + 4 * h) = w;
             }
-            if (h == 0) *reinterpret_cast<uint32_t*>(block) = float_to_half_sat(dq) | (float_to_half_sat(total) << 16);
+            if (h == 0) *reinterpret_cast<uint32_t*>(blk) = float_to_half_sat(dq) | (float_to_half_sat(total) << 16);
         }
     }
 }
@@ -978,7 +1058,8 @@ __global__ __launch_bounds__(kThreads) void batch_join_flat_kernel(BatchArgs a) 
         o[2] = __builtin_fmaf(w, v.z, o[2]);
         o[3] = __builtin_fmaf(w, v.w, o[3]);
     }
-    finish4<HD>(a, t, h, d, o, l, none, g);
+    normed4(o, l, none);
+    finish4<HD>(a, t, h, d, o, g);
 }
 
 // Many chunks: workgroup (row, 64 dims); weights to LDS, wave w sums chunks w, w + 4, ... in order, then the waves in order.
@@ -1109,7 +1190,8 @@ void set_outputs(BatchArgs* a, const Outputs& o) {
     a->q8_stride = o.q8_stride;
 }
 
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kMaxStride = 1 << 26;   // a step's rows are within 32 bits of its first
+
 constexpr long long kMostBlocks = 0xffffffffLL / kThreads;
 
 template <int KT, int VT, int HD>
@@ -1228,8 +1310,8 @@ extern "C" int rmi_gqa_prompt_attn(int type, const void* q, int q_stride, const 
                                    void* stream) {
     if (type != RMI_ROWS_F16 && type != RMI_ROWS_BF16) return fail(RMI_ERR_UNSUPPORTED, "gqa_prompt_attn: rows of F16 or BF16");
     if (!heads_ok(n_head, n_kv, head_dim) || !batch_ok(n_req, ntok, max_len) || !(scale > 0.0f && scale <= FLT_MAX) || q_stride % 8 || k_stride % 8 ||
-        v_stride % 8 || (ntok > 1 && (q_stride < n_head * head_dim || k_stride < n_kv * head_dim || v_stride < n_kv * head_dim)))
-        return fail(RMI_ERR_SHAPE, "gqa_prompt_attn: invalid arguments (strides are multiples of 8 elements)");
+        v_stride % 8 || k_stride > kMaxStride || v_stride > kMaxStride || (ntok > 1 && (q_stride < n_head * head_dim || k_stride < n_kv * head_dim || v_stride < n_kv * head_dim)))
+        return fail(RMI_ERR_SHAPE, "gqa_prompt_attn: invalid arguments (strides are multiples of 8 elements, up to 2^26)");
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned4(row_start))
         return fail(RMI_ERR_POINTER, "gqa_prompt_attn: null or misaligned pointer");
     const Outputs out{gate_src, gate_stride, y, y_stride, q8, q8_stride};
