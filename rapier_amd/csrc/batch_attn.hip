@@ -28,7 +28,8 @@ typedef float floatx2 __attribute__((ext_vector_type(2)));
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kFewRows = 16;
-constexpr int kTileRows = 128, kWaveRows = 32;
+constexpr int kWaveRows = 32;      // of a wave of the form of more rows
+constexpr int kTileRows = 128;     // rows of four such waves, the unit of a split
 constexpr int kChunkUnit = 128;    // a chunk is a whole number of them
 constexpr int kMaxChunks = 1024;   // named in the messages
 constexpr float kPScale = 8.0f;    // p goes as 2^8 p: fp16's subnormals begin 2^-22 below a row's maximum
@@ -517,7 +518,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void batch_few_kern
 }
 
 // ---- more rows: tiles in LDS -------------------------------------------------------------------------------------------------
-// Four waves of 32 query rows over steps of STEP positions, v_mfma_f32_32x32x16: lane l32 = l % 32, h = l / 32; A rows, B and D
+// WAVES waves of 32 query rows over steps of STEP positions, v_mfma_f32_32x32x16: lane l32 = l % 32, h = l / 32; A rows, B and D
 // columns are l32; A and B hold k = 8 h + 0..7; D register r is row 8 (r / 4) + 4 h + r % 4.
 //   scores    D[position][row] += K[position][dims] . q_row[dims]: a lane has half of its row's scores, so a row's maximum and sum
 //             take one exchange with lane l ^ 32, and what scales a row is a lane's own value
@@ -525,7 +526,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void batch_few_kern
 //             (h, e) of 16 positions is position 8 (e / 4) + 4 h + e % 4, and V's transposed reads (ds_read_b64_tr_b16: 16 lanes
 //             give the addresses of 4 positions x 16 dims and get a dim's four positions each) take the same order.
 // q and o stay in registers.  16-bit K and V go from memory into LDS without passing registers, the next step's over this step's
-// products; codes are turned to fp16 on the way.  LDS rows have no padding (the direct loads write 1024 bytes in a row);
+// products; codes go there as they are, two steps ahead, and are turned to fp16 tiles by the next step.  LDS rows have no padding (the direct loads write 1024 bytes in a row);
 // instead their 16-byte (K) or 32-byte (V) pieces are permuted by the row, so that the lanes of a read fall on different banks:
 // K piece c of row p is at c ^ (p % 16), V piece c at c ^ {0, 3, 5, 6}[p % 4].
 constexpr int kPaged = 1, kRowsF16 = 2, kRowsBF16 = 3;   // where K and V come from
@@ -540,6 +541,10 @@ __device__ __forceinline__ void load_lds(const uint8_t* base, uint32_t off, uint
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(static_cast<int>(to))), "v"(off),
                  "s"(u)
                  : "memory");
+}
+// the same for four bytes a lane, each lane's from a place of its own
+__device__ __forceinline__ void load_lds4(const uint8_t* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(static_cast<int>(to))), "v"(from) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*) p));
@@ -558,6 +563,13 @@ __device__ __forceinline__ void stream(u32x4 (&ready)[AHEAD], READ&& read, PRODU
     }
 }
 
+// the same value, of which the compiler does not know that a loop leaves it as it is: what is made of it then is made anew in each
+// round, by an instruction or two, and not kept in registers that there are none of
+__device__ __forceinline__ int fresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 __device__ __forceinline__ int v_swizzle(int p) { return (0x6530 >> (4 * (p & 3))) & 7; }
 
 template <int HD>
@@ -568,22 +580,24 @@ struct TileShape {
     static constexpr int kTile = 2 * kHalf;
 };
 
-template <int SRC, int KT, int VT, int HD>
-__global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
+template <int SRC, int KT, int VT, int HD, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) {
     using S = TileShape<HD>;
+    constexpr int THREADS = 64 * WAVES, ROWS = kWaveRows * WAVES;   // query rows of a workgroup
     constexpr bool BF = SRC == kRowsBF16, PAGED = SRC == kPaged;
-    constexpr bool DIRECT_K = KT == kKvF16, DIRECT_V = VT == kKvF16;   // no codes to turn
+    constexpr bool CODES = KT != kKvF16;             // K and V are codes to be turned to fp16 (both or neither)
+    constexpr int LEAD = CODES ? 2 : 1;              // steps that loads are ahead
     constexpr int STEP = S::kStep, ROW = S::kRow, NS = STEP / 32;      // 32-position pieces of a step
     constexpr int NK = HD / 16, ND = HD / 32;
     constexpr int AHEAD = HD == 256 ? 2 : 4;         // operands from LDS on their way
     constexpr bool V_EARLY = HD == 128;              // the first of V over the softmax
-    constexpr int WR = STEP / kWaves;                // rows of a step that a wave loads
+    constexpr int WR = STEP / WAVES;                // rows of a step that a wave loads
     constexpr int PER = 1024 / ROW, NL = WR / PER;   // rows a direct load, loads a wave
     constexpr int NG = STEP / 16;                    // 16-position pieces, each in one page
-    constexpr int NU = STEP * (HD / 16) / kThreads;  // 16-dim units a thread turns
     constexpr int NB = HD / kKvBlock;
     constexpr int kKB = kv_row_bytes(KT, HD), kVB = kv_row_bytes(VT, HD);
-    __shared__ __attribute__((aligned(16))) uint8_t pool[2 * S::kTile];
+    constexpr int RAW = STEP * (kKB + kVB + 2 * NB);   // a step's codes and scales
+    __shared__ __attribute__((aligned(16))) uint8_t pool[2 * S::kTile + (CODES ? 2 * RAW : 0)];
     __shared__ int odd[2];   // a tile's V had a value that is not finite
     static_assert(sizeof(pool) >= kMaxReq * sizeof(int), "the requests' tiles are counted in the tiles' place");
 
@@ -596,7 +610,7 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
     {
         auto tiles_of = [&](int k) {
             const int rows = request(a, k, a.row_start[k], a.row_start[k + 1]).n * G;
-            return a.skip_few && rows <= kFewRows ? 0 : (rows + kTileRows - 1) / kTileRows;
+            return a.skip_few && rows <= kFewRows ? 0 : (rows + ROWS - 1) / ROWS;
         };
         if (tid < 2) odd[tid] = 0;
         if (a.n_req <= 64) {   // a request a lane
@@ -604,7 +618,7 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
             if (!tile_of_rank(a, [&](int) { return mine; }, rank, &i, &level)) return;   // uniform
         } else {
             int* tiles = reinterpret_cast<int*>(pool);
-            for (int k = tid; k < a.n_req; k += kThreads) tiles[k] = tiles_of(k);
+            for (int k = tid; k < a.n_req; k += THREADS) tiles[k] = tiles_of(k);
             __syncthreads();
             const bool has = tile_of_rank(a, [&](int k) { return tiles[k]; }, rank, &i, &level);
             __syncthreads();   // read before the first tile overwrites it
@@ -615,9 +629,9 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
     level = __builtin_amdgcn_readfirstlane(level);
     const Req rq = request(a, i, word(a.row_start, i), word(a.row_start, i + 1));
     const int rows = rq.n * G, base = rq.len - rq.n, c0 = chunk * a.chunk;
-    const int first = base + level * kTileRows / G, last = base + min(level * kTileRows + kTileRows - 1, rows - 1) / G;   // of the workgroup's tokens
+    const int first = base + level * ROWS / G, last = base + min(level * ROWS + ROWS - 1, rows - 1) / G;   // of the workgroup's tokens
     if (chunk > 0 && c0 > last) return;
-    const int row0 = level * kTileRows + kWaveRows * wv, row = row0 + l32, rowc = min(row, rows - 1), tok = rowc / G;
+    const int row0 = level * ROWS + kWaveRows * wv, row = row0 + l32, rowc = min(row, rows - 1), tok = rowc / G;
     const int head = kv * G + rowc - tok * G;
     const int lim = row < rows ? base + tok : -1;   // the row sees every position up to here
     const int wfirst = base + min(row0, rows - 1) / G, wlast = row0 < rows ? base + min(row0 + kWaveRows - 1, rows - 1) / G : -1;
@@ -633,11 +647,11 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
     const int size = 1 << a.shift;
     const size_t kpage = kv_page_bytes(KT, size, a.n_kv, HD), vpage = kv_page_bytes(VT, size, a.n_kv, HD);
     // bytes from a position's row to the next
-    const size_t kstride = !PAGED ? 2 * static_cast<size_t>(a.k_stride) : DIRECT_K ? static_cast<size_t>(a.n_kv) * kKB : kKB;
-    const size_t vstride = !PAGED ? 2 * static_cast<size_t>(a.v_stride) : DIRECT_V ? static_cast<size_t>(a.n_kv) * kVB : kVB;
+    const size_t kstride = !PAGED ? 2 * static_cast<size_t>(a.k_stride) : !CODES ? static_cast<size_t>(a.n_kv) * kKB : kKB;
+    const size_t vstride = !PAGED ? 2 * static_cast<size_t>(a.v_stride) : !CODES ? static_cast<size_t>(a.n_kv) * kVB : kVB;
     const int* const ids = a.table + static_cast<size_t>(i) * a.table_stride;
     int id[NG];       // pages of the step that is loaded next
-    uint32_t bad = 0, next_bad = 0;   // of its 16-position pieces: not a page
+    uint32_t next_bad = 0;   // of its 16-position pieces: not a page
     auto find_pages = [&](int sb) {
         next_bad = 0;
         if constexpr (PAGED) {
@@ -651,88 +665,117 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
             }
         }
     };
-    // rows of 16-bit values straight into LDS: lane l writes piece l % (ROW / 16) of row l / (ROW / 16)
-    auto direct = [&](const uint8_t* src, size_t page_bytes, size_t stride, size_t at0, int sb, uint8_t* to, bool k) {
-        constexpr int PIECES = ROW / 16;
-        const int p0 = WR * wv, lr = lane / PIECES, c = lane % PIECES;
+    // Rows of 16-bit values straight into LDS: a load's lane l writes piece l % PIECES of its row l / PIECES.  Both permutations are
+    // exclusive ors and linear in the row, so the n-th load's piece is the first's with a constant.
+    constexpr int PIECES = ROW / 16;
+    const int p0 = WR * wv, lr = lane / PIECES;
+    const uint32_t k_piece0 = 16 * (lane % PIECES ^ ((p0 + lr) & 15)), v_piece0 = 16 * (lane % PIECES ^ (v_swizzle(lr) << 1));
+    const uint32_t k_row = static_cast<uint32_t>(lr) * static_cast<uint32_t>(kstride), v_row = static_cast<uint32_t>(lr) * static_cast<uint32_t>(vstride);
+    auto direct = [&](const uint8_t* src, size_t page_bytes, size_t stride, size_t at0, int sb, uint32_t to, bool k) {
+        const uint32_t piece0 = fresh(k ? k_piece0 : v_piece0);
         const uint8_t* from;
-        int most = WR - 1;   // the last row that may be read
+        int over = 0;   // how many of the wave's rows lie behind the call's (prompts: the last step of the last rows)
         if constexpr (PAGED) {
             int page = id[0];
 #pragma unroll
             for (int g = 1; g < NG; ++g) page = p0 / 16 == g ? id[g] : page;
             from = src + static_cast<size_t>(page) * page_bytes + at0 + ((sb + p0) & (size - 1)) * stride;
         } else {
-            const int p = min(sb + p0, last);
-            most = min(most, last - p);
-            from = src + (static_cast<size_t>(rq.start) + p) * stride + at0;
+            const int r = min(rq.start + sb + p0, a.ntok - 1);
+            over = r + WR - a.ntok;
+            from = src + static_cast<size_t>(r) * stride + at0;
         }
 #pragma unroll
         for (int n = 0; n < NL; ++n) {
-            const int r = n * PER + lr, p = p0 + r;
-            const int piece = k ? c ^ (p & 15) : c ^ (v_swizzle(p) << 1);
-            load_lds(from, static_cast<uint32_t>(min(r, most)) * static_cast<uint32_t>(stride) + 16 * piece, lds_address(to + (p0 + n * PER) * ROW));
-        }
-    };
-    // a thread's units of codes: unit = position and 16 dims of it
-    constexpr int UP = kThreads / (HD / 16);   // positions to a thread's next unit
-    const int upos = tid / (HD / 16), ucol = tid % (HD / 16);
-    Dims16<KT> kx[DIRECT_K ? 1 : NU];
-    Dims16<VT> vx[DIRECT_V ? 1 : NU];
-    uint32_t ksc[DIRECT_K ? 1 : NU], vsc[DIRECT_V ? 1 : NU];
-    auto fetch = [&](auto& x, auto& sc, const uint8_t* src, size_t page_bytes, auto type, int sb) {
-        constexpr int T = decltype(type)::value;
-        constexpr int B = kv_row_bytes(T, HD);
-        const KvRow<T> r0 = kv_row<T>(0, kv, a.n_kv, size, HD);
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            const int p = upos + u * UP, off = (sb + p) & (size - 1);
-            int page = id[0];
-#pragma unroll
-            for (int g = 1; g < NG; ++g) page = p / 16 == g ? id[g] : page;
-            const uint8_t* pg = src + static_cast<size_t>(page) * page_bytes;
-            const uint8_t* code = pg + r0.code + static_cast<size_t>(off) * B + ucol * (B / (HD / 16));
-            if constexpr (T == kKvI8) {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(code);
-                x[u].w[0] = v[0], x[u].w[1] = v[1], x[u].w[2] = v[2], x[u].w[3] = v[3];
-            } else if constexpr (T == kKvI4) {
-                const uint2 v = *reinterpret_cast<const uint2*>(code);
-                x[u].w[0] = v.x, x[u].w[1] = v.y;
-            }
-            sc[u] = pg[r0.scale + static_cast<size_t>(off) * NB + ucol / 2];
-        }
-    };
-    auto put = [&](auto& x, auto& sc, auto type, uint8_t* to, bool k) {
-        constexpr int T = decltype(type)::value;
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            const int p = upos + u * UP;
-            const Scale2 s = scale2<T>(sc[u], sc[u]);
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int piece = 2 * ucol + hf, at = k ? piece ^ (p & 15) : piece ^ (v_swizzle(p) << 1);
-                *reinterpret_cast<half8*>(to + p * ROW + 16 * at) = operand<T>(x[u], hf, s);
-            }
+            const uint32_t piece = piece0 ^ (k ? 16 * (n * PER & 15) : 32 * v_swizzle(n * PER));
+            const uint32_t lds = to + (p0 + n * PER) * ROW;
+            if (over <= 0) load_lds(from + n * PER * stride, (k ? k_row : v_row) + piece, lds);
+            else load_lds(from, static_cast<uint32_t>(min(n * PER + lr, WR - 1 - over)) * static_cast<uint32_t>(stride) + piece, lds);
         }
     };
     const size_t k_at = PAGED ? kv_row<KT>(0, kv, a.n_kv, size, HD).code : static_cast<size_t>(kv) * ROW;
     const size_t v_at = PAGED ? kv_row<VT>(0, kv, a.n_kv, size, HD).code : static_cast<size_t>(kv) * ROW;
-    // a step's rows on their way: into LDS, or codes into registers
+    const uint32_t pool0 = lds_address(pool);
+    // Codes and their scales into LDS as they are: rows of a page lie one behind another, so a wave's 1024 bytes are in a row.
+    // Waves take K's and V's codes in turn, the first two the scales.
+    auto raw_codes = [&](const uint8_t* src, size_t page_bytes, size_t at0, auto type, int sb, uint32_t to, int turn) {
+        constexpr int B = kv_row_bytes(decltype(type)::value, HD), R = 1024 / B;   // rows a load
+        static_assert(R <= 16, "within a page's 16");
+        if (turn >= STEP / R) return;   // uniform
+        const int p = turn * R;
+        int page = id[0];
+#pragma unroll
+        for (int g = 1; g < NG; ++g) page = p / 16 == g ? id[g] : page;
+        load_lds(src + static_cast<size_t>(page) * page_bytes + at0 + static_cast<size_t>((sb + p) & (size - 1)) * B, 16 * lane, to + 1024 * turn);
+    };
+    auto raw_scales = [&](const uint8_t* src, size_t page_bytes, size_t at0, int sb, uint32_t to) {
+        const int l = fresh(lane), p = 4 * l / NB;   // the lane's four bytes
+        int page = id[0];
+#pragma unroll
+        for (int g = 1; g < NG; ++g) page = p / 16 == g ? id[g] : page;
+        load_lds4(src + static_cast<size_t>(page) * page_bytes + at0 + static_cast<size_t>((sb + p) & (size - 1)) * NB + (4 * l) % NB, to);
+    };
+    // a step's rows on their way, to tile or raw buffer `buf`
     auto load = [&](int buf, int sb) {
-        uint8_t* to = pool + buf * S::kTile;
-        if constexpr (DIRECT_K) direct(a.k, kpage, kstride, k_at, sb, to, true);
-        else fetch(kx, ksc, a.k, kpage, std::integral_constant<int, KT>{}, sb);
-        if constexpr (DIRECT_V) direct(a.v, vpage, vstride, v_at, sb, to + S::kHalf, false);
-        else fetch(vx, vsc, a.v, vpage, std::integral_constant<int, VT>{}, sb);
+        if constexpr (CODES) {
+            const uint32_t to = pool0 + 2 * S::kTile + buf * RAW;
+#pragma unroll
+            for (int n = 0; n < S::kHalf / 2 / (1024 * WAVES); ++n) {   // as many as rows of eight bits take
+                raw_codes(a.k, kpage, k_at, std::integral_constant<int, KT>{}, sb, to, wv + n * WAVES);
+                raw_codes(a.v, vpage, v_at, std::integral_constant<int, VT>{}, sb, to + STEP * kKB, wv + n * WAVES);
+            }
+            if (wv == 0) raw_scales(a.k, kpage, kv_row<KT>(0, kv, a.n_kv, size, HD).scale, sb, to + STEP * (kKB + kVB));
+            if (wv == 1) raw_scales(a.v, vpage, kv_row<VT>(0, kv, a.n_kv, size, HD).scale, sb, to + STEP * (kKB + kVB + NB));
+        } else {
+            const uint32_t to = pool0 + buf * S::kTile;
+            direct(a.k, kpage, kstride, k_at, sb, to, true);
+            direct(a.v, vpage, vstride, v_at, sb, to + S::kHalf, false);
+        }
+    };
+    // raw buffer `buf` to tile `buf`: a thread turns 16 dims of a position at a time
+    auto turn_rows = [&](auto type, const uint8_t* codes, const uint8_t* scales, uint8_t* to, bool k) {
+        constexpr int T = decltype(type)::value;
+        constexpr int UP = THREADS / (HD / 16);   // positions to a thread's next unit
+        const int t = fresh(tid), pos = t / (HD / 16), col = t % (HD / 16);
+#pragma unroll
+        for (int u = 0; u < STEP / UP; ++u) {
+            const int p = pos + u * UP;
+            Dims16<T> x;
+            if constexpr (T == kKvI8) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(codes + p * HD + 16 * col);
+                x.w[0] = v[0], x.w[1] = v[1], x.w[2] = v[2], x.w[3] = v[3];
+            } else if constexpr (T == kKvI4) {
+                const uint2 v = *reinterpret_cast<const uint2*>(codes + p * (HD / 2) + 8 * col);
+                x.w[0] = v.x, x.w[1] = v.y;
+            }
+            const uint32_t sc = scales[p * NB + col / 2];
+            const Scale2 s = scale2<T>(sc, sc);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const int piece = 2 * col + hf, at = k ? piece ^ (p & 15) : piece ^ (v_swizzle(p) << 1);
+                *reinterpret_cast<half8*>(to + p * ROW + 16 * at) = operand<T>(x, hf, s);
+            }
+        }
     };
     auto turn = [&](int buf) {
-        uint8_t* to = pool + buf * S::kTile;
-        if constexpr (!DIRECT_K) put(kx, ksc, std::integral_constant<int, KT>{}, to, true);
-        if constexpr (!DIRECT_V) put(vx, vsc, std::integral_constant<int, VT>{}, to + S::kHalf, false);
+        if constexpr (CODES) {
+            const uint8_t* from = pool + 2 * S::kTile + buf * RAW;
+            uint8_t* to = pool + buf * S::kTile;
+            const uint8_t* scales = from + STEP * (kKB + kVB);
+            turn_rows(std::integral_constant<int, KT>{}, from, scales, to, true);
+            turn_rows(std::integral_constant<int, VT>{}, from + STEP * kKB, scales + STEP * NB, to + S::kHalf, false);
+        }
     };
 
     find_pages(c0);
     if (nsteps > 0) load(0, c0);
+    uint32_t bad = next_bad, bad2 = 0;   // of this step and the next
+    find_pages(c0 + STEP);
+    if constexpr (CODES) {   // codes come two steps ahead
+        if (nsteps > 1) load(1, c0 + STEP);
+        bad2 = next_bad;
+        find_pages(c0 + 2 * STEP);
+    }
     // q is here before the loop: inside it, a wait for q would be one for the tiles on their way
 #pragma unroll
     for (int k = 0; k < NK; ++k) asm volatile("" : "+v"(q[k]));
@@ -769,9 +812,12 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
         return (w & E) != E && (w & (E << 16)) != (E << 16);
     };
 
-    bad = next_bad;
-    find_pages(c0 + STEP);
-    turn(0);
+    if constexpr (CODES) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        turn(0);
+    }
     for (int st = 0; st < nsteps; ++st) {
         const int sb = c0 + st * STEP, buf = st & 1;
         const uint8_t* const tile = pool + buf * S::kTile;
@@ -780,11 +826,12 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
         __builtin_amdgcn_s_barrier();   // this step's tile is there, and the other one is read
         asm volatile("" ::: "memory");
         const uint32_t step_bad = bad;
-        if (more) {
-            load(buf ^ 1, sb + STEP);
-            bad = next_bad;
-            find_pages(sb + 2 * STEP);
-        }
+        if (st + LEAD < nsteps) load(CODES ? buf : buf ^ 1, sb + LEAD * STEP);
+        bad = CODES ? bad2 : next_bad;
+        bad2 = next_bad;
+        find_pages(sb + (LEAD + 1) * STEP);
+        // half of the waves turn the next step's codes before their products, half after: a SIMD has one of each
+        if (CODES && more && wv >= WAVES / 2) turn(buf ^ 1);
         const bool tail = sb + STEP - 1 > first;   // uniform: not every row sees the whole step
         if (tail) {
             // what is not finite leaves V's tile, so that a product with a masked zero is zero, and is added by itself to the rows
@@ -792,8 +839,8 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
             uint8_t* const vt = pool + buf * S::kTile + S::kHalf;
             bool found = false;
 #pragma unroll
-            for (int n = 0; n < S::kHalf / (16 * kThreads); ++n) {
-                u32x4* at = reinterpret_cast<u32x4*>(vt + 16 * (tid + n * kThreads));
+            for (int n = 0; n < S::kHalf / (16 * THREADS); ++n) {
+                u32x4* at = reinterpret_cast<u32x4*>(vt + 16 * (tid + n * THREADS));
                 u32x4 w = *at;
                 if (!(finite(w[0]) && finite(w[1]) && finite(w[2]) && finite(w[3]))) {
                     constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
@@ -817,16 +864,17 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
             for (int j = 0; j < NS; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[j][r] = 0.0f;
+            const int ka = fresh(kat), va = fresh(vat);
             auto k_piece = [&](int n) {   // dims 16 k .. of positions 32 j ..
                 const int j = n / NK, k = n % NK;
-                return *reinterpret_cast<const u32x4*>(tile + 32 * j * ROW + (kat ^ ((k & 7) << 5)) + (k >> 3) * 256);
+                return *reinterpret_cast<const u32x4*>(tile + 32 * j * ROW + (ka ^ ((k & 7) << 5)) + (k >> 3) * 256);
             };
             const uint8_t* const vt = tile + S::kHalf;
             auto v_piece = [&](int n) {   // 16 positions 16 k .. of dims 32 d ..
                 const int k = n / ND, d = n % ND;
                 typedef short s16x4 __attribute__((ext_vector_type(4)));
                 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-                const uint8_t* at = vt + 16 * k * ROW + (vat ^ ((d & 3) << 6)) + (d >> 2) * 256;
+                const uint8_t* at = vt + 16 * k * ROW + (va ^ ((d & 3) << 6)) + (d >> 2) * 256;
                 const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*) at));
                 const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*) (at + 8 * ROW)));
                 return u32x4{x.x, x.y, y.x, y.y};
@@ -835,7 +883,9 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
 #pragma unroll
             for (int n = 0; n < AHEAD; ++n) ready[n] = k_piece(n);
             __builtin_amdgcn_sched_barrier(0x6);
+            __builtin_amdgcn_s_setprio(1);
             stream<AHEAD, NS * NK>(ready, k_piece, [&](int n, u32x4 x) { s[n / NK] = mfma32<BF>(x, q[n % NK], s[n / NK]); });
+            __builtin_amdgcn_s_setprio(0);
             auto v_first = [&] {
 #pragma unroll
                 for (int n = 0; n < AHEAD; ++n) ready[n] = v_piece(n);
@@ -914,7 +964,7 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
                         for (int r = 0; r < 16; ++r) {
                             const int dim = 32 * d + 8 * (r >> 2) + 4 * h + (r & 3);
                             float v;
-                            if constexpr (!DIRECT_V) v = odd_value<VT>(vr[scale + d]);
+                            if constexpr (CODES) v = odd_value<VT>(vr[scale + d]);
                             else if constexpr (BF) v = __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(vr)[dim]) << 16);
                             else v = half_bits_to_float(reinterpret_cast<const uint16_t*>(vr)[dim]);
                             if (!(fabsf(v) <= FLT_MAX) && at <= lim) o[d][r] = __builtin_fmaf(x, v, o[d][r]);
@@ -923,9 +973,11 @@ __global__ __launch_bounds__(kThreads, 2) void batch_tile_kernel(BatchArgs a) {
                 }
             }
             if constexpr (!V_EARLY) v_first();
+            __builtin_amdgcn_s_setprio(1);
             stream<AHEAD, 2 * NS * ND>(ready, v_piece, [&](int n, u32x4 x) { o[n % ND] = mfma32<BF>(x, p[n / ND], o[n % ND]); });
+            __builtin_amdgcn_s_setprio(0);
         }
-        if (more) turn(buf ^ 1);
+        if (CODES && more && wv < WAVES / 2) turn(buf ^ 1);
     }
 
     l_run += xor_lane<32>(l_run);
@@ -1139,10 +1191,12 @@ bool batch_ok(int n_req, int ntok, int max_new) { return n_req >= 1 && n_req <= 
 int chunks_of(int max_ctx, int split) { return static_cast<int>((static_cast<long long>(max_ctx) + split - 1) / split); }
 bool split_ok(int max_ctx, int split) { return split >= kChunkUnit && split % kChunkUnit == 0 && chunks_of(max_ctx, split) <= kMaxChunks; }
 
-// the most tiles of rows that n_req requests of ntok tokens in all can have
-long long most_tiles(int n_req, int ntok, int max_new, int G) {
-    const long long rows = static_cast<long long>(ntok) * G, each = (static_cast<long long>(std::min(max_new, ntok)) * G + kTileRows - 1) / kTileRows;
-    return std::min(rows / kTileRows + n_req, each * n_req);
+// tiles of `held` rows: the most that a request of max_new tokens has, and that n_req requests of ntok tokens in all have
+int most_levels(int ntok, int max_new, int G, int held) {
+    return static_cast<int>((static_cast<long long>(std::min(max_new, ntok)) * G + held - 1) / held);
+}
+long long most_tiles(int n_req, int ntok, int max_new, int G, int held) {
+    return std::min(static_cast<long long>(ntok) * G / held + n_req, static_cast<long long>(most_levels(ntok, max_new, G, held)) * n_req);
 }
 
 struct Outputs {
@@ -1194,9 +1248,14 @@ constexpr int kMaxStride = 1 << 26;   // a step's rows are within 32 bits of its
 
 constexpr long long kMostBlocks = 0xffffffffLL / kThreads;
 
+// waves of a tile's workgroup
+constexpr int kPromptWaves = 4;
+constexpr int tile_waves(int ktype) { return ktype == kKvF16 ? 4 : 8; }
+
 template <int KT, int VT, int HD>
 void launch_paged(const BatchArgs& a, bool tiles, long long few_blocks, long long tile_blocks, hipStream_t s) {
-    if (tiles) hipLaunchKernelGGL((batch_tile_kernel<kPaged, KT, VT, HD>), dim3(static_cast<unsigned>(tile_blocks)), dim3(kThreads), 0, s, a);
+    constexpr int W = tile_waves(KT);
+    if (tiles) hipLaunchKernelGGL((batch_tile_kernel<kPaged, KT, VT, HD, W>), dim3(static_cast<unsigned>(tile_blocks)), dim3(64 * W), 0, s, a);
     hipLaunchKernelGGL((batch_few_kernel<KT, VT, HD>), dim3(static_cast<unsigned>(few_blocks)), dim3(kThreads), 0, s, a);
     if (a.chunks > kFlatChunks) {
         hipLaunchKernelGGL((batch_join_kernel<HD>), dim3(a.ntok, a.n_head, HD / 64), dim3(kThreads), 0, s, a);
@@ -1290,13 +1349,14 @@ extern "C" int rmi_gqa_paged_attn(int qtype, const void* q, int ktype, const voi
     a.chunks = chunks;
     a.wo = static_cast<float*>(workspace);
     a.wml = a.wo + static_cast<size_t>(chunks) * ntok * n_head * head_dim;
-    a.levels = static_cast<int>((static_cast<long long>(std::min(max_new, ntok)) * G + kTileRows - 1) / kTileRows);
+    const int held = kWaveRows * tile_waves(ktype);
+    a.levels = most_levels(ntok, max_new, G, held);
     a.skip_few = 1;
     a.bf16 = qtype == RMI_ROWS_BF16;
     a.post = scale * kLog2e;
     const bool tiles = static_cast<long long>(std::min(max_new, ntok)) * G > kFewRows;
-    const long long few = static_cast<long long>(n_req) * n_kv * chunks, tile = most_tiles(n_req, ntok, max_new, G) * n_kv * chunks;
-    if (few > kMostBlocks || (tiles && tile > kMostBlocks) || static_cast<long long>(ntok) * n_head > kMostBlocks)
+    const long long few = static_cast<long long>(n_req) * n_kv * chunks, tile = most_tiles(n_req, ntok, max_new, G, held) * n_kv * chunks;
+    if (few > kMostBlocks || (tiles && tile > kMostBlocks / 2) || static_cast<long long>(ntok) * n_head > kMostBlocks)
         return fail(RMI_ERR_SHAPE, "gqa_paged_attn: too many workgroups");
     auto* s = static_cast<hipStream_t>(stream);
     if (head_dim == 256) launch_paged<256>(a, ktype, vtype, tiles, few, tile, s);
@@ -1338,15 +1398,16 @@ extern "C" int rmi_gqa_prompt_attn(int type, const void* q, int q_stride, const 
     a.n_kv = n_kv;
     a.chunk = (ntok + kChunkUnit - 1) / kChunkUnit * kChunkUnit;
     a.chunks = 1;
-    a.levels = static_cast<int>((static_cast<long long>(std::min(max_len, ntok)) * G + kTileRows - 1) / kTileRows);
+    const int held = kWaveRows * kPromptWaves;
+    a.levels = most_levels(ntok, max_len, G, held);
     a.bf16 = type == RMI_ROWS_BF16;
     a.post = scale * kLog2e;
-    const long long blocks = most_tiles(n_req, ntok, max_len, G) * n_kv;
+    const long long blocks = most_tiles(n_req, ntok, max_len, G, held) * n_kv;
     if (blocks > kMostBlocks) return fail(RMI_ERR_SHAPE, "gqa_prompt_attn: too many workgroups");
     auto go = [&](auto* kernel) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kPromptWaves), 0, static_cast<hipStream_t>(stream), a);
         return launch_status("gqa_prompt_attn");
     };
-    if (a.bf16) return head_dim == 256 ? go(&batch_tile_kernel<kRowsBF16, kKvF16, kKvF16, 256>) : go(&batch_tile_kernel<kRowsBF16, kKvF16, kKvF16, 128>);
-    return head_dim == 256 ? go(&batch_tile_kernel<kRowsF16, kKvF16, kKvF16, 256>) : go(&batch_tile_kernel<kRowsF16, kKvF16, kKvF16, 128>);
+    if (a.bf16) return head_dim == 256 ? go(&batch_tile_kernel<kRowsBF16, kKvF16, kKvF16, 256, kPromptWaves>) : go(&batch_tile_kernel<kRowsBF16, kKvF16, kKvF16, 128, kPromptWaves>);
+    return head_dim == 256 ? go(&batch_tile_kernel<kRowsF16, kKvF16, kKvF16, 256, kPromptWaves>) : go(&batch_tile_kernel<kRowsF16, kKvF16, kKvF16, 128, kPromptWaves>);
 }
