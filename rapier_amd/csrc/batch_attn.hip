@@ -117,6 +117,30 @@ __device__ __forceinline__ bool tile_of_rank(const BatchArgs& a, F&& count, uint
     return false;
 }
 
+// The chunk of a few-rows workgroup by its rank among those of the call: the requests' chunks one behind another, so that the
+// workgroups that have work are the first ones, as many to each XCD (they go there in turn), and a round of one for each compute
+// unit is one.  (Launched as requests times the longest one's chunks, with the others' ends empty: 32 requests of 1 K to 4 K
+// positions in chunks of 1792 78 us; so 70.)
+__device__ __forceinline__ bool chunk_of_rank(const BatchArgs& a, uint32_t rank, int G, int* req, int* chunk) {
+    const int lane = threadIdx.x & 63;
+    for (int i0 = 0; i0 < a.n_req; i0 += 64) {
+        const int i = min(i0 + lane, a.n_req - 1);
+        const Req r = request(a, i, a.row_start[i], a.row_start[i + 1]);
+        const int rows = r.n * G;
+        uint32_t n = i0 + lane < a.n_req && rows > 0 && rows <= kFewRows ? max((r.len + a.chunk - 1) / a.chunk, 1) : 0;
+        const uint32_t upto = wave_scan(n, [](uint32_t x, uint32_t y) { return x + y; });
+        const uint64_t past = __ballot(upto > rank);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            *req = i0 + l;
+            *chunk = static_cast<int>(rank) - __builtin_amdgcn_readlane(static_cast<int>(upto - n), l);
+            return true;
+        }
+        rank -= static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
+    }
+    return false;
+}
+
 // ---- 16-bit rows -----------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) { return u2(__builtin_convertvector(floatx2{a, b}, half2v)); }
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
@@ -212,11 +236,11 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void batch_few_kern
     __shared__ float stat[kWaves][2][kFewRows], fac[kWaves][kFewRows], sum[2][kFewRows];
 
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
-    const int kv = blockIdx.x % a.n_kv, chunk = (blockIdx.x / a.n_kv) % a.chunks, i = blockIdx.x / a.n_kv / a.chunks;
-    const int G = a.n_head / a.n_kv;
+    const int kv = blockIdx.x % a.n_kv, G = a.n_head / a.n_kv;
+    int i = 0, chunk = 0;
+    if (!chunk_of_rank(a, blockIdx.x / a.n_kv, G, &i, &chunk)) return;   // uniform
     const Req rq = request(a, i, word(a.row_start, i), word(a.row_start, i + 1));
     const int rows = rq.n * G, base = rq.len - rq.n, last = rq.len - 1, c0 = chunk * a.chunk;
-    if (rows == 0 || rows > kFewRows || (chunk > 0 && c0 > last)) return;   // uniform
     const int row = l16, rowc = min(row, rows - 1), tok = rowc / G;
     const uint16_t* qr = reinterpret_cast<const uint16_t*>(a.q) + (static_cast<ptrdiff_t>(rq.start + tok) * a.q_stride + (kv * G + rowc - tok * G) * HD) + 32 * g4;
     u32x4 qb[NI][2];
@@ -565,8 +589,9 @@ __device__ __forceinline__ void stream(u32x4 (&ready)[AHEAD], READ&& read, PRODU
 
 // the same value, of which the compiler does not know that a loop leaves it as it is: what is made of it then is made anew in each
 // round, by an instruction or two, and not kept in registers that there are none of
+template <bool ON>
 __device__ __forceinline__ int fresh(int x) {
-    asm volatile("" : "+v"(x));
+    if constexpr (ON) asm volatile("" : "+v"(x));
     return x;
 }
 
@@ -672,7 +697,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
     const uint32_t k_piece0 = 16 * (lane % PIECES ^ ((p0 + lr) & 15)), v_piece0 = 16 * (lane % PIECES ^ (v_swizzle(lr) << 1));
     const uint32_t k_row = static_cast<uint32_t>(lr) * static_cast<uint32_t>(kstride), v_row = static_cast<uint32_t>(lr) * static_cast<uint32_t>(vstride);
     auto direct = [&](const uint8_t* src, size_t page_bytes, size_t stride, size_t at0, int sb, uint32_t to, bool k) {
-        const uint32_t piece0 = fresh(k ? k_piece0 : v_piece0);
+        const uint32_t piece0 = fresh<CODES>(k ? k_piece0 : v_piece0);
         const uint8_t* from;
         int over = 0;   // how many of the wave's rows lie behind the call's (prompts: the last step of the last rows)
         if constexpr (PAGED) {
@@ -709,7 +734,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
         load_lds(src + static_cast<size_t>(page) * page_bytes + at0 + static_cast<size_t>((sb + p) & (size - 1)) * B, 16 * lane, to + 1024 * turn);
     };
     auto raw_scales = [&](const uint8_t* src, size_t page_bytes, size_t at0, int sb, uint32_t to) {
-        const int l = fresh(lane), p = 4 * l / NB;   // the lane's four bytes
+        const int l = fresh<CODES>(lane), p = 4 * l / NB;   // the lane's four bytes
         int page = id[0];
 #pragma unroll
         for (int g = 1; g < NG; ++g) page = p / 16 == g ? id[g] : page;
@@ -736,7 +761,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
     auto turn_rows = [&](auto type, const uint8_t* codes, const uint8_t* scales, uint8_t* to, bool k) {
         constexpr int T = decltype(type)::value;
         constexpr int UP = THREADS / (HD / 16);   // positions to a thread's next unit
-        const int t = fresh(tid), pos = t / (HD / 16), col = t % (HD / 16);
+        const int t = fresh<CODES>(tid), pos = t / (HD / 16), col = t % (HD / 16);
 #pragma unroll
         for (int u = 0; u < STEP / UP; ++u) {
             const int p = pos + u * UP;
@@ -864,7 +889,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
             for (int j = 0; j < NS; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[j][r] = 0.0f;
-            const int ka = fresh(kat), va = fresh(vat);
+            const int ka = fresh<CODES>(kat), va = fresh<CODES>(vat);
             auto k_piece = [&](int n) {   // dims 16 k .. of positions 32 j ..
                 const int j = n / NK, k = n % NK;
                 return *reinterpret_cast<const u32x4*>(tile + 32 * j * ROW + (ka ^ ((k & 7) << 5)) + (k >> 3) * 256);
@@ -1284,10 +1309,21 @@ extern "C" int rmi_gqa_paged_split(long long total_ctx, int max_ctx, int n_req, 
         return 0;
     }
     const int G = n_head / n_kv;
-    // about 512 workgroups, two a compute unit
     long long chunk;
-    if (static_cast<long long>(max_new) * G <= kFewRows) chunk = std::min<long long>(total_ctx, static_cast<long long>(max_ctx) * n_req) * n_kv / 512;
-    else chunk = std::max(1LL, static_cast<long long>(ntok) * G / kTileRows) * n_kv * max_ctx / 512;
+    if (static_cast<long long>(max_new) * G <= kFewRows) {
+        // Few rows: one round of workgroups, one for each of 256 compute units, since past the memory's rate it is their beginnings,
+        // ends and records that cost.  A request of any length has half a chunk too many on average; eight workgroups are left for
+        // more.  More rounds where one would leave a chunk much longer than its share.
+        const long long total = std::min<long long>(total_ctx, static_cast<long long>(max_ctx) * n_req);
+        long long rounds = 1, slots;
+        do {
+            slots = 512 * rounds - static_cast<long long>(n_req - 1) * n_kv - (n_req > 1 ? 16 : 0);   // halves
+            chunk = slots > 0 ? (2 * total * n_kv + slots - 1) / slots : max_ctx;
+        } while (++rounds <= 8 && 256 * chunk > 2 * total * n_kv);
+    } else {
+        // more rows: about 512 workgroups, two a compute unit
+        chunk = std::max(1LL, static_cast<long long>(ntok) * G / kTileRows) * n_kv * max_ctx / 512;
+    }
     chunk = std::max<long long>(chunk, (static_cast<long long>(max_ctx) + kMaxChunks - 1) / kMaxChunks);
     chunk = std::min<long long>(std::max(chunk, 1LL), max_ctx);
     return static_cast<int>((chunk + kChunkUnit - 1) / kChunkUnit * kChunkUnit);

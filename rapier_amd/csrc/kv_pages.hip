@@ -20,7 +20,8 @@ namespace {
 // ---- plan and trim -----------------------------------------------------------------------------------------------------
 // Both are two prefix sums over the requests and a copy.  Every workgroup takes the sums of all requests for itself (16 KB of
 // lengths at most, from the L2), so one launch does and no workgroup waits for another; tokens and pages are then dealt out over
-// all of them, each finding its request by bisection of the sums in LDS.  Latency-bound: 32 requests and 999 take a few us.
+// all of them, each finding its request by bisection of the sums in LDS.  Latency-bound: loads, two sums with their barriers, a bisection, a
+// load; 32 requests of one token 4 us.
 constexpr int kPlanThreads = 256;
 constexpr uint32_t kSat = 1u << 30;   // sums stop here: min(a + b, kSat) is associative, and lengths may be anything
 constexpr uint32_t kRefused = 1u << 31;
@@ -34,16 +35,12 @@ __device__ __forceinline__ void scan_requests(uint32_t* a, int n, uint32_t* sums
     const int per = (n + kPlanThreads - 1) / kPlanThreads, first = tid * per, end = min(first + per, n);
     uint32_t mine = 0;
     for (int i = first; i < end; ++i) mine = sat_add(mine, a[i]);
-    uint32_t upto = mine;
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-        const uint32_t o = __shfl_up(upto, k, 64);
-        if (lane >= k) upto = sat_add(upto, o);
-    }
+    const uint32_t upto = wave_scan(mine, sat_add);
     if (lane == 63) sums[wv] = upto;
     __syncthreads();
     uint32_t before = 0;
-    for (int w = 0; w < wv; ++w) before = sat_add(before, sums[w]);
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 64 - 1; ++w) before = sat_add(before, w < wv ? sums[w] : 0);
     const uint32_t prev = __shfl_up(upto, 1, 64);
     if (lane > 0) before = sat_add(before, prev);
     for (int i = first; i < end; ++i) {
@@ -74,37 +71,52 @@ struct PlanArgs {
 
 __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PlanArgs a) {
     __shared__ uint32_t rows[kMaxReq + 1], offs[kMaxReq + 1];   // row starts; pages taken before, with kRefused
+    __shared__ int pasts[kMaxReq];
     __shared__ uint32_t sums[kPlanThreads / 64], taken;
+    constexpr int E = kMaxReq / kPlanThreads;   // requests a thread has, 256 apart
     const int tid = threadIdx.x, n = a.n_req;
+    int past[E], count[E];   // in flight together
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+        if (k * kPlanThreads < n) {   // uniform
+            const int i = min(k * kPlanThreads + tid, n - 1);
+            past[k] = a.past[i];
+            count[k] = a.count[i];
+        }
     const int n_free = min(max(a.n_free[0], 0), a.n_pages);
-    const long long room = static_cast<long long>(a.table_stride) << a.shift;
-    auto lengths_ok = [&](int past, int count) { return past >= 0 && count >= 0 && static_cast<long long>(past) + count <= min(room, static_cast<long long>(kSat)); };
+    const long long room = min(static_cast<long long>(a.table_stride) << a.shift, static_cast<long long>(kSat));
+    const uint32_t max_tok = static_cast<uint32_t>(a.max_tok);
+    // f(request, its past and count) for each of the thread's
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+            if (k * kPlanThreads + tid < n) f(k * kPlanThreads + tid, past[k], count[k]);
+    };
+    auto fits = [&](int i, int p, int c) { return p >= 0 && c >= 0 && static_cast<long long>(p) + c <= room && rows[i] + static_cast<uint32_t>(c) <= max_tok; };
+    auto need = [&](int p, int c) { return static_cast<uint32_t>(pages_of(p + c, a.shift) - pages_of(p, a.shift)); };
     if (tid == 0) taken = 0;
-    for (int i = tid; i < n; i += kPlanThreads) rows[i] = static_cast<uint32_t>(min(max(a.count[i], 0), static_cast<int>(kSat)));
+    each([&](int i, int p, int c) {
+        rows[i] = static_cast<uint32_t>(min(max(c, 0), static_cast<int>(kSat)));
+        pasts[i] = p;
+    });
     __syncthreads();
     scan_requests(rows, n, sums);
-    const uint32_t max_tok = static_cast<uint32_t>(a.max_tok);
-    auto fits = [&](int i, int past, int count) { return lengths_ok(past, count) && rows[i] + static_cast<uint32_t>(count) <= max_tok; };
-    for (int i = tid; i < n; i += kPlanThreads) {
-        const int past = a.past[i], count = a.count[i];
-        offs[i] = fits(i, past, count) ? static_cast<uint32_t>(pages_of(past + count, a.shift) - pages_of(past, a.shift)) : 0;
-    }
+    each([&](int i, int p, int c) { offs[i] = fits(i, p, c) ? need(p, c) : 0; });
     __syncthreads();
     scan_requests(offs, n, sums);
     const uint32_t wanted = offs[n];
-    for (int i = tid; i < n; i += kPlanThreads) {
-        const int past = a.past[i], count = a.count[i];
-        const bool good = fits(i, past, count);
-        const uint32_t before = offs[i], need = good ? static_cast<uint32_t>(pages_of(past + count, a.shift) - pages_of(past, a.shift)) : 0;
-        const bool ok = good && (need == 0 || before + need <= static_cast<uint32_t>(n_free));
+    each([&](int i, int p, int c) {
+        const bool good = fits(i, p, c);
+        const uint32_t before = offs[i], pages = good ? need(p, c) : 0;
+        const bool ok = good && (pages == 0 || before + pages <= static_cast<uint32_t>(n_free));
         if (!ok) offs[i] = before | kRefused;   // only this thread reads it before the barrier
-        else if (need) atomicMax(&taken, before + need);
+        else if (pages) atomicMax(&taken, before + pages);
         if (blockIdx.x == 0) {
             a.row_start[i] = static_cast<int>(min(rows[i], max_tok));
-            a.kv_len[i] = ok ? past + count : 0;
+            a.kv_len[i] = ok ? p + c : 0;
             a.status[i] = ok ? RMI_PAGES_OK : good ? RMI_PAGES_NONE_LEFT : RMI_PAGES_BAD_LENGTH;
         }
-    }
+    });
     __syncthreads();
     if (blockIdx.x == 0 && tid == 0) {
         a.row_start[n] = static_cast<int>(min(rows[n], max_tok));
@@ -116,10 +128,9 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PlanArgs a) {
         if (t < used) {
             const int i = request_of(rows, n, t);
             const uint32_t off = offs[i];
-            const int past = a.past[i];
-            p = static_cast<int>(static_cast<uint32_t>(past) + (t - rows[i]));   // anything if the lengths are bad
+            p = static_cast<int>(static_cast<uint32_t>(pasts[i]) + (t - rows[i]));   // anything if the lengths are bad
             if (!(off & kRefused)) {
-                const int held = pages_of(past, a.shift), at = p >> a.shift;
+                const int held = pages_of(pasts[i], a.shift), at = p >> a.shift;
                 const int page = at < held ? a.table[static_cast<size_t>(i) * a.table_stride + at]
                                            : a.free_pages[n_free - 1 - static_cast<int>(off) - (at - held)];
                 if (page >= 0 && page < a.n_pages) slot = (page << a.shift) | (p & ((1 << a.shift) - 1));
@@ -133,7 +144,7 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PlanArgs a) {
         const int i = request_of(offs, n, k);
         const uint32_t off = offs[i];
         if (!(off & kRefused))
-            a.table[static_cast<size_t>(i) * a.table_stride + pages_of(a.past[i], a.shift) + (k - off)] = a.free_pages[n_free - 1 - static_cast<int>(k)];
+            a.table[static_cast<size_t>(i) * a.table_stride + pages_of(pasts[i], a.shift) + (k - off)] = a.free_pages[n_free - 1 - static_cast<int>(k)];
     }
 }
 
@@ -148,6 +159,7 @@ __global__ __launch_bounds__(kPlanThreads) void page_trim_kernel(TrimArgs a) {
     __shared__ uint32_t sums[kPlanThreads / 64];
     const int tid = threadIdx.x, n = a.n_req;
     const int n_free = min(max(a.n_free[0], 0), a.n_pages);
+#pragma unroll 4
     for (int i = tid; i < n; i += kPlanThreads) {
         const int len = a.len[i], keep = a.keep[i];
         const int end = min(pages_of(len, a.shift), a.table_stride), first = pages_of(keep, a.shift);
@@ -417,8 +429,9 @@ extern "C" int rmi_page_plan(const int* past, const int* count, int n_req, int p
     if (!apart(in, 4, out, 7)) return fail(RMI_ERR_POINTER, "page_plan: an output lies on another argument");
     const PlanArgs a{past, count, free_pages, n_free, table, row_start, kv_len, slot, pos, n_left, status,
                      n_req, page_shift_of(page_size), n_pages, table_stride, max_tok};
-    // four tokens a thread: more workgroups only repeat the sums
-    const int blocks = std::min(256, (max_tok + 4 * kPlanThreads - 1) / (4 * kPlanThreads));
+    // a token a thread up to four workgroups a compute unit: each repeats the sums, but a thread's tokens wait for one another.
+    // 999 requests with 121 K tokens, four tokens a thread 13.2 us, one 9.5
+    const int blocks = std::min(1024, (max_tok + kPlanThreads - 1) / kPlanThreads);
     hipLaunchKernelGGL(page_plan_kernel, dim3(blocks), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream), a);
     return launch_status("page_plan");
 }
