@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace rmi {
 namespace {
@@ -43,7 +44,7 @@ struct BatchArgs {
     float *wo, *wml;   // records: o [chunk][row][head][HD], (m, l) [chunk][row][head][2]
     int q_stride, k_stride, v_stride, gate_stride, y_stride, q8_stride;   // elements (q8: bytes)
     int table_stride, n_req, ntok, max_new, max_ctx, n_head, n_kv, shift, n_pages;
-    int chunk, chunks, levels, skip_few, bf16;
+    int chunk, chunks, tiles, levels, skip_few, bf16;   // tiles: of rows, at most; levels: of a request's tiles, at most
     float post;   // score = q.k * post, in base 2
 };
 
@@ -115,6 +116,29 @@ __device__ __forceinline__ bool tile_of_rank(const BatchArgs& a, F&& count, uint
         k -= n;
     }
     return false;
+}
+
+// tile_of_rank for tiles of ROWS rows, in a workgroup of THREADS; counts: kMaxReq words of LDS, free again afterwards
+template <int ROWS, int THREADS>
+__device__ __forceinline__ bool find_tile(const BatchArgs& a, int* counts, uint32_t rank, int G, int* req, int* level) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    auto tiles_of = [&](int k) {
+        const int rows = request(a, k, a.row_start[k], a.row_start[k + 1]).n * G;
+        return a.skip_few && rows <= kFewRows ? 0 : (rows + ROWS - 1) / ROWS;
+    };
+    bool has;
+    if (a.n_req <= 64) {   // a request a lane
+        const int mine = tiles_of(min(lane, a.n_req - 1));
+        has = tile_of_rank(a, [&](int) { return mine; }, rank, req, level);
+    } else {
+        for (int k = tid; k < a.n_req; k += THREADS) counts[k] = tiles_of(k);
+        __syncthreads();
+        has = tile_of_rank(a, [&](int k) { return counts[k]; }, rank, req, level);
+        __syncthreads();   // read before the first tile overwrites them
+    }
+    *req = __builtin_amdgcn_readfirstlane(*req);
+    *level = __builtin_amdgcn_readfirstlane(*level);
+    return has;
 }
 
 // The chunk of a few-rows workgroup by its rank among those of the call: the requests' chunks one behind another, so that the
@@ -605,6 +629,154 @@ struct TileShape {
     static constexpr int kTile = 2 * kHalf;
 };
 
+// ---- a step of 32 query rows -------------------------------------------------------------------------------------------------
+// where a V row's values are, for the few that are read past the tile
+struct VRow {
+    const uint8_t* p;
+    size_t scale;   // codes: from p to the row's scale bytes
+    bool ok;        // there is one
+};
+
+// Scores, softmax and P V of the positions sb .. sb + STEP - 1 in the tiles kt and vt for the wave's 32 rows.  lim: the last position
+// that the lane's row sees, last: that any row of the workgroup sees; cut: uniform, some row does not see the whole step; bad: 16-position
+// pieces without a page.  v_ready() is called when K is read, has_odd() tells (uniformly) whether a value that is not finite was
+// taken out of vt, v_row(position) where it is.  FRESH: no addresses kept in registers.  V_EARLY: the first of V over the softmax.
+template <bool BF, int HD, int VT, bool FRESH, bool V_EARLY, typename READY, typename ODD, typename ROWS>
+__device__ __forceinline__ void tile_step(const uint8_t* kt, const uint8_t* vt, int kat, int vat, const u32x4 (&q)[HD / 16], floatx16 (&o)[HD / 32],
+                                          float& m_run, float& l_run, float post, int sb, int last, int lim, int h, uint32_t bad, bool cut,
+                                          READY&& v_ready, ODD&& has_odd, ROWS&& v_row) {
+    constexpr int STEP = TileShape<HD>::kStep, ROW = TileShape<HD>::kRow, NS = STEP / 32, NK = HD / 16, ND = HD / 32;
+    constexpr int AHEAD = HD == 256 ? 2 : 4;   // operands from LDS on their way
+    floatx16 s[NS];
+#pragma unroll
+    for (int j = 0; j < NS; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[j][r] = 0.0f;
+    const int ka = fresh<FRESH>(kat), va = fresh<FRESH>(vat);
+    auto k_piece = [&](int n) {   // dims 16 k .. of positions 32 j ..
+        const int j = n / NK, k = n % NK;
+        return *reinterpret_cast<const u32x4*>(kt + 32 * j * ROW + (ka ^ ((k & 7) << 5)) + (k >> 3) * 256);
+    };
+    auto v_piece = [&](int n) {   // 16 positions 16 k .. of dims 32 d ..
+        const int k = n / ND, d = n % ND;
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const uint8_t* at = vt + 16 * k * ROW + (va ^ ((d & 3) << 6)) + (d >> 2) * 256;
+        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*) at));
+        const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*) (at + 8 * ROW)));
+        return u32x4{x.x, x.y, y.x, y.y};
+    };
+    // the matrix cores go to the wave that has its operands, so that the two waves of a SIMD take turns at them and at the softmax
+    u32x4 ready[AHEAD];
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) ready[n] = k_piece(n);
+    __builtin_amdgcn_sched_barrier(0x6);
+    __builtin_amdgcn_s_setprio(1);
+    stream<AHEAD, NS * NK>(ready, k_piece, [&](int n, u32x4 x) { s[n / NK] = mfma32<BF>(x, q[n % NK], s[n / NK]); });
+    __builtin_amdgcn_s_setprio(0);
+    auto v_first = [&] {
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) ready[n] = v_piece(n);
+        __builtin_amdgcn_sched_barrier(0x6);
+    };
+    if constexpr (V_EARLY) {
+        v_ready();
+        v_first();
+    }
+    if (bad)
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (bad >> (2 * j + (r >> 3)) & 1) s[j][r] = __builtin_nanf("");
+    if (cut)
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (sb + 32 * j + 8 * (r >> 2) + 4 * h + (r & 3) > lim) s[j][r] = -INFINITY;
+    float top = s[0][0];
+#pragma unroll
+    for (int j = 0; j < NS; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[j][r]);
+    top = fmaxf(top, xor_lane<32>(top)) * post;   // post > 0
+    const float m_new = top > m_run + kLazy ? top : m_run;
+    const float m_ref = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: exp2(-inf) = 0, no NaN
+    const float alpha = m_run == m_new || m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_ref);   // -inf: o is 0
+    m_run = m_new;
+    const float shift = kPScale - m_ref;
+    float sum = 0.0f;
+    u32x4 p[2 * NS];
+#pragma unroll
+    for (int j = 0; j < NS; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], post, shift)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r + 1], post, shift));
+            sum += x + y;
+            p[2 * j + (r >> 3)][(r & 7) >> 1] = BF ? pack_bf16(x, y) : pack_f16(x, y);
+        }
+    l_run = __builtin_fmaf(l_run, alpha, sum);
+    if (__ballot(alpha != 1.0f)) {   // uniform: some row's maximum moved
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+    }
+    if constexpr (!V_EARLY) v_ready();
+    if (has_odd()) {   // uniform
+        for (int pp = 0; pp < STEP; ++pp) {
+            const int at = sb + pp;
+            if (at > last) break;
+            // the row's p of this position, from the half that has it
+            const int j = pp >> 5, r = 4 * ((pp >> 3) & 3) + (pp & 3);
+            float x = 0.0f;
+#pragma unroll
+            for (int jj = 0; jj < NS; ++jj)
+#pragma unroll
+                for (int rr = 0; rr < 16; ++rr)
+                    if (j == jj && r == rr) x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[jj][rr], post, shift));
+            const float other = xor_lane<32>(x);
+            if (((pp >> 2) & 1) != h) x = other;
+            const int hh = fresh<true>(h);   // with the barriers below: no address or load of another dim takes a register here
+            const VRow row = v_row(at);
+            if (!row.ok) continue;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+#pragma unroll
+                for (int r2 = 0; r2 < 16; ++r2) {
+                    const int dim = 32 * d + 8 * (r2 >> 2) + 4 * hh + (r2 & 3);
+                    float v;
+                    if constexpr (VT != kKvF16) v = odd_value<VT>(row.p[row.scale + d]);
+                    else if constexpr (BF) v = __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row.p)[dim]) << 16);
+                    else v = half_bits_to_float(reinterpret_cast<const uint16_t*>(row.p)[dim]);
+                    if (!(fabsf(v) <= FLT_MAX) && at <= lim) o[d][r2] = __builtin_fmaf(x, v, o[d][r2]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+    if constexpr (!V_EARLY) v_first();
+    __builtin_amdgcn_s_setprio(1);
+    stream<AHEAD, 2 * NS * ND>(ready, v_piece, [&](int n, u32x4 x) { o[n % ND] = mfma32<BF>(x, p[n / ND], o[n % ND]); });
+    __builtin_amdgcn_s_setprio(0);
+}
+
+// what is not finite leaves the 16 bytes at `at`; whether there was any
+template <bool BF>
+__device__ __forceinline__ bool clear_odd(u32x4* at) {
+    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+    u32x4 w = *at;
+    bool found = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if ((w[e] & E) == E) w[e] &= 0xffff0000u, found = true;
+        if ((w[e] & (E << 16)) == (E << 16)) w[e] &= 0xffffu, found = true;
+    }
+    if (found) *at = w;
+    return found;
+}
+
 template <int SRC, int KT, int VT, int HD, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) {
     using S = TileShape<HD>;
@@ -612,11 +784,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
     constexpr bool BF = SRC == kRowsBF16, PAGED = SRC == kPaged;
     constexpr bool CODES = KT != kKvF16;             // K and V are codes to be turned to fp16 (both or neither)
     constexpr int LEAD = CODES ? 2 : 1;              // steps that loads are ahead
-    constexpr int STEP = S::kStep, ROW = S::kRow, NS = STEP / 32;      // 32-position pieces of a step
+    constexpr int STEP = S::kStep, ROW = S::kRow;
     constexpr int NK = HD / 16, ND = HD / 32;
-    constexpr int AHEAD = HD == 256 ? 2 : 4;         // operands from LDS on their way
-    constexpr bool V_EARLY = HD == 128;              // the first of V over the softmax
-    constexpr int WR = STEP / WAVES;                // rows of a step that a wave loads
+    // the waves that load 16-bit rows, and rows of a step of each.  Eight waves: the first four, whose loads hold them up for 500 cycles
+    // and more, so that the other wave of a SIMD is ahead of them and one is at its products while the other is at its softmax (8001
+    // tokens 505 us with two workgroups of four waves, 485 so)
+    constexpr int LOADERS = 4, WR = STEP / LOADERS;
     constexpr int PER = 1024 / ROW, NL = WR / PER;   // rows a direct load, loads a wave
     constexpr int NG = STEP / 16;                    // 16-position pieces, each in one page
     constexpr int NB = HD / kKvBlock;
@@ -628,30 +801,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
 
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, h = lane >> 5;
     const int G = a.n_head / a.n_kv;
-    // KV heads innermost: workgroups go to the XCDs round robin, so a head's tiles meet its K and V in one or two L2s
-    const int kv = blockIdx.x % a.n_kv, chunk = (blockIdx.x / a.n_kv) % a.chunks;
-    const uint32_t rank = blockIdx.x / a.n_kv / a.chunks;
+    // KV heads innermost: workgroups go to the XCDs round robin, so a head's tiles meet its K and V in one or two L2s.  Chunks
+    // outermost: those that not every request has are the last, and lie over the XCDs as the tiles do.  (Chunks next to the heads, as
+    // many or none by turns, were 16 I8 requests of 16 tokens behind 1 K to 4 K in 896s 67 or 103 us, as it fell out.)
+    const int kv = blockIdx.x % a.n_kv, chunk = blockIdx.x / a.n_kv / a.tiles;
+    const uint32_t rank = blockIdx.x / a.n_kv % a.tiles;
     int i = 0, level = 0;
-    {
-        auto tiles_of = [&](int k) {
-            const int rows = request(a, k, a.row_start[k], a.row_start[k + 1]).n * G;
-            return a.skip_few && rows <= kFewRows ? 0 : (rows + ROWS - 1) / ROWS;
-        };
-        if (tid < 2) odd[tid] = 0;
-        if (a.n_req <= 64) {   // a request a lane
-            const int mine = tiles_of(min(lane, a.n_req - 1));
-            if (!tile_of_rank(a, [&](int) { return mine; }, rank, &i, &level)) return;   // uniform
-        } else {
-            int* tiles = reinterpret_cast<int*>(pool);
-            for (int k = tid; k < a.n_req; k += THREADS) tiles[k] = tiles_of(k);
-            __syncthreads();
-            const bool has = tile_of_rank(a, [&](int k) { return tiles[k]; }, rank, &i, &level);
-            __syncthreads();   // read before the first tile overwrites it
-            if (!has) return;   // uniform
-        }
-    }
-    i = __builtin_amdgcn_readfirstlane(i);
-    level = __builtin_amdgcn_readfirstlane(level);
+    if (tid < 2) odd[tid] = 0;
+    if (!find_tile<ROWS, THREADS>(a, reinterpret_cast<int*>(pool), rank, G, &i, &level)) return;   // uniform
     const Req rq = request(a, i, word(a.row_start, i), word(a.row_start, i + 1));
     const int rows = rq.n * G, base = rq.len - rq.n, c0 = chunk * a.chunk;
     const int first = base + level * ROWS / G, last = base + min(level * ROWS + ROWS - 1, rows - 1) / G;   // of the workgroup's tokens
@@ -695,9 +852,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
     constexpr int PIECES = ROW / 16;
     const int p0 = WR * wv, lr = lane / PIECES;
     const uint32_t k_piece0 = 16 * (lane % PIECES ^ ((p0 + lr) & 15)), v_piece0 = 16 * (lane % PIECES ^ (v_swizzle(lr) << 1));
-    const uint32_t k_row = static_cast<uint32_t>(lr) * static_cast<uint32_t>(kstride), v_row = static_cast<uint32_t>(lr) * static_cast<uint32_t>(vstride);
+    const uint32_t k_line = static_cast<uint32_t>(lr) * static_cast<uint32_t>(kstride), v_line = static_cast<uint32_t>(lr) * static_cast<uint32_t>(vstride);
     auto direct = [&](const uint8_t* src, size_t page_bytes, size_t stride, size_t at0, int sb, uint32_t to, bool k) {
-        const uint32_t piece0 = fresh<CODES>(k ? k_piece0 : v_piece0);
+        const uint32_t piece0 = fresh<PAGED>(k ? k_piece0 : v_piece0);
         const uint8_t* from;
         int over = 0;   // how many of the wave's rows lie behind the call's (prompts: the last step of the last rows)
         if constexpr (PAGED) {
@@ -714,7 +871,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
         for (int n = 0; n < NL; ++n) {
             const uint32_t piece = piece0 ^ (k ? 16 * (n * PER & 15) : 32 * v_swizzle(n * PER));
             const uint32_t lds = to + (p0 + n * PER) * ROW;
-            if (over <= 0) load_lds(from + n * PER * stride, (k ? k_row : v_row) + piece, lds);
+            if (over <= 0) load_lds(from + n * PER * stride, (k ? k_line : v_line) + piece, lds);
             else load_lds(from, static_cast<uint32_t>(min(n * PER + lr, WR - 1 - over)) * static_cast<uint32_t>(stride) + piece, lds);
         }
     };
@@ -734,7 +891,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
         load_lds(src + static_cast<size_t>(page) * page_bytes + at0 + static_cast<size_t>((sb + p) & (size - 1)) * B, 16 * lane, to + 1024 * turn);
     };
     auto raw_scales = [&](const uint8_t* src, size_t page_bytes, size_t at0, int sb, uint32_t to) {
-        const int l = fresh<CODES>(lane), p = 4 * l / NB;   // the lane's four bytes
+        const int l = fresh<PAGED>(lane), p = 4 * l / NB;   // the lane's four bytes
         int page = id[0];
 #pragma unroll
         for (int g = 1; g < NG; ++g) page = p / 16 == g ? id[g] : page;
@@ -751,7 +908,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
             }
             if (wv == 0) raw_scales(a.k, kpage, kv_row<KT>(0, kv, a.n_kv, size, HD).scale, sb, to + STEP * (kKB + kVB));
             if (wv == 1) raw_scales(a.v, vpage, kv_row<VT>(0, kv, a.n_kv, size, HD).scale, sb, to + STEP * (kKB + kVB + NB));
-        } else {
+        } else if (wv < LOADERS) {   // uniform
             const uint32_t to = pool0 + buf * S::kTile;
             direct(a.k, kpage, kstride, k_at, sb, to, true);
             direct(a.v, vpage, vstride, v_at, sb, to + S::kHalf, false);
@@ -761,7 +918,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
     auto turn_rows = [&](auto type, const uint8_t* codes, const uint8_t* scales, uint8_t* to, bool k) {
         constexpr int T = decltype(type)::value;
         constexpr int UP = THREADS / (HD / 16);   // positions to a thread's next unit
-        const int t = fresh<CODES>(tid), pos = t / (HD / 16), col = t % (HD / 16);
+        const int t = fresh<PAGED>(tid), pos = t / (HD / 16), col = t % (HD / 16);
 #pragma unroll
         for (int u = 0; u < STEP / UP; ++u) {
             const int p = pos + u * UP;
@@ -832,9 +989,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
     const int kat = l32 * ROW + ((h ^ (l32 & 15)) << 4);
     const int vp = 4 * h + ((lane & 15) >> 2);
     const int vat = vp * ROW + ((((lane >> 4) & 1) ^ v_swizzle(vp)) << 5) + 8 * (lane & 3);
-    auto finite = [](uint32_t w) {
-        constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
-        return (w & E) != E && (w & (E << 16)) != (E << 16);
+    auto v_row = [&](int at) {
+        VRow r = {a.v, 0, true};
+        if constexpr (PAGED) {
+            const int page = word(ids, min(at >> a.shift, a.table_stride - 1));
+            const KvRow<VT> row = kv_row<VT>(at & (size - 1), kv, a.n_kv, size, HD);
+            r.ok = page >= 0 && page < a.n_pages;
+            r.p += static_cast<size_t>(r.ok ? page : 0) * vpage + row.code;
+            r.scale = row.scale - row.code;
+        } else {
+            r.p += (static_cast<size_t>(rq.start) + at) * vstride + v_at;
+        }
+        return r;
     };
 
     if constexpr (CODES) {
@@ -864,144 +1030,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
             uint8_t* const vt = pool + buf * S::kTile + S::kHalf;
             bool found = false;
 #pragma unroll
-            for (int n = 0; n < S::kHalf / (16 * THREADS); ++n) {
-                u32x4* at = reinterpret_cast<u32x4*>(vt + 16 * (tid + n * THREADS));
-                u32x4 w = *at;
-                if (!(finite(w[0]) && finite(w[1]) && finite(w[2]) && finite(w[3]))) {
-                    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if ((w[e] & E) == E) w[e] &= 0xffff0000u;
-                        if ((w[e] & (E << 16)) == (E << 16)) w[e] &= 0xffffu;
-                    }
-                    *at = w;
-                    found = true;
-                }
-            }
+            for (int n = 0; n < S::kHalf / (16 * THREADS); ++n) found |= clear_odd<BF>(reinterpret_cast<u32x4*>(vt + 16 * (tid + n * THREADS)));
             if (found) odd[buf] = st + 1;   // every writer stores the same
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
         }
-        if (sb <= wlast) {   // uniform in the wave
-            floatx16 s[NS];
-#pragma unroll
-            for (int j = 0; j < NS; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[j][r] = 0.0f;
-            const int ka = fresh<CODES>(kat), va = fresh<CODES>(vat);
-            auto k_piece = [&](int n) {   // dims 16 k .. of positions 32 j ..
-                const int j = n / NK, k = n % NK;
-                return *reinterpret_cast<const u32x4*>(tile + 32 * j * ROW + (ka ^ ((k & 7) << 5)) + (k >> 3) * 256);
-            };
-            const uint8_t* const vt = tile + S::kHalf;
-            auto v_piece = [&](int n) {   // 16 positions 16 k .. of dims 32 d ..
-                const int k = n / ND, d = n % ND;
-                typedef short s16x4 __attribute__((ext_vector_type(4)));
-                typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-                const uint8_t* at = vt + 16 * k * ROW + (va ^ ((d & 3) << 6)) + (d >> 2) * 256;
-                const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*) at));
-                const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*) (at + 8 * ROW)));
-                return u32x4{x.x, x.y, y.x, y.y};
-            };
-            u32x4 ready[AHEAD];
-#pragma unroll
-            for (int n = 0; n < AHEAD; ++n) ready[n] = k_piece(n);
-            __builtin_amdgcn_sched_barrier(0x6);
-            __builtin_amdgcn_s_setprio(1);
-            stream<AHEAD, NS * NK>(ready, k_piece, [&](int n, u32x4 x) { s[n / NK] = mfma32<BF>(x, q[n % NK], s[n / NK]); });
-            __builtin_amdgcn_s_setprio(0);
-            auto v_first = [&] {
-#pragma unroll
-                for (int n = 0; n < AHEAD; ++n) ready[n] = v_piece(n);
-                __builtin_amdgcn_sched_barrier(0x6);
-            };
-            if constexpr (V_EARLY) v_first();
-            if (step_bad)
-#pragma unroll
-                for (int j = 0; j < NS; ++j)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (step_bad >> (2 * j + (r >> 3)) & 1) s[j][r] = __builtin_nanf("");
-            const bool cut = sb + STEP - 1 > wfirst || row0 + kWaveRows > rows;   // uniform in the wave
-            if (cut)
-#pragma unroll
-                for (int j = 0; j < NS; ++j)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (sb + 32 * j + 8 * (r >> 2) + 4 * h + (r & 3) > lim) s[j][r] = -INFINITY;
-            float top = s[0][0];
-#pragma unroll
-            for (int j = 0; j < NS; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[j][r]);
-            top = fmaxf(top, xor_lane<32>(top)) * post;   // post > 0
-            const float m_new = top > m_run + kLazy ? top : m_run;
-            const float m_ref = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: exp2(-inf) = 0, no NaN
-            const float alpha = m_run == m_new || m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_ref);   // -inf: o is 0
-            m_run = m_new;
-            const float shift = kPScale - m_ref;
-            float sum = 0.0f;
-            u32x4 p[2 * NS];
-#pragma unroll
-            for (int j = 0; j < NS; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; r += 2) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], post, shift)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r + 1], post, shift));
-                    sum += x + y;
-                    p[2 * j + (r >> 3)][(r & 7) >> 1] = BF ? pack_bf16(x, y) : pack_f16(x, y);
-                }
-            l_run = __builtin_fmaf(l_run, alpha, sum);
-            if (__ballot(alpha != 1.0f)) {   // uniform: some row's maximum moved
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
-            }
-            if (tail && odd[buf] == st + 1) {   // uniform
-                for (int pp = 0; pp < STEP; ++pp) {
-                    const int at = sb + pp;
-                    if (at > last) break;
-                    // the row's p of this position, from the half that has it
-                    const int j = pp >> 5, r = 4 * ((pp >> 3) & 3) + (pp & 3);
-                    float x = 0.0f;
-#pragma unroll
-                    for (int jj = 0; jj < NS; ++jj)
-#pragma unroll
-                        for (int rr = 0; rr < 16; ++rr)
-                            if (j == jj && r == rr) x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[jj][rr], post, shift));
-                    const float other = xor_lane<32>(x);
-                    if (((pp >> 2) & 1) != h) x = other;
-                    const uint8_t* vr = a.v;
-                    size_t scale = 0;
-                    if constexpr (PAGED) {
-                        const int page = word(ids, min(at >> a.shift, a.table_stride - 1));
-                        const KvRow<VT> vrow = kv_row<VT>(at & (size - 1), kv, a.n_kv, size, HD);
-                        if (page < 0 || page >= a.n_pages) continue;
-                        vr += static_cast<size_t>(page) * vpage + vrow.code;
-                        scale = vrow.scale - vrow.code;
-                    } else {
-                        vr += (static_cast<size_t>(rq.start) + at) * vstride + v_at;
-                    }
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int dim = 32 * d + 8 * (r >> 2) + 4 * h + (r & 3);
-                            float v;
-                            if constexpr (CODES) v = odd_value<VT>(vr[scale + d]);
-                            else if constexpr (BF) v = __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(vr)[dim]) << 16);
-                            else v = half_bits_to_float(reinterpret_cast<const uint16_t*>(vr)[dim]);
-                            if (!(fabsf(v) <= FLT_MAX) && at <= lim) o[d][r] = __builtin_fmaf(x, v, o[d][r]);
-                        }
-                    }
-                }
-            }
-            if constexpr (!V_EARLY) v_first();
-            __builtin_amdgcn_s_setprio(1);
-            stream<AHEAD, 2 * NS * ND>(ready, v_piece, [&](int n, u32x4 x) { o[n % ND] = mfma32<BF>(x, p[n / ND], o[n % ND]); });
-            __builtin_amdgcn_s_setprio(0);
-        }
+        if (sb <= wlast)   // uniform in the wave
+            tile_step<BF, HD, VT, PAGED, HD == 128>(tile, tile + S::kHalf, kat, vat, q, o, m_run, l_run, post, sb, last, lim, h, step_bad,
+                                                    sb + STEP - 1 > wfirst || row0 + kWaveRows > rows, [] {},
+                                                    [&] { return tail && odd[buf] == st + 1; }, v_row);
         if (CODES && more && wv < WAVES / 2) turn(buf ^ 1);
     }
 
@@ -1075,6 +1113,148 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
             }
             if (h == 0) *reinterpret_cast<uint32_t*>(blk) = float_to_half_sat(dq) | (float_to_half_sat(total) << 16);
         }
+    }
+}
+
+// ---- few tiles: 32 rows a workgroup, the positions in four parts --------------------------------------------------------------
+// Short prompts: tiles of 128 rows would leave compute units empty and each wave alone with a long chain of steps.  Here a workgroup
+// has 32 rows, its waves take steps of the positions in turn, each with K and V tiles of its own in LDS (no barriers), and their
+// parts are joined at the end.  A wave loads K of its next step when this step's scores are done and V when its product is.
+// 500 tokens x 16 heads 24 us, tiles of 128 rows 31.6.
+template <bool BF, int HD>
+__global__ __launch_bounds__(kThreads, 1) void batch_parts_kernel(BatchArgs a) {
+    using S = TileShape<HD>;
+    constexpr int STEP = S::kStep, ROW = S::kRow, NK = HD / 16, ND = HD / 32, PER = 1024 / ROW, NL = STEP / PER, PIECES = ROW / 16;
+    constexpr int ROWS = kWaveRows;
+    __shared__ __attribute__((aligned(16))) uint8_t pool[kWaves * S::kTile];
+    __shared__ float stat[kWaves][2][ROWS];
+    static_assert(sizeof(pool) >= kWaves * ROWS * HD * sizeof(float), "the parts' rows are joined in the tiles' place");
+    static_assert(sizeof(pool) >= kMaxReq * sizeof(int), "the requests' tiles are counted in the tiles' place");
+
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, h = lane >> 5;
+    const int G = a.n_head / a.n_kv, kv = blockIdx.x % a.n_kv;
+    int i = 0, level = 0;
+    if (!find_tile<ROWS, kThreads>(a, reinterpret_cast<int*>(pool), blockIdx.x / a.n_kv, G, &i, &level)) return;   // uniform
+    const Req rq = request(a, i, word(a.row_start, i), word(a.row_start, i + 1));
+    const int rows = rq.n * G, row0 = level * ROWS, row = row0 + l32, rowc = min(row, rows - 1), tok = rowc / G, head = kv * G + rowc - tok * G;
+    const int first = row0 / G, last = min(row0 + ROWS - 1, rows - 1) / G, lim = row < rows ? tok : -1;
+    const int nsteps = (last + STEP) / STEP;   // of all waves
+
+    u32x4 q[NK];
+    {
+        const uint16_t* qr = reinterpret_cast<const uint16_t*>(a.q) + (static_cast<ptrdiff_t>(rq.start + tok) * a.q_stride + head * HD) + 8 * h;
+#pragma unroll
+        for (int k = 0; k < NK; ++k) q[k] = *reinterpret_cast<const u32x4*>(qr + 16 * k);
+    }
+    const size_t kstride = 2 * static_cast<size_t>(a.k_stride), vstride = 2 * static_cast<size_t>(a.v_stride);
+    uint8_t* const kt = pool + wv * S::kTile;
+    uint8_t* const vt = kt + S::kHalf;
+    const uint32_t klds = lds_address(kt), vlds = lds_address(vt);
+    const int lr = lane / PIECES;   // as in the tiles above, with all of a step's rows a wave's
+    const uint32_t k_piece0 = 16 * (lane % PIECES ^ (lr & 15)), v_piece0 = 16 * (lane % PIECES ^ (v_swizzle(lr) << 1));
+    auto load = [&](const uint8_t* src, size_t stride, int sb, uint32_t to, uint32_t piece0, bool k) {
+        const int r = min(rq.start + sb, a.ntok - 1), over = r + STEP - a.ntok;
+        const uint8_t* from = src + static_cast<size_t>(r) * stride + static_cast<size_t>(kv) * ROW;
+#pragma unroll
+        for (int n = 0; n < NL; ++n) {
+            const uint32_t piece = piece0 ^ (k ? 16 * (n * PER & 15) : 32 * v_swizzle(n * PER));
+            if (over <= 0) load_lds(from + n * PER * stride, static_cast<uint32_t>(lr) * static_cast<uint32_t>(stride) + piece, to + 1024 * n);
+            else load_lds(from, static_cast<uint32_t>(min(n * PER + lr, STEP - 1 - over)) * static_cast<uint32_t>(stride) + piece, to + 1024 * n);
+        }
+    };
+    auto load_k = [&](int sb) { load(a.k, kstride, sb, klds, k_piece0, true); };
+    auto load_v = [&](int sb) { load(a.v, vstride, sb, vlds, v_piece0, false); };
+    if (wv < nsteps) {
+        load_k(wv * STEP);
+        load_v(wv * STEP);
+    }
+#pragma unroll
+    for (int k = 0; k < NK; ++k) asm volatile("" : "+v"(q[k]));   // here before the loop
+
+    floatx16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    float m_run = -INFINITY, l_run = 0.0f;
+    const int kat = l32 * ROW + ((h ^ (l32 & 15)) << 4), vp = 4 * h + ((lane & 15) >> 2);
+    const int vat = vp * ROW + ((((lane >> 4) & 1) ^ v_swizzle(vp)) << 5) + 8 * (lane & 3);
+    const bool short_rows = row0 + ROWS > rows;
+    auto v_row = [&](int at) { return VRow{a.v + (static_cast<size_t>(rq.start) + at) * vstride + static_cast<size_t>(kv) * ROW, 0, true}; };
+    for (int st = wv; st < nsteps; st += kWaves) {   // uniform in the wave
+        const int sb = st * STEP;
+        const bool more = st + kWaves < nsteps, tail = sb + STEP - 1 > first;
+        bool odd = false;
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");   // K; V's loads came after
+        tile_step<BF, HD, kKvF16, false, false>(
+            kt, vt, kat, vat, q, o, m_run, l_run, a.post, sb, last, lim, h, 0, tail || short_rows,
+            [&] {
+                if (more) {
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K is read
+                    load_k(sb + kWaves * STEP);
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");   // V; the next K came after
+                } else {
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                }
+                if (tail) {   // as in the tiles above
+                    bool found = false;
+#pragma unroll 4
+                    for (int n = 0; n < S::kHalf / 1024; ++n) found |= clear_odd<BF>(reinterpret_cast<u32x4*>(vt + 16 * (lane + 64 * n)));
+                    odd = __ballot(found) != 0;
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                }
+            },
+            [&] { return odd; }, v_row);
+        if (more) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // V is read
+            load_v(sb + kWaves * STEP);
+        }
+    }
+
+    l_run += xor_lane<32>(l_run);
+    if (h == 0) {
+        stat[wv][0][l32] = m_run;
+        stat[wv][1][l32] = l_run;
+    }
+    // a thread's pieces of the joined rows: four dims of every UP-th row; their gates on the way
+    constexpr int L4 = HD / 4, UP = kThreads / L4, NR = ROWS / UP;
+    const int piece = tid % L4, r0 = tid / L4;
+    float g[NR][4];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        const int rw = min(row0 + r0 + n * UP, rows - 1), t = rw / G;
+        load_gate<HD>(a, rq.start + t, kv * G + rw - t * G, 4 * piece, g[n]);
+    }
+    __syncthreads();   // the tiles are read
+    float* const slab = reinterpret_cast<float*>(pool);   // [part][row][HD], a row's pieces of four permuted by exclusive or with the row
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+            *reinterpret_cast<float4*>(slab + (wv * ROWS + l32) * HD + 4 * ((8 * d + r / 2 + h) ^ l32)) = make_float4(o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        const int r = r0 + n * UP, rw = row0 + r;
+        if (rw >= rows) break;   // the lanes of a block of eight stay together
+        float m = stat[0][0][r];
+#pragma unroll
+        for (int p = 1; p < kWaves; ++p) m = fmaxf(m, stat[p][0][r]);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int p = 0; p < kWaves; ++p) {
+            const float f = __builtin_amdgcn_exp2f(stat[p][0][r] - ref);
+            const float4 x = *reinterpret_cast<const float4*>(slab + (p * ROWS + r) * HD + 4 * (piece ^ r));
+            l = __builtin_fmaf(stat[p][1][r], f, l);
+            v[0] = __builtin_fmaf(x.x, f, v[0]);
+            v[1] = __builtin_fmaf(x.y, f, v[1]);
+            v[2] = __builtin_fmaf(x.z, f, v[2]);
+            v[3] = __builtin_fmaf(x.w, f, v[3]);
+        }
+        const int t = rw / G;
+        normed4(v, l, false);
+        finish4<HD>(a, rq.start + t, kv * G + rw - t * G, 4 * piece, v, g[n]);
     }
 }
 
@@ -1274,7 +1454,6 @@ constexpr int kMaxStride = 1 << 26;   // a step's rows are within 32 bits of its
 constexpr long long kMostBlocks = 0xffffffffLL / kThreads;
 
 // waves of a tile's workgroup
-constexpr int kPromptWaves = 4;
 constexpr int tile_waves(int ktype) { return ktype == kKvF16 ? 4 : 8; }
 
 template <int KT, int VT, int HD>
@@ -1296,6 +1475,33 @@ void launch_paged(const BatchArgs& a, int ktype, int vtype, bool tiles, long lon
     else if (ktype == kKvI4) launch_paged<kKvI4, kKvI4, HD>(a, tiles, few_blocks, tile_blocks, s);
     else if (vtype == kKvI8) launch_paged<kKvI8, kKvI8, HD>(a, tiles, few_blocks, tile_blocks, s);
     else launch_paged<kKvI8, kKvI4, HD>(a, tiles, few_blocks, tile_blocks, s);
+}
+
+// The chunk of a call with more rows, from what its parts cost (us; 256 dims, 32 positions a step): a workgroup's beginning and end
+// 4.5, a step 1.3 alone on its compute unit and 2.2 beside another, so that a round of up to 256 workgroups takes 4.5 + 1.3 steps and
+// one of up to 512 4.5 + 2.2 steps; the join 5 and its records at 4 TB/s.  Measured against the chunks around it, F16: 999 tokens
+// behind 8001 positions 2048 (182 / 159 / 184 us at 1024 / 2048 / 4096), behind 65501 16384 (1530 at 15872, five chunks and two
+// rounds, 1050 at 16384), 300 behind 2000 512 (41 / 40 / 55 at 256 / 512 / 1024), 16 requests of 5 behind 4096 512 (62 / 50 / 55),
+// 8 of 200 behind 1000 one chunk (62 / 54 at 512 / 1024).
+long long tile_chunk(long long total_ctx, int max_ctx, int n_req, int ntok, int max_new, int G, int n_head, int n_kv, int head_dim) {
+    const int new_each = std::min(max_new, ntok);
+    // as if all tokens were in requests of the longest kind
+    const double tiles = std::max(1.0, std::floor(static_cast<double>(ntok) / new_each + 0.5)) * most_levels(ntok, new_each, G, kTileRows) * n_kv;
+    // contexts: the requests' average, or the longest where most tokens are one request's
+    const double len = ntok < 2LL * new_each ? max_ctx : std::min(static_cast<double>(max_ctx), static_cast<double>(total_ctx) / n_req), step = 32.0 * 256 / head_dim;
+    double best = 0.0;
+    long long chunk = 0;
+    for (int k = 1, before = 0; k <= 512; ++k) {
+        const int c = static_cast<int>((static_cast<long long>(max_ctx) + static_cast<long long>(k) * kChunkUnit - 1) / (static_cast<long long>(k) * kChunkUnit)) * kChunkUnit;
+        if (c == before) continue;
+        before = c;
+        const int chunks = chunks_of(max_ctx, c);
+        const double groups = tiles * (n_req == 1 ? chunks : std::min<double>(chunks, len / c + (chunks > 1 ? 0.5 : 0.0))), steps = std::ceil(std::min<double>(c, max_ctx) / step);
+        const double round = 4.5 + (groups <= 256 ? 1.3 : 2.2) * steps, rounds = std::max(1.0, std::ceil(groups * (n_req > 1 ? 1.06 : 1.0) / 512));   // ragged: some more than the average says
+        const double cost = round * rounds + (chunks > 1 ? 5.0 + static_cast<double>(chunks) * ntok * n_head * head_dim * 4 / 4e6 : 0.0);
+        if (chunk == 0 || cost < best) best = cost, chunk = c;
+    }
+    return chunk;
 }
 
 }  // namespace
@@ -1321,8 +1527,7 @@ extern "C" int rmi_gqa_paged_split(long long total_ctx, int max_ctx, int n_req, 
             chunk = slots > 0 ? (2 * total * n_kv + slots - 1) / slots : max_ctx;
         } while (++rounds <= 8 && 256 * chunk > 2 * total * n_kv);
     } else {
-        // more rows: about 512 workgroups, two a compute unit
-        chunk = std::max(1LL, static_cast<long long>(ntok) * G / kTileRows) * n_kv * max_ctx / 512;
+        chunk = tile_chunk(total_ctx, max_ctx, n_req, ntok, max_new, G, n_head, n_kv, head_dim);
     }
     chunk = std::max<long long>(chunk, (static_cast<long long>(max_ctx) + kMaxChunks - 1) / kMaxChunks);
     chunk = std::min<long long>(std::max(chunk, 1LL), max_ctx);
@@ -1391,7 +1596,8 @@ extern "C" int rmi_gqa_paged_attn(int qtype, const void* q, int ktype, const voi
     a.bf16 = qtype == RMI_ROWS_BF16;
     a.post = scale * kLog2e;
     const bool tiles = static_cast<long long>(std::min(max_new, ntok)) * G > kFewRows;
-    const long long few = static_cast<long long>(n_req) * n_kv * chunks, tile = most_tiles(n_req, ntok, max_new, G, held) * n_kv * chunks;
+    a.tiles = static_cast<int>(most_tiles(n_req, ntok, max_new, G, held));   // at most 2^24 64 / 128 + 4096
+    const long long few = static_cast<long long>(n_req) * n_kv * chunks, tile = static_cast<long long>(a.tiles) * n_kv * chunks;
     if (few > kMostBlocks || (tiles && tile > kMostBlocks / 2) || static_cast<long long>(ntok) * n_head > kMostBlocks)
         return fail(RMI_ERR_SHAPE, "gqa_paged_attn: too many workgroups");
     auto* s = static_cast<hipStream_t>(stream);
@@ -1434,16 +1640,32 @@ extern "C" int rmi_gqa_prompt_attn(int type, const void* q, int q_stride, const 
     a.n_kv = n_kv;
     a.chunk = (ntok + kChunkUnit - 1) / kChunkUnit * kChunkUnit;
     a.chunks = 1;
-    const int held = kWaveRows * kPromptWaves;
-    a.levels = most_levels(ntok, max_len, G, held);
     a.bf16 = type == RMI_ROWS_BF16;
     a.post = scale * kLog2e;
-    const long long blocks = most_tiles(n_req, ntok, max_len, G, held) * n_kv;
+    // Three forms.  Eight waves over 256 rows, which share a tile's K and V, from about two rounds of workgroups on: one prompt of 8001
+    // tokens (504 tiles, 16 heads, 4 KV heads of 256 dims) 505 us with 128 rows, 485 with 256; of 4000 (252) 190 / 196.  32 rows with the
+    // positions in four parts where prompts are long enough for steps to part and tiles few: one prompt of 128 / 500 / 750 tokens (64 /
+    // 252 / 376 tiles of 32) 14.0 / 24.1 / 36 us, tiles of 128 rows 17.5 / 31.6 / 41; but 20 prompts of 25 tokens on average (260 tiles,
+    // 3 levels) 26.5 / 16.6 and ten of 100 (540 tiles) 40 / 23.5.  128 rows else.
+    const bool wide = most_tiles(n_req, ntok, max_len, G, 8 * kWaveRows) * n_kv >= 480;
+    const bool parts = !wide && most_levels(ntok, max_len, G, 4 * kWaveRows) >= 4 && most_tiles(n_req, ntok, max_len, G, kWaveRows) * n_kv <= 400;
+    const int held = parts ? kWaveRows : (wide ? 8 : 4) * kWaveRows;
+    a.levels = most_levels(ntok, max_len, G, held);
+    a.tiles = static_cast<int>(most_tiles(n_req, ntok, max_len, G, held));
+    const long long blocks = static_cast<long long>(a.tiles) * n_kv;
     if (blocks > kMostBlocks) return fail(RMI_ERR_SHAPE, "gqa_prompt_attn: too many workgroups");
-    auto go = [&](auto* kernel) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kPromptWaves), 0, static_cast<hipStream_t>(stream), a);
+    auto go = [&](auto* kernel, int waves) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * waves), 0, static_cast<hipStream_t>(stream), a);
         return launch_status("gqa_prompt_attn");
     };
-    if (a.bf16) return head_dim == 256 ? go(&batch_tile_kernel<kRowsBF16, kKvF16, kKvF16, 256, kPromptWaves>) : go(&batch_tile_kernel<kRowsBF16, kKvF16, kKvF16, 128, kPromptWaves>);
-    return head_dim == 256 ? go(&batch_tile_kernel<kRowsF16, kKvF16, kKvF16, 256, kPromptWaves>) : go(&batch_tile_kernel<kRowsF16, kKvF16, kKvF16, 128, kPromptWaves>);
+    auto with = [&](auto bf, auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        constexpr bool BF = decltype(bf)::value;
+        constexpr int SRC = BF ? kRowsBF16 : kRowsF16;
+        if (parts) return go(&batch_parts_kernel<BF, HD>, kWaves);
+        if (wide) return go(&batch_tile_kernel<SRC, kKvF16, kKvF16, HD, 8>, 8);
+        return go(&batch_tile_kernel<SRC, kKvF16, kKvF16, HD, 4>, 4);
+    };
+    auto of_type = [&](auto bf) { return head_dim == 256 ? with(bf, std::integral_constant<int, 256>{}) : with(bf, std::integral_constant<int, 128>{}); };
+    return a.bf16 ? of_type(std::true_type{}) : of_type(std::false_type{});
 }

@@ -389,7 +389,8 @@ def test_prompt_unseen_rows(rmi, name, hd):
 
 
 def test_prompt_equals_pages(rmi):
-    """a prompt over its packed rows and over an fp16 page pool whose slots are in order: the same products, the same bits"""
+    """a prompt over its packed rows and over an fp16 page pool whose slots are in order: the same rows.  The forms add a row's weights
+    in different orders, so each is held to the formula by its bound, and with it to the other"""
     t = torch()
     rng = np.random.default_rng(1)
     n, n_kv, G, hd = 200, 2, 4, 256
@@ -400,4 +401,6 @@ def test_prompt_equals_pages(rmi):
     rmi.gqa_prompt_attn(q, nh * hd, k, n_kv * hd, v, n_kv * hd, start, None, 0, y[0], nh * hd, None, 0, 1, n, n, nh, n_kv, hd, scale)
     rmi.gqa_paged_attn(q, rmi.KV_F16, k, rmi.KV_F16, v, ints([0, 1, 2, 3]), 4, start, ints([n]), None, 0, y[1], nh * hd, None, 0, None, 1, n,
                        n, n, nh, n_kv, hd, 64, 4, 256, scale)
-    assert t.equal(y[0], y[1])
+    want, bound = ref.attention(*(x[:n].double().cpu().numpy() for x in (q, k, v)), 0, float(np.float32(scale)), None, 2.0 ** -11, 2.0 ** -11)
+    for got in y:
+        assert (np.abs(got.double().cpu().numpy() - want) <= bound).all()
