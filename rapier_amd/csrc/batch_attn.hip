@@ -44,7 +44,7 @@ struct BatchArgs {
     float *wo, *wml;   // records: o [chunk][row][head][HD], (m, l) [chunk][row][head][2]
     int q_stride, k_stride, v_stride, gate_stride, y_stride, q8_stride;   // elements (q8: bytes)
     int table_stride, n_req, ntok, max_new, max_ctx, n_head, n_kv, shift, n_pages;
-    int chunk, chunks, tiles, levels, skip_few, bf16;   // tiles: of rows, at most; levels: of a request's tiles, at most
+    int chunk, chunks, levels, bf16;   // levels: the most tiles of a prompt
     float post;   // score = q.k * post, in base 2
 };
 
@@ -124,7 +124,7 @@ __device__ __forceinline__ bool find_tile(const BatchArgs& a, int* counts, uint3
     const int tid = threadIdx.x, lane = tid & 63;
     auto tiles_of = [&](int k) {
         const int rows = request(a, k, a.row_start[k], a.row_start[k + 1]).n * G;
-        return a.skip_few && rows <= kFewRows ? 0 : (rows + ROWS - 1) / ROWS;
+        return (rows + ROWS - 1) / ROWS;
     };
     bool has;
     if (a.n_req <= 64) {   // a request a lane
@@ -141,29 +141,30 @@ __device__ __forceinline__ bool find_tile(const BatchArgs& a, int* counts, uint3
     return has;
 }
 
-// The chunk of a few-rows workgroup by its rank among those of the call: the requests' chunks one behind another, so that the
-// workgroups that have work are the first ones, as many to each XCD (they go there in turn), and a round of one for each compute
-// unit is one.  (Launched as requests times the longest one's chunks, with the others' ends empty: 32 requests of 1 K to 4 K
-// positions in chunks of 1792 78 us; so 70.)
-__device__ __forceinline__ bool chunk_of_rank(const BatchArgs& a, uint32_t rank, int G, int* req, int* chunk) {
+// A paged call's work by its rank: the requests' items one behind another, count(request) of each, so that the workgroups that have
+// work are the first ones, as many to each XCD (they go there in turn), and a round of one for each compute unit is one.  (Launched
+// as every request's items to the longest one's, 32 requests of one token behind 1 K to 4 K positions took 78 us in chunks of 1792,
+// so 70; two of 40 tokens behind 30 K and 15 K, I8, in chunks of 768, 128 and XX.)  False: the call has no such item.
+template <typename F>
+__device__ __forceinline__ bool item_of_rank(const BatchArgs& a, uint32_t rank, F&& count, int* req, int* item) {
     const int lane = threadIdx.x & 63;
     for (int i0 = 0; i0 < a.n_req; i0 += 64) {
         const int i = min(i0 + lane, a.n_req - 1);
-        const Req r = request(a, i, a.row_start[i], a.row_start[i + 1]);
-        const int rows = r.n * G;
-        uint32_t n = i0 + lane < a.n_req && rows > 0 && rows <= kFewRows ? max((r.len + a.chunk - 1) / a.chunk, 1) : 0;
+        const uint32_t n = i0 + lane < a.n_req ? count(request(a, i, a.row_start[i], a.row_start[i + 1])) : 0;
         const uint32_t upto = wave_scan(n, [](uint32_t x, uint32_t y) { return x + y; });
         const uint64_t past = __ballot(upto > rank);
         if (past) {
             const int l = __builtin_ctzll(past);
             *req = i0 + l;
-            *chunk = static_cast<int>(rank) - __builtin_amdgcn_readlane(static_cast<int>(upto - n), l);
+            *item = static_cast<int>(rank) - __builtin_amdgcn_readlane(static_cast<int>(upto - n), l);
             return true;
         }
         rank -= static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
     }
     return false;
 }
+// chunks of a request's positions, one at least (its rows are written there)
+__device__ __forceinline__ int chunks_in(const BatchArgs& a, int len) { return max((len + a.chunk - 1) / a.chunk, 1); }
 
 // ---- 16-bit rows -----------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) { return u2(__builtin_convertvector(floatx2{a, b}, half2v)); }
@@ -262,7 +263,8 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void batch_few_kern
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
     const int kv = blockIdx.x % a.n_kv, G = a.n_head / a.n_kv;
     int i = 0, chunk = 0;
-    if (!chunk_of_rank(a, blockIdx.x / a.n_kv, G, &i, &chunk)) return;   // uniform
+    auto count = [&](const Req& r) { return r.n > 0 && r.n * G <= kFewRows ? chunks_in(a, r.len) : 0; };
+    if (!item_of_rank(a, blockIdx.x / a.n_kv, count, &i, &chunk)) return;   // uniform
     const Req rq = request(a, i, word(a.row_start, i), word(a.row_start, i + 1));
     const int rows = rq.n * G, base = rq.len - rq.n, last = rq.len - 1, c0 = chunk * a.chunk;
     const int row = l16, rowc = min(row, rows - 1), tok = rowc / G;
@@ -801,14 +803,21 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
 
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, h = lane >> 5;
     const int G = a.n_head / a.n_kv;
-    // KV heads innermost: workgroups go to the XCDs round robin, so a head's tiles meet its K and V in one or two L2s.  Chunks
-    // outermost: those that not every request has are the last, and lie over the XCDs as the tiles do.  (Chunks next to the heads, as
-    // many or none by turns, were 16 I8 requests of 16 tokens behind 1 K to 4 K in 896s 67 or 103 us, as it fell out.)
-    const int kv = blockIdx.x % a.n_kv, chunk = blockIdx.x / a.n_kv / a.tiles;
-    const uint32_t rank = blockIdx.x / a.n_kv % a.tiles;
-    int i = 0, level = 0;
+    // KV heads innermost: workgroups go to the XCDs round robin, so a head's tiles meet its K and V in one or two L2s
+    const int kv = blockIdx.x % a.n_kv;
+    const uint32_t rank = blockIdx.x / a.n_kv;
+    int i = 0, level = 0, chunk = 0;
     if (tid < 2) odd[tid] = 0;
-    if (!find_tile<ROWS, THREADS>(a, reinterpret_cast<int*>(pool), rank, G, &i, &level)) return;   // uniform
+    if constexpr (PAGED) {
+        auto tiles = [&](int n) { return (n * G + ROWS - 1) / ROWS; };
+        int item = 0;
+        if (!item_of_rank(a, rank, [&](const Req& r) { return r.n * G > kFewRows ? tiles(r.n) * chunks_in(a, r.len) : 0; }, &i, &item)) return;   // uniform
+        const int n = tiles(request(a, i, word(a.row_start, i), word(a.row_start, i + 1)).n);
+        chunk = item / n;
+        level = n - 1 - item % n;
+    } else {
+        if (!find_tile<ROWS, THREADS>(a, reinterpret_cast<int*>(pool), rank, G, &i, &level)) return;   // uniform
+    }
     const Req rq = request(a, i, word(a.row_start, i), word(a.row_start, i + 1));
     const int rows = rq.n * G, base = rq.len - rq.n, c0 = chunk * a.chunk;
     const int first = base + level * ROWS / G, last = base + min(level * ROWS + ROWS - 1, rows - 1) / G;   // of the workgroup's tokens
@@ -1488,7 +1497,8 @@ long long tile_chunk(long long total_ctx, int max_ctx, int n_req, int ntok, int 
     // as if all tokens were in requests of the longest kind
     const double tiles = std::max(1.0, std::floor(static_cast<double>(ntok) / new_each + 0.5)) * most_levels(ntok, new_each, G, kTileRows) * n_kv;
     // contexts: the requests' average, or the longest where most tokens are one request's
-    const double len = ntok < 2LL * new_each ? max_ctx : std::min(static_cast<double>(max_ctx), static_cast<double>(total_ctx) / n_req), step = 32.0 * 256 / head_dim;
+    const bool one = n_req == 1 || ntok < 2LL * new_each;
+    const double len = one ? max_ctx : std::min(static_cast<double>(max_ctx), static_cast<double>(total_ctx) / n_req), step = 32.0 * 256 / head_dim;
     double best = 0.0;
     long long chunk = 0;
     for (int k = 1, before = 0; k <= 512; ++k) {
@@ -1496,8 +1506,8 @@ long long tile_chunk(long long total_ctx, int max_ctx, int n_req, int ntok, int 
         if (c == before) continue;
         before = c;
         const int chunks = chunks_of(max_ctx, c);
-        const double groups = tiles * (n_req == 1 ? chunks : std::min<double>(chunks, len / c + (chunks > 1 ? 0.5 : 0.0))), steps = std::ceil(std::min<double>(c, max_ctx) / step);
-        const double round = 4.5 + (groups <= 256 ? 1.3 : 2.2) * steps, rounds = std::max(1.0, std::ceil(groups * (n_req > 1 ? 1.06 : 1.0) / 512));   // ragged: some more than the average says
+        const double groups = tiles * (one ? chunks : std::min<double>(chunks, len / c + (chunks > 1 ? 0.5 : 0.0))), steps = std::ceil(std::min<double>(c, max_ctx) / step);
+        const double round = 4.5 + (groups <= 256 ? 1.3 : 2.2) * steps, rounds = std::max(1.0, std::ceil(groups * (one ? 1.0 : 1.06) / 512));   // ragged: some more than the average says
         const double cost = round * rounds + (chunks > 1 ? 5.0 + static_cast<double>(chunks) * ntok * n_head * head_dim * 4 / 4e6 : 0.0);
         if (chunk == 0 || cost < best) best = cost, chunk = c;
     }
@@ -1591,13 +1601,10 @@ extern "C" int rmi_gqa_paged_attn(int qtype, const void* q, int ktype, const voi
     a.wo = static_cast<float*>(workspace);
     a.wml = a.wo + static_cast<size_t>(chunks) * ntok * n_head * head_dim;
     const int held = kWaveRows * tile_waves(ktype);
-    a.levels = most_levels(ntok, max_new, G, held);
-    a.skip_few = 1;
     a.bf16 = qtype == RMI_ROWS_BF16;
     a.post = scale * kLog2e;
     const bool tiles = static_cast<long long>(std::min(max_new, ntok)) * G > kFewRows;
-    a.tiles = static_cast<int>(most_tiles(n_req, ntok, max_new, G, held));   // at most 2^24 64 / 128 + 4096
-    const long long few = static_cast<long long>(n_req) * n_kv * chunks, tile = static_cast<long long>(a.tiles) * n_kv * chunks;
+    const long long few = static_cast<long long>(n_req) * n_kv * chunks, tile = most_tiles(n_req, ntok, max_new, G, held) * n_kv * chunks;
     if (few > kMostBlocks || (tiles && tile > kMostBlocks / 2) || static_cast<long long>(ntok) * n_head > kMostBlocks)
         return fail(RMI_ERR_SHAPE, "gqa_paged_attn: too many workgroups");
     auto* s = static_cast<hipStream_t>(stream);
@@ -1642,17 +1649,18 @@ extern "C" int rmi_gqa_prompt_attn(int type, const void* q, int q_stride, const 
     a.chunks = 1;
     a.bf16 = type == RMI_ROWS_BF16;
     a.post = scale * kLog2e;
-    // Three forms.  Eight waves over 256 rows, which share a tile's K and V, from about two rounds of workgroups on: one prompt of 8001
-    // tokens (504 tiles, 16 heads, 4 KV heads of 256 dims) 505 us with 128 rows, 485 with 256; of 4000 (252) 190 / 196.  32 rows with the
-    // positions in four parts where prompts are long enough for steps to part and tiles few: one prompt of 128 / 500 / 750 tokens (64 /
-    // 252 / 376 tiles of 32) 14.0 / 24.1 / 36 us, tiles of 128 rows 17.5 / 31.6 / 41; but 20 prompts of 25 tokens on average (260 tiles,
-    // 3 levels) 26.5 / 16.6 and ten of 100 (540 tiles) 40 / 23.5.  128 rows else.
-    const bool wide = most_tiles(n_req, ntok, max_len, G, 8 * kWaveRows) * n_kv >= 480;
+    // Three forms.  Eight waves over 256 rows, which share a tile's K and V, for long prompts from about two rounds of workgroups on:
+    // one prompt of 8001 tokens (504 tiles, 16 heads, 4 KV heads of 256 dims) 505 us with 128 rows, 485 with 256; of 4000 (252) 190 /
+    // 196; 40 of 200 (664, up to 13 levels) 103 / 110.  32 rows with the positions in four parts where prompts are long enough for
+    // steps to part and tiles few: one prompt of 128 / 500 / 750 tokens (64 / 252 / 376 tiles of 32) 14.0 / 24.1 / 36 us, tiles of 128
+    // rows 17.5 / 31.6 / 41; but 20 prompts of 25 tokens on average (260 tiles, 3 levels) 26.5 / 16.6 and ten of 100 (540 tiles) 40 /
+    // 23.5.  128 rows else.
+    const int most_rows = 8 * kWaveRows;
+    const bool wide = most_levels(ntok, max_len, G, most_rows) >= 64 && most_tiles(n_req, ntok, max_len, G, most_rows) * n_kv >= 480;
     const bool parts = !wide && most_levels(ntok, max_len, G, 4 * kWaveRows) >= 4 && most_tiles(n_req, ntok, max_len, G, kWaveRows) * n_kv <= 400;
     const int held = parts ? kWaveRows : (wide ? 8 : 4) * kWaveRows;
     a.levels = most_levels(ntok, max_len, G, held);
-    a.tiles = static_cast<int>(most_tiles(n_req, ntok, max_len, G, held));
-    const long long blocks = static_cast<long long>(a.tiles) * n_kv;
+    const long long blocks = most_tiles(n_req, ntok, max_len, G, held) * n_kv;
     if (blocks > kMostBlocks) return fail(RMI_ERR_SHAPE, "gqa_prompt_attn: too many workgroups");
     auto go = [&](auto* kernel, int waves) {
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * waves), 0, static_cast<hipStream_t>(stream), a);
