@@ -5,8 +5,8 @@
 //
 // Query row r of a request and KV head is token r / G, head r % G of the head's G.  Token t of n new ones is at position
 // len - n + t and sees the positions up to its own.  Three kernels:
-//   few     up to 16 rows a request (decode, short drafts): workgroup (request, KV head, chunk of positions), K and V straight from
-//           the pages into matrix operands; bound by the cache
+//   few     up to 16 rows a request, 32 of a quantised cache (decode, drafts): workgroup (request, KV head, chunk of positions), K
+//           and V straight from the pages into matrix operands; bound by the cache
 //   tile    more rows: workgroup (128 rows, KV head, chunk), K and V tiles in LDS
 //   join    the chunks' records (m, l, o) of a row, where the context is split
 // A paged call with requests of both kinds launches both of the first two; each takes its own requests.
@@ -44,7 +44,7 @@ struct BatchArgs {
     float *wo, *wml;   // records: o [chunk][row][head][HD], (m, l) [chunk][row][head][2]
     int q_stride, k_stride, v_stride, gate_stride, y_stride, q8_stride;   // elements (q8: bytes)
     int table_stride, n_req, ntok, max_new, max_ctx, n_head, n_kv, shift, n_pages;
-    int chunk, chunks, levels, bf16;   // levels: the most tiles of a prompt
+    int chunk, chunks, levels, few, bf16;   // levels: the most tiles of a prompt; few: the rows that the form of few rows takes
     float post;   // score = q.k * post, in base 2
 };
 
@@ -144,7 +144,7 @@ __device__ __forceinline__ bool find_tile(const BatchArgs& a, int* counts, uint3
 // A paged call's work by its rank: the requests' items one behind another, count(request) of each, so that the workgroups that have
 // work are the first ones, as many to each XCD (they go there in turn), and a round of one for each compute unit is one.  (Launched
 // as every request's items to the longest one's, 32 requests of one token behind 1 K to 4 K positions took 78 us in chunks of 1792,
-// so 70; two of 40 tokens behind 30 K and 15 K, I8, in chunks of 768, 128 and XX.)  False: the call has no such item.
+// so 70; two of 40 tokens behind 30 K and 15 K, I8, in chunks of 768, 128 and 83.)  False: the call has no such item.
 template <typename F>
 __device__ __forceinline__ bool item_of_rank(const BatchArgs& a, uint32_t rank, F&& count, int* req, int* item) {
     const int lane = threadIdx.x & 63;
@@ -250,31 +250,37 @@ struct Half {
     Rsrc kr, ks, vr, vs;
 };
 
-template <int KT, int VT, int HD>
-__global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void batch_few_kernel(BatchArgs a) {
+template <int KT, int VT, int HD, int RB>
+__global__ __launch_bounds__(kThreads, KT == kKvF16 || RB == 2 ? 1 : 2) void batch_few_kernel(BatchArgs a) {
     constexpr int NI = HD / 64;        // K: 16-dim pieces a lane takes of a position, two to a 32-dim run
     constexpr int VD = HD / 16;        // V: dims a lane takes of a position
     constexpr int NB = HD / kKvBlock;  // scale bytes of a row
+    constexpr int ROWS = kFewRows * RB;
     constexpr int kKB = kv_row_bytes(KT, HD), kVB = kv_row_bytes(VT, HD);
-    __shared__ __attribute__((aligned(16))) float slab[kWaves][kFewRows][HD];   // the rows that are joined
-    __shared__ float pb[kWaves][kFewRows][32];   // a step's p where a V is not finite
-    __shared__ float stat[kWaves][2][kFewRows], fac[kWaves][kFewRows], sum[2][kFewRows];
+    __shared__ __attribute__((aligned(16))) float slab[kWaves][ROWS][HD];   // the rows that are joined
+    __shared__ float pb[kWaves][ROWS][32];   // a step's p where a V is not finite
+    __shared__ float stat[kWaves][2][ROWS], fac[kWaves][ROWS], sum[2][ROWS];
 
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
     const int kv = blockIdx.x % a.n_kv, G = a.n_head / a.n_kv;
     int i = 0, chunk = 0;
-    auto count = [&](const Req& r) { return r.n > 0 && r.n * G <= kFewRows ? chunks_in(a, r.len) : 0; };
+    auto count = [&](const Req& r) { return r.n > 0 && r.n * G <= ROWS ? chunks_in(a, r.len) : 0; };
     if (!item_of_rank(a, blockIdx.x / a.n_kv, count, &i, &chunk)) return;   // uniform
     const Req rq = request(a, i, word(a.row_start, i), word(a.row_start, i + 1));
     const int rows = rq.n * G, base = rq.len - rq.n, last = rq.len - 1, c0 = chunk * a.chunk;
-    const int row = l16, rowc = min(row, rows - 1), tok = rowc / G;
-    const uint16_t* qr = reinterpret_cast<const uint16_t*>(a.q) + (static_cast<ptrdiff_t>(rq.start + tok) * a.q_stride + (kv * G + rowc - tok * G) * HD) + 32 * g4;
-    u32x4 qb[NI][2];
+    const bool second = RB == 2 && rows > kFewRows;   // uniform: the second 16 rows are there
+    u32x4 qb[RB][NI][2];
+    int lim[RB];   // row 16 b + l16 sees every position up to here
 #pragma unroll
-    for (int k = 0; k < NI; ++k)
+    for (int b = 0; b < RB; ++b) {
+        const int row = kFewRows * b + l16, rowc = min(row, rows - 1), tok = rowc / G;
+        const uint16_t* qr = reinterpret_cast<const uint16_t*>(a.q) + (static_cast<ptrdiff_t>(rq.start + tok) * a.q_stride + (kv * G + rowc - tok * G) * HD) + 32 * g4;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) qb[k][hf] = *reinterpret_cast<const u32x4*>(qr + 128 * (k >> 1) + 16 * (k & 1) + 8 * hf);
-    const int lim = row >= rows ? -1 : base + tok;   // the row sees every position up to here
+        for (int k = 0; k < NI; ++k)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) qb[b][k][hf] = *reinterpret_cast<const u32x4*>(qr + 128 * (k >> 1) + 16 * (k & 1) + 8 * hf);
+        lim[b] = row >= rows ? -1 : base + tok;
+    }
     const int end = min(last + 1, c0 + a.chunk);
     const int total = max(end - c0 + 31, 0) / 32, nsteps = max(total - wv + kWaves - 1, 0) / kWaves;
 
@@ -356,94 +362,117 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void batch_few_kern
     load_v(sb, id);
     int nid[2] = {page_at(sb + 32 * kWaves), page_at(sb + 32 * kWaves + 16)};
 
-    float post = a.post * kSixteen<KT>;
-    if (a.bf16) {   // uniform: q as fp16, a row's largest brought to [2^13, 2^14)
-        uint32_t m = 0;
+    float post[RB];
 #pragma unroll
-        for (int k = 0; k < NI; ++k)
+    for (int b = 0; b < RB; ++b) {
+        post[b] = a.post * kSixteen<KT>;
+        if (a.bf16) {   // uniform: q as fp16, a row's largest brought to [2^13, 2^14)
+            uint32_t m = 0;
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
+            for (int k = 0; k < NI; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) m = max_magnitude(m, qb[k][hf][e]);
-        float top = __uint_as_float(max(m << 16, m & 0xffff0000u));
-        top = fmaxf(top, xor_lane<16>(top));
-        top = fmaxf(top, xor_lane<32>(top));
-        const int sh = q_shift(top);
-        post *= ldexpf(1.0f, -sh);
+                for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-        for (int k = 0; k < NI; ++k)
+                    for (int e = 0; e < 4; ++e) m = max_magnitude(m, qb[b][k][hf][e]);
+            float top = __uint_as_float(max(m << 16, m & 0xffff0000u));
+            top = fmaxf(top, xor_lane<16>(top));
+            top = fmaxf(top, xor_lane<32>(top));
+            const int sh = q_shift(top);
+            post[b] *= ldexpf(1.0f, -sh);
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
+            for (int k = 0; k < NI; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) qb[k][hf][e] = bf16_to_f16(qb[k][hf][e], sh);
+                for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) qb[b][k][hf][e] = bf16_to_f16(qb[b][k][hf][e], sh);
+        }
     }
-    floatx4 o[VD];
+    floatx4 o[RB][VD];
+    float m_run[RB], l_run[RB];   // l_run: this lane's positions only
 #pragma unroll
-    for (int e = 0; e < VD; ++e) o[e] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m_run = -INFINITY, l_run = 0.0f;   // l_run: this lane's positions only
+    for (int b = 0; b < RB; ++b) {
+#pragma unroll
+        for (int e = 0; e < VD; ++e) o[b][e] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        m_run[b] = -INFINITY;
+        l_run[b] = 0.0f;
+    }
 
     for (int st = 0; st < nsteps; ++st) {
-        float sc[8];   // j: position sb + 4 g4 + j, or 16 + 4 g4 + j - 4 further
+        float sc[RB][8];   // j: position sb + 4 g4 + j, or 16 + 4 g4 + j - 4 further
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            floatx4 acc[RB];
+#pragma unroll
+            for (int b = 0; b < RB; ++b) acc[b] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int k = 0; k < NI; ++k) {
                 Scale2 s = {};
                 if constexpr (KT != kKvF16) {   // block 4 (k / 2) + g4
-                    const uint32_t b = (ksc[t][k >> 1] >> (8 * g4)) & 0xffu;
-                    s = scale2<KT>(b, b);
+                    const uint32_t byte = (ksc[t][k >> 1] >> (8 * g4)) & 0xffu;
+                    s = scale2<KT>(byte, byte);
                 }
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) acc = mfma16(operand<KT>(kx[t][k], hf, s), __builtin_bit_cast(half8, qb[k][hf]), acc);
+                for (int hf = 0; hf < 2; ++hf) {
+                    const half8 kk = operand<KT>(kx[t][k], hf, s);
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) acc[b] = mfma16(kk, __builtin_bit_cast(half8, qb[b][k][hf]), acc[b]);
+                }
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sc[4 * t + r] = acc[r] * post;
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sc[b][4 * t + r] = acc[b][r] * post[b];
         }
         const int bad = (id[0] < 0 && sb < end ? 1 : 0) | (id[1] < 0 && sb + 16 < end ? 2 : 0);   // uniform
         // the loads are not under a branch: behind one, every wait would be for all that might be out
         const int next = sb + 32 * kWaves;
         load_k(next, nid);
-        if (bad)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (bad >> (j >> 2) & 1) sc[j] = __builtin_nanf("");
         const bool tail = sb + 31 > base;   // uniform: not every row sees the whole step
-        uint32_t seen = 0xffu;
-        if (tail || row >= rows) {
-            seen = 0;
+        half8 ph[RB];
+        uint32_t seen[RB];
+        float p[RB][8];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            if (bad)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (bad >> (j >> 2) & 1) sc[b][j] = __builtin_nanf("");
+            seen[b] = 0xffu;
+            if (tail || kFewRows * (b + 1) > rows) {
+                seen[b] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (sb + 4 * g4 + (j < 4 ? j : 12 + j) <= lim[b]) seen[b] |= 1u << j;
+                    else sc[b][j] = -INFINITY;
+                }
+            }
+            float mloc = sc[b][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) mloc = fmaxf(mloc, sc[b][j]);
+            mloc = fmaxf(mloc, xor_lane<16>(mloc));
+            mloc = fmaxf(mloc, xor_lane<32>(mloc));
+            const float m_new = mloc > m_run[b] + kLazy ? mloc : m_run[b];
+            const float m_ref = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: exp2(-inf) = 0, no NaN
+            const float alpha = m_run[b] == m_new || m_run[b] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run[b] - m_ref);   // -inf: o is 0
+            float lsum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (sb + 4 * g4 + (j < 4 ? j : 12 + j) <= lim) seen |= 1u << j;
-                else sc[j] = -INFINITY;
+                p[b][j] = __builtin_amdgcn_exp2f(sc[b][j] - m_ref + kPScale);
+                lsum += p[b][j];
             }
+            l_run[b] = l_run[b] * alpha + lsum;
+            m_run[b] = m_new;
+            if (__ballot(alpha != 1.0f)) {   // uniform: some row's maximum moved
+                float al[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) al[r] = __shfl(alpha, 4 * g4 + r, 64);
+#pragma unroll
+                for (int e = 0; e < VD; ++e)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[b][e][r] *= al[r];
+            }
+            ph[b] = h8(pack_f16(p[b][0], p[b][1]), pack_f16(p[b][2], p[b][3]), pack_f16(p[b][4], p[b][5]), pack_f16(p[b][6], p[b][7]));
         }
-        float mloc = sc[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) mloc = fmaxf(mloc, sc[j]);
-        mloc = fmaxf(mloc, xor_lane<16>(mloc));
-        mloc = fmaxf(mloc, xor_lane<32>(mloc));
-        const float m_new = mloc > m_run + kLazy ? mloc : m_run;
-        const float m_ref = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: exp2(-inf) = 0, no NaN
-        const float alpha = m_run == m_new || m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_ref);   // -inf: o is 0
-        float p[8], lsum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(sc[j] - m_ref + kPScale);
-            lsum += p[j];
-        }
-        l_run = l_run * alpha + lsum;
-        m_run = m_new;
-        if (__ballot(alpha != 1.0f)) {   // uniform: some row's maximum moved
-            float al[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) al[r] = __shfl(alpha, 4 * g4 + r, 64);
-#pragma unroll
-            for (int e = 0; e < VD; ++e)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[e][r] *= al[r];
-        }
-        const half8 ph = h8(pack_f16(p[0], p[1]), pack_f16(p[2], p[3]), pack_f16(p[4], p[5]), pack_f16(p[6], p[7]));
         Scale2 vsp[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -464,7 +493,9 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void batch_few_kern
             if (__ballot(!finite16(big))) {
                 float(*pw)[32] = pb[wv];   // [row][position], -1: not seen
 #pragma unroll
-                for (int j = 0; j < 8; ++j) pw[l16][4 * g4 + (j < 4 ? j : 12 + j)] = seen >> j & 1 ? p[j] : -1.0f;
+                for (int b = 0; b < RB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) pw[kFewRows * b + l16][4 * g4 + (j < 4 ? j : 12 + j)] = seen[b] >> j & 1 ? p[b][j] : -1.0f;
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 for (int pp = 0; pp < 32; ++pp) {
                     const int p1 = sb + pp, pid = pp < 16 ? id[0] : id[1];
@@ -478,10 +509,12 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void batch_few_kern
                         else v = odd_value<VT>(page[at.scale + VD * l16 / kKvBlock]);
                         if (fabsf(v) <= FLT_MAX) continue;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float x = pw[4 * g4 + r][pp];
-                            if (!(x < 0.0f)) o[e][r] = __builtin_fmaf(x, v, o[e][r]);
-                        }
+                        for (int b = 0; b < RB; ++b)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float x = pw[kFewRows * b + 4 * g4 + r][pp];
+                                if (!(x < 0.0f)) o[b][e][r] = __builtin_fmaf(x, v, o[b][e][r]);
+                            }
                     }
                 }
 #pragma unroll
@@ -503,8 +536,12 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void batch_few_kern
             uint32_t ev[4], od[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) v_pair<VT, VD>(vx[2 * j], vx[2 * j + 1], e, vsp[j], ev[j], od[j]);
-            o[2 * e] = mfma16(ph, h8(ev[0], ev[1], ev[2], ev[3]), o[2 * e]);
-            o[2 * e + 1] = mfma16(ph, h8(od[0], od[1], od[2], od[3]), o[2 * e + 1]);
+            const half8 v0 = h8(ev[0], ev[1], ev[2], ev[3]), v1 = h8(od[0], od[1], od[2], od[3]);
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                o[b][2 * e] = mfma16(ph[b], v0, o[b][2 * e]);
+                o[b][2 * e + 1] = mfma16(ph[b], v1, o[b][2 * e + 1]);
+            }
         }
         load_v(next, nid);
         sb = next;
@@ -512,19 +549,24 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 ? 1 : 2) void batch_few_kern
         nid[0] = page_at(sb + 32 * kWaves), nid[1] = page_at(sb + 32 * kWaves + 16);
     }
 
-    l_run += xor_lane<16>(l_run);
-    l_run += xor_lane<32>(l_run);
-    if (g4 == 0) {
-        stat[wv][0][l16] = m_run;
-        stat[wv][1][l16] = l_run;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        if (b == 1 && !second) break;
+        l_run[b] += xor_lane<16>(l_run[b]);
+        l_run[b] += xor_lane<32>(l_run[b]);
+        if (g4 == 0) {
+            stat[wv][0][kFewRows * b + l16] = m_run[b];
+            stat[wv][1][kFewRows * b + l16] = l_run[b];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < VD; e += 4)
+                *reinterpret_cast<float4*>(&slab[wv][kFewRows * b + 4 * g4 + r][DimsV<VT, VD>::dim(l16, e)]) =
+                    make_float4(o[b][e][r], o[b][e + 1][r], o[b][e + 2][r], o[b][e + 3][r]);
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int e = 0; e < VD; e += 4)
-            *reinterpret_cast<float4*>(&slab[wv][4 * g4 + r][DimsV<VT, VD>::dim(l16, e)]) = make_float4(o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]);
     __syncthreads();
-    if (threadIdx.x < kFewRows) {   // the parts' weights and the joined sum of every row
+    if (threadIdx.x < (second ? ROWS : kFewRows)) {   // the parts' weights and the joined sum of every row
         const int r = threadIdx.x;
         float m = stat[0][0][r];
 #pragma unroll
@@ -811,7 +853,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
     if constexpr (PAGED) {
         auto tiles = [&](int n) { return (n * G + ROWS - 1) / ROWS; };
         int item = 0;
-        if (!item_of_rank(a, rank, [&](const Req& r) { return r.n * G > kFewRows ? tiles(r.n) * chunks_in(a, r.len) : 0; }, &i, &item)) return;   // uniform
+        if (!item_of_rank(a, rank, [&](const Req& r) { return r.n * G > a.few ? tiles(r.n) * chunks_in(a, r.len) : 0; }, &i, &item)) return;   // uniform
         const int n = tiles(request(a, i, word(a.row_start, i), word(a.row_start, i + 1)).n);
         chunk = item / n;
         level = n - 1 - item % n;
@@ -1413,6 +1455,15 @@ long long most_tiles(int n_req, int ntok, int max_new, int G, int held) {
     return std::min(static_cast<long long>(ntok) * G / held + n_req, static_cast<long long>(most_levels(ntok, max_new, G, held)) * n_req);
 }
 
+// The rows of a request that the form of few rows takes in a call: 32, two blocks of 16, where no request has more and the cache is
+// quantised (a code is turned once for both blocks), else 16.  16 requests of 5 tokens behind 4096 positions (16 heads, 4 KV heads of
+// 256 dims) I8 33 us with two blocks and 68 in tiles, I4 32 and 66; 200 of 5 behind 500 I8 74 and 117; F16 in tiles 50, with two
+// blocks 54.  Beside longer requests two blocks would cost single tokens a workgroup: their records leave one to a compute unit.
+int few_rows(bool quantised, int ntok, int max_new, int G) {
+    const long long most = static_cast<long long>(std::min(max_new, ntok)) * G;
+    return quantised && most > kFewRows && most <= 2 * kFewRows ? 2 * kFewRows : kFewRows;
+}
+
 struct Outputs {
     const float* gate;
     int gate_stride;
@@ -1462,14 +1513,17 @@ constexpr int kMaxStride = 1 << 26;   // a step's rows are within 32 bits of its
 
 constexpr long long kMostBlocks = 0xffffffffLL / kThreads;
 
-// waves of a tile's workgroup
+// waves of a paged tile's workgroup
 constexpr int tile_waves(int ktype) { return ktype == kKvF16 ? 4 : 8; }
 
 template <int KT, int VT, int HD>
 void launch_paged(const BatchArgs& a, bool tiles, long long few_blocks, long long tile_blocks, hipStream_t s) {
     constexpr int W = tile_waves(KT);
     if (tiles) hipLaunchKernelGGL((batch_tile_kernel<kPaged, KT, VT, HD, W>), dim3(static_cast<unsigned>(tile_blocks)), dim3(64 * W), 0, s, a);
-    hipLaunchKernelGGL((batch_few_kernel<KT, VT, HD>), dim3(static_cast<unsigned>(few_blocks)), dim3(kThreads), 0, s, a);
+    auto* few = &batch_few_kernel<KT, VT, HD, 1>;
+    if constexpr (KT != kKvF16)
+        if (a.few > kFewRows) few = &batch_few_kernel<KT, VT, HD, 2>;
+    hipLaunchKernelGGL(few, dim3(static_cast<unsigned>(few_blocks)), dim3(kThreads), 0, s, a);
     if (a.chunks > kFlatChunks) {
         hipLaunchKernelGGL((batch_join_kernel<HD>), dim3(a.ntok, a.n_head, HD / 64), dim3(kThreads), 0, s, a);
     } else if (a.chunks > 1) {
@@ -1526,7 +1580,7 @@ extern "C" int rmi_gqa_paged_split(long long total_ctx, int max_ctx, int n_req, 
     }
     const int G = n_head / n_kv;
     long long chunk;
-    if (static_cast<long long>(max_new) * G <= kFewRows) {
+    if (static_cast<long long>(std::min(max_new, ntok)) * G <= few_rows(true, ntok, max_new, G)) {   // F16's tiles of 17 to 32 rows take these chunks within 10 % of their best
         // Few rows: one round of workgroups, one for each of 256 compute units, since past the memory's rate it is their beginnings,
         // ends and records that cost.  A request of any length has half a chunk too many on average; eight workgroups are left for
         // more.  More rounds where one would leave a chunk much longer than its share.
@@ -1603,7 +1657,8 @@ extern "C" int rmi_gqa_paged_attn(int qtype, const void* q, int ktype, const voi
     const int held = kWaveRows * tile_waves(ktype);
     a.bf16 = qtype == RMI_ROWS_BF16;
     a.post = scale * kLog2e;
-    const bool tiles = static_cast<long long>(std::min(max_new, ntok)) * G > kFewRows;
+    a.few = few_rows(ktype != kKvF16, ntok, max_new, G);
+    const bool tiles = static_cast<long long>(std::min(max_new, ntok)) * G > a.few;
     const long long few = static_cast<long long>(n_req) * n_kv * chunks, tile = most_tiles(n_req, ntok, max_new, G, held) * n_kv * chunks;
     if (few > kMostBlocks || (tiles && tile > kMostBlocks / 2) || static_cast<long long>(ntok) * n_head > kMostBlocks)
         return fail(RMI_ERR_SHAPE, "gqa_paged_attn: too many workgroups");
