@@ -510,7 +510,8 @@ int rmi_attn_prep_paged(const float* q3, int q3_stride, const float* qn, const f
  * Left as they are: rows behind the last request's, and rows of a request with more than max_new new tokens or more than max_ctx
  * positions.  A token at a negative position (kv_len below the number of new tokens) gives zeros.  A token that sees a position
  * whose page id is outside the pool or past the table's row gives NaN.  What a token does not see has no part in its result,
- * whatever it holds; a NaN or an infinity in what it sees makes it NaN or infinite.
+ * whatever it holds; a NaN in what it sees, or an infinity in V, makes it NaN or infinite (an infinite score is the formula's:
+ * +inf gives NaN, -inf a weight of zero).
  * The contexts are worked on in chunks of `split` positions, a multiple of 128 that leaves at most 1024 chunks of max_ctx;
  * rmi_gqa_paged_split gives it for a batch of total_ctx positions in all, to be settled once (results differ in the last bits
  * between splits).  workspace holds rmi_gqa_paged_workspace_bytes(...) bytes, 16-byte aligned (null where split >= max_ctx), and
@@ -526,9 +527,10 @@ int rmi_gqa_paged_attn(int qtype, const void* q, int ktype, const void* kpool, i
 
 /* Causal attention over whole prompts packed row by row, without a cache: rows row_start[i] .. row_start[i + 1] - 1 of q
  * ([n_head][head_dim]), k and v ([n_kv][head_dim]), all of one type, are request i's; row t of it sees its rows up to t.  Rows are
- * q_stride, k_stride and v_stride elements apart (multiples of 8, those of k and v up to 2^26; q, k and v 16-byte aligned); an F16 cache's rows, contiguous or
- * pages in order, can be k and v.  BF16 rows are multiplied as bf16, the weights rounded to it.  Requests of more than max_len
- * rows are left out, rows behind the last request's are left as they are.  Gate, y, Q8_1 and what is not finite as above. */
+ * q_stride, k_stride and v_stride elements apart (multiples of 8, those of k and v up to 2^25; q, k and v 16-byte aligned); an F16
+ * cache's rows, contiguous or pages in order, can be k and v.  BF16 rows are multiplied as bf16, the weights rounded to it.
+ * Requests of more than max_len rows are left out, rows behind the last request's are left as they are.  Gate, y, Q8_1 and what
+ * is not finite as above. */
 int rmi_gqa_prompt_attn(int type, const void* q, int q_stride, const void* k, int k_stride, const void* v, int v_stride,
                         const int* row_start, const float* gate_src, int gate_stride, void* y, int y_stride, uint8_t* q8,
                         int q8_stride, int n_req, int ntok, int max_len, int n_head, int n_kv, int head_dim, float scale,

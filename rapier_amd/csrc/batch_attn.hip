@@ -33,7 +33,7 @@ constexpr int kWaveRows = 32;      // of a wave of the form of more rows
 constexpr int kTileRows = 128;     // rows of four such waves, the unit of a split
 constexpr int kChunkUnit = 128;    // a chunk is a whole number of them
 constexpr int kMaxChunks = 1024;   // named in the messages
-constexpr float kPScale = 8.0f;    // p goes as 2^8 p: fp16's subnormals begin 2^-22 below a row's maximum
+constexpr float kPScale = 8.0f;    // p goes as 2^8 p in fp16, whose subnormals then begin 2^-22 below a row's maximum (bf16 has no need)
 constexpr float kLazy = 7.0f;      // a maximum moves once a score passes it by more than 2^7 (2^15 p is an fp16 number)
 
 struct BatchArgs {
@@ -749,7 +749,7 @@ __device__ __forceinline__ void tile_step(const uint8_t* kt, const uint8_t* vt, 
     const float m_ref = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: exp2(-inf) = 0, no NaN
     const float alpha = m_run == m_new || m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_ref);   // -inf: o is 0
     m_run = m_new;
-    const float shift = kPScale - m_ref;
+    const float shift = (BF ? 0.0f : kPScale) - m_ref;
     float sum = 0.0f;
     u32x4 p[2 * NS];
 #pragma unroll
@@ -1509,7 +1509,7 @@ void set_outputs(BatchArgs* a, const Outputs& o) {
     a->q8_stride = o.q8_stride;
 }
 
-constexpr int kMaxStride = 1 << 26;   // a step's rows are within 32 bits of its first
+constexpr int kMaxStride = 1 << 25;   // the 64 rows of a step are within 32 bits of its first, in bytes
 
 constexpr long long kMostBlocks = 0xffffffffLL / kThreads;
 
@@ -1675,7 +1675,7 @@ extern "C" int rmi_gqa_prompt_attn(int type, const void* q, int q_stride, const 
     if (type != RMI_ROWS_F16 && type != RMI_ROWS_BF16) return fail(RMI_ERR_UNSUPPORTED, "gqa_prompt_attn: rows of F16 or BF16");
     if (!heads_ok(n_head, n_kv, head_dim) || !batch_ok(n_req, ntok, max_len) || !(scale > 0.0f && scale <= FLT_MAX) || q_stride % 8 || k_stride % 8 ||
         v_stride % 8 || k_stride > kMaxStride || v_stride > kMaxStride || (ntok > 1 && (q_stride < n_head * head_dim || k_stride < n_kv * head_dim || v_stride < n_kv * head_dim)))
-        return fail(RMI_ERR_SHAPE, "gqa_prompt_attn: invalid arguments (strides are multiples of 8 elements, up to 2^26)");
+        return fail(RMI_ERR_SHAPE, "gqa_prompt_attn: invalid arguments (strides are multiples of 8 elements, k's and v's up to 2^25)");
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned4(row_start))
         return fail(RMI_ERR_POINTER, "gqa_prompt_attn: null or misaligned pointer");
     const Outputs out{gate_src, gate_stride, y, y_stride, q8, q8_stride};
@@ -1716,7 +1716,7 @@ extern "C" int rmi_gqa_prompt_attn(int type, const void* q, int q_stride, const 
     const int held = parts ? kWaveRows : (wide ? 8 : 4) * kWaveRows;
     a.levels = most_levels(ntok, max_len, G, held);
     const long long blocks = most_tiles(n_req, ntok, max_len, G, held) * n_kv;
-    if (blocks > kMostBlocks) return fail(RMI_ERR_SHAPE, "gqa_prompt_attn: too many workgroups");
+    if (blocks > kMostBlocks / (wide ? 2 : 1)) return fail(RMI_ERR_SHAPE, "gqa_prompt_attn: too many workgroups");
     auto go = [&](auto* kernel, int waves) {
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * waves), 0, static_cast<hipStream_t>(stream), a);
         return launch_status("gqa_prompt_attn");

@@ -8,7 +8,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstring>
 
 #include "kv_rows.h"
 #include "overlap.h"
@@ -364,32 +363,24 @@ __global__ __launch_bounds__(64 * kPrepWaves) void prep_paged_kernel(PagedPrepAr
     }
 }
 
-// The turns of each pair in one position, from the rotation's parameters; kept by their values for the thread's next call (a pow
-// for each of 32 pairs costs as much as the rest of a call).
-struct Turns {
-    rmi_rope_params rope;
-    int n_rot = -1;
-    double size, turns[kMaxPairs];
-};
-bool rope_turns(const rmi_rope_params& r, int n_rot, const Turns** out) {
-    static thread_local Turns kept;
-    if (kept.n_rot != n_rot || std::memcmp(&kept.rope, &r, sizeof r) != 0) {
-        Yarn y;
-        if (!yarn_setup(r, n_rot, &y)) return false;
-        kept.n_rot = -1;
-        for (int i = 0; i < n_rot / 2; ++i) {
-            double f = std::pow(static_cast<double>(r.freq_base), -2.0 * i / n_rot);
-            if (y.on) {
-                const double ramp = (1.0 - std::fmin(1.0, std::fmax(0.0, (i - y.low) / std::fmax(0.001, y.high - y.low)))) * y.ext;
-                f = f / y.factor * (1.0 - ramp) + f * ramp;
-            }
-            kept.turns[i] = f / 6.28318530717958647692;
+// The turns of each pair in one position, from the rotation's parameters.  base^(-2 i / n_rot) is a product of one power for i / 8
+// and one for i % 8: a pow for each of 32 pairs costs as much as the rest of a call.
+bool rope_turns(const rmi_rope_params& r, int n_rot, double* turns, double* size) {
+    Yarn y;
+    if (!yarn_setup(r, n_rot, &y)) return false;
+    double low[8];
+    for (int k = 0; k < 8; ++k) low[k] = std::pow(static_cast<double>(r.freq_base), -2.0 * k / std::max(n_rot, 1));
+    double high = 1.0;
+    for (int i = 0; i < n_rot / 2; ++i) {
+        if (i % 8 == 0) high = std::pow(static_cast<double>(r.freq_base), -2.0 * i / n_rot);
+        double f = high * low[i % 8];
+        if (y.on) {
+            const double ramp = (1.0 - std::fmin(1.0, std::fmax(0.0, (i - y.low) / std::fmax(0.001, y.high - y.low)))) * y.ext;
+            f = f / y.factor * (1.0 - ramp) + f * ramp;
         }
-        kept.size = y.on ? y.mscale : 1.0;
-        kept.rope = r;
-        kept.n_rot = n_rot;
+        turns[i] = f / 6.28318530717958647692;
     }
-    *out = &kept;
+    *size = y.on ? y.mscale : 1.0;
     return true;
 }
 
@@ -500,9 +491,8 @@ extern "C" int rmi_attn_prep_paged(const float* q3, int q3_stride, const float* 
                          block_of(kn, kn ? head_dim * 4 : 0), ints(slot, ntok), ints(pos, ntok)};
     const RowSet out[] = {block_of(kpool, pools[0]), block_of(vpool, pools[1]), block_of(qout, static_cast<size_t>(ntok) * n_head * head_dim * 2)};
     if (!apart(in, 5, out, 3)) return fail(RMI_ERR_POINTER, "attn_prep_paged: a pool or qout lies on another argument");
-    const Turns* turns;
-    if (!rope_turns(*rope, n_rot, &turns)) return fail(RMI_ERR_SHAPE, "attn_prep_paged: invalid YaRN parameters");
     PagedPrepArgs a{};
+    if (!rope_turns(*rope, n_rot, a.turns, &a.size)) return fail(RMI_ERR_SHAPE, "attn_prep_paged: invalid YaRN parameters");
     a.q3 = q3;
     a.qn = qn;
     a.kn = kn;
@@ -520,8 +510,6 @@ extern "C" int rmi_attn_prep_paged(const float* q3, int q3_stride, const float* 
     a.neighbours = pairs == RMI_ROPE_NEIGHBOURS;
     a.bf16 = qtype == RMI_ROWS_BF16;
     a.eps = eps;
-    a.size = turns->size;
-    std::memcpy(a.turns, turns->turns, sizeof(double) * (n_rot / 2));
     const int items = n_head + 2 * n_kv;
     // rows a wave: as many as leave about a thousand workgroups (they share a token's angles), one for few tokens (latency)
     a.per_wave = std::min((items + kPrepWaves - 1) / kPrepWaves, static_cast<int>((static_cast<long long>(items) * ntok + 4095) / 4096));

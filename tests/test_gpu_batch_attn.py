@@ -131,6 +131,22 @@ def test_paged(rmi, kt, vt, n_kv, G, hd, page):
         check_q8(y[used], blocks[used], ref.HALF_STEP[b.qname])
 
 
+@pytest.mark.parametrize("kt,vt", TYPES)
+@pytest.mark.parametrize("lens,G", [([(0, 5), (31, 8), (32, 7), (95, 6), (127, 5), (128, 8), (700, 8), (1100, 5), (64, 1), (15, 0), (200, 4)], 4),
+                                    ([(p, 1) for p in (0, 15, 31, 63, 64, 300)] + [(9, 0)], 24), ([(40, 32), (0, 17), (5, 31), (3, 1)], 1),
+                                    ([(40, 6), (0, 4), (511, 3)], 5)])
+def test_paged_drafts(rmi, kt, vt, lens, G):
+    """17 to 32 rows a request beside fewer"""
+    rng = np.random.default_rng(G + 7 * kt + vt)
+    for hd, page, name in ((256, 64, "float16"), (128, 16, "bfloat16")):
+        b = Batch(rng, lens, kt, vt, 2, G, hd, page, name, gate=G == 4)
+        for split in (128, 256, 1280):
+            y, blocks = b.run(rmi, split)
+            b.check(y, blocks)
+            used = slice(0, b.start[-1])
+            check_q8(y[used], blocks[used], ref.HALF_STEP[b.qname])
+
+
 @pytest.mark.parametrize("page", [32, 128])
 @pytest.mark.parametrize("new", [1, 2, 4, 5, 16, 17, 32, 33, 65])
 def test_paged_lengths(rmi, new, page):
@@ -157,7 +173,7 @@ def test_paged_large_and_small_q(rmi, qname):
 
 
 @pytest.mark.parametrize("kt,vt", TYPES)
-@pytest.mark.parametrize("new", [4, 40])
+@pytest.mark.parametrize("new", [4, 7, 40])
 def test_unseen_rows_have_no_part(rmi, kt, vt, new):
     """K and V of a new token that are NaN or infinite: the tokens before it do not notice, the others are not finite"""
     rng = np.random.default_rng(new + kt)
@@ -196,10 +212,11 @@ def test_unseen_rows_have_no_part(rmi, kt, vt, new):
             assert np.isinf(y[s + at:s + new, :4, 6]).all()
 
 
-@pytest.mark.parametrize("new", [1, 3, 40])
-def test_pages_that_are_none(rmi, new):
+@pytest.mark.parametrize("kt,vt", [(F16, F16), (I8, I4)])
+@pytest.mark.parametrize("new", [1, 3, 7, 40])
+def test_pages_that_are_none(rmi, new, kt, vt):
     rng = np.random.default_rng(new)
-    b = Batch(rng, [(100, new), (200, new), (90, new), (60, new)], F16, F16, 2, 4, 128, 32)
+    b = Batch(rng, [(100, new), (200, new), (90, new), (60, new)], kt, vt, 2, 4, 128, 32)
     table = b.table.copy()
     table[0, 2] = b.n_pages          # positions 64 ..
     table[1, 0] = -1
@@ -307,9 +324,87 @@ def test_pool_past_32_bits(rmi):
         del pools
 
 
+@pytest.mark.parametrize("kt,vt", [(F16, F16), (I8, I8)])
+def test_more_requests_than_lanes(rmi, kt, vt):
+    """200 requests of no, one and many tokens: each of the forms has some of several waves' worth"""
+    rng = np.random.default_rng(21 + kt)
+    new = rng.choice([0, 1, 1, 2, 4, 33, 70], 200, p=[0.1, 0.3, 0.2, 0.2, 0.1, 0.06, 0.04])
+    lens = [(int(p), int(n)) for p, n in zip(rng.integers(0, 400, 200), new)]
+    b = Batch(rng, lens, kt, vt, 1, 4, 128, 16)
+    for split in (128, 512):
+        b.check(*b.run(rmi, split))
+    b.check(*b.run(rmi))
+
+
+def test_most_requests(rmi):
+    rng = np.random.default_rng(3)
+    lens = [(int(p), int(n)) for p, n in zip(rng.integers(0, 40, 4096), rng.integers(0, 3, 4096))]
+    b = Batch(rng, lens, F16, F16, 1, 1, 128, 16, gate=False)
+    b.check(*b.run(rmi))
+    b.check(*b.run(rmi, max_new=20))   # both forms are launched, one has none
+
+
+@pytest.mark.parametrize("new", [1, 6, 40])
+def test_bounds_far_above(rmi, new):
+    """bounds of the longest context and of all the tokens: the chunks are many and long, the lengths are what they are"""
+    rng = np.random.default_rng(new)
+    b = Batch(rng, [(300, new), (0, new), (31, 1)], I8, I8, 1, 4, 128, 32)
+    y, blocks = b.run(rmi, max_ctx=1 << 30, max_new=1 << 30)
+    b.check(y, blocks)
+
+
+@pytest.mark.parametrize("qname", ["float16", "bfloat16"])
+@pytest.mark.parametrize("kt,vt", [(F16, F16), (I8, I4)])
+@pytest.mark.parametrize("new", [1, 7, 40])
+def test_q_that_is_not_finite(rmi, qname, kt, vt, new):
+    """one head of one token: its row is NaN, the others do not notice"""
+    rng = np.random.default_rng(new)
+    b = Batch(rng, [(200, new), (50, new)], kt, vt, 2, 4, 128, 16, qname)
+    plain, _ = b.run(rmi, 128, q8=False)
+    at = b.start[1] - 1
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        b.tq[at, 5, 77] = bad
+        y, _ = b.run(rmi, 128, q8=False)
+        assert np.isnan(y[at, 5]).all()
+        y[at, 5] = plain[at, 5]
+        assert np.array_equal(y, plain)
+
+
+@pytest.mark.parametrize("kt,vt", [(F16, F16), (I4, I4)])
+def test_shared_pages(rmi, kt, vt):
+    """requests that read the same pages: each as if it were alone"""
+    t = torch()
+    rng = np.random.default_rng(12)
+    b = Batch(rng, [(250, 6)] * 3 + [(240, 1), (0, 40)], kt, vt, 2, 4, 128, 16)
+    b.table[1] = b.table[2] = b.table[0]
+    b.table[3, :16] = b.table[0, :16]
+    for split in (128, 256):
+        b.check(*b.run(rmi, split))
+
+
+def test_two_calls_at_once(rmi):
+    """on two streams, each with a workspace of its own: the bits of each alone"""
+    t = torch()
+    rng = np.random.default_rng(14)
+    b = [Batch(rng, [(900, 1), (2000, 4), (60, 30)], kt, kt, 4, 4, 256, 64) for kt in (F16, I8)]
+    first = [x.run(rmi, 128) for x in b]
+    streams = [t.cuda.Stream() for _ in b]
+    for x in b:
+        x.y.zero_()
+        x.blocks.zero_()
+    t.cuda.synchronize()
+    for _ in range(5):
+        for x, s in zip(b, streams):
+            rmi.gqa_paged_attn(*x.args, stream=s)
+    t.cuda.synchronize()
+    for x, (y, blocks) in zip(b, first):
+        used = slice(0, x.start[-1])
+        assert np.array_equal(x.y.double().cpu().numpy()[used], y[used]) and np.array_equal(x.blocks.cpu().numpy()[used], blocks[used])
+
+
 # ---- whole prompts -------------------------------------------------------------------------------------------------------
-def prompt_case(rmi, rng, lens, name, n_kv, G, hd, gate=True, pad=0, q8=True, max_len=None):
-    """rows of q, k and v side by side in one tensor (pad elements between them)"""
+def prompt_case(rmi, rng, lens, name, n_kv, G, hd, gate=True, pad=0, q8=True, max_len=None, heads=None):
+    """rows of q, k and v side by side in one tensor (pad elements between them); heads: those of each KV head that are looked at"""
     t = torch()
     nh, n = n_kv * G, sum(lens)
     width = (nh + 2 * n_kv) * hd + pad
@@ -329,9 +424,10 @@ def prompt_case(rmi, rng, lens, name, n_kv, G, hd, gate=True, pad=0, q8=True, ma
         if max_len and m > max_len:
             assert (got[s:s + m] == 77.0).all()
             continue
-        want, bound = ref.attention(q[s:s + m].reshape(m, nh, hd), k[s:s + m].reshape(m, n_kv, hd), v[s:s + m].reshape(m, n_kv, hd), 0,
-                                    scale, None if g is None else g[s:s + m, :, 1].astype(np.float64), ref.HALF_STEP[name], ref.HALF_STEP[name])
-        off = np.abs(got[s:s + m, :nh * hd].reshape(m, nh, hd) - want)
+        some = np.arange(nh).reshape(n_kv, G)[:, heads or slice(None)].reshape(-1)
+        want, bound = ref.attention(q[s:s + m].reshape(m, nh, hd)[:, some], k[s:s + m].reshape(m, n_kv, hd), v[s:s + m].reshape(m, n_kv, hd), 0,
+                                    scale, None if g is None else g[s:s + m, some, 1].astype(np.float64), ref.HALF_STEP[name], ref.HALF_STEP[name])
+        off = np.abs(got[s:s + m, :nh * hd].reshape(m, nh, hd)[:, some] - want)
         assert not (~(off <= bound)).any(), f"prompt {i} of {m}: off by {np.nanmax(off):.3g}, bound {bound.max():.3g}"
     assert (got[n:] == 77.0).all() and (got[:, nh * hd:] == 77.0).all()
     if q8:
@@ -358,13 +454,76 @@ def test_prompts_many(rmi):
 
 @pytest.mark.parametrize("name", ["float16", "bfloat16"])
 @pytest.mark.parametrize("hd", [128, 256])
-def test_prompt_unseen_rows(rmi, name, hd):
+def test_prompt_forms(rmi, name, hd):
+    """the workgroups of eight waves, with heads enough for many of them, and those of four over prompts of several tiles"""
+    rng = np.random.default_rng(hd)
+    prompt_case(rmi, rng, [257, 0, 5], name, 8, 64, hd, gate=hd == 128, heads=[0, 63])
+    prompt_case(rmi, rng, [150, 149, 151, 9, 180, 150, 150], name, 4, 4, hd, heads=[1])
+
+
+@pytest.mark.parametrize("G", [4, 8])
+@pytest.mark.parametrize("lens", [[70], [160, 3]])
+def test_prompt_rows_far_apart(rmi, lens, G):
+    """rows as far apart as may be, the last steps cut at the call's end"""
+    t = torch()
+    rng = np.random.default_rng(5)
+    n, hd, stride = sum(lens), 128, 1 << 25
+    far = t.empty(n, stride, dtype=t.float16, device="cuda")
+    q, k, v = (rng.standard_normal((n, h, hd)).astype(np.float16) for h in (G, 1, 1))
+    far[:, :hd] = t.from_numpy(k[:, 0]).cuda()
+    far[:, hd:2 * hd] = t.from_numpy(v[:, 0]).cuda()
+    y = t.empty(n, G, hd, dtype=t.float16, device="cuda")
+    start, scale = np.concatenate([[0], np.cumsum(lens)]), float(np.float32(hd ** -0.5))
+    rmi.gqa_prompt_attn(t.from_numpy(q).cuda(), G * hd, far, stride, far[:, hd:], stride, ints(start), None, 0, y, G * hd, None, 0, len(lens), n,
+                        max(lens), G, 1, hd, scale)
+    got = y.double().cpu().numpy()
+    for s, m in zip(start, lens):
+        want, bound = ref.attention(*(x[s:s + m].astype(np.float64) for x in (q, k, v)), 0, scale, None, 2.0 ** -11, 2.0 ** -11)
+        assert (np.abs(got[s:s + m] - want) <= bound).all()
+
+
+def test_prompt_large_values(rmi):
+    """bf16 values near the type's largest: the sums on the way stay inside fp32 (a weight is at most 2^7, 100 of them)"""
+    t = torch()
+    rng = np.random.default_rng(17)
+    for lens in ([100], [30] * 8):
+        args, y = prompt_case(rmi, rng, lens, "bfloat16", 1, 8, 128, gate=False, q8=False)
+        plain = y.double().cpu().numpy()
+        rows = args[0]
+        rows[:, 9 * 128:] *= 2.0 ** 110   # of the order of 2^112, times 2^14 for all the weights
+        rmi.gqa_prompt_attn(*args)
+        n = sum(lens)
+        got = y.double().cpu().numpy()[:n, :1024]
+        assert np.array_equal(got, plain[:n, :1024] * 2.0 ** 110)
+
+
+@pytest.mark.parametrize("name", ["float16", "bfloat16"])
+@pytest.mark.parametrize("lens,n_kv,G", [([100, 40], 1, 8), ([20] * 30, 2, 4), ([257, 9], 8, 64)])
+def test_prompt_q_that_is_not_finite(rmi, name, lens, n_kv, G):
+    rng = np.random.default_rng(G)
+    args, y = prompt_case(rmi, rng, lens, name, n_kv, G, 128, gate=False, q8=False, heads=[0])
+    plain = y.double().cpu().numpy()
+    at, h = lens[0] - 1, n_kv * G - 2
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        args[0][at, 128 * h + 5] = bad
+        rmi.gqa_prompt_attn(*args)
+        got = y.double().cpu().numpy()
+        mine = slice(128 * h, 128 * (h + 1))
+        assert np.isnan(got[at, mine]).all()
+        got[at, mine] = plain[at, mine]
+        assert np.array_equal(got, plain)
+
+
+@pytest.mark.parametrize("name", ["float16", "bfloat16"])
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("lens,n_kv,G", [([40, 100, 9], 1, 4), ([40, 100, 9], 1, 3), ([40, 257, 9], 8, 64), ([40, 100, 9] + [90] * 18, 1, 4)])
+def test_prompt_unseen_rows(rmi, name, hd, lens, n_kv, G):
     """a row whose k and v are not finite: no part in the rows before it, nor in other prompts"""
     rng = np.random.default_rng(6)
-    args, y = prompt_case(rmi, rng, [40, 100, 9], name, 1, 4, hd, gate=False)
+    args, y = prompt_case(rmi, rng, lens, name, n_kv, G, hd, gate=False, q8=False, heads=[0])
     plain = y.double().cpu().numpy()
-    row, nh = args[0], 4
-    k, v = row[:, nh * hd:(nh + 1) * hd], row[:, (nh + 1) * hd:(nh + 2) * hd]
+    row, nh, end = args[0], n_kv * G, 40 + lens[1]
+    k, v = row[:, nh * hd:(nh + 1) * hd], row[:, (nh + n_kv) * hd:(nh + n_kv + 1) * hd]   # KV head 0
     keep = k[70].clone(), v[70].clone()
     v[70, 3:60:5] = float("nan")
     v[70, 64] = float("inf")
@@ -373,16 +532,17 @@ def test_prompt_unseen_rows(rmi, name, hd):
             k[70] = float("nan")
         rmi.gqa_prompt_attn(*args)
         got = y.double().cpu().numpy()
-        before = np.r_[0:70, 140:149]
+        before = np.r_[0:70, end:len(got)]
         assert np.array_equal(got[before], plain[before])
-        after = got[70:140, :nh * hd].reshape(70, nh, hd)
+        assert np.array_equal(got[:, G * hd:], plain[:, G * hd:])
+        after = got[70:end, :G * hd].reshape(end - 70, G, hd)
         odd = np.zeros(hd, bool)
         odd[3:60:5] = odd[64] = True
         assert not np.isfinite(after[..., odd]).any()
         if k_too:
             assert np.isnan(after).all()
         else:
-            assert np.array_equal(after[..., ~odd], plain[70:140, :nh * hd].reshape(70, nh, hd)[..., ~odd]) and np.isinf(after[..., 64]).all()
+            assert np.array_equal(after[..., ~odd], plain[70:end, :G * hd].reshape(end - 70, G, hd)[..., ~odd]) and np.isinf(after[..., 64]).all()
     k[70], v[70] = keep
     rmi.gqa_prompt_attn(*args)
     assert np.array_equal(y.double().cpu().numpy(), plain)

@@ -95,7 +95,9 @@ def test_prompt_attention(rmi):
         rmi._call("rmi_gqa_prompt_attn", t, q, qs, k, ks, v, vs, row, gate, gs, y, ys, q8, q8s, n, ntok, longest, nh, nkv, hd, scale, None)
 
     for bad in ({"t": 2}, {"n": 0}, {"ntok": 0}, {"longest": 0}, {"nh": 10}, {"hd": 192}, {"scale": 0.0}, {"qs": 4092}, {"qs": 4088}, {"ks": 1020}, {"ks": 1016},
-                {"vs": 1025}, {"q": NULL}, {"k": off(at(2), 8)}, {"v": NULL}, {"row": NULL}, {"gate": off(at(7), 1)}, {"y": NULL, "q8": NULL},
+                {"vs": 1025}, {"ks": 2 ** 25 + 8}, {"vs": 2 ** 25 + 8}, {"n": 4097}, {"ntok": 2 ** 24 + 1}, {"scale": float("nan")},
+                {"ntok": 2 ** 24, "longest": 2 ** 24, "nh": 64 * 64, "nkv": 64, "qs": 64 * 64 * 256, "ks": 2 ** 14, "vs": 2 ** 14, "ys": 2 ** 20, "q8s": 2 ** 21, "gate": NULL, "k": at(2 ** 24), "v": at(2 ** 25), "y": at(2 ** 26), "q8": NULL, "hd": 256},
+                {"q": NULL}, {"k": off(at(2), 8)}, {"v": NULL}, {"row": NULL}, {"gate": off(at(7), 1)}, {"y": NULL, "q8": NULL},
                 {"y": off(at(8), 4)}, {"ys": 4094}, {"q8s": 4000}, {"y": at(1)}, {"y": at(3)}, {"q8": at(2)}, {"y": at(9)}, {"q8": off(at(7), 1024)},
                 {"y": at(5)}):
         with pytest.raises(ValueError, match="gqa_prompt_attn"):
