@@ -363,17 +363,15 @@ __global__ __launch_bounds__(64 * kPrepWaves) void prep_paged_kernel(PagedPrepAr
     }
 }
 
-// The turns of each pair in one position, from the rotation's parameters.  base^(-2 i / n_rot) is a product of one power for i / 8
-// and one for i % 8: a pow for each of 32 pairs costs as much as the rest of a call.
+// The turns of each pair in one position, from the rotation's parameters: base^(-2 i / n_rot) by products of one power in the host's
+// 80-bit numbers, 128 of which lose less than fp64 does by one rounding (a pow for each pair takes the host longer).
 bool rope_turns(const rmi_rope_params& r, int n_rot, double* turns, double* size) {
     Yarn y;
     if (!yarn_setup(r, n_rot, &y)) return false;
-    double low[8];
-    for (int k = 0; k < 8; ++k) low[k] = std::pow(static_cast<double>(r.freq_base), -2.0 * k / std::max(n_rot, 1));
-    double high = 1.0;
-    for (int i = 0; i < n_rot / 2; ++i) {
-        if (i % 8 == 0) high = std::pow(static_cast<double>(r.freq_base), -2.0 * i / n_rot);
-        double f = high * low[i % 8];
+    const long double ratio = n_rot > 2 ? std::pow(static_cast<long double>(r.freq_base), -2.0L / n_rot) : 1.0L;
+    long double power = 1.0L;
+    for (int i = 0; i < n_rot / 2; ++i, power *= ratio) {
+        double f = static_cast<double>(power);
         if (y.on) {
             const double ramp = (1.0 - std::fmin(1.0, std::fmax(0.0, (i - y.low) / std::fmax(0.001, y.high - y.low)))) * y.ext;
             f = f / y.factor * (1.0 - ramp) + f * ramp;
