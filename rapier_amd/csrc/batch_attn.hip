@@ -246,6 +246,11 @@ __device__ __forceinline__ void finish4(const BatchArgs& a, int t, int h, int d,
 // The waves take steps of 32 positions in turn.  A step's positions lie in one or two pages: each half has its own buffer, whose
 // length ends at the last position (rows past it read as zeros) and is zero for a page that is not one.  K of the next step is
 // loaded when this step's scores are done, V when its product is.
+// RB blocks of 16 rows share a step's operands (few_rows says when).
+// Bound by the cache, which is read once: 32 requests of one token behind 1 K to 4 K positions F16 (16 heads, 4 KV heads of 256 dims)
+// 65 us, 5.2 TB/s, one behind 65501 positions I8 25 us, 5.5 TB/s (a large copy 5.12).  Of small calls, and of a round's every
+// workgroup, 5 us go into starts: lengths, then page ids, then codes, each a wait for memory.  F16 holds two waves' registers in one (at
+// two waves a SIMD the loads ahead no longer fit: slower).
 struct Half {
     Rsrc kr, ks, vr, vs;
 };
@@ -618,8 +623,13 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 || RB == 2 ? 1 : 2) void bat
 //             (h, e) of 16 positions is position 8 (e / 4) + 4 h + e % 4, and V's transposed reads (ds_read_b64_tr_b16: 16 lanes
 //             give the addresses of 4 positions x 16 dims and get a dim's four positions each) take the same order.
 // q and o stay in registers.  16-bit K and V go from memory into LDS without passing registers, the next step's over this step's
-// products; codes go there as they are, two steps ahead, and are turned to fp16 tiles by the next step.  LDS rows have no padding (the direct loads write 1024 bytes in a row);
-// instead their 16-byte (K) or 32-byte (V) pieces are permuted by the row, so that the lanes of a read fall on different banks:
+// products; codes go there as they are, two steps ahead, and are turned to fp16 tiles by the next step.  Turning codes on their way
+// from memory held up every wave: 999 tokens behind 8 K of I8 / I4 249 us, 179 so.
+// Bound by the matrix cores and LDS together: a step of 256 rows x 32 positions is 2048 cycles of products and 256 KB of operands, 2048
+// cycles at 128 bytes each, with the softmax beside them, and takes some 3400: one prompt of 8001 tokens x 16 heads of 256 dims
+// 472 us, 1.11 PFLOP/s (a large library product 1.18), the matrix cores busy for 56 % of it.  Codes cost 7 % more over F16 pages (999
+// tokens behind 7 K: 159 us with the join, I8 170, I4 163).
+// LDS rows have no padding (the direct loads write 1024 bytes in a row); instead their 16-byte (K) or 32-byte (V) pieces are permuted by the row, so that the lanes of a read fall on different banks:
 // K piece c of row p is at c ^ (p % 16), V piece c at c ^ {0, 3, 5, 6}[p % 4].
 constexpr int kPaged = 1, kRowsF16 = 2, kRowsBF16 = 3;   // where K and V come from
 
@@ -683,12 +693,12 @@ struct VRow {
 
 // Scores, softmax and P V of the positions sb .. sb + STEP - 1 in the tiles kt and vt for the wave's 32 rows.  lim: the last position
 // that the lane's row sees, last: that any row of the workgroup sees; cut: uniform, some row does not see the whole step; bad: 16-position
-// pieces without a page.  v_ready() is called when K is read, has_odd() tells (uniformly) whether a value that is not finite was
+// pieces without a page.  scored() is called when the last product of the scores is issued, v_ready() when K is read, has_odd() tells (uniformly) whether a value that is not finite was
 // taken out of vt, v_row(position) where it is.  FRESH: no addresses kept in registers.  V_EARLY: the first of V over the softmax.
-template <bool BF, int HD, int VT, bool FRESH, bool V_EARLY, typename READY, typename ODD, typename ROWS>
+template <bool BF, int HD, int VT, bool FRESH, bool V_EARLY, typename SCORED, typename READY, typename ODD, typename ROWS>
 __device__ __forceinline__ void tile_step(const uint8_t* kt, const uint8_t* vt, int kat, int vat, const u32x4 (&q)[HD / 16], floatx16 (&o)[HD / 32],
                                           float& m_run, float& l_run, float post, int sb, int last, int lim, int h, uint32_t bad, bool cut,
-                                          READY&& v_ready, ODD&& has_odd, ROWS&& v_row) {
+                                          SCORED&& scored, READY&& v_ready, ODD&& has_odd, ROWS&& v_row) {
     constexpr int STEP = TileShape<HD>::kStep, ROW = TileShape<HD>::kRow, NS = STEP / 32, NK = HD / 16, ND = HD / 32;
     constexpr int AHEAD = HD == 256 ? 2 : 4;   // operands from LDS on their way
     floatx16 s[NS];
@@ -718,6 +728,7 @@ __device__ __forceinline__ void tile_step(const uint8_t* kt, const uint8_t* vt, 
     __builtin_amdgcn_s_setprio(1);
     stream<AHEAD, NS * NK>(ready, k_piece, [&](int n, u32x4 x) { s[n / NK] = mfma32<BF>(x, q[n % NK], s[n / NK]); });
     __builtin_amdgcn_s_setprio(0);
+    scored();
     auto v_first = [&] {
 #pragma unroll
         for (int n = 0; n < AHEAD; ++n) ready[n] = v_piece(n);
@@ -883,16 +894,24 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
     const size_t kstride = !PAGED ? 2 * static_cast<size_t>(a.k_stride) : !CODES ? static_cast<size_t>(a.n_kv) * kKB : kKB;
     const size_t vstride = !PAGED ? 2 * static_cast<size_t>(a.v_stride) : !CODES ? static_cast<size_t>(a.n_kv) * kVB : kVB;
     const int* const ids = a.table + static_cast<size_t>(i) * a.table_stride;
-    int id[NG];       // pages of the step that is loaded next
+    int id[NG];              // pages of the step that is loaded next
+    int asked[NG];           // what the table says of the one after
     uint32_t next_bad = 0;   // of its 16-position pieces: not a page
+    // A step's page ids, by scalar loads, which come back in any order: a read of LDS beside them would wait for them, so they are
+    // asked for where none is on its way, before the softmax
+    auto ask_pages = [&](int sb) {
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) asked[g] = word(ids, max(min(min(sb + 16 * g, last) >> a.shift, a.table_stride - 1), 0));
+        }
+    };
     auto find_pages = [&](int sb) {
         next_bad = 0;
         if constexpr (PAGED) {
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const int p = sb + 16 * g, at = min(p, last) >> a.shift;
-                const int x = p <= last && at < a.table_stride ? word(ids, at) : -1;
-                const bool ok = x >= 0 && x < a.n_pages;
+                const int p = sb + 16 * g, x = asked[g];
+                const bool ok = p <= last && p >> a.shift < a.table_stride && x >= 0 && x < a.n_pages;
                 if (p <= last && !ok) next_bad |= 1u << g;
                 id[g] = ok ? x : 0;
             }
@@ -930,7 +949,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
     const size_t v_at = PAGED ? kv_row<VT>(0, kv, a.n_kv, size, HD).code : static_cast<size_t>(kv) * ROW;
     const uint32_t pool0 = lds_address(pool);
     // Codes and their scales into LDS as they are: rows of a page lie one behind another, so a wave's 1024 bytes are in a row.
-    // Waves take K's and V's codes in turn, the first two the scales.
+    // The loading waves take K's and V's codes in turn, two of them the scales.
     auto raw_codes = [&](const uint8_t* src, size_t page_bytes, size_t at0, auto type, int sb, uint32_t to, int turn) {
         constexpr int B = kv_row_bytes(decltype(type)::value, HD), R = 1024 / B;   // rows a load
         static_assert(R <= 16, "within a page's 16");
@@ -942,72 +961,91 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
         load_lds(src + static_cast<size_t>(page) * page_bytes + at0 + static_cast<size_t>((sb + p) & (size - 1)) * B, 16 * lane, to + 1024 * turn);
     };
     auto raw_scales = [&](const uint8_t* src, size_t page_bytes, size_t at0, int sb, uint32_t to) {
-        const int l = fresh<PAGED>(lane), p = 4 * l / NB;   // the lane's four bytes
+        const uint32_t l = static_cast<uint32_t>(fresh<PAGED>(lane)), p = 4 * l / NB;   // the lane's four bytes
         int page = id[0];
 #pragma unroll
         for (int g = 1; g < NG; ++g) page = p / 16 == g ? id[g] : page;
-        load_lds4(src + static_cast<size_t>(page) * page_bytes + at0 + static_cast<size_t>((sb + p) & (size - 1)) * NB + (4 * l) % NB, to);
+        load_lds4(src + static_cast<size_t>(page) * page_bytes + at0 + static_cast<size_t>((sb + static_cast<int>(p)) & (size - 1)) * NB + (4 * l) % NB, to);
     };
     // a step's rows on their way, to tile or raw buffer `buf`
     auto load = [&](int buf, int sb) {
+        if (wv >= LOADERS) return;   // uniform
         if constexpr (CODES) {
             const uint32_t to = pool0 + 2 * S::kTile + buf * RAW;
 #pragma unroll
-            for (int n = 0; n < S::kHalf / 2 / (1024 * WAVES); ++n) {   // as many as rows of eight bits take
-                raw_codes(a.k, kpage, k_at, std::integral_constant<int, KT>{}, sb, to, wv + n * WAVES);
-                raw_codes(a.v, vpage, v_at, std::integral_constant<int, VT>{}, sb, to + STEP * kKB, wv + n * WAVES);
+            for (int n = 0; n < S::kHalf / 2 / (1024 * LOADERS); ++n) {   // as many as rows of eight bits take
+                raw_codes(a.k, kpage, k_at, std::integral_constant<int, KT>{}, sb, to, wv + n * LOADERS);
+                raw_codes(a.v, vpage, v_at, std::integral_constant<int, VT>{}, sb, to + STEP * kKB, wv + n * LOADERS);
             }
             if (wv == 0) raw_scales(a.k, kpage, kv_row<KT>(0, kv, a.n_kv, size, HD).scale, sb, to + STEP * (kKB + kVB));
             if (wv == 1) raw_scales(a.v, vpage, kv_row<VT>(0, kv, a.n_kv, size, HD).scale, sb, to + STEP * (kKB + kVB + NB));
-        } else if (wv < LOADERS) {   // uniform
+        } else {
             const uint32_t to = pool0 + buf * S::kTile;
             direct(a.k, kpage, kstride, k_at, sb, to, true);
             direct(a.v, vpage, vstride, v_at, sb, to + S::kHalf, false);
         }
     };
-    // raw buffer `buf` to tile `buf`: a thread turns 16 dims of a position at a time
-    auto turn_rows = [&](auto type, const uint8_t* codes, const uint8_t* scales, uint8_t* to, bool k) {
+    // raw buffer `buf` to tile `buf`: a thread turns 16 dims of K and of V of a position at a time, both read before either is turned
+    auto codes16 = [](auto type, const uint8_t* codes, int at) {
         constexpr int T = decltype(type)::value;
-        constexpr int UP = THREADS / (HD / 16);   // positions to a thread's next unit
-        const int t = fresh<PAGED>(tid), pos = t / (HD / 16), col = t % (HD / 16);
+        Dims16<T> x;
+        if constexpr (T == kKvI8) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(codes + 16 * at);
+            x.w[0] = v[0], x.w[1] = v[1], x.w[2] = v[2], x.w[3] = v[3];
+        } else if constexpr (T == kKvI4) {
+            const uint2 v = *reinterpret_cast<const uint2*>(codes + 8 * at);
+            x.w[0] = v.x, x.w[1] = v.y;
+        }
+        return x;
+    };
+    auto swap_halves = [](auto& x, bool yes) {
+        constexpr int W = sizeof(x.w) / sizeof(x.w[0]) / 2;
 #pragma unroll
-        for (int u = 0; u < STEP / UP; ++u) {
-            const int p = pos + u * UP;
-            Dims16<T> x;
-            if constexpr (T == kKvI8) {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(codes + p * HD + 16 * col);
-                x.w[0] = v[0], x.w[1] = v[1], x.w[2] = v[2], x.w[3] = v[3];
-            } else if constexpr (T == kKvI4) {
-                const uint2 v = *reinterpret_cast<const uint2*>(codes + p * (HD / 2) + 8 * col);
-                x.w[0] = v.x, x.w[1] = v.y;
-            }
-            const uint32_t sc = scales[p * NB + col / 2];
-            const Scale2 s = scale2<T>(sc, sc);
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int piece = 2 * col + hf, at = k ? piece ^ (p & 15) : piece ^ (v_swizzle(p) << 1);
-                *reinterpret_cast<half8*>(to + p * ROW + 16 * at) = operand<T>(x, hf, s);
-            }
+        for (int e = 0; e < W; ++e) {
+            const uint32_t lo = x.w[e], hi = x.w[e + W];
+            x.w[e] = yes ? hi : lo;
+            x.w[e + W] = yes ? lo : hi;
         }
     };
     auto turn = [&](int buf) {
         if constexpr (CODES) {
-            const uint8_t* from = pool + 2 * S::kTile + buf * RAW;
-            uint8_t* to = pool + buf * S::kTile;
-            const uint8_t* scales = from + STEP * (kKB + kVB);
-            turn_rows(std::integral_constant<int, KT>{}, from, scales, to, true);
-            turn_rows(std::integral_constant<int, VT>{}, from + STEP * kKB, scales + STEP * NB, to + S::kHalf, false);
+            constexpr int UP = THREADS / (HD / 16);   // positions to a thread's next unit
+            const uint8_t* const raw = pool + 2 * S::kTile + buf * RAW;
+            const uint8_t* const scales = raw + STEP * (kKB + kVB);
+            uint8_t* const to = pool + buf * S::kTile;
+            const uint32_t t = static_cast<uint32_t>(fresh<true>(tid)), pos = t / (HD / 16), col = t % (HD / 16);
+#pragma unroll
+            for (int u = 0; u < STEP / UP; ++u) {
+                const uint32_t p = pos + u * UP, n = t + u * THREADS;   // unit n = p HD / 16 + col
+                Dims16<KT> k = codes16(std::integral_constant<int, KT>{}, raw, n);
+                const uint32_t ks = scales[n / 2];
+                Dims16<VT> v = codes16(std::integral_constant<int, VT>{}, raw + STEP * kKB, n);
+                const uint32_t vs = scales[STEP * NB + n / 2];
+                const Scale2 k2 = scale2<KT>(ks, ks), v2 = scale2<VT>(vs, vs);
+                uint8_t* const row = to + p * ROW;
+                // columns from the ninth on write their second half first: a row's 16 lanes would meet on half of the banks
+                const uint32_t other = col & 8;
+                const uint32_t at_k = (16 * ((2 * col) ^ (p & 15))) ^ (2 * other), at_v = (32 * (col ^ v_swizzle(p))) ^ (2 * other);
+                swap_halves(k, other != 0);
+                swap_halves(v, other != 0);
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) *reinterpret_cast<half8*>(row + (at_k ^ (16 * hf))) = operand<KT>(k, hf, k2);
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) *reinterpret_cast<half8*>(row + S::kHalf + (at_v ^ (16 * hf))) = operand<VT>(v, hf, v2);
+            }
         }
     };
 
+    ask_pages(c0);
     find_pages(c0);
     if (nsteps > 0) load(0, c0);
     uint32_t bad = next_bad, bad2 = 0;   // of this step and the next
-    find_pages(c0 + STEP);
+    ask_pages(c0 + STEP);
     if constexpr (CODES) {   // codes come two steps ahead
+        find_pages(c0 + STEP);
         if (nsteps > 1) load(1, c0 + STEP);
         bad2 = next_bad;
-        find_pages(c0 + 2 * STEP);
+        ask_pages(c0 + 2 * STEP);
     }
     // q is here before the loop: inside it, a wait for q would be one for the tiles on their way
 #pragma unroll
@@ -1068,10 +1106,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
         __builtin_amdgcn_s_barrier();   // this step's tile is there, and the other one is read
         asm volatile("" ::: "memory");
         const uint32_t step_bad = bad;
-        if (st + LEAD < nsteps) load(CODES ? buf : buf ^ 1, sb + LEAD * STEP);
-        bad = CODES ? bad2 : next_bad;
-        bad2 = next_bad;
-        find_pages(sb + (LEAD + 1) * STEP);
+        auto load_ahead = [&] {
+            find_pages(sb + LEAD * STEP);
+            if (st + LEAD < nsteps) load(CODES ? buf : buf ^ 1, sb + LEAD * STEP);
+            bad = CODES ? bad2 : next_bad;
+            bad2 = next_bad;
+        };
+        if (!CODES) load_ahead();
         // half of the waves turn the next step's codes before their products, half after: a SIMD has one of each
         if (CODES && more && wv >= WAVES / 2) turn(buf ^ 1);
         const bool tail = sb + STEP - 1 > first;   // uniform: not every row sees the whole step
@@ -1087,9 +1128,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void batch_tile_kernel(BatchArgs a) 
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
         }
-        if (sb <= wlast)   // uniform in the wave
+        auto scored = [&] {
+            if (CODES) load_ahead();   // at the step's start it held up the waves that turn codes then: 900 cycles became 1340
+            ask_pages(sb + (LEAD + 1) * STEP);
+        };
+        if (sb > wlast) scored();   // uniform in the wave (with `else` for the next line the compiler spills half of o)
+        if (sb <= wlast)
             tile_step<BF, HD, VT, PAGED, HD == 128>(tile, tile + S::kHalf, kat, vat, q, o, m_run, l_run, post, sb, last, lim, h, step_bad,
-                                                    sb + STEP - 1 > wfirst || row0 + kWaveRows > rows, [] {},
+                                                    sb + STEP - 1 > wfirst || row0 + kWaveRows > rows, scored, [] {},
                                                     [&] { return tail && odd[buf] == st + 1; }, v_row);
         if (CODES && more && wv < WAVES / 2) turn(buf ^ 1);
     }
@@ -1238,7 +1284,7 @@ __global__ __launch_bounds__(kThreads, 1) void batch_parts_kernel(BatchArgs a) {
         bool odd = false;
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");   // K; V's loads came after
         tile_step<BF, HD, kKvF16, false, false>(
-            kt, vt, kat, vat, q, o, m_run, l_run, a.post, sb, last, lim, h, 0, tail || short_rows,
+            kt, vt, kat, vat, q, o, m_run, l_run, a.post, sb, last, lim, h, 0, tail || short_rows, [] {},
             [&] {
                 if (more) {
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K is read
@@ -1336,7 +1382,8 @@ __device__ __forceinline__ bool row_chunks(const BatchArgs& a, int t, int* chunk
     return true;
 }
 
-// Few chunks: a wave a row, HD / 64 dims a lane.
+// Few chunks: a wave a row of 256 dims or two of 128, four dims a lane.  Bound by its bytes: 999 tokens, 16 heads of 256 dims, four
+// chunks, 95 MB with gates and outputs, 19.8 us (4.8 TB/s).
 constexpr int kFlatChunks = 8;
 
 template <int HD>
@@ -1370,7 +1417,8 @@ __global__ __launch_bounds__(kThreads) void batch_join_flat_kernel(BatchArgs a) 
     finish4<HD>(a, t, h, d, o, g);
 }
 
-// Many chunks: workgroup (row, 64 dims); weights to LDS, wave w sums chunks w, w + 4, ... in order, then the waves in order.
+// Many chunks: workgroup (row, 64 dims); weights to LDS, wave w sums chunks w, w + 4, ... in order, then the waves in order.  One token
+// of 16 heads over 64 chunks 4.6 us.
 constexpr int kJoinBatch = 16;
 
 template <int HD>

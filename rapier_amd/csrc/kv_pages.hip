@@ -20,7 +20,7 @@ namespace {
 // Both are two prefix sums over the requests and a copy.  Every workgroup takes the sums of all requests for itself (16 KB of
 // lengths at most, from the L2), so one launch does and no workgroup waits for another; tokens and pages are then dealt out over
 // all of them, each finding its request by bisection of the sums in LDS.  Latency-bound: loads, two sums with their barriers, a bisection, a
-// load; 32 requests of one token 4 us.
+// load; a plan of 32 requests of one token 4.4 us, of 999 with 121 K tokens 9.3 us; a trim 2.5 and 4.4.
 constexpr int kPlanThreads = 256;
 constexpr uint32_t kSat = 1u << 30;   // sums stop here: min(a + b, kSat) is associative, and lengths may be anything
 constexpr uint32_t kRefused = 1u << 31;
@@ -175,7 +175,8 @@ __global__ __launch_bounds__(kPlanThreads) void page_trim_kernel(TrimArgs a) {
 }
 
 // ---- rows of slots -------------------------------------------------------------------------------------------------------
-// kv_read's unit (eight dims a lane), each row at its own slot
+// kv_read's unit (eight dims a lane), each row at its own slot: 1999 rows of 4 x 256 dims F16 4.3 us, of which 2 are the beginning and
+// end of a launch (16.4 MB with the outputs)
 constexpr int kReadThreads = 256;
 
 template <int T, bool OUT16, bool VEC>
@@ -201,7 +202,8 @@ __global__ __launch_bounds__(kReadThreads) void kv_page_read_kernel(const uint8_
 // dims; a row's loads go out before the work on the row before it.  The frequencies are the host's (2 pi left out, YaRN's ramp in
 // them), so that an angle is one fp64 product, its fraction, and two polynomials; pow and sincos on the device were half of
 // attn_prep_axes' time.  q is normed and rotated in fp32 and rounded to 16 bits; K in fp64, rounded to fp32 once, so that what a
-// cache holds does not hang on the order of a sum (a code at a border would).
+// cache holds does not hang on the order of a sum (a code at a border would).  Bound by the rows: 1999 tokens of 16 + 4 heads of 256
+// dims, 74 MB, 17.8 us (4.2 TB/s); 32 tokens, a wave a row, 4.6 us of waits: slot, row, weights, then the angles' barrier.
 constexpr int kPrepWaves = 4;
 constexpr int kMaxPairs = 128;
 
