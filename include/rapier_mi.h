@@ -459,7 +459,9 @@ int rmi_logits_process(const float* logits, int n, int ncols, int col_stride, fl
  * of a layer are two pools under the same page ids.  Slot s is position s % page_size of page s / page_size.  A block table has
  * a row of table_stride page ids for each of up to 4096 requests: position p of request i is in page
  * table[i * table_stride + p / page_size].  Lengths, page ids and slots are device words and checked there: none leads outside a
- * pool, a table or a call's rows.  No two pages of one table that are in use may be the same. */
+ * pool, a table or a call's rows.  A page that is
+ * written is in use by one request, once; pages that are only read may be several requests' (then the caller counts their users:
+ * rmi_page_trim gives back what it is told). */
 enum { RMI_PAGES_OK = 0, RMI_PAGES_BAD_LENGTH = 1, RMI_PAGES_NONE_LEFT = 2 };   /* status of a request in a plan */
 
 /* The plan of a round in which request i, of past[i] positions so far, gets count[i] >= 0 new tokens.
