@@ -66,14 +66,9 @@ __device__ __forceinline__ Req request(const BatchArgs& a, int i, int first, int
     return r;
 }
 
-__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
-    v += xor_lane<32>(v);
-    v += xor_lane<16>(v);
-    v += xor_lane<8>(v);
-    v += xor_lane<4>(v);
-    v += xor_lane<2>(v);
-    v += xor_lane<1>(v);
-    return v;
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {   // a scalar
+    const uint32_t upto = wave_scan(v, [](uint32_t x, uint32_t y) { return x + y; });
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
 }
 
 // The workgroup's tile by its rank among all of the call.  A request's tile at `level` is its rows 128 level ..; tiles go by level,
@@ -85,7 +80,7 @@ __device__ __forceinline__ bool tile_of_rank(const BatchArgs& a, F&& count, uint
     auto above = [&](int l) {   // tiles at level l and higher
         uint32_t s = 0;
         for (int i = lane; i < a.n_req; i += 64) s += static_cast<uint32_t>(max(count(i) - l, 0));
-        return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(wave_sum(s))));
+        return wave_sum(s);
     };
     if (rank >= above(0)) return false;
     int lo = 0, hi = a.levels;   // above(lo) > rank, above(hi) <= rank (nothing is at the bound)
