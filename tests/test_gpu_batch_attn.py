@@ -514,6 +514,50 @@ def test_prompt_q_that_is_not_finite(rmi, name, lens, n_kv, G):
         assert np.array_equal(got, plain)
 
 
+@pytest.mark.parametrize("lens,n_kv,G", [([100, 40, 3], 1, 8), ([20] * 30, 2, 4), ([257, 9, 2], 8, 64)])
+def test_prompt_row_starts_that_are_not(rmi, lens, n_kv, G):
+    """row starts beyond the call, negative or descending lead nowhere outside it"""
+    rng = np.random.default_rng(4)
+    args, y = prompt_case(rmi, rng, lens, "bfloat16", n_kv, G, 128, gate=False, q8=False, heads=[0])
+    for start in ([0, 1, 10 ** 9, 10 ** 9], [-5, -9, 3, 2], [7, 3, 1, 0], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 5], [0, 200, 0, 200]):
+        args[6][:4] = ints(np.array(start, np.int64).astype(np.int32))
+        rmi.gqa_prompt_attn(*args)
+        torch().cuda.synchronize()
+
+
+@pytest.mark.parametrize("lens,n_kv,G", [([100, 40], 1, 8), ([20] * 30, 2, 4), ([257, 9], 8, 64)])
+def test_prompt_graph_and_stream(rmi, lens, n_kv, G):
+    """a captured call reads the row starts when it runs; on another stream the same bits"""
+    t = torch()
+    rng = np.random.default_rng(len(lens))
+    args, y = prompt_case(rmi, rng, lens, "float16", n_kv, G, 128, heads=[1])
+    first, start, blocks = y.clone(), args[6], args[11]
+    other = t.cuda.Stream()
+    other.wait_stream(t.cuda.current_stream())
+    y.fill_(77.0)
+    t.cuda.synchronize()
+    rmi.gqa_prompt_attn(*args, stream=other)
+    other.synchronize()
+    assert t.equal(y, first)
+    graph = t.cuda.CUDAGraph()
+    with t.cuda.graph(graph):
+        rmi.gqa_prompt_attn(*args)
+    keep = start.clone()
+    for cut in (0, 7, 3, 0):   # the first prompt's last rows become the second's first
+        start.copy_(keep)
+        start[1:-1] -= cut
+        got = []
+        for run in (graph.replay, lambda: rmi.gqa_prompt_attn(*args)):
+            y.fill_(77.0)
+            blocks.fill_(0xee)
+            t.cuda.synchronize()
+            run()
+            t.cuda.synchronize()
+            got.append((y.clone(), blocks.clone()))
+        assert t.equal(got[0][0], got[1][0]) and t.equal(got[0][1], got[1][1])
+        assert t.equal(got[0][0], first) == (cut == 0)
+
+
 @pytest.mark.parametrize("name", ["float16", "bfloat16"])
 @pytest.mark.parametrize("hd", [128, 256])
 @pytest.mark.parametrize("lens,n_kv,G", [([40, 100, 9], 1, 4), ([40, 100, 9], 1, 3), ([40, 257, 9], 8, 64), ([40, 100, 9] + [90] * 18, 1, 4)])
