@@ -4,12 +4,13 @@
 // No counterpart in the reference, which serves one request (gqa_head_kernel, qw:384-442; its ingest's score pass, qw:444-559).
 //
 // Query row r of a request and KV head is token r / G, head r % G of the head's G.  Token t of n new ones is at position
-// len - n + t and sees the positions up to its own.  Three kernels:
+// len - n + t and sees the positions up to its own.  Kernels:
 //   few     up to 16 rows a request, 32 of a quantised cache (decode, drafts): workgroup (request, KV head, chunk of positions), K
 //           and V straight from the pages into matrix operands; bound by the cache
-//   tile    more rows: workgroup (128 rows, KV head, chunk), K and V tiles in LDS
+//   tile    more rows: workgroup (128 or 256 rows, KV head, chunk), K and V tiles in LDS
+//   parts   prompts of few tiles: workgroup (32 rows, KV head), its waves taking steps of the positions in turn
 //   join    the chunks' records (m, l, o) of a row, where the context is split
-// A paged call with requests of both kinds launches both of the first two; each takes its own requests.
+// A paged call with requests of both kinds launches the first two; each takes its own requests.
 #include "kv_operand.h"
 #include "kv_pages.h"
 #include "overlap.h"
