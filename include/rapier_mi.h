@@ -470,7 +470,7 @@ enum { RMI_PAGES_OK = 0, RMI_PAGES_BAD_LENGTH = 1, RMI_PAGES_NONE_LEFT = 2 };   
  *                         in request order the first page taken is free_pages[n_free[0] - 1], the next the one before
  *   kv_len[i], status[i]  past + count and RMI_PAGES_OK; or 0 and a reason, and the request gets no page: its lengths are
  *                         negative, longer than the table's row or than 2^30, or its rows pass max_tok; or it needs pages and the
- *                         sum of those needed up to and with it passes n_free
+ *                         sum of those needed up to and with it passes n_free (it keeps the pages of past, and its rows)
  *   slot, pos [max_tok]   per row its token's slot (-1: refused, or behind the last request) and position (0 behind the last)
  *   n_left                what is left of the free list, free_pages[0 .. n_left)
  * free_pages holds n_pages words, max_tok <= 2^30.  Outputs share no byte with each other or with inputs (n_left is not n_free:
@@ -479,7 +479,8 @@ int rmi_page_plan(const int* past, const int* count, int n_req, int page_size, i
                   const int* n_free, int* table, int table_stride, int max_tok, int* row_start, int* kv_len, int* slot,
                   int* pos, int* n_left, int* status, void* stream);
 /* Gives back the pages past the positions that requests keep: pages ceil(keep / page_size) .. ceil(len / page_size) - 1 of each,
- * in the order of requests and positions, to free_pages[n_free[0]] on; n_out the new count.  keep = len gives back nothing (nor
+ * in the order of requests and positions, to free_pages[n_free[0]] on; n_out the new count.  len is what a request holds pages for:
+ * after a plan the larger of kv_len and past, since kv_len is 0 where the plan refused.  keep = len gives back nothing (nor
  * does keep < 0 or keep > len), keep = 0 all of a request.  Pages past n_pages free ones are dropped.  The table is left as
  * it is.  Outputs share no byte with each other or with inputs. */
 int rmi_page_trim(const int* len, const int* keep, int n_req, int page_size, int n_pages, const int* table, int table_stride,

@@ -800,7 +800,8 @@ def page_plan(past, count, n_req, page_size, n_pages, free_pages, n_free, table,
 
 
 def page_trim(length, keep, n_req, page_size, n_pages, table, table_stride, n_free, free_pages, n_out, stream=None):
-    """the pages past the first keep[i] of length[i] positions of each request, back to the free list"""
+    """the pages past the first keep[i] of length[i] positions of each request, back to the free list (after a plan, length is the
+    larger of kv_len and past: a request that it refused has kv_len 0 and still holds its pages)"""
     _call("rmi_page_trim", _i32(length), _i32(keep), n_req, page_size, n_pages, _i32(table), table_stride, _i32(n_free),
           _i32(free_pages), _i32(n_out), _s(stream, table, length, keep, n_free, free_pages, n_out))
 
