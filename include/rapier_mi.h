@@ -510,8 +510,8 @@ int rmi_attn_prep_paged(const float* q3, int q3_stride, const float* qn, const f
  * Any mix of single tokens, drafts and prompt chunks.  Cache types as rmi_gqa_tree_decode's; products on fp16 operands (bf16 q
  * is brought to fp16 by a power of two a row, the weights are rounded to fp16), sums in fp32.  scale > 0.  Sigmoid gate, y (of
  * qtype, 8-byte aligned, y_stride a multiple of 4) and Q8_1 as rmi_gqa_tree_decode's.
- * Left as they are: rows behind the last request's, and rows of a request with more than max_new new tokens or more than max_ctx
- * positions.  A token at a negative position (kv_len below the number of new tokens) gives zeros.  A token that sees a position
+ * Left as they are: rows before the first request's and behind the last's, and rows of a request with more than max_new new tokens
+ * or more than max_ctx positions.  A token at a negative position (kv_len below the number of new tokens) gives zeros.  A token that sees a position
  * whose page id is outside the pool or past the table's row gives NaN.  What a token does not see has no part in its result,
  * whatever it holds; a NaN in what it sees, or an infinity in V, makes it NaN or infinite (an infinite score is the formula's:
  * +inf gives NaN, -inf a weight of zero).
@@ -532,7 +532,7 @@ int rmi_gqa_paged_attn(int qtype, const void* q, int ktype, const void* kpool, i
  * ([n_head][head_dim]), k and v ([n_kv][head_dim]), all of one type, are request i's; row t of it sees its rows up to t.  Rows are
  * q_stride, k_stride and v_stride elements apart (multiples of 8, those of k and v up to 2^25; q, k and v 16-byte aligned); an F16
  * cache's rows, contiguous or pages in order, can be k and v.  BF16 rows are multiplied as bf16, the weights rounded to it.
- * Requests of more than max_len rows are left out, rows behind the last request's are left as they are.  Gate, y, Q8_1 and what
+ * Requests of more than max_len rows are left out, rows of no request are left as they are.  Gate, y, Q8_1 and what
  * is not finite as above. */
 int rmi_gqa_prompt_attn(int type, const void* q, int q_stride, const void* k, int k_stride, const void* v, int v_stride,
                         const int* row_start, const float* gate_src, int gate_stride, void* y, int y_stride, uint8_t* q8,

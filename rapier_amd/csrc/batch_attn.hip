@@ -1352,21 +1352,21 @@ __global__ __launch_bounds__(kThreads, 1) void batch_parts_kernel(BatchArgs a) {
 }
 
 // ---- join ------------------------------------------------------------------------------------------------------------------
-// the request of a call's row t: the last whose rows begin at or before it, 64 starts at a time
+// the request of a call's row t: the last whose rows begin at or before it (the first if none does), 64 starts at a time
 __device__ __forceinline__ int request_of_row(const BatchArgs& a, int t) {
     const int lane = threadIdx.x & 63;
     int lo = 0, n = a.n_req;   // among requests [lo, lo + n)
     while (n > 1) {
         const int step = (n + 63) / 64, at = lo + lane * step;
         const bool in = lane * step < n && a.row_start[min(at, a.n_req - 1)] <= t;
-        const int k = max(__popcll(__ballot(in)) - 1, 0);   // starts ascend
+        const int k = max(static_cast<int>(__popcll(__ballot(in))) - 1, 0);   // starts ascend; the count is unsigned, and there may be none
         n = min(step, n - k * step);
         lo += k * step;
     }
     return lo;
 }
 
-// A row's chunks; false: the row is not written (behind the last request, or past the call's bounds)
+// A row's chunks; false: the row is not written (no request's, or past the call's bounds)
 __device__ __forceinline__ bool row_chunks(const BatchArgs& a, int t, int* chunks, bool* none) {
     const int i = __builtin_amdgcn_readfirstlane(request_of_row(a, t));
     const Req r = request(a, i, word(a.row_start, i), word(a.row_start, i + 1));
