@@ -1694,7 +1694,7 @@ extern "C" int rmi_gqa_paged_attn(int qtype, const void* q, int ktype, const voi
     a.n_kv = n_kv;
     a.shift = page_shift_of(page_size);
     a.n_pages = n_pages;
-    a.chunk = split;
+    a.chunk = std::min(split, (max_ctx + kChunkUnit - 1) / kChunkUnit * kChunkUnit);   // a length and a chunk fit an int
     a.chunks = chunks;
     a.wo = static_cast<float*>(workspace);
     a.wml = a.wo + static_cast<size_t>(chunks) * ntok * n_head * head_dim;
