@@ -623,7 +623,7 @@ __global__ __launch_bounds__(kThreads, KT == kKvF16 || RB == 2 ? 1 : 2) void bat
 // from memory held up every wave: 999 tokens behind 8 K of I8 / I4 249 us, 179 so.
 // Bound by the matrix cores and LDS together: a step of 256 rows x 32 positions is 2048 cycles of products and 256 KB of operands, 2048
 // cycles at 128 bytes each, with the softmax beside them, and takes some 3400: one prompt of 8001 tokens x 16 heads of 256 dims
-// 457 to 502 us, 1.05 to 1.15 PFLOP/s (a large library product 1.18), the matrix cores busy for 56 % of it.  Codes cost 7 % more over F16 pages (999
+// 457 to 502 us, 1.05 to 1.15 PFLOP/s (a large library product 1.18), the matrix cores busy for 58 % of it.  Codes cost 7 % more over F16 pages (999
 // tokens behind 7 K: 159 us with the join, I8 170, I4 163).
 // LDS rows have no padding (the direct loads write 1024 bytes in a row); instead their 16-byte (K) or 32-byte (V) pieces are permuted by the row, so that the lanes of a read fall on different banks:
 // K piece c of row p is at c ^ (p % 16), V piece c at c ^ {0, 3, 5, 6}[p % 4].
